@@ -6,6 +6,9 @@ include/dz_host.h and include/dz_cuda.h (dranzer_b200/libdz_cuda.so):
   quantize_pack / quantize_unpack      src/include/core/quantize.h:129-140
   QuantizedWeightMatrix,
   matmul_quantized_weight              src/include/core/quantized_matmul.h:13-42
+  quantize_pack_grouped,
+  GroupedWeightMatrix, KV4Cache        none: 4-bit weights with group scales, the
+                                       4-bit ring cache and its attention
   Bundle (code-retaining loader),
   save_quantized_bundle                src/include/core/bundle.h:52-85
   Model, KVCache.forward_tokens        model_forward_token, src/core/transformer.c:755
@@ -19,18 +22,20 @@ import ctypes
 
 import numpy as np
 
-from ._native import (DzBundleInfo, DzBundleMeta, DzError, DzGenerationControls, DzGenerationResult,
-                      DzModelDesc, DzSampling, DzTensorBlob, check, lib)
+from ._native import (DzBundleInfo, DzBundleMeta, DzError, DzGenerationControls, DzGenerationResult, DzGroupedBlob,
+                      DzKv4, DzKv4Append, DzKv4Attention, DzModelDesc, DzSampling, DzTensorBlob, check, lib)
 
 __all__ = ["GRAN_TENSOR", "GRAN_ROW", "GRAN_COLUMN", "GREEDY", "TOPK", "TOPP", "STREAM_INIT",
            "STREAM_DROPOUT", "STREAM_SAMPLING", "STREAM_TESTING", "DzError", "available",
            "rng_stream", "synth_gaussian", "synth_prompt_ids", "quantized_scale_count",
            "quantized_packed_size", "quantize_pack", "quantize_unpack", "quantized_slice", "positional_encoding", "fnv1a",
            "QuantizedWeightMatrix", "matmul_quantized_weight", "Bundle", "save_quantized_bundle",
-           "minimal_tokenizer", "model_tensor_layout", "Sampling", "Controls", "Model", "KVCache"]
+           "TYPE_F32", "TYPE_F16", "TYPE_BF16", "quantize_pack_grouped", "quantize_unpack_grouped",
+           "GroupedWeightMatrix", "KV4Cache", "minimal_tokenizer", "model_tensor_layout", "Sampling", "Controls", "Model", "KVCache"]
 
 GRAN_TENSOR, GRAN_ROW, GRAN_COLUMN = 0, 1, 2
 GREEDY, TOPK, TOPP = 0, 1, 2
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 PREFILL_AUTO, PREFILL_TOKENS, PREFILL_BATCHED = 0, 1, 2
 KIND_PROJECTION, KIND_EMBEDDING, KIND_BIAS, KIND_NORM = 0, 1, 2, 3
 STREAM_INIT = 0x9E3779B97F4A7C15
@@ -220,6 +225,143 @@ class QuantizedWeightMatrix:
 def matmul_quantized_weight(A, weights):
     """C = A . deq(W) (matmul_quantized_weight, src/core/quantized_matmul.c:253-295)."""
     return weights.matmul(A)
+
+
+# ------------------------------------------------------- 4-bit group scales
+
+def quantize_pack_grouped(values, group):
+    """(scales [ceil(rows / group), cols], packed) of a rows x cols float32
+    matrix, 4 bits, one scale per `group` rows of a column
+    (dz_quantize_pack_grouped)."""
+    w = np.ascontiguousarray(values, np.float32)
+    if w.ndim != 2 or group not in (32, 64, 128):
+        raise ValueError("values must be 2-D (rows x cols) and groups hold 32, 64 or 128 rows")
+    rows, cols = w.shape
+    scales = np.empty((-(-rows // group), cols), np.float32)
+    packed = np.empty((rows * cols + 1) // 2, np.uint8)
+    if lib().dz_quantize_pack_grouped(_p(w), rows, cols, group, _p(scales), scales.size, _p(packed), packed.size) != 0:
+        raise ValueError("quantize_pack_grouped rejected the input (non-finite value or bad arguments)")
+    return scales, packed
+
+
+def quantize_unpack_grouped(scales, packed, rows, cols, group):
+    s = np.ascontiguousarray(scales, np.float32)
+    p = np.ascontiguousarray(packed, np.uint8)
+    out = np.empty((rows, cols), np.float32)
+    if lib().dz_quantize_unpack_grouped(_p(s), s.size, _p(p), p.size, rows, cols, group, _p(out)) != 0:
+        raise ValueError("quantize_unpack_grouped rejected the payload (non-canonical codes or bad scales)")
+    return out
+
+
+class GroupedWeightMatrix:
+    """A 4-bit matrix with one scale per `group` rows of a column, resident on a
+    device (dz_cuda_gmatrix_create). scales: float32 or float16."""
+
+    def __init__(self, scales, packed, rows, cols, group, device=0):
+        s = np.ascontiguousarray(scales)
+        if s.dtype != np.float16:
+            s = np.ascontiguousarray(s, np.float32)
+        p = np.ascontiguousarray(packed, np.uint8)
+        self._create(s.ctypes.data, s.size, TYPE_F16 if s.dtype == np.float16 else TYPE_F32, p.ctypes.data, p.size,
+                     rows, cols, group, device)
+
+    @classmethod
+    def encode(cls, values, group, device=0):
+        w = np.ascontiguousarray(values, np.float32)
+        s, p = quantize_pack_grouped(w, group)
+        return cls(s, p, w.shape[0], w.shape[1], group, device)
+
+    @classmethod
+    def from_device(cls, scales_ptr, packed_ptr, rows, cols, group, scale_type=TYPE_F32, device=0):
+        """From codes and scales that lie in device memory already (copied)."""
+        self = cls.__new__(cls)
+        if rows < 1 or cols < 1 or group < 1:
+            raise ValueError("rows, cols and group must be positive")
+        self._create(scales_ptr, -(-rows // group) * cols, scale_type, packed_ptr, (rows * cols + 1) // 2, rows, cols,
+                     group, device)
+        return self
+
+    def _create(self, scales, scale_count, scale_type, packed, packed_size, rows, cols, group, device):
+        self.rows, self.cols, self.group, self.device = rows, cols, group, device
+        blob = DzGroupedBlob(rows, cols, group, packed, packed_size, scales, scale_count, scale_type)
+        h = ctypes.c_void_p()
+        check(lib().dz_cuda_gmatrix_create(device, ctypes.byref(blob), ctypes.byref(h)), "gmatrix_create")
+        self.handle = h.value
+
+    @property
+    def nbytes(self):
+        return lib().dz_cuda_gmatrix_bytes(self.handle)
+
+    def unpack(self):
+        out = np.empty((self.rows, self.cols), np.float32)
+        check(lib().dz_cuda_gmatrix_unpack(self.handle, _p(out)), "gmatrix_unpack")
+        return out
+
+    def matmul(self, A):
+        a = np.ascontiguousarray(A, np.float32)
+        if a.ndim == 1:
+            a = a[None, :]
+        m, k = a.shape
+        c = np.empty((m, self.cols), np.float32)
+        check(lib().dz_cuda_matmul_grouped(_p(a), self.handle, _p(c), m, k), "matmul_grouped")
+        return c
+
+    def matmul_async(self, a_ptr, c_ptr, m, stream_ptr=None, type=TYPE_F32, lda=None, ldc=None):
+        """C = A . W on device buffers of element type `type`, row strides in elements."""
+        status = lib().dz_cuda_matmul_grouped_async(a_ptr, self.rows if lda is None else lda, self.handle, c_ptr,
+                                                    self.cols if ldc is None else ldc, m, self.rows, type, stream_ptr)
+        if status:
+            check(status, "matmul_grouped_async")
+
+    def close(self):
+        if getattr(self, "handle", None):
+            lib().dz_cuda_gmatrix_free(self.handle)
+            self.handle = None
+
+    __del__ = close
+
+
+class KV4Cache:
+    """4-bit ring caches of one layer over device buffers that the caller owns
+    (dz_kv4_t): codes [batch, kv_heads, capacity, head_dim / 2] bytes, scales
+    [batch, kv_heads, capacity, head_dim / 64] float32, given as addresses.
+    Positions are a device int64 [batch] array (negative: skip the sequence);
+    operands are device addresses, rows [batch * n_tokens], strides in
+    elements (None: contiguous)."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales, batch, kv_heads, head_dim, capacity, sinks=0, device=0):
+        self.batch, self.kv_heads, self.head_dim = batch, kv_heads, head_dim
+        self.capacity, self.sinks, self.device = capacity, sinks, device
+        self.c = DzKv4(device, k_codes, v_codes, k_scales, v_scales, batch, kv_heads, head_dim, capacity, sinks)
+        self._ref = ctypes.byref(self.c)
+
+    def append(self, positions, n_tokens, *, type=TYPE_F32, q_heads=0, q=None, k=None, v=None, q_stride=None,
+               k_stride=None, v_stride=None, q_out=None, q_out_stride=None, k_out=None, v_out=None,
+               k_out_stride=None, v_out_stride=None, q_gain=None, k_gain=None, eps=1e-6, rope_base=0.0,
+               halves=False, stream_ptr=None):
+        """Norm and rotate q and k per head, quantize k and v into their slots
+        (dz_cuda_kv4_append)."""
+        wq, wk = q_heads * self.head_dim, self.kv_heads * self.head_dim
+        a = DzKv4Append(type, q_heads, q, k, v, wq if q_stride is None else q_stride,
+                        wk if k_stride is None else k_stride, wk if v_stride is None else v_stride, q_out,
+                        wq if q_out_stride is None else q_out_stride, k_out, v_out,
+                        wk if k_out_stride is None else k_out_stride, wk if v_out_stride is None else v_out_stride,
+                        q_gain, k_gain, eps, rope_base, 1 if halves else 0)
+        status = lib().dz_cuda_kv4_append(self._ref, ctypes.byref(a), positions, n_tokens, stream_ptr)
+        if status:
+            check(status, "kv4_append")
+
+    def attention(self, positions, n_tokens, *, type=TYPE_F32, q_heads, q, out, q_stride=None, out_stride=None,
+                  scale=None, window=0, stream_ptr=None):
+        """Attention of the n_tokens newest queries of every sequence
+        (dz_cuda_kv4_attention); scale None: 1 / sqrt(head_dim)."""
+        w = q_heads * self.head_dim
+        a = DzKv4Attention(type, q_heads, q, w if q_stride is None else q_stride, out,
+                           w if out_stride is None else out_stride,
+                           self.head_dim ** -0.5 if scale is None else scale, window)
+        status = lib().dz_cuda_kv4_attention(self._ref, ctypes.byref(a), positions, n_tokens, stream_ptr)
+        if status:
+            check(status, "kv4_attention")
 
 
 # -------------------------------------------------------------------- bundles

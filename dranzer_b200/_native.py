@@ -77,6 +77,28 @@ class DzGenerationResult(ctypes.Structure):
                 ("stopped_on_stop_sequence", U32), ("stop_sequence_index", U32)]
 
 
+class DzGroupedBlob(ctypes.Structure):
+    _fields_ = [("rows", SZ), ("cols", SZ), ("group", SZ), ("packed", P), ("packed_size", SZ), ("scales", P),
+                ("scale_count", SZ), ("scale_type", I32)]
+
+
+class DzKv4(ctypes.Structure):
+    _fields_ = [("device", I32), ("k_codes", P), ("v_codes", P), ("k_scales", P), ("v_scales", P), ("batch", SZ),
+                ("kv_heads", SZ), ("head_dim", SZ), ("capacity", SZ), ("sinks", SZ)]
+
+
+class DzKv4Append(ctypes.Structure):
+    _fields_ = [("type", I32), ("q_heads", SZ), ("q", P), ("k", P), ("v", P), ("q_stride", SZ), ("k_stride", SZ),
+                ("v_stride", SZ), ("q_out", P), ("q_out_stride", SZ), ("k_out", P), ("v_out", P),
+                ("k_out_stride", SZ), ("v_out_stride", SZ), ("q_gain", P), ("k_gain", P), ("eps", F64),
+                ("rope_base", F64), ("rope_pairing", I32)]
+
+
+class DzKv4Attention(ctypes.Structure):
+    _fields_ = [("type", I32), ("q_heads", SZ), ("q", P), ("q_stride", SZ), ("out", P), ("out_stride", SZ),
+                ("scale", F32), ("window", SZ)]
+
+
 # name -> (restype, argtypes); every exported symbol of include/dz_host.h and include/dz_cuda.h
 SIGNATURES = {
     # dz_host.h
@@ -90,6 +112,8 @@ SIGNATURES = {
     "dz_quantized_packed_size": (I32, [SZ, I32, P]),
     "dz_quantize_pack": (I32, [P, SZ, SZ, I32, I32, P, SZ, P, SZ]),
     "dz_quantize_unpack": (I32, [P, SZ, P, SZ, SZ, SZ, I32, I32, P]),
+    "dz_quantize_pack_grouped": (I32, [P, SZ, SZ, SZ, P, SZ, P, SZ]),
+    "dz_quantize_unpack_grouped": (I32, [P, SZ, P, SZ, SZ, SZ, SZ, P]),
     "dz_quantize_dequantize_into": (I32, [P, P, SZ, SZ, I32, I32, P]),
     "dz_quantize_dequantize": (I32, [P, SZ, SZ, I32, I32, P]),
     "dz_positional_encoding": (I32, [P, SZ, SZ]),
@@ -117,6 +141,14 @@ SIGNATURES = {
     "dz_cuda_matmul_quantized": (I32, [P, P, P, SZ, SZ]),
     "dz_cuda_matmul_quantized_async": (I32, [P, P, P, SZ, SZ, P]),
     "dz_cuda_matmul_quantized_noalloc": (I32, [P, P, P, SZ, SZ, P]),
+    "dz_cuda_gmatrix_create": (I32, [I32, P, P]),
+    "dz_cuda_gmatrix_free": (None, [P]),
+    "dz_cuda_gmatrix_bytes": (SZ, [P]),
+    "dz_cuda_gmatrix_unpack": (I32, [P, P]),
+    "dz_cuda_matmul_grouped": (I32, [P, P, P, SZ, SZ]),
+    "dz_cuda_matmul_grouped_async": (I32, [P, SZ, P, P, SZ, SZ, SZ, I32, P]),
+    "dz_cuda_kv4_append": (I32, [P, P, P, SZ, P]),
+    "dz_cuda_kv4_attention": (I32, [P, P, P, SZ, P]),
     "dz_cuda_model_create": (I32, [P, P, SZ, I32, P]),
     "dz_cuda_model_free": (None, [P]),
     "dz_cuda_model_step_bytes": (SZ, [P]),

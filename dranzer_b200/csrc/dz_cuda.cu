@@ -20,6 +20,7 @@
 #include <tuple>
 #include <vector>
 
+#include "shim.cuh"
 #include "decode.cuh"
 #include "qmv.cuh"
 #include "qmma.cuh"
@@ -40,7 +41,7 @@ using namespace dz;
 static thread_local int g_status = DZ_OK;
 static thread_local char g_message[512] = "";
 
-static int fail(int status, const char* fmt, ...) {
+int dz::fail(int status, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_message, sizeof(g_message), fmt, ap);
@@ -49,14 +50,6 @@ static int fail(int status, const char* fmt, ...) {
     return status;
 }
 
-#define DZ_CUDA(call)                                                                      \
-    do {                                                                                   \
-        cudaError_t e_ = (call);                                                           \
-        if (e_ != cudaSuccess)                                                             \
-            return fail(e_ == cudaErrorMemoryAllocation ? DZ_E_NOMEM : DZ_E_DEVICE,        \
-                        "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__); \
-    } while (0)
-
 extern "C" int dz_cuda_last_error(char* buf, size_t n) {
     if (buf && n) {
         strncpy(buf, g_message, n - 1);
@@ -64,20 +57,6 @@ extern "C" int dz_cuda_last_error(char* buf, size_t n) {
     }
     return g_status;
 }
-
-// Switches to a handle's device for the duration of a call.
-struct DeviceGuard {
-    int prev = -1;
-    bool ok = true;
-    explicit DeviceGuard(int dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
-    }
-    ~DeviceGuard() {
-        int cur;
-        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-    }
-};
 
 extern "C" int dz_cuda_available(void) {
     int n = 0;

@@ -271,6 +271,53 @@ int dz_quantize_pack(const float *src, size_t rows, size_t cols, int bits, int g
     return 0;
 }
 
+/* Whether the sizes of a group-scaled rows x cols matrix belong together. */
+static int grouped_sizes_ok(size_t rows, size_t cols, size_t group, size_t scale_count, size_t packed_size) {
+    size_t need_bytes = 0;
+    if (rows == 0 || cols == 0 || rows > SIZE_MAX / cols || (group != 32 && group != 64 && group != 128) ||
+        dz_quantized_packed_size(rows * cols, 4, &need_bytes) != 0 || packed_size != need_bytes) return 0;
+    return scale_count == ((rows - 1) / group + 1) * cols;
+}
+
+int dz_quantize_pack_grouped(const float *src, size_t rows, size_t cols, size_t group, float *scales,
+                             size_t scale_count, uint8_t *packed, size_t packed_size) {
+    if (!src || !scales || !packed || !grouped_sizes_ok(rows, cols, group, scale_count, packed_size)) return -1;
+    memset(scales, 0, scale_count * sizeof(float));
+    memset(packed, 0, packed_size);
+    for (size_t r = 0; r < rows; r++) {
+        float *peaks = scales + (r / group) * cols;
+        for (size_t c = 0; c < cols; c++) {
+            const float v = src[r * cols + c], m = fabsf(v);
+            if (!finite_bits(v)) return -1;
+            if (m > peaks[c]) peaks[c] = m;
+        }
+    }
+    for (size_t r = 0; r < rows; r++)
+        for (size_t c = 0; c < cols; c++) {
+            const size_t i = r * cols + c;
+            const uint32_t code = quant_code(src[i], scales[(r / group) * cols + c], 7);
+            packed[i >> 1] |= (uint8_t)(code << ((i & 1u) * 4));
+        }
+    for (size_t g = 0; g < scale_count; g++)
+        if (scales[g] > 0.0f) scales[g] = scales[g] / 7.0f;
+    return 0;
+}
+
+int dz_quantize_unpack_grouped(const float *scales, size_t scale_count, const uint8_t *packed,
+                               size_t packed_size, size_t rows, size_t cols, size_t group, float *dst) {
+    if (!scales || !packed || !dst || !grouped_sizes_ok(rows, cols, group, scale_count, packed_size)) return -1;
+    for (size_t g = 0; g < scale_count; g++)
+        if (!finite_bits(scales[g]) || scales[g] < 0.0f) return -1;
+    for (size_t r = 0; r < rows; r++)
+        for (size_t c = 0; c < cols; c++) {
+            const size_t i = r * cols + c;
+            const int code = (packed[i >> 1] >> ((i & 1u) * 4)) & 15;
+            if (code > 14) return -1;
+            dst[i] = scales[(r / group) * cols + c] * (float)(code - 7);
+        }
+    return 0;
+}
+
 /* One group of quantize_dequantize_into (quantize_group, src/core/
  * quantize.c:54-116): values src[i * stride], i < count. The original is read
  * before the store so the in-place form measures against it. */

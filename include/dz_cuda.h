@@ -94,6 +94,62 @@ int dz_cuda_matmul_quantized_async(const float *A_dev, const dz_cuda_qmatrix_t *
 int dz_cuda_matmul_quantized_noalloc(const float *A_dev, const dz_cuda_qmatrix_t *weights, float *C_dev,
                                      size_t m, size_t k, void *stream);
 
+/* ---- Group-scaled 4-bit weight matrix (dz_grouped_blob_t), beside the
+ * tensor / row / column granularities above. No counterpart in the reference,
+ * whose finest scales are per row or column. */
+typedef struct dz_cuda_gmatrix dz_cuda_gmatrix_t;
+/* Lays the matrix out on `device`; `packed` and `scales` may be host or device
+ * memory and are copied. DZ_E_INVALID for a code of 15, a scale that is
+ * negative or not finite, or sizes that do not belong together. Synchronous;
+ * for sources in device memory it first waits for all work on `device`. */
+int dz_cuda_gmatrix_create(int device, const dz_grouped_blob_t *weights, dz_cuda_gmatrix_t **out);
+void dz_cuda_gmatrix_free(dz_cuda_gmatrix_t *matrix);
+/* Device bytes of codes + scales a product streams. */
+size_t dz_cuda_gmatrix_bytes(const dz_cuda_gmatrix_t *matrix);
+/* dst[k * n] = scale * (code - 7), computed on the device. Host destination. */
+int dz_cuda_gmatrix_unpack(const dz_cuda_gmatrix_t *matrix, float *dst);
+/* C (m x n) = A (m x k) . W on device buffers, enqueued on `stream` (a
+ * cudaStream_t) without synchronisation. A and C have element type `type` and
+ * row strides lda >= k, ldc >= n in elements; they must not overlap. Products
+ * and sums carry at least 22 bits relative to the largest of each 128
+ * consecutive activations of a row, one rounding to `type` at the end; a row
+ * that holds an infinity or a NaN reads NaN. Meant for few rows (16 at a time
+ * pass over the weights). Nothing is allocated and the handle holds no
+ * scratch: calls on one matrix may overlap, and a call may be captured. */
+int dz_cuda_matmul_grouped_async(const void *A_dev, size_t lda, const dz_cuda_gmatrix_t *weights, void *C_dev,
+                                 size_t ldc, size_t m, size_t k, int type, void *stream);
+/* The same on contiguous fp32 host buffers, synchronous. */
+int dz_cuda_matmul_grouped(const float *A, const dz_cuda_gmatrix_t *weights, float *C, size_t m, size_t k);
+
+/* ---- 4-bit ring caches (dz_kv4_t), on device buffers, enqueued on `stream`
+ * without synchronisation; nothing is allocated. positions[batch] (device,
+ * int64): the position of each sequence's first new token; a sequence with a
+ * negative position is skipped and its rows are left as they were. No
+ * counterpart in the reference, whose caches are fp32. */
+
+/* For n_tokens new tokens of every sequence: queries and keys normed per head
+ * (y = gain * x / sqrt(mean(x^2) + eps)), rotated by position * base^(-2p /
+ * head_dim) for pair p, queries written to q_out, keys and values quantized
+ * into their slots: per 64 elements scale = fp32(peak / 7), code =
+ * clamp(round_half_away(x * fp32(7 / peak)), -7, 7) + 7 (the framework's
+ * quantizer). Keys are normed and rotated in 64 bits and rounded once to fp32
+ * before it. 64 elements that hold an infinity or a NaN are stored with a NaN
+ * scale. An output row may be its own input row (same pointer and stride);
+ * otherwise outputs overlap no input. n_tokens <= capacity - sinks. */
+int dz_cuda_kv4_append(const dz_kv4_t *cache, const dz_kv4_append_t *args, const int64_t *positions,
+                       size_t n_tokens, void *stream);
+
+/* softmax(scale * q . k) . v over the cache for the n_tokens queries of every
+ * sequence, whose own keys have been appended (positions as in that append).
+ * The query at position i sees position p <= i that the ring retains after
+ * the append, when p < sinks, or window is 0, or p > i - window. With a
+ * window, window + n_tokens - 1 <= capacity - sinks is asked (so that no
+ * query has lost a token of its window), and n_tokens <= capacity - sinks
+ * always. fp32 scores, softmax statistics and sums. out must not overlap q or
+ * the cache. */
+int dz_cuda_kv4_attention(const dz_kv4_t *cache, const dz_kv4_attention_t *args, const int64_t *positions,
+                          size_t n_tokens, void *stream);
+
 /* ---- Model: the parameters of a v2/v3 bundle kept as codes on the device.
  * `tensors` are the n blobs of model_param_tensors() order
  * (src/core/model_params.c:39-103), as dz_bundle_tensors() returns them; they are

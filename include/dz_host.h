@@ -42,6 +42,18 @@ int dz_quantize_unpack(const float *scales, size_t scales_count, const uint8_t *
                        size_t packed_size, size_t rows, size_t cols, int bits, int granularity,
                        float *dst);
 
+/* The quantizer with one scale per `group` (32, 64 or 128) consecutive rows of
+ * a column of a rows x cols matrix, 4 bits: dz_quantize_pack's codes and
+ * scales for every such group. scales [ceil(rows / group)][cols], packed
+ * dz_quantized_packed_size(rows * cols, 4) bytes (dz_grouped_blob_t). -1 for
+ * bad arguments or a value that is not finite. dz_quantize_unpack_grouped is
+ * its inverse (dst[k * n] = scale * (code - 7)); -1 for a code of 15 or a
+ * negative or non-finite scale. No counterpart in the reference. */
+int dz_quantize_pack_grouped(const float *src, size_t rows, size_t cols, size_t group, float *scales,
+                             size_t scale_count, uint8_t *packed, size_t packed_size);
+int dz_quantize_unpack_grouped(const float *scales, size_t scale_count, const uint8_t *packed,
+                               size_t packed_size, size_t rows, size_t cols, size_t group, float *dst);
+
 /* Error of one simulated quantization, quant_error_t
  * (src/include/core/quantize.h:58-80): the same fields in the same order. */
 typedef struct {
