@@ -153,81 +153,6 @@ cudaError_t dz_kv4_append_launch(const Kv4AppendArgs& a, int type, int head_dim,
     return cudaGetLastError();
 }
 
-// ---------------------------------------------------------------- attention
-
-// One warp per (row, query head), lanes over the head dimension, the visible
-// positions one after the other with an online softmax.
-template <typename T, int E>
-__global__ void __launch_bounds__(128) dz_kv4_attn_simple_kernel(const __grid_constant__ Kv4AttnArgs a) {
-    constexpr int HD = 32 * E;
-    const int lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const long long row = unit / a.q_heads;
-    const int h = (int)(unit % a.q_heads);
-    if (row >= (long long)a.c.batch * a.n_tokens) return;
-    const int b = (int)(row / a.n_tokens), j = (int)(row % a.n_tokens);
-    const long long first = a.positions[b];
-    if (first < 0) return;
-    const long long pos = first + j, last = first + a.n_tokens - 1, ring = a.c.capacity - a.c.sinks;
-    const int hk = h / (a.q_heads / a.c.kv_heads);
-    float q[E], acc[E];
-#pragma unroll
-    for (int i = 0; i < E; i++) {
-        q[i] = dz_to_float(static_cast<const T*>(a.q)[row * a.ldq + (long long)h * HD + lane * E + i]) * a.scale;
-        acc[i] = 0.0f;
-    }
-    const long long nsink = a.c.sinks < pos + 1 ? a.c.sinks : pos + 1;
-    long long lo = last - ring + 1;
-    if (lo < a.c.sinks) lo = a.c.sinks;
-    if (a.window && pos - a.window + 1 > lo) lo = pos - a.window + 1;
-    const long long base = ((long long)b * a.c.kv_heads + hk) * a.c.capacity;
-    float m = -INFINITY, l = 0.0f;
-    const long long count = nsink + (pos + 1 > lo ? pos + 1 - lo : 0);
-    for (long long i = 0; i < count; i++) {
-        const long long p = i < nsink ? i : lo + (i - nsink);
-        const long long at = base + kv4_slot(p, a.c.sinks, ring);
-        const int group = lane * E / KV4_GROUP;
-        float s = 0.0f, v[E];
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const long long el = at * HD + lane * E + e;
-            s = fmaf(q[e], (float)(((a.c.k_codes[el >> 1] >> ((el & 1) * 4)) & 15) - 7), s);
-            v[e] = (float)(((a.c.v_codes[el >> 1] >> ((el & 1) * 4)) & 15) - 7);
-        }
-        s *= a.c.k_scales[at * (HD / KV4_GROUP) + group];
-        const float vs = a.c.v_scales[at * (HD / KV4_GROUP) + group];
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        const float mn = s > m ? s : m;
-        const float f = m == -INFINITY ? 0.0f : expf(m - mn), w = expf(s - mn);
-        l = l * f + w;
-#pragma unroll
-        for (int e = 0; e < E; e++) acc[e] = acc[e] * f + w * vs * v[e];
-        m = mn;
-    }
-#pragma unroll
-    for (int e = 0; e < E; e++)
-        static_cast<T*>(a.out)[row * a.ldo + (long long)h * HD + lane * E + e] = dz_from_float<T>(acc[e] / l);
-}
-
-template <typename T> static void kv4_attn_t(const Kv4AttnArgs& a, int head_dim, unsigned grid, cudaStream_t st) {
-    if (head_dim == 128)
-        dz_kv4_attn_simple_kernel<T, 4><<<grid, 128, 0, st>>>(a);
-    else
-        dz_kv4_attn_simple_kernel<T, 2><<<grid, 128, 0, st>>>(a);
-}
-
-cudaError_t dz_kv4_attn_launch(const Kv4AttnArgs& a, int type, int head_dim, int, cudaStream_t st) {
-    const unsigned grid = (unsigned)(((long long)a.c.batch * a.n_tokens * a.q_heads + 3) / 4);
-    if (type == DZ_TYPE_F32)
-        kv4_attn_t<float>(a, head_dim, grid, st);
-    else if (type == DZ_TYPE_F16)
-        kv4_attn_t<__half>(a, head_dim, grid, st);
-    else
-        kv4_attn_t<__nv_bfloat16>(a, head_dim, grid, st);
-    return cudaGetLastError();
-}
-
 }  // namespace dz
 
 using namespace dz;

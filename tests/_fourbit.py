@@ -107,14 +107,19 @@ def visible(pos, last, sinks, capacity, window):
     return list(range(min(sinks, pos + 1))) + list(range(oldest, pos + 1))
 
 
-def attend(q, k, v, scale):
+def attend(q, k, v, scale, v_scales):
     """One query head over its visible keys and values (64 bits), and the bound
     of an fp32 evaluation: scores within (hd / 16 + 8) u of sum |q k|, the
-    exponential within 2^-21, n / 16 + 64 additions."""
+    exponential within 2^-21, n / 16 + 64 additions. Weights times value scales
+    enter the product in fp16 parts, scaled so that the largest lies in [2^13,
+    2^14] or is at most halved from there: below fp16's smallest normal number
+    the step is 2^-24, an error of 2^-25 in 2^13, so each token's weight is off
+    by at most 2^-38 of the largest, times a level of at most 7."""
     q, k, v = (t.astype(np.float64) for t in (q, k, v))
     s = scale * (k @ q)
     e = np.exp(s - s.max())
     p = e / e.sum()
     wide = (abs(scale) * (np.abs(k) @ np.abs(q))).max()
     weight = p @ np.abs(v)
-    return p @ v, (2 * (q.size / 16 + 8) * U * wide + 2.0 ** -21 + (len(s) / 16 + 64) * U) * weight, weight
+    least = 7 * len(p) * 2.0 ** -38 * (p[:, None] * v_scales).max()
+    return p @ v, (2 * (q.size / 16 + 8) * U * wide + 2.0 ** -21 + (len(s) / 16 + 64) * U) * weight + least, weight

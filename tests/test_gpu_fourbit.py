@@ -188,6 +188,9 @@ class Ring:
     def snapshot(self):
         return [(c.cpu().numpy().copy(), s.cpu().numpy().copy()) for c, s in zip(self.codes, self.scales)]
 
+    def scale_rows(self, which, b, h, slots):
+        return _np(self.scales[which])[(b * self.heads + h) * self.cap + np.asarray(slots)]
+
     def rows(self, which, b, h, slots):
         """Values [len(slots), hd] of the keys (0) or values (1)."""
         at = ((b * self.heads + h) * self.cap + np.asarray(slots))
@@ -373,9 +376,9 @@ def _check_attention(gpu, ring, kind, n, hq, window, first, q, scale, rows_out=N
                 key = (b, h // (hq // hk))
                 if key not in cached:
                     every = list(range(ring.cap))
-                    cached[key] = ring.rows(0, *key, every), ring.rows(1, *key, every)
-                k, v = (c[slots] for c in cached[key])
-                ref, bound, weight = fb.attend(qv[b, j, h], k, v, scale)
+                    cached[key] = ring.rows(0, *key, every), ring.rows(1, *key, every), ring.scale_rows(1, *key, every)
+                k, v, s = (c[slots] for c in cached[key])
+                ref, bound, weight = fb.attend(qv[b, j, h], k, v, scale, s)
                 if kind == "bf16":
                     bound = bound + 2.0 ** -11 * weight   # weights of the values in 11 bits
                 err = np.abs(got[b, j, h] - ref)
@@ -544,7 +547,7 @@ def test_run_of_the_operators(gpu):
         seen = [fb.slot(i, 4, cap) for i in fb.visible(p, p, 4, cap, 128)]
         for h in range(hq):
             ref, bound, _ = fb.attend(_np(rot)[b, h * hd:(h + 1) * hd], ring.rows(0, b, h // 2, seen),
-                                      ring.rows(1, b, h // 2, seen), hd ** -0.5)
+                                      ring.rows(1, b, h // 2, seen), hd ** -0.5, ring.scale_rows(1, b, h // 2, seen))
             assert (np.abs(_np(att)[b, h * hd:(h + 1) * hd] - ref) <= bound + fb.rounding(ref, "f32")).all()
     ref, bound = fb.product(_np(att), wo.unpack().astype(np.float64))
     assert (np.abs(_np(y) - ref) <= bound + fb.rounding(ref, "f32")).all()
