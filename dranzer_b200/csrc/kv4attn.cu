@@ -1,28 +1,33 @@
 // Attention over the 4-bit ring caches (kv4.cuh), in a translation unit of its
 // own.
 //
-// One cluster of 1 to 8 blocks handles one (sequence, key head) and up to NT x
-// 8 / PARTS of its (query token, query head) pairs; the visible tokens go in
-// tiles of 32 to the cluster's warps in turn, each warp keeps its own softmax
-// state, and the states join in shared memory, then across the cluster.
+// A unit is one (sequence, key head) and up to 4 NT (fp32: 2 NT) of its (query
+// token, query head) pairs. Its visible tokens go in tiles of 32 to a team of
+// 1, 2, 4 or 8 warps in turn, or to the warps of a cluster of 2 to 16 blocks;
+// each warp keeps its own softmax state and the states join in shared memory,
+// then across the cluster. A warp's start and its part in a join cost as much
+// as several tiles, so a team is no larger than it takes to fill the SMs.
 //
-// Products. Codes become levels -7..7 in fp16, which is exact, in the A
-// operand of mma.m16n8k16; the B columns are the pairs:
-//   scores   A = 16 tokens x 16 elements of K, B = the query, per 64-element
-//            group, each group's sum times the token's scale in fp32;
-//   values   A = 16 elements of V^T x 16 tokens, B = weight x value scale.
-// fp32 and fp16 queries and weights enter as two fp16 columns (PARTS = 2), hi
-// = fp16(x) and lo = fp16(x - hi): 22 to 24 bits, so that products keep fp32
-// accuracy; the query scaled by a power of two that puts its largest element
-// in [2^14, 2^15). bf16 queries are exact in one column, and their weights are
-// rounded to fp16's 11 bits (2^-12 relative, an eighth of the output's own
-// rounding).
+// Products, in the 8-bit integer MMA (m16n8k32), whose sums of a tile or a
+// 64-element group are exact. Codes are its A operand as they are, unsigned
+// bytes holding code or 16 x code, so that one or two logic operations widen
+// four of them; the 7 that a code stands above its level is taken off by the
+// value that an accumulator starts at. B columns are digits of base 256:
+//   scores   A = 16 tokens x 32 elements of K, B = the query's balanced digits.
+//            Its elements are integers after a power of two per 64-element
+//            group. Group sums times the token's scale add up in fp32.
+//   values   A = 16 elements of V^T x 32 tokens, B = the digits of weight x
+//            value scale, integers after a power of two per tile and group.
+//            Tile sums add up in fp32.
+// fp32 takes three digits: 2^-23 of the group's largest element, or of the
+// tile's largest weight x scale, is lost at most; fp16 and bf16 take two, 2^-15
+// of either, well below their outputs' rounding. A pair takes 4 (fp32, one of them
+// idle) or 2 columns of the 8. An accumulator starts at the bits of 1.5 x 2^23
+// (less the 7s): its bits read as a float are 1.5 x 2^23 plus the sum.
 //
-// Weights. p = 2^(x - m) against the pair's running maximum m; what enters the
-// product is p x scale / R x 2^14, with R at least the largest p x scale of
-// the pair so far (in units of 2^m). R follows the products themselves, not the
-// scales alone, because a token that takes all the weight may hold nothing,
-// as first tokens often do, and the rest then decides the result.
+// Measured against levels widened to fp16 pairs in m16n8k16 (two fp16 parts
+// per fp32 weight): 860 instructions per tile of 32 tokens at head dimension
+// 128, over half of the ALU's issue rate in widening.
 #include <atomic>
 #include <cmath>
 
@@ -34,9 +39,10 @@ namespace dz {
 constexpr int KA_WARPS = 8;
 constexpr int KA_TILE = 32;     // tokens of a tile
 constexpr int KA_STAGES = 3;
-constexpr float KA_TOP = 16384.0f;     // 2^14
 constexpr int KA_DEVICES = 64;  // devices whose launch state is kept
-constexpr float KA_RMIN = 1e-30f;
+constexpr int KA_CLUSTER = 16;            // blocks of a cluster at most
+constexpr int KA_ZERO = 0x4B400000;       // 1.5 x 2^23
+constexpr float KA_ZEROF = 12582912.0f;
 
 template <int HD> struct KaCfg {
     static constexpr int ROW = HD / 2;                 // code bytes of a row
@@ -58,10 +64,17 @@ template <int BYTES> __device__ __forceinline__ void ka_copy_small(uint32_t dst,
 __device__ __forceinline__ void ka_commit() { asm volatile("cp.async.commit_group;"); }
 template <int N> __device__ __forceinline__ void ka_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N)); }
 
-__device__ __forceinline__ void ka_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+// A unsigned; B signed (the query's digits) or unsigned (the weights').
+__device__ __forceinline__ void ka_mma_s(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ka_mma_u(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
@@ -71,52 +84,37 @@ __device__ __forceinline__ float ka_exp2(float x) {
     return y;
 }
 
-// Levels of the nibbles at bits 0 and 16 (low) or 4 and 20 (high) of w, as
-// fp16 pairs. 0x6400 is 1024, whose step is 1: or-ing a nibble in adds it (or
-// 16 x it), and the subtraction is exact.
-__device__ __forceinline__ uint32_t ka_low(uint32_t w) {
-    const uint32_t x = (w & 0x000F000Fu) | 0x64006400u;
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6407)));  // 1031
-    return *reinterpret_cast<const uint32_t*>(&y);
-}
-__device__ __forceinline__ uint32_t ka_high(uint32_t w) {
-    const uint32_t x = (w & 0x00F000F0u) | 0x64006400u;
-    const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x2C00)),   // 1/16
-                              __half2half2(__ushort_as_half(0xD470)));                                         // -71
-    return *reinterpret_cast<const uint32_t*>(&y);
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float ka_max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
 }
 
-__device__ __forceinline__ uint32_t ka_pack(float a, float b) {   // a in the low half
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 ka_unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
-
-// Column `part` of two values: hi, or what hi leaves.
-template <int PARTS> __device__ __forceinline__ uint32_t ka_column(float a, float b, bool low) {
-    const uint32_t hi = ka_pack(a, b);
-    if (PARTS == 1) return hi;
-    const float2 f = ka_unpack(hi);
-    const uint32_t lo = ka_pack(a - f.x, b - f.y);
-    return low ? lo : hi;
+// Byte d of four words (sel = d | (4 + d) << 4).
+__device__ __forceinline__ uint32_t ka_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t sel) {
+    return __byte_perm(__byte_perm(a, b, sel), __byte_perm(c, d, sel), 0x5410);
 }
 
-template <typename T, int HD, int PARTS, int NT>
-__global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 2 : 1) dz_kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a,
-                                                                                    int cluster, int pair_blocks) {
+template <typename T, int HD, int ND, int NT>
+__global__ void __launch_bounds__(KA_WARPS * 32, NT <= 2 ? 2 : 1) dz_kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a,
+                                                                                    int team, int cluster, int pair_blocks,
+                                                                                    int units) {
     using C = KaCfg<HD>;
-    constexpr int NP = 2 / PARTS;            // pairs of a lane in one n-tile
-    constexpr int PAIRS = NT * 8 / PARTS;    // pairs of a block
+    constexpr int CPP = ND == 3 ? 4 : 2;     // columns of a pair
+    constexpr int PPT = 8 / CPP;             // pairs of an n-tile; lane t has columns of pair 2 t / CPP
+    constexpr int PAIRS = NT * PPT;          // pairs of a block
     constexpr int GR = C::GROUPS;
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rank = blockIdx.x % cluster;
-    int unit = blockIdx.x / cluster;
+    const int rank = blockIdx.x % cluster, tw = warp % team;      // the warp's place in its team
+    int unit = blockIdx.x / cluster * (KA_WARPS / team) + warp / team;
+    if (unit >= units) return;               // whole teams of a single block
     const int pb = unit % pair_blocks;
     unit /= pair_blocks;
     const int hk = unit % a.c.kv_heads, b = unit / a.c.kv_heads;
     const long long first = a.positions[b];
-    if (first < 0) return;                   // the whole cluster leaves
+    if (first < 0) return;                   // the whole team, or cluster, leaves
     const int share = a.q_heads / a.c.kv_heads, pairs = share * a.n_tokens, pair0 = pb * PAIRS;
 
     // ---- the virtual index v = 0..count-1 runs over the sinks, then over positions lo, lo + 1, ...
@@ -149,105 +147,129 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 2 : 1) dz_kv4_attn_ke
     auto issue = [&](int tile, int stage) {
         const uint32_t s = my_s + stage * C::STAGE;
         const int v0 = tile * KA_TILE;
+        const int s0 = slot_of(v0);
+        // whole, neither across the sinks' end nor round the ring: one run of slots
+        const bool run = v0 + KA_TILE <= count && (v0 >= nsink || v0 + KA_TILE <= nsink) && s0 + KA_TILE <= cap;
+        const int r = lane / CH, c = lane % CH;
+        const uint32_t d = s + r * C::ROW + (HD == 128 ? (c ^ (r & 2)) : c) * 16;   // (r + 8 i) & 2 == r & 2
+        const uint32_t ds = s + 2 * C::CODES + lane * GR * 4;
+        if (run) {
+            const uint8_t* k = kc + (long long)s0 * C::ROW + lane * 16;
+            const uint8_t* v = vc + (long long)s0 * C::ROW + lane * 16;
+#pragma unroll
+            for (int i = 0; i < KA_TILE / RPI; i++) {
+                ka_copy16(d + i * 512, k + i * 512, true);
+                ka_copy16(d + C::CODES + i * 512, v + i * 512, true);
+            }
+            ka_copy_small<GR * 4>(ds, ksc + ((long long)s0 + lane) * GR, true);
+            ka_copy_small<GR * 4>(ds + C::SCALES, vsc + ((long long)s0 + lane) * GR, true);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < KA_TILE / RPI; i++) {
-            const int r = lane / CH + i * RPI, c = lane % CH;
-            const bool valid = v0 + r < count;
-            const long long off = (long long)(valid ? slot_of(v0 + r) : 0) * C::ROW + c * 16;
-            const uint32_t d = s + r * C::ROW + (HD == 128 ? (c ^ (r & 2)) : c) * 16;
-            ka_copy16(d, kc + off, valid);
-            ka_copy16(d + C::CODES, vc + off, valid);
+            const int v = v0 + r + i * RPI;
+            const long long off = (long long)(v < count ? slot_of(v) : 0) * C::ROW + c * 16;
+            ka_copy16(d + i * 512, kc + off, v < count);
+            ka_copy16(d + C::CODES + i * 512, vc + off, v < count);
         }
         const bool valid = v0 + lane < count;
         const long long off = (long long)(valid ? slot_of(v0 + lane) : 0) * GR;
-        ka_copy_small<GR * 4>(s + 2 * C::CODES + lane * GR * 4, ksc + off, valid);
-        ka_copy_small<GR * 4>(s + 2 * C::CODES + C::SCALES + lane * GR * 4, vsc + off, valid);
+        ka_copy_small<GR * 4>(ds, ksc + off, valid);
+        ka_copy_small<GR * 4>(ds + C::SCALES, vsc + off, valid);
     };
 
-    const int ntiles = (count + KA_TILE - 1) / KA_TILE, step = KA_WARPS * cluster;
-    const int tile0 = rank * KA_WARPS + warp;
+    const int ntiles = (count + KA_TILE - 1) / KA_TILE, step = team * cluster;
+    const int tile0 = rank * team + tw;
 #pragma unroll
     for (int i = 0; i < KA_STAGES - 1; i++) {
         if (tile0 + i * step < ntiles) issue(tile0 + i * step, i);
         ka_commit();
     }
 
-    // ---- query fragments: column g of n-tile n is part (g % PARTS) of pair
-    // pair0 + n * 8 / PARTS + g / PARTS; the lane's elements follow the order in
-    // which a code word's nibbles become A registers
-    uint32_t qf[NT][GR * 4][2];
-    float qfac[NT];                          // scale x log2 e / the pair's power of two, column layout (g)
+    // ---- query digits: column g of n-tile n is digit g % CPP of pair pair0 +
+    // n PPT + g / CPP; lane t has elements 16 t .. 16 t + 15 of each group, the
+    // even ones in B step 0, the odd ones in step 1, as the codes' nibbles fall
+    const uint32_t dsel = (uint32_t)(g % CPP) * 0x11u + 0x40u;          // digit d: d | (4 + d) << 4
+    uint32_t qd[NT][GR][2][2];
+    int zero[NT][GR][2];                     // where the accumulators of columns 2t, 2t + 1 start
+    float qw[NT][GR][2];                     // and what their sums count: 256^digit / the group's power / 16
+    bool qbad[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const int pair = pair0 + n * (8 / PARTS) + g / PARTS;
+        const int pair = pair0 + n * PPT + g / CPP;
         const bool live = pair < pairs;
         const T* q = static_cast<const T*>(a.q) +
                      ((long long)b * a.n_tokens + (live ? pair / share : 0)) * a.ldq +
-                     (long long)(hk * share + (live ? pair % share : 0)) * HD;
-        float x[GR * 16];
-        float top = 0.0f;
+                     (long long)(hk * share + (live ? pair % share : 0)) * HD + 16 * t;
         bool bad = false;
 #pragma unroll
-        for (int i = 0; i < GR * 16; i++) {
-            x[i] = live ? dz_to_float(q[(i / 16) * 64 + 16 * t + i % 16]) : 0.0f;
-            top = fmaxf(top, fabsf(x[i]));
-            bad |= !(fabsf(x[i]) <= 3.402823466e38f);
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        bad = __any_sync(0xfu << (lane & 28), bad);
-        // 2^(14 - e) for top in [2^e, 2^(e+1)), as a product of two powers so that neither over- nor underflows
-        int e = top > 0.0f && !bad ? ilogbf(top) : 0;
-        e = max(e, -140);
-        const int up = 14 - e, u0 = up / 2, u1 = up - u0;
-        const float f0 = __int_as_float((127 + u0) << 23), f1 = __int_as_float((127 + u1) << 23);
-        const float d0 = __int_as_float((127 - u0) << 23), d1 = __int_as_float((127 - u1) << 23);
-        qfac[n] = bad ? __int_as_float(0x7fc00000) : a.scale * 1.4426950408889634f * d0 * d1;
+        for (int gr = 0; gr < GR; gr++) {
+            float x[16], top = 0.0f;
 #pragma unroll
-        for (int w = 0; w < GR * 2; w++) {   // word w of the lane: elements 8 w .. 8 w + 7 of its x
-            float y[8];
+            for (int i = 0; i < 16; i++) {
+                x[i] = live ? dz_to_float(q[64 * gr + i]) : 0.0f;
+                top = fmaxf(top, fabsf(x[i]));
+                bad |= !(fabsf(x[i]) <= 3.402823466e38f);
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            constexpr int BITS = ND == 3 ? 22 : 14;
+            constexpr float LIMIT = ND == 3 ? 8355711.0f : 32639.0f;   // the top digit must stay below 128
+            int e = min(127 + BITS - (int)(__float_as_uint(top) >> 23), 126);
+            if (top * __int_as_float((127 + e) << 23) > LIMIT) e--;
+            const float f = __int_as_float((127 + e) << 23);
+            uint32_t y[16];
 #pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = x[8 * w + i] * f0 * f1;
+            for (int i = 0; i < 16; i++) y[i] = (uint32_t)(__float2int_rn(x[i] * f) + (ND == 3 ? 0x8080 : 0x80));
+            const uint32_t flip = g % CPP < ND - 1 ? 0x80808080u : 0u, keep = g % CPP < ND ? ~0u : 0u;
+            int sum = 0;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                qf[n][2 * w + h][0] = ka_column<PARTS>(y[2 * h], y[2 * h + 4], g & 1);
-                qf[n][2 * w + h][1] = ka_column<PARTS>(y[2 * h + 1], y[2 * h + 5], g & 1);
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t* z = y + 8 * j + h;
+                    qd[n][gr][h][j] = (ka_bytes(z[0], z[2], z[4], z[6], dsel) ^ flip) & keep;
+                    sum = __dp4a((int)qd[n][gr][h][j], 0x01010101, sum);
+                }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int start0 = KA_ZERO - 112 * sum;
+            const float digit = g % CPP == 0 ? 0.0625f : g % CPP == 1 ? 16.0f : g % CPP == 2 ? 4096.0f : 0.0f;
+            const float weight = digit * __int_as_float((127 - e) << 23);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                zero[n][gr][i] = __shfl_sync(0xffffffffu, start0, 8 * t + 4 * i);
+                qw[n][gr][i] = __shfl_sync(0xffffffffu, weight, 8 * t + 4 * i);
             }
         }
+        qbad[n] = __any_sync(0xfu << (lane & 28), bad);
     }
-    // ---- the same factor, and the visible range, of the lane's pairs in score layout (t)
-    float sfac[NT][NP];
-    int see_sink[NT][NP], see_hi[NT][NP], see_lo[NT][NP];
+    // ---- the score factor and the visible range of the lane's pairs
+    float sfac[NT];                          // scale x log2 e (NaN for a query that holds one)
+    int see_sink[NT], see_hi[NT], see_lo[NT];
     const bool masked = a.n_tokens > 1;
 #pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int i = 0; i < NP; i++) {
-            const int col = PARTS == 2 ? 2 * t : 2 * t + i;
-            sfac[n][i] = __shfl_sync(0xffffffffu, qfac[n], col * 4);
-            const int pair = min(pair0 + n * (8 / PARTS) + col / PARTS, pairs - 1);
-            const long long pos = first + pair / share;
-            see_sink[n][i] = (int)min(pos, (long long)INT32_MAX);
-            see_hi[n][i] = (int)max(-1LL, pos - lo);
-            see_lo[n][i] = a.window ? (int)max(-1LL, pos - a.window - lo) : -1;
-        }
+    for (int n = 0; n < NT; n++) {
+        const bool bad = __shfl_sync(0xffffffffu, qbad[n], 8 * t);
+        sfac[n] = bad ? __int_as_float(0x7fc00000) : a.scale * 1.4426950408889634f;
+        const int pair = min(pair0 + n * PPT + 2 * t / CPP, pairs - 1);
+        const long long pos = first + pair / share;
+        see_sink[n] = (int)min(pos, (long long)INT32_MAX);
+        see_hi[n] = (int)max(-1LL, pos - lo);
+        see_lo[n] = a.window ? (int)max(-1LL, pos - a.window - lo) : -1;
+    }
 
-    float m[NT][NP], l[NT][NP], R[NT], rinv[NT];
-    float acc[NT][GR * 4][4];
+    float m[NT], l[NT];
+    float acc[NT][GR * 4][2];                // elements 64 gr + 8 g + 2 k (and 16 x that of + 1), the lane's digits
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        R[n] = KA_RMIN;
-        rinv[n] = KA_TOP / KA_RMIN;
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NP; i++) {
-            m[n][i] = -INFINITY;
-            l[n][i] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < GR * 4; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) acc[n][i][r] = 0.0f;
+        for (int i = 0; i < GR * 4; i++) acc[n][i][0] = acc[n][i][1] = 0.0f;
     }
+    // the weights' digits as C columns 2t and 2t + 1 count them
+    const float wd0 = ND == 3 && (t & 1) ? 65536.0f : 1.0f, wd1 = ND == 3 && (t & 1) ? 0.0f : 256.0f;
 
     int stage = 0, next = KA_STAGES - 1;
     for (int tile = tile0; tile < ntiles; tile += step) {
@@ -260,244 +282,231 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 2 : 1) dz_kv4_attn_ke
         next = next + 1 == KA_STAGES ? 0 : next + 1;
         const float* ks = reinterpret_cast<const float*>(st + 2 * C::CODES);
         const float* vs = ks + KA_TILE * GR;
+        constexpr uint32_t HIGH = 0xF0F0F0F0u, LOW = 0x0F0F0F0Fu;
 
-        // scores: x[n][blk][row half][pair]
-        float x[NT][2][2][NP];
+        // scores of tokens g, g + 8, g + 16, g + 24
+        float x[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[n][r] = 0.0f;
 #pragma unroll
         for (int blk = 0; blk < 2; blk++) {
             const int r0 = blk * 16 + g, r1 = r0 + 8;
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int i = 0; i < NP; i++) x[n][blk][0][i] = x[n][blk][1][i] = 0.0f;
-#pragma unroll
             for (int gr = 0; gr < GR; gr++) {
                 // 8 bytes at 8 t of the group's 32: rows r0 and r1 (r1 & 2 == r0 & 2)
-                const int at = HD == 128 ? ((2 * gr + (t >> 1)) ^ (r0 & 2)) * 16 + 8 * (t & 1) : 8 * t;
+                const int at = HD == 128 ? ((2 * gr + (t >> 1)) ^ (g & 2)) * 16 + 8 * (t & 1) : 8 * t;
                 const uint2 w0 = *reinterpret_cast<const uint2*>(st + r0 * C::ROW + at);
                 const uint2 w1 = *reinterpret_cast<const uint2*>(st + r1 * C::ROW + at);
-                float s[NT][4];
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) s[n][r] = 0.0f;
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const uint32_t p = u ? w0.y : w0.x, q = u ? w1.y : w1.x;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t a0 = ka_low(p >> (8 * h)), a2 = ka_high(p >> (8 * h));
-                        const uint32_t a1 = ka_low(q >> (8 * h)), a3 = ka_high(q >> (8 * h));
-#pragma unroll
-                        for (int n = 0; n < NT; n++)
-                            ka_mma(s[n], a0, a1, a2, a3, qf[n][4 * gr + 2 * u + h][0], qf[n][4 * gr + 2 * u + h][1]);
-                    }
-                }
                 const float k0 = ks[r0 * GR + gr], k1 = ks[r1 * GR + gr];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    if (PARTS == 2) {
-                        x[n][blk][0][0] = fmaf(s[n][0] + s[n][1], k0, x[n][blk][0][0]);
-                        x[n][blk][1][0] = fmaf(s[n][2] + s[n][3], k1, x[n][blk][1][0]);
-                    } else {
-                        x[n][blk][0][0] = fmaf(s[n][0], k0, x[n][blk][0][0]);
-                        x[n][blk][0][NP - 1] = fmaf(s[n][1], k0, x[n][blk][0][NP - 1]);
-                        x[n][blk][1][0] = fmaf(s[n][2], k1, x[n][blk][1][0]);
-                        x[n][blk][1][NP - 1] = fmaf(s[n][3], k1, x[n][blk][1][NP - 1]);
-                    }
+                    int c[4] = {zero[n][gr][0], zero[n][gr][1], zero[n][gr][0], zero[n][gr][1]};
+                    ka_mma_s(c, (w0.x << 4) & HIGH, (w1.x << 4) & HIGH, (w0.y << 4) & HIGH, (w1.y << 4) & HIGH,
+                             qd[n][gr][0][0], qd[n][gr][0][1]);
+                    ka_mma_s(c, w0.x & HIGH, w1.x & HIGH, w0.y & HIGH, w1.y & HIGH, qd[n][gr][1][0], qd[n][gr][1][1]);
+                    const float u0 = qw[n][gr][0], u1 = qw[n][gr][1];
+                    const float s0 = fmaf(__int_as_float(c[1]) - KA_ZEROF, u1, (__int_as_float(c[0]) - KA_ZEROF) * u0);
+                    const float s1 = fmaf(__int_as_float(c[3]) - KA_ZEROF, u1, (__int_as_float(c[2]) - KA_ZEROF) * u0);
+                    x[n][2 * blk] = fmaf(s0, k0, x[n][2 * blk]);
+                    x[n][2 * blk + 1] = fmaf(s1, k1, x[n][2 * blk + 1]);
                 }
             }
         }
         const int v0 = tile * KA_TILE;
-        uint32_t bw[NT][2][GR][2];           // B columns of the weights
         const bool edge = masked || v0 + KA_TILE > count;
+        uint32_t bw[NT][GR][2];              // digits of weight x value scale
+        float back[NT][GR][2];               // what columns 2t, 2t + 1 count
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            float top[NP];
 #pragma unroll
-            for (int i = 0; i < NP; i++) {
-                top[i] = -INFINITY;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float& y = x[n][r >> 1][r & 1][i];
-                    y *= sfac[n][i];
-                    if (edge) {
-                        const int v = v0 + r * 8 + g, rel = v - nsink;
-                        const bool see = v < nsink ? v <= see_sink[n][i] : rel <= see_hi[n][i] && rel > see_lo[n][i];
-                        if (!see || v >= count) y = -INFINITY;
-                    }
-                    top[i] = fmaxf(top[i], y);
-                }
-                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 4));
-                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 8));
-                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
-            }
-            if (__any_sync(0xffffffffu, top[0] > m[n][0] || top[NP - 1] > m[n][NP - 1])) {
-                float c[NP];
-#pragma unroll
-                for (int i = 0; i < NP; i++) {
-                    const float mn = fmaxf(m[n][i], top[i]);
-                    c[i] = m[n][i] == -INFINITY ? 1.0f : ka_exp2(m[n][i] - mn);   // nothing was summed before
-                    l[n][i] *= c[i];
-                    m[n][i] = mn;
-                }
-                // R is in units of 2^m of its column's pair
-                const float c0 = __shfl_sync(0xffffffffu, c[0], g >> 1), c1 = __shfl_sync(0xffffffffu, c[NP - 1], g >> 1);
-                R[n] *= PARTS == 2 || !(g & 1) ? c0 : c1;
-                rinv[n] = KA_TOP / R[n];
-            }
-            // weights, and their move to B layout: tokens t + 4 i (i = 0..3) of
-            // each 16, column g
-            float pb_[2][4];
-#pragma unroll
-            for (int i = 0; i < NP; i++) {
-                const float ref = m[n][i] == -INFINITY ? 0.0f : m[n][i];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float& y = x[n][r >> 1][r & 1][i];
-                    y = ka_exp2(y - ref);
-                    l[n][i] += y;
+            for (int r = 0; r < 4; r++) {
+                if (ND == 3) x[n][r] += __shfl_xor_sync(0xffffffffu, x[n][r], 1);   // the pair's other digits
+                x[n][r] *= sfac[n];
+                if (edge) {
+                    const int v = v0 + r * 8 + g, rel = v - nsink;
+                    const bool see = v < nsink ? v <= see_sink[n] : rel <= see_hi[n] && rel > see_lo[n];
+                    if (!see || v >= count) x[n][r] = -INFINITY;
                 }
             }
-#pragma unroll
-            for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int src = (t + 4 * (i & 1)) * 4 + (g >> 1);
-                    const float y0 = __shfl_sync(0xffffffffu, x[n][blk][i >> 1][0], src);
-                    if (PARTS == 2) {
-                        pb_[blk][i] = y0;
-                    } else {
-                        const float y1 = __shfl_sync(0xffffffffu, x[n][blk][i >> 1][NP - 1], src);
-                        pb_[blk][i] = (g & 1) ? y1 : y0;
-                    }
-                }
-            // weight x value scale (a token of weight 0 may hold a NaN scale: masked for this pair)
-            float w[2][GR][4], wtop = 0.0f;
-#pragma unroll
-            for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int gr = 0; gr < GR; gr++) {
-                        const float s = vs[(blk * 16 + t + 4 * i) * GR + gr];
-                        w[blk][gr][i] = pb_[blk][i] != 0.0f ? pb_[blk][i] * s : 0.0f;
-                        wtop = fmaxf(wtop, w[blk][gr][i]);
-                    }
-            wtop = fmaxf(wtop, __shfl_xor_sync(0xffffffffu, wtop, 1));
-            wtop = fmaxf(wtop, __shfl_xor_sync(0xffffffffu, wtop, 2));
-            if (__any_sync(0xffffffffu, wtop > R[n] || R[n] < KA_RMIN)) {
-                const bool mine = wtop > R[n] || R[n] < KA_RMIN;
-                const float rn = mine ? fmaxf(2.0f * wtop, KA_RMIN) : R[n];
-                const float f = R[n] / rn;
-                R[n] = rn;
-                rinv[n] = KA_TOP / rn;
-                const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+            float top = fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            if (__any_sync(0xffffffffu, top > m[n])) {
+                const float mn = fmaxf(m[n], top);
+                const float c = m[n] == -INFINITY ? 0.0f : ka_exp2(m[n] - mn);   // nothing was summed before
+                l[n] *= c;
+                m[n] = mn;
 #pragma unroll
                 for (int i = 0; i < GR * 4; i++) {
-                    acc[n][i][0] *= f0;
-                    acc[n][i][1] *= f1;
-                    acc[n][i][2] *= f0;
-                    acc[n][i][3] *= f1;
+                    acc[n][i][0] *= c;
+                    acc[n][i][1] *= c;
                 }
             }
+            const float ref = m[n] == -INFINITY ? 0.0f : m[n];
 #pragma unroll
-            for (int blk = 0; blk < 2; blk++)
+            for (int r = 0; r < 4; r++) {
+                x[n][r] = ka_exp2(x[n][r] - ref);
+                l[n] += x[n][r];
+            }
+            // the weights in B layout: tokens t + 4 i, column g
+            float p[8];
 #pragma unroll
-                for (int gr = 0; gr < GR; gr++) {
-                    float* y = w[blk][gr];
-                    const uint32_t b0 = ka_column<PARTS>(y[0] * rinv[n], y[1] * rinv[n], g & 1);
-                    const uint32_t b1 = ka_column<PARTS>(y[2] * rinv[n], y[3] * rinv[n], g & 1);
-                    bw[n][blk][gr][0] = b0;
-                    bw[n][blk][gr][1] = b1;
+            for (int i = 0; i < 8; i++)
+                p[i] = __shfl_sync(0xffffffffu, x[n][i >> 1], (t + 4 * (i & 1)) * 4 + g / 2);
+#pragma unroll
+            for (int gr = 0; gr < GR; gr++) {
+                float w[8], wtop = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    float s = vs[(t + 4 * i) * GR + gr];
+                    if (masked && p[i] == 0.0f) s = 0.0f;    // a token that another query sees may hold a NaN scale
+                    w[i] = p[i] * s;
+                    wtop = ka_max_nan(wtop, w[i]);
                 }
+                wtop = ka_max_nan(wtop, __shfl_xor_sync(0xffffffffu, wtop, 1));
+                wtop = ka_max_nan(wtop, __shfl_xor_sync(0xffffffffu, wtop, 2));
+                // the power of two that puts the largest in [2^22, 2^23) (or [2^14, 2^15): it may round up to
+                // the next power, which has to fit the digits); 2^23 added, the float's low bytes are the
+                // integer. Below 2^-102 the weights fade out.
+                constexpr uint32_t TOP = ND == 3 ? 22 : 14;
+                const uint32_t e = max(__float_as_uint(wtop) & 0x7F800000u, 25u << 23);
+                const float f = __uint_as_float(((254u + TOP) << 23) - e);
+                uint32_t y[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] = __float_as_uint(fmaf(w[i], f, 8388608.0f));
+                bw[n][gr][0] = ka_bytes(y[0], y[1], y[2], y[3], dsel);
+                bw[n][gr][1] = ka_bytes(y[4], y[5], y[6], y[7], dsel);
+                // its inverse, NaN where a weight is not finite
+                const float inv = fmaf(wtop, 0.0f, __uint_as_float(e - (TOP << 23)));
+                back[n][gr][0] = __shfl_sync(0xffffffffu, inv, 8 * t) * wd0;
+                back[n][gr][1] = __shfl_sync(0xffffffffu, inv, 8 * t + 4) * wd1;
+            }
         }
         // values
 #pragma unroll
-        for (int blk = 0; blk < 2; blk++)
+        for (int gr = 0; gr < GR; gr++) {
+            int start[NT][4];
 #pragma unroll
-            for (int gr = 0; gr < GR; gr++) {
-                uint32_t wv[4];
+            for (int n = 0; n < NT; n++) {
+                int c[4] = {0, 0, 0, 0};     // the digits' sums over the tile
+                ka_mma_u(c, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, bw[n][gr][0], bw[n][gr][1]);
+                start[n][0] = KA_ZERO - 7 * c[0];
+                start[n][1] = KA_ZERO - 7 * c[1];
+                start[n][2] = KA_ZERO - 112 * c[0];
+                start[n][3] = KA_ZERO - 112 * c[1];
+            }
+            uint32_t w[8];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int r = blk * 16 + t + 4 * i;
-                    const int at = HD == 128 ? ((2 * gr + (g >> 2)) ^ (r & 2)) * 16 + 4 * (g & 3) : 4 * g;
-                    wv[i] = *reinterpret_cast<const uint32_t*>(st + C::CODES + r * C::ROW + at);
-                }
+            for (int i = 0; i < 8; i++) {
+                const int r = t + 4 * i;
+                const int at = HD == 128 ? ((2 * gr + (g >> 2)) ^ (t & 2)) * 16 + 4 * (g & 3) : 4 * g;
+                w[i] = *reinterpret_cast<const uint32_t*>(st + C::CODES + r * C::ROW + at);
+            }
 #pragma unroll
-                for (int byte = 0; byte < 4; byte++) {
-                    const uint32_t sel = (uint32_t)byte * 0x11u | (uint32_t)(4 + byte) * 0x1100u;
-                    const uint32_t r01 = __byte_perm(wv[0], wv[1], sel), r23 = __byte_perm(wv[2], wv[3], sel);
-                    const uint32_t a0 = ka_low(r01), a1 = ka_high(r01), a2 = ka_low(r23), a3 = ka_high(r23);
+            for (int byte = 0; byte < 4; byte++) {
+                // byte `byte` of four tokens: element 8 g + 2 byte in the low halves, the next one in the high halves
+                const uint32_t sel = (uint32_t)byte * 0x11u + 0x40u;
+                const uint32_t b0 = ka_bytes(w[0], w[1], w[2], w[3], sel), b1 = ka_bytes(w[4], w[5], w[6], w[7], sel);
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
-                        ka_mma(acc[n][gr * 4 + byte], a0, a1, a2, a3, bw[n][blk][gr][0], bw[n][blk][gr][1]);
+                for (int n = 0; n < NT; n++) {
+                    int c[4] = {start[n][0], start[n][1], start[n][2], start[n][3]};
+                    ka_mma_u(c, b0 & LOW, b0 & HIGH, b1 & LOW, b1 & HIGH, bw[n][gr][0], bw[n][gr][1]);
+                    float* o = acc[n][4 * gr + byte];
+                    o[0] = fmaf(__int_as_float(c[0]) - KA_ZEROF, back[n][gr][0], o[0]);
+                    o[0] = fmaf(__int_as_float(c[1]) - KA_ZEROF, back[n][gr][1], o[0]);
+                    o[1] = fmaf(__int_as_float(c[2]) - KA_ZEROF, back[n][gr][0], o[1]);
+                    o[1] = fmaf(__int_as_float(c[3]) - KA_ZEROF, back[n][gr][1], o[1]);
                 }
             }
+        }
     }
 
-    // ---- join: each warp's (m, l, sum) to shared memory, over the ring
+    // ---- the warp's sums in units of its 2^m: lane (g, t) has elements 64 gr + 8 g .. + 7 of pair 2 t / CPP
     ka_wait<0>();
-    __syncthreads();
-    float* so = reinterpret_cast<float*>(smem);                 // [warp][pair][HD]
-    float* sm = so + KA_WARPS * PAIRS * HD;                     // [warp][pair]
-    float* sl = sm + KA_WARPS * PAIRS;
-    float* co = sl + KA_WARPS * PAIRS;                          // the block's own [pair][HD], [pair], [pair]
-    float* cm = co + PAIRS * HD;
-    float* cl = cm + PAIRS;
+    __syncwarp();
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const float back = R[n] * (1.0f / KA_TOP);
-        const float e0 = __shfl_sync(0xffffffffu, back, 8 * t), e1 = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 4);
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 8);
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
 #pragma unroll
-        for (int i = 0; i < NP; i++) {
-            float s = l[n][i];
-            s += __shfl_xor_sync(0xffffffffu, s, 4);
-            s += __shfl_xor_sync(0xffffffffu, s, 8);
-            s += __shfl_xor_sync(0xffffffffu, s, 16);
-            const int pair = n * (8 / PARTS) + (PARTS == 2 ? t : 2 * t + i);
-            if (g == 0) {
-                sm[warp * PAIRS + pair] = m[n][i];
-                sl[warp * PAIRS + pair] = s;
+        for (int k = 0; k < GR * 4; k++) {
+            if (ND == 3) {
+                acc[n][k][0] += __shfl_xor_sync(0xffffffffu, acc[n][k][0], 1);
+                acc[n][k][1] += __shfl_xor_sync(0xffffffffu, acc[n][k][1], 1);
             }
-            float* o = so + (warp * PAIRS + pair) * HD;
-#pragma unroll
-            for (int k = 0; k < GR * 4; k++) {
-                const int d = (k >> 2) * 64 + 8 * g + 2 * (k & 3);
-                if (PARTS == 2) {
-                    o[d] = (acc[n][k][0] + acc[n][k][1]) * e0;
-                    o[d + 1] = (acc[n][k][2] + acc[n][k][3]) * e0;
-                } else {
-                    o[d] = acc[n][k][i] * (i ? e1 : e0);
-                    o[d + 1] = acc[n][k][2 + i] * (i ? e1 : e0);
-                }
-            }
+            acc[n][k][1] *= 0.0625f;
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < PAIRS * HD; i += KA_WARPS * 32) {
-        const int pair = i / HD;
-        float mx = -INFINITY;
+    auto store_out = [&](int p, int d, float v) {
+        static_cast<T*>(a.out)[((long long)b * a.n_tokens + p / share) * a.ldo +
+                               (long long)(hk * share + p % share) * HD + d] = dz_from_float<T>(v);
+    };
+    const bool speaks = ND == 2 || !(t & 1);   // of two lanes with the same sums
+    if (team * cluster == 1) {
 #pragma unroll
-        for (int w = 0; w < KA_WARPS; w++) mx = fmaxf(mx, sm[w * PAIRS + pair]);
+        for (int n = 0; n < NT; n++) {
+            const int p = pair0 + n * PPT + 2 * t / CPP;
+            if (p >= pairs || !speaks) continue;
+            T* o = static_cast<T*>(a.out) + ((long long)b * a.n_tokens + p / share) * a.ldo +
+                   (long long)(hk * share + p % share) * HD + 8 * g;
+            const float inv = 1.0f / l[n];
+#pragma unroll
+            for (int gr = 0; gr < GR; gr++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) o[64 * gr + k] = dz_from_float<T>(acc[n][4 * gr + k / 2][k % 2] * inv);
+        }
+        return;
+    }
+
+    // ---- join: each warp's sums, m and l over its ring; [pair][OS]
+    constexpr int OS = HD + 16;              // float4 stores of 2 g and 4 t meet a bank twice at most
+    constexpr int MINE = KA_STAGES * C::STAGE / 4;
+    static_assert(PAIRS * OS + 2 * PAIRS <= MINE, "a warp's part of the join lies over its ring");
+    float* so = reinterpret_cast<float*>(my);
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int pair = n * PPT + 2 * t / CPP;
+        if (!speaks) continue;
+#pragma unroll
+        for (int gr = 0; gr < GR; gr++)
+#pragma unroll
+            for (int k = 0; k < 4; k += 2)
+                *reinterpret_cast<float4*>(so + pair * OS + 64 * gr + 8 * g + 2 * k) =
+                    make_float4(acc[n][4 * gr + k][0], acc[n][4 * gr + k][1], acc[n][4 * gr + k + 1][0],
+                                acc[n][4 * gr + k + 1][1]);
+        if (g == 0) {
+            so[PAIRS * OS + pair] = m[n];
+            so[PAIRS * OS + PAIRS + pair] = l[n];
+        }
+    }
+    // the team's barrier (teams of one block have barriers of their own: their lengths differ)
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / team), "r"(team * 32) : "memory");
+    const float* t0 = reinterpret_cast<const float*>(smem) + (warp - tw) * MINE;
+    float* co = reinterpret_cast<float*>(smem + C::RING);       // a cluster's block: [pair][HD], [pair], [pair]
+    for (int i = tw * 32 + lane; i < PAIRS * HD; i += team * 32) {
+        const int pair = i / HD, d = i % HD, p = pair0 + pair;
+        if (p >= pairs) break;
+        float mx = -INFINITY;
+        for (int w = 0; w < team; w++) mx = fmaxf(mx, t0[w * MINE + PAIRS * OS + pair]);
         const float ref = mx == -INFINITY ? 0.0f : mx;
         float o = 0.0f, s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < KA_WARPS; w++) {
-            const float f = ka_exp2(sm[w * PAIRS + pair] - ref);
-            o = fmaf(so[w * PAIRS * HD + i], f, o);
-            s = fmaf(sl[w * PAIRS + pair], f, s);
+        for (int w = 0; w < team; w++) {
+            const float* q = t0 + w * MINE;
+            const float f = ka_exp2(q[PAIRS * OS + pair] - ref);
+            o = fmaf(q[pair * OS + d], f, o);
+            s = fmaf(q[PAIRS * OS + PAIRS + pair], f, s);
         }
-        const int p = pair0 + pair;
         if (cluster == 1) {
-            if (p < pairs)
-                static_cast<T*>(a.out)[((long long)b * a.n_tokens + p / share) * a.ldo +
-                                       (long long)(hk * share + p % share) * HD + i % HD] = dz_from_float<T>(o / s);
+            store_out(p, d, o / s);
         } else {
             co[i] = o;
-            if (i % HD == 0) {
-                cm[pair] = mx;
-                cl[pair] = s;
+            if (d == 0) {
+                co[PAIRS * HD + pair] = mx;
+                co[PAIRS * HD + PAIRS + pair] = s;
             }
         }
     }
@@ -523,86 +532,106 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT == 1 ? 2 : 1) dz_kv4_attn_ke
             o = fmaf(remote(c, i), f, o);
             s = fmaf(remote(c, PAIRS * HD + PAIRS + pair), f, s);
         }
-        static_cast<T*>(a.out)[((long long)b * a.n_tokens + p / share) * a.ldo +
-                               (long long)(hk * share + p % share) * HD + i % HD] = dz_from_float<T>(o / s);
+        store_out(p, i % HD, o / s);
     }
     // no block leaves while another may still read its shared memory
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-template <int HD, int PARTS, int NT> constexpr int ka_smem() {
-    constexpr int pairs = NT * 8 / PARTS;
-    constexpr int join = ((KA_WARPS + 1) * pairs * HD + 2 * (KA_WARPS + 1) * pairs) * 4;
-    return KaCfg<HD>::RING > join ? KaCfg<HD>::RING : join;
+template <int HD, int ND, int NT> constexpr int ka_smem() {
+    constexpr int pairs = NT * (ND == 3 ? 2 : 4);
+    return KaCfg<HD>::RING + (pairs * HD + 2 * pairs) * 4;
 }
 
-// Blocks of a cluster: one pass over the SMs' room with as many blocks as fit,
-// while each warp still has a tile or two of the longest context that the ring
-// allows.
-static int ka_cluster(long long units, long long longest, int sms, int per_sm) {
-    int best = 1;
-    double cost = 1e30;
-    for (int c = 1; c <= 8; c *= 2) {
-        if (c > 1 && longest < (long long)c * KA_WARPS * KA_TILE) break;
-        const double waves = (double)((units * c + (long long)sms * per_sm - 1) / ((long long)sms * per_sm));
-        const double t = waves / c + 0.02 * c;
-        if (t < cost) {
-            cost = t;
-            best = c;
+// Clusters of 1..16 blocks of a kernel that a device holds at once (a cluster
+// stays within one GPC, so that larger ones leave SMs idle).
+struct KaRoom {
+    std::atomic<bool> known{false};
+    std::atomic<int> clusters[KA_CLUSTER + 1];
+};
+
+// Warps of a team and blocks of a cluster for `units` units of up to `longest`
+// visible tokens: the least number of tiles that a warp works through one
+// after the other, its start (as long as 4 tiles) and the joins (3 each) among
+// them. 256 x 16 units of 640 tokens: 76 us with a warp each, 123 with eight;
+// 16 units of 130000: 564 us with eight, 118 with 64.
+static void ka_shape(const KaRoom& room, long long units, long long longest, int* team, int* cluster) {
+    const long long tiles = (longest + KA_TILE - 1) / KA_TILE;
+    double best = 1e30;
+    auto consider = [&](int w, int c) {
+        const long long warps = (long long)w * c, slots = (long long)room.clusters[c].load(std::memory_order_relaxed) * (KA_WARPS / w);
+        const double waves = (double)((units + slots - 1) / slots), each = (double)((tiles + warps - 1) / warps);
+        const double t = waves * (each + 4.0 + (warps > 1 ? 3.0 : 0.0) + (c > 1 ? 3.0 : 0.0));
+        if (t < best) {
+            best = t;
+            *team = w;
+            *cluster = c;
         }
-    }
-    return best;
+    };
+    for (int w = 1; w <= KA_WARPS; w *= 2) consider(w, 1);
+    for (int c = 2; c <= KA_CLUSTER && (long long)(c - 1) * KA_WARPS < tiles; c++) consider(KA_WARPS, c);
 }
 
-template <typename T, int HD, int PARTS, int NT>
-static cudaError_t ka_launch(const Kv4AttnArgs& a, int device, int sms, cudaStream_t st) {
-    auto* k = dz_kv4_attn_kernel<T, HD, PARTS, NT>;
-    constexpr int smem = ka_smem<HD, PARTS, NT>(), pairs_per_block = NT * 8 / PARTS;
-    static std::atomic<bool> ready[KA_DEVICES];
-    if (device >= KA_DEVICES || !ready[device].load(std::memory_order_relaxed)) {
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <typename T, int HD, int ND, int NT>
+static cudaError_t ka_launch(const Kv4AttnArgs& a, int device, cudaStream_t st) {
+    auto* k = dz_kv4_attn_kernel<T, HD, ND, NT>;
+    constexpr int smem = ka_smem<HD, ND, NT>(), pairs_per_block = NT * (ND == 3 ? 2 : 4);
+    static KaRoom rooms[KA_DEVICES];
+    if (device < 0 || device >= KA_DEVICES) return cudaErrorInvalidDevice;
+    KaRoom& room = rooms[device];
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(KA_WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    if (!room.known.load(std::memory_order_acquire)) {
+        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        for (int c = 1; c <= KA_CLUSTER && e == cudaSuccess; c++) {
+            cfg.gridDim = dim3(c);
+            cfg.numAttrs = 1;
+            attr[0].val.clusterDim.x = c;
+            int n = 0;
+            e = cudaOccupancyMaxActiveClusters(&n, k, &cfg);
+            room.clusters[c].store(n > 0 ? n : 1, std::memory_order_relaxed);
+        }
         if (e != cudaSuccess) return e;
-        if (device < KA_DEVICES) ready[device].store(true, std::memory_order_relaxed);
+        room.known.store(true, std::memory_order_release);
     }
     const int pairs = a.n_tokens * (a.q_heads / a.c.kv_heads);
     const int blocks = (pairs + pairs_per_block - 1) / pairs_per_block;
     const long long units = (long long)a.c.batch * a.c.kv_heads * blocks;
     const long long ring = a.c.capacity - a.c.sinks;
     const long long longest = a.c.sinks + (a.window && a.window < ring ? a.window + a.n_tokens : ring);
-    const int cluster = ka_cluster(units, longest, sms, NT == 1 ? 2 : 1);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * cluster));
-    cfg.blockDim = dim3(KA_WARPS * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
+    int team, cluster;
+    ka_shape(room, units, longest, &team, &cluster);
+    const long long grid = (units + KA_WARPS / team - 1) / (KA_WARPS / team) * cluster;
+    cfg.gridDim = dim3((unsigned)grid);
     attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k, a, cluster, blocks);
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, k, a, team, cluster, blocks, (int)units);
 }
 
-template <typename T, int PARTS>
-static cudaError_t ka_launch_t(const Kv4AttnArgs& a, int head_dim, int device, int sms, cudaStream_t st) {
-    const bool one = a.n_tokens * (a.q_heads / a.c.kv_heads) <= 8 / PARTS;
-    if (head_dim == 128)
-        return one ? ka_launch<T, 128, PARTS, 1>(a, device, sms, st) : ka_launch<T, 128, PARTS, 2>(a, device, sms, st);
-    return one ? ka_launch<T, 64, PARTS, 1>(a, device, sms, st) : ka_launch<T, 64, PARTS, 2>(a, device, sms, st);
+template <typename T, int HD, int ND>
+static cudaError_t ka_launch_n(const Kv4AttnArgs& a, int device, cudaStream_t st) {
+    const int tiles = (a.n_tokens * (a.q_heads / a.c.kv_heads) + (ND == 3 ? 1 : 3)) / (ND == 3 ? 2 : 4);
+    if (tiles == 1) return ka_launch<T, HD, ND, 1>(a, device, st);
+    if (tiles == 2) return ka_launch<T, HD, ND, 2>(a, device, st);
+    return ka_launch<T, HD, ND, 4>(a, device, st);
+}
+
+template <typename T, int ND>
+static cudaError_t ka_launch_t(const Kv4AttnArgs& a, int head_dim, int device, cudaStream_t st) {
+    return head_dim == 128 ? ka_launch_n<T, 128, ND>(a, device, st) : ka_launch_n<T, 64, ND>(a, device, st);
 }
 
 cudaError_t dz_kv4_attn_launch(const Kv4AttnArgs& a, int type, int head_dim, int device, cudaStream_t st) {
-    static std::atomic<int> sms[KA_DEVICES];   // SM count per device, looked up once
-    int n = device < KA_DEVICES ? sms[device].load(std::memory_order_relaxed) : 0;
-    if (!n) {
-        const cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
-        if (e != cudaSuccess) return e;
-        if (device < KA_DEVICES) sms[device].store(n, std::memory_order_relaxed);
-    }
-    if (type == DZ_TYPE_F32) return ka_launch_t<float, 2>(a, head_dim, device, n, st);
-    if (type == DZ_TYPE_F16) return ka_launch_t<__half, 2>(a, head_dim, device, n, st);
-    return ka_launch_t<__nv_bfloat16, 1>(a, head_dim, device, n, st);
+    if (type == DZ_TYPE_F32) return ka_launch_t<float, 3>(a, head_dim, device, st);
+    if (type == DZ_TYPE_F16) return ka_launch_t<__half, 2>(a, head_dim, device, st);
+    return ka_launch_t<__nv_bfloat16, 2>(a, head_dim, device, st);
 }
 
 }  // namespace dz

@@ -29,17 +29,24 @@ def dequant(scales, packed, rows, cols, group):
     return level * scales.astype(np.float64).repeat(group, 0)[:rows]
 
 
-def product(x, w):
-    """y and its bound: each activation is held to 2^-22 of the largest of its
-    128 consecutive ones, each of the K / 32 + 64 additions rounds once, and so
-    does the scale of a sum."""
+HELD = {"f32": 2.0 ** -22, "f16": 1 / 32639, "bf16": 1 / 32639}
+
+
+def product(x, w, kind="f32"):
+    """y and its bound. fp32 activations are held to 2^-22 of the largest of
+    their 128 consecutive ones, 16-bit ones to 1 / 32639: each is rounded to an
+    integer after a power of two that puts the largest in [2^22, 2^23) or
+    [2^14, 2^15), halved where that is above 8355711 or 32639 (the top digit
+    would not fit). The largest is then at least 4177855 or 16319.5, and half
+    a step is 1/2. Each of the K / 32 + 64 additions
+    rounds once, and so does the scale of a sum."""
     x = x.astype(np.float64)
     m, k = x.shape
     pad = -k % 128
     top = np.abs(np.pad(x, ((0, 0), (0, pad)))).reshape(m, -1, 128).max(-1)
     a = np.abs(w)
     block = np.pad(a, ((0, pad), (0, 0))).reshape(-1, 128, w.shape[1]).sum(1)
-    bound = 2.0 ** -22 * (top @ block) + (k / 32 + 64) * U * (np.abs(x) @ a)
+    bound = HELD[kind] * (top @ block) + (k / 32 + 64) * U * (np.abs(x) @ a)
     return x @ w, bound
 
 
@@ -107,19 +114,26 @@ def visible(pos, last, sinks, capacity, window):
     return list(range(min(sinks, pos + 1))) + list(range(oldest, pos + 1))
 
 
-def attend(q, k, v, scale, v_scales):
+def attend(q, k, v, scale, v_scales, kind="f32"):
     """One query head over its visible keys and values (64 bits), and the bound
-    of an fp32 evaluation: scores within (hd / 16 + 8) u of sum |q k|, the
-    exponential within 2^-21, n / 16 + 64 additions. Weights times value scales
-    enter the product in fp16 parts, scaled so that the largest lies in [2^13,
-    2^14] or is at most halved from there: below fp16's smallest normal number
-    the step is 2^-24, an error of 2^-25 in 2^13, so each token's weight is off
-    by at most 2^-38 of the largest, times a level of at most 7."""
+    of an evaluation with fp32 sums: scores within (hd / 16 + 8) u of sum |q k|,
+    the exponential within 2^-21, n / 16 + 64 additions. On top of that the
+    query's elements and the weights x value scales enter as integers:
+    - an element is off by half a step where the largest of its 64 is at least
+      4177855 steps (fp32) or 16319.5 (16 bits), HELD as in product();
+    - a weight by half a step where the largest of its tile of 32 tokens, all
+      within 31 places of it, is at least 2^22 (2^14) steps, times a level of
+      at most 7."""
     q, k, v = (t.astype(np.float64) for t in (q, k, v))
     s = scale * (k @ q)
     e = np.exp(s - s.max())
     p = e / e.sum()
     wide = (abs(scale) * (np.abs(k) @ np.abs(q))).max()
+    tops = np.abs(q).reshape(-1, GROUP).max(1)
+    held = (abs(scale) * HELD[kind] * (np.abs(k).reshape(len(k), -1, GROUP).sum(2) @ tops)).max()
     weight = p @ np.abs(v)
-    least = 7 * len(p) * 2.0 ** -38 * (p[:, None] * v_scales).max()
-    return p @ v, (2 * (q.size / 16 + 8) * U * wide + 2.0 ** -21 + (len(s) / 16 + 64) * U) * weight + least, weight
+    w = np.pad(p * v_scales.max(1), 31)
+    near = np.lib.stride_tricks.sliding_window_view(w, 63).max(1)
+    least = 7 * (2.0 ** -23 if kind == "f32" else 2.0 ** -15) * near.sum()
+    score = (q.size / 16 + 8) * U * wide + held
+    return p @ v, (2 * score + 2.0 ** -21 + (len(s) / 16 + 64) * U) * weight + least
