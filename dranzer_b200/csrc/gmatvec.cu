@@ -2,6 +2,7 @@
 // the C entry points, in a translation unit of their own.
 #include "dz_cuda.h"
 
+#include <atomic>
 #include <cmath>
 #include <new>
 
@@ -14,26 +15,27 @@ __device__ __forceinline__ int gmv_code(const uint8_t* packed, long long i) {
     return (packed[i >> 1] >> ((i & 1) * 4)) & 15;
 }
 
+// Where element (k, n) of a record lies: its word, the bit of its nibble.
+__device__ __forceinline__ int gmv_word(int kk, int c) {
+    return (kk >> 5) * 128 + ((c & 7) * 4 + ((kk >> 3) & 3)) * 4 + (c >> 3);
+}
+__device__ __forceinline__ int gmv_bit(int kk) { return (kk & 4) ? 8 * (kk & 3) : 8 * (kk & 3) + 4; }
+
 // One thread per word of the records' codes. `bad` is set for a code of 15.
 __global__ void dz_gmv_repack_kernel(const uint8_t* __restrict__ packed, GmvMatrix w, int* __restrict__ bad) {
     const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const long long total = (long long)w.ntiles * w.nblocks * (GMV_CODES / 4);
-    if (i >= total) return;
+    if (i >= (long long)w.ntiles * w.nblocks * (GMV_CODES / 4)) return;
     const int word = (int)(i % (GMV_CODES / 4));
     const long long r = i / (GMV_CODES / 4);
-    const int half = word >> 7, lane = (word >> 2) & 31, q = word & 3;
-    const int g = lane >> 2, t = lane & 3;
-    const int n = (int)(r / w.nblocks) * GMV_TILE + g + 8 * (q & 1);
-    const int k0 = (int)(r % w.nblocks) * GMV_BLOCK + 64 * half + 32 * (q >> 1) + 8 * t;
+    const int piece = word >> 7, lane = (word >> 2) & 31, q = word & 3;
+    const int n = (int)(r / w.nblocks) * GMV_TILE + (lane >> 2) + 8 * q;
+    const int k0 = (int)(r % w.nblocks) * GMV_BLOCK + 32 * piece + 8 * (lane & 3);
     uint32_t v = 0;
     if (n < w.N) {
-        for (int j = 0; j < 8; j++) {
-            const int k = k0 + j;
-            if (k >= w.K) break;
+        for (int k = k0; k < min(k0 + 8, w.K); k++) {
             const int c = gmv_code(packed, (long long)k * w.N + n);
             if (c > 14) *bad = 1;
-            const uint32_t level = (uint32_t)(c - 7) & 15u;
-            v |= level << (j < 4 ? 8 * j + 4 : 8 * (j - 4));
+            v |= ((uint32_t)(c - 7) & 15u) << gmv_bit(k);
         }
     }
     *reinterpret_cast<uint32_t*>(w.rec + r * w.rec_bytes + 4 * word) = v;
@@ -65,67 +67,516 @@ template <typename S> __global__ void dz_gmv_dequant_kernel(GmvMatrix w, float* 
     if (i >= (long long)w.K * w.N) return;
     const int k = (int)(i / w.N), n = (int)(i % w.N);
     const uint8_t* rec = w.rec + ((long long)(n / GMV_TILE) * w.nblocks + k / GMV_BLOCK) * w.rec_bytes;
-    const int kk = k % GMV_BLOCK, j = kk & 7, c = n % GMV_TILE;
-    const int word = (kk >> 6) * 128 + ((c & 7) * 4 + ((kk >> 3) & 3)) * 4 + 2 * ((kk >> 5) & 1) + (c >> 3);
-    const int byte = rec[4 * word + (j & 3)];
-    const int level = (int)((uint32_t)(j < 4 ? byte >> 4 : byte & 15) << 28) >> 28;
+    const int kk = k % GMV_BLOCK, c = n % GMV_TILE;
+    const uint32_t word = reinterpret_cast<const uint32_t*>(rec)[gmv_word(kk, c)];
+    const int level = (int)(word << (28 - gmv_bit(kk))) >> 28;
     dst[i] = dz_to_float(reinterpret_cast<const S*>(rec + GMV_CODES)[kk / w.group * GMV_TILE + c]) * (float)level;
 }
 
-// One block per (tile, row): thread (p, c) sums column c over the groups p,
-// p + 16, ... in fp32; the 16 parts add in order in shared memory.
-template <typename T, typename S> __global__ void __launch_bounds__(256) dz_gmv_simple_kernel(GmvArgs a) {
-    __shared__ float part[16][GMV_TILE];
-    const GmvMatrix& w = a.w;
-    const int c = threadIdx.x % GMV_TILE, p = threadIdx.x / GMV_TILE, m = blockIdx.y;
-    const T* x = static_cast<const T*>(a.x) + (long long)m * a.ldx;
-    float acc = 0.0f;
-    for (int k0 = p * w.group; k0 < w.K; k0 += 16 * w.group) {
-        const uint8_t* rec = w.rec + ((long long)blockIdx.x * w.nblocks + k0 / GMV_BLOCK) * w.rec_bytes;
-        float s = 0.0f;
-        for (int k = k0; k < min(k0 + w.group, w.K); k++) {
-            const int kk = k % GMV_BLOCK, j = kk & 7;
-            const int word = (kk >> 6) * 128 + ((c & 7) * 4 + ((kk >> 3) & 3)) * 4 + 2 * ((kk >> 5) & 1) + (c >> 3);
-            const int byte = rec[4 * word + (j & 3)];
-            const int level = (int)((uint32_t)(j < 4 ? byte >> 4 : byte & 15) << 28) >> 28;
-            const float v = dz_to_float(x[k]);   // v - v: NaN for an infinity
-            s = fmaf((float)level, v, s) + (v - v);
+// ------------------------------------------------------------------ product
+//
+// Integer formulation. Each 128 consecutive activations of a row (one block of
+// the layout) are scaled by a power of two, rounded to integers X and cut into
+// ND balanced base-256 digits (X = 65536 top + 256 mid + low for ND = 3).
+// Digits and levels meet in the 8-bit integer MMA, whose sums over one scale
+// group are exact (16 x 7 x 128 x 128 < 2^22); B column ND m + d is digit d of
+// row m. An accumulator starts at the bits of 1.5 x 2^23, whose step is 1, so
+// that its bits read as a float are 1.5 x 2^23 plus the sum: one subtraction
+// converts it. Group sums times scale and times the power of two add up in
+// fp32. fp32 activations take three digits, the largest of a block in [2^22,
+// 2^23): 2^-23 of it at most is lost. fp16 and bf16 ones take two, the largest
+// in [2^14, 2^15): 2^-15 of it, an eighth of fp16's own step at the largest
+// element and less than the output's rounding for any row that the type holds
+// well; two digits make a third fewer MMAs and digit bytes.
+//
+// Work. A cluster of 1 to 8 blocks takes a contiguous range of tiles; its
+// blocks take a share of the rows of W each (so that each converts only its
+// share of the activations), and a block's eight warps equal contiguous
+// ranges of its (tile, block) records, whatever tile borders lie inside. A
+// warp streams its records through its own ring of cp.async stages and meets
+// no barrier before the end: the warp that has a tile's first record keeps its
+// sum in the tile's place, a warp that continues a tile keeps it in its own.
+// Then the parts add up in a fixed order, over warps, then over the cluster.
+
+constexpr int GMV_DEVICES = 64;         // devices whose launch state is kept
+constexpr int GMV_SMEM = 227 * 1024 - 128;// shared memory a block may have
+constexpr int GMV_SMEM2 = 113 * 1024 - 128;// and if two are to fit an SM
+constexpr int GMV_WARPS = 8;
+constexpr int GMV_STAGES = 4;
+constexpr int GMV_MAX_ROWS = 16;        // rows of one pass
+constexpr int GMV_ZERO = 0x4B400000;    // 1.5 x 2^23
+
+struct GmvPlan {
+    int rows;         // rows of this launch
+    int cluster;      // blocks that share a tile
+    int clusters;     // clusters of the grid
+    int slice;        // records of a tile that a block has, at most
+    int tiles;        // tiles of a cluster, at most
+};
+
+__device__ __forceinline__ void gmv_mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+
+// E consecutive activations (16 bytes: 4 fp32 or 8 of 16 bits) from element k
+// of a row of K, zero past the end. wide: rows start on 16-byte boundaries.
+template <int E> __device__ __forceinline__ uint4 gmv_load(const void* x, long long row, int k, int K, bool wide) {
+    uint4 q;
+    if (E == 4) {
+        const uint32_t* p = static_cast<const uint32_t*>(x) + row + k;
+        if (wide && k + E <= K) return *reinterpret_cast<const uint4*>(p);
+        q.x = k < K ? p[0] : 0u;
+        q.y = k + 1 < K ? p[1] : 0u;
+        q.z = k + 2 < K ? p[2] : 0u;
+        q.w = k + 3 < K ? p[3] : 0u;
+        return q;
+    }
+    const uint16_t* p = static_cast<const uint16_t*>(x) + row + k;
+    if (wide && k + E <= K) return *reinterpret_cast<const uint4*>(p);
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) h[i] = k + i < K ? p[i] : 0u;
+    q.x = h[0] | h[1] << 16;
+    q.y = h[2] | h[3] << 16;
+    q.z = h[4] | h[5] << 16;
+    q.w = h[6] | h[7] << 16;
+    return q;
+}
+
+__device__ __forceinline__ void gmv_store(void* y, int type, long long at, float v) {
+    if (type == DZ_TYPE_F32) static_cast<float*>(y)[at] = v;
+    else if (type == DZ_TYPE_F16) static_cast<__half*>(y)[at] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
+}
+
+// Where share i of n things among `of` begins: shares differ by at most one.
+__device__ __forceinline__ int gmv_share(unsigned n, unsigned i, unsigned of) {
+    const unsigned q = n / of, r = n - q * of;
+    return (int)(q * i + r * i / of);
+}
+
+// Shared memory: the rings (over them, at a tile's end, nothing), the digit
+// columns, the digits' weights, a warp's tile in accumulator order, the parts.
+template <int ND, int NT> struct GmvSmem {
+    static constexpr int LD = 8 * NT + 1;                    // floats between the columns of W in a warp's tile
+    static constexpr int TILE = (GMV_TILE * LD + 3) / 4 * 4;
+    static __host__ __device__ int ring(int rec) { return GMV_WARPS * GMV_STAGES * rec; }
+    static __host__ __device__ int stride(int slice) { return slice * GMV_BLOCK + 32; }   // bytes between digit columns
+    static __host__ __device__ int digits(int rows, int slice) { return ND * rows * stride(slice); }
+    static __host__ __device__ int total(int rec, const GmvPlan& p) {
+        return ring(rec) + digits(p.rows, p.slice) + p.slice * 8 * NT * 4 + GMV_WARPS * TILE * 4 +
+               (p.tiles + GMV_WARPS) * GMV_TILE * p.rows * 4;
+    }
+};
+
+template <int GPB, typename S, int ND, int NT>   // scale groups of a block, scale type, digits, column tiles of 8
+__global__ void __launch_bounds__(GMV_WARPS * 32, NT < 3 || (NT == 3 && GPB < 4) ? 2 : 1) dz_gmv_kernel(const __grid_constant__ GmvArgs a,
+                                                                                const __grid_constant__ GmvPlan plan) {
+    using L = GmvSmem<ND, NT>;
+    constexpr int REC = GMV_CODES + GPB * GMV_TILE * (int)sizeof(S), CHUNKS = REC / 16;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int head_tile[GMV_WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int rank = blockIdx.x % plan.cluster, who = blockIdx.x / plan.cluster;
+    const int M = plan.rows, stride = L::stride(plan.slice);
+    uint8_t* digits = smem + L::ring(REC);
+    float* fx = reinterpret_cast<float*>(digits + L::digits(M, plan.slice));   // [record of the slice][8 NT]
+    float* mine = fx + plan.slice * 8 * NT + warp * L::TILE;
+    float* parts = fx + plan.slice * 8 * NT + GMV_WARPS * L::TILE;             // [tile][M][32]
+    float* heads = parts + plan.tiles * GMV_TILE * M;                          // [warp][M][32]
+
+    // (32-bit divisions only: a 64-bit one costs some hundred cycles before the first load)
+    const unsigned nblocks = a.w.nblocks;
+    const int kb0 = (int)(nblocks * rank / (unsigned)plan.cluster);
+    const int nb = (int)(nblocks * (rank + 1) / (unsigned)plan.cluster) - kb0;   // >= 1: cluster <= nblocks
+    const int tile0 = (int)(gmv_share(a.w.ntiles, who, plan.clusters));
+    const int nt = gmv_share(a.w.ntiles, who + 1, plan.clusters) - tile0;
+
+    // ---- this warp's records: numbers r0..r1-1 of the block's nt x nb, tile major
+    const unsigned all = (unsigned)nt * nb;
+    const int r0 = gmv_share(all, warp, GMV_WARPS), r1 = gmv_share(all, warp + 1, GMV_WARPS);
+    const long long tile_bytes = (long long)a.w.nblocks * REC, skip = tile_bytes - (long long)nb * REC;
+    int ti = r0 / nb, kb = r0 - ti * nb;                                       // the consumer's place
+    const uint8_t* src = a.w.rec + (tile0 + ti) * tile_bytes + (long long)(kb0 + kb) * REC + lane * 16;
+    int pk = kb, left = r1 - r0;                                               // the producer's
+    uint8_t* my = smem + warp * GMV_STAGES * REC;
+    const uint32_t my_s = (uint32_t)__cvta_generic_to_shared(my) + lane * 16;
+    int pstage = 0;
+    auto produce = [&] {
+        if (left > 0) {
+            left--;
+            const uint32_t dst = my_s + pstage * REC;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; c += 32)
+                if (c + 32 <= CHUNKS || lane < CHUNKS - c)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * 16), "l"(src + c * 16));
+            src += REC;
+            if (++pk == nb) {
+                pk = 0;
+                src += skip;
+            }
         }
-        acc = fmaf(s, dz_to_float(reinterpret_cast<const S*>(rec + GMV_CODES)[k0 % GMV_BLOCK / w.group * GMV_TILE + c]),
-                   acc);
+        asm volatile("cp.async.commit_group;");
+        pstage = pstage + 1 == GMV_STAGES ? 0 : pstage + 1;
+    };
+    produce();
+    // the weights are nobody's output; activations and y wait for the kernel before
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    // ---- activations to digits. A unit is one row's share of one block, 128
+    // elements: 16 bytes a lane, so a warp takes one (fp32) or two (16 bits) at
+    // a time; four such loads go out ahead of the rest of the ring (behind it
+    // they would wait for the weights) and four more while the last are worked on
+    {
+        constexpr int E = ND == 3 ? 4 : 8, UNITS = E / 4, AHEAD = 4;
+        const bool wide = (((uintptr_t)a.x | (uintptr_t)(a.ldx * (16 / E))) & 15) == 0;
+        const int le = UNITS == 1 ? lane : lane & 15;
+        int m = 0, kx = warp * UNITS + (UNITS == 1 ? 0 : lane >> 4);   // this lane's units: every 8 UNITS-th of M x nb
+        while (kx >= nb) { kx -= nb; m++; }
+        uint4 raw[2][AHEAD];
+        int um[2][AHEAD], uk[2][AHEAD];
+        auto fetch = [&](uint4 (&r)[AHEAD], int (&rm)[AHEAD], int (&rk)[AHEAD]) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                rm[u] = m;
+                rk[u] = kx;
+                r[u] = make_uint4(0, 0, 0, 0);
+                if (m < M) {
+                    r[u] = gmv_load<E>(a.x, (long long)m * a.ldx, (kb0 + kx) * GMV_BLOCK + E * le, a.w.K, wide);
+                    kx += GMV_WARPS * UNITS;
+                    while (kx >= nb) { kx -= nb; m++; }
+                }
+            }
+        };
+        auto work = [&](const uint4 (&r)[AHEAD], const int (&rm)[AHEAD], const int (&rk)[AHEAD]) {
+            unsigned top[AHEAD];             // bits of the largest magnitude: above 0x7f7fffff it is not finite
+            float v[AHEAD][E];
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                const uint32_t q[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
+                top[u] = 0;
+#pragma unroll
+                for (int j = 0; j < E; j++) {
+                    if (E == 4) v[u][j] = __uint_as_float(q[j]);
+                    else if (a.type == DZ_TYPE_F16) v[u][j] = __half2float(__ushort_as_half((unsigned short)(q[j / 2] >> 16 * (j & 1))));
+                    else v[u][j] = __uint_as_float(j & 1 ? q[j / 2] & 0xffff0000u : q[j / 2] << 16);
+                    top[u] = max(top[u], __float_as_uint(v[u][j]) & 0x7fffffffu);
+                }
+                top[u] = __reduce_max_sync(UNITS == 1 ? 0xffffffffu : lane < 16 ? 0xffffu : 0xffff0000u, top[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                // the power stays a normal float: a block below 2^-104 keeps fewer bits
+                constexpr int BITS = ND == 3 ? 22 : 14;
+                constexpr float LIMIT = ND == 3 ? 8355711.0f : 32639.0f;   // the top digit must stay below 128
+                int s = min(127 + BITS - (int)(top[u] >> 23), 126);
+                if (__uint_as_float(top[u]) * __int_as_float((127 + s) << 23) > LIMIT) s--;
+                const float f = __int_as_float((127 + s) << 23);
+                uint32_t y[E];   // X + 0x8080 (0x80): its bytes less 128 are the lower digits, its last byte the top one
+#pragma unroll
+                for (int j = 0; j < E; j++)
+                    y[j] = (uint32_t)(__float2int_rn(v[u][j] * f) + (ND == 3 ? 0x8080 : 0x80));
+                if (rm[u] >= M) continue;
+                uint8_t* to = digits + ND * rm[u] * stride + rk[u] * GMV_BLOCK + E * le;
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const uint32_t sel = (uint32_t)d | (uint32_t)(4 + d) << 4, flip = d < ND - 1 ? 0x80808080u : 0u;
+#pragma unroll
+                    for (int j = 0; j < E; j += 4)
+                        *reinterpret_cast<uint32_t*>(to + d * stride + j) =
+                            __byte_perm(__byte_perm(y[j], y[j + 1], sel), __byte_perm(y[j + 2], y[j + 3], sel), 0x5410) ^ flip;
+                }
+                if (le < ND) {   // the digit's weight, the levels' factor 16 taken back
+                    const float back = __int_as_float((127 - s) << 23) * (le == 0 ? 0.0625f : le == 1 ? 16.0f : 4096.0f);
+                    fx[rk[u] * 8 * NT + ND * rm[u] + le] = top[u] > 0x7f7fffffu ? __int_as_float(0x7fc00000) : back;
+                }
+            }
+        };
+        fetch(raw[0], um[0], uk[0]);
+#pragma unroll
+        for (int i = 0; i < GMV_STAGES - 2; i++) produce();
+        // both lane halves go round until neither has a unit left
+        while (__any_sync(0xffffffffu, um[0][0] < M)) {
+            fetch(raw[1], um[1], uk[1]);
+            work(raw[0], um[0], uk[0]);
+            if (!__any_sync(0xffffffffu, um[1][0] < M)) break;
+            fetch(raw[0], um[0], uk[0]);
+            work(raw[1], um[1], uk[1]);
+        }
     }
-    part[p][c] = acc;
     __syncthreads();
-    const int n = blockIdx.x * GMV_TILE + c;
-    if (p == 0 && n < w.N) {
+
+    // ---- records
+    const uint8_t* col[NT];   // this lane's digit columns (columns past ND M read the last one; nobody reads their sums)
+#pragma unroll
+    for (int n = 0; n < NT; n++) col[n] = digits + min(n * 8 + g, ND * M - 1) * stride + 8 * t;
+    float out[NT][8];         // columns g, g + 8 (0..3), g + 16, g + 24 (4..7) of W by columns 2t, 2t + 1 of B
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int r = 0; r < 8; r++) out[n][r] = 0.0f;
+    bool head = kb != 0 && r0 < r1;   // the first tile is another warp's to begin
+    if (lane == 0) head_tile[warp] = head ? ti : -1;
+    int cstage = 0;
+    for (int r = r0; r < r1; r++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(GMV_STAGES - 2));
+        __syncwarp();
+        produce();
+        const uint8_t* st = my + cstage * REC;
+        cstage = cstage + 1 == GMV_STAGES ? 0 : cstage + 1;
+        const S* scale = reinterpret_cast<const S*>(st + GMV_CODES) + g;
+        float part[NT][8];
+#pragma unroll
+        for (int gi = 0; gi < GPB; gi++) {
+            int acc[NT][2][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int q = 0; q < 8; q++) acc[n][q >> 2][q & 3] = GMV_ZERO;
+#pragma unroll
+            for (int k = gi * (4 / GPB); k < (gi + 1) * (4 / GPB); k++) {   // 32 rows each
+                const uint4 w = *reinterpret_cast<const uint4*>(st + k * 512 + lane * 16);
+                uint2 b[NT];
+#pragma unroll
+                for (int n = 0; n < NT; n++) b[n] = *reinterpret_cast<const uint2*>(col[n] + kb * GMV_BLOCK + k * 32);
+                constexpr uint32_t HIGH = 0xF0F0F0F0u;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    gmv_mma(acc[n][0], w.x & HIGH, w.y & HIGH, (w.x << 4) & HIGH, (w.y << 4) & HIGH, b[n]);
+                    gmv_mma(acc[n][1], w.z & HIGH, w.w & HIGH, (w.z << 4) & HIGH, (w.w << 4) & HIGH, b[n]);
+                }
+            }
+            float s[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) s[q] = dz_to_float(scale[gi * GMV_TILE + 8 * q]);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    const float v = __int_as_float(acc[n][q >> 2][q & 3]) - 12582912.0f;
+                    part[n][q] = gi ? fmaf(v, s[q >> 1], part[n][q]) : v * s[q >> 1];
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const float2 f = *reinterpret_cast<const float2*>(fx + kb * 8 * NT + 8 * n + 2 * t);
+#pragma unroll
+            for (int q = 0; q < 8; q++) out[n][q] = fmaf(part[n][q], q & 1 ? f.y : f.x, out[n][q]);
+        }
+        if (++kb < nb && r + 1 < r1) continue;
+        // the tile ends, or the warp's range does: add the digits, keep the part
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                mine[(g + 8 * (q >> 1)) * L::LD + 8 * n + 2 * t + (q & 1)] = out[n][q];
+                out[n][q] = 0.0f;
+            }
+        __syncwarp();
+        float* to = head ? heads + warp * GMV_TILE * M : parts + ti * GMV_TILE * M;
+#pragma unroll 4
+        for (int m = 0; m < M; m++) {
+            const float* p = mine + lane * L::LD + ND * m;
+            to[m * GMV_TILE + lane] = ND == 3 ? p[0] + p[1] + p[2] : p[0] + p[1];
+        }
+        __syncwarp();
+        head = false;
+        kb = 0;
+        ti++;
+    }
+    asm volatile("cp.async.wait_group 0;");
+    __syncthreads();
+
+    // ---- the block's parts in one place: warps that continue a tile, in order
+    for (int o = threadIdx.x; o < GMV_TILE * M; o += GMV_WARPS * 32)
+#pragma unroll
+        for (int w = 1; w < GMV_WARPS; w++)
+            if (head_tile[w] >= 0) parts[head_tile[w] * GMV_TILE * M + o] += heads[w * GMV_TILE * M + o];
+    if (plan.cluster == 1) {
+        __syncthreads();
+    } else {
+        asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+    }
+    const uint32_t parts_s = (uint32_t)__cvta_generic_to_shared(parts);
+    for (int i = rank * GMV_WARPS * 32 + threadIdx.x; i < nt * GMV_TILE * M; i += plan.cluster * GMV_WARPS * 32) {
+        const int tile = i / (GMV_TILE * M), m = i / GMV_TILE % M, n = (tile0 + tile) * GMV_TILE + i % GMV_TILE;
         float s = 0.0f;
-        for (int i = 0; i < 16; i++) s += part[i][c];
-        static_cast<T*>(a.y)[(long long)m * a.ldy + n] = dz_from_float<T>(s);
+        if (plan.cluster == 1) {
+            s = parts[i];
+        } else {
+            for (int c = 0; c < plan.cluster; c++) {
+                uint32_t at;
+                float v;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(parts_s + 4 * i), "r"(c));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+                s += v;
+            }
+        }
+        if (n < a.w.N) gmv_store(a.y, a.type, (long long)m * a.ldy + n, s);
+    }
+    // no block leaves while another may still read its shared memory
+    if (plan.cluster > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+template <int GPB, typename S, int ND, int NT>
+static cudaError_t gmv_launch_t(const GmvArgs& a, const GmvPlan& plan, int device, cudaStream_t st) {
+    auto* k = dz_gmv_kernel<GPB, S, ND, NT>;
+    static std::atomic<bool> ready[GMV_DEVICES];
+    if (device >= GMV_DEVICES || !ready[device].load(std::memory_order_relaxed)) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, GMV_SMEM);
+        if (e != cudaSuccess) return e;
+        if (device < GMV_DEVICES) ready[device].store(true, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(plan.clusters * plan.cluster));
+    cfg.blockDim = dim3(GMV_WARPS * 32);
+    cfg.dynamicSmemBytes = (size_t)GmvSmem<ND, NT>::total(a.w.rec_bytes, plan);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = plan.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = plan.cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, k, a, plan);
+}
+
+// Column tiles of 8 for `rows` rows: the instantiations below.
+static int gmv_col_tiles(int nd, int rows) {
+    const int n = (nd * rows + 7) / 8;
+    return n <= 3 ? n : nd == 3 ? 6 : 4;
+}
+
+template <int GPB, typename S>
+static cudaError_t gmv_launch_n(const GmvArgs& a, const GmvPlan& plan, int device, cudaStream_t st) {
+    if (a.type == DZ_TYPE_F32) {
+        switch (gmv_col_tiles(3, plan.rows)) {
+        case 1: return gmv_launch_t<GPB, S, 3, 1>(a, plan, device, st);
+        case 2: return gmv_launch_t<GPB, S, 3, 2>(a, plan, device, st);
+        case 3: return gmv_launch_t<GPB, S, 3, 3>(a, plan, device, st);
+        default: return gmv_launch_t<GPB, S, 3, 6>(a, plan, device, st);
+        }
+    }
+    switch (gmv_col_tiles(2, plan.rows)) {
+    case 1: return gmv_launch_t<GPB, S, 2, 1>(a, plan, device, st);
+    case 2: return gmv_launch_t<GPB, S, 2, 2>(a, plan, device, st);
+    case 3: return gmv_launch_t<GPB, S, 2, 3>(a, plan, device, st);
+    default: return gmv_launch_t<GPB, S, 2, 4>(a, plan, device, st);
     }
 }
 
-template <typename T> static void gmv_launch_t(const GmvArgs& a, dim3 grid, cudaStream_t st) {
-    if (a.w.scale_f16)
-        dz_gmv_simple_kernel<T, __half><<<grid, 256, 0, st>>>(a);
-    else
-        dz_gmv_simple_kernel<T, float><<<grid, 256, 0, st>>>(a);
+static int gmv_smem(const GmvArgs& a, const GmvPlan& p) {
+    const int nd = a.type == DZ_TYPE_F32 ? 3 : 2, nt = gmv_col_tiles(nd, p.rows), rec = a.w.rec_bytes;
+    if (nd == 3)
+        return nt == 1   ? GmvSmem<3, 1>::total(rec, p)
+               : nt == 2 ? GmvSmem<3, 2>::total(rec, p)
+               : nt == 3 ? GmvSmem<3, 3>::total(rec, p)
+                         : GmvSmem<3, 6>::total(rec, p);
+    return nt == 1   ? GmvSmem<2, 1>::total(rec, p)
+           : nt == 2 ? GmvSmem<2, 2>::total(rec, p)
+           : nt == 3 ? GmvSmem<2, 3>::total(rec, p)
+                     : GmvSmem<2, 4>::total(rec, p);
 }
 
-cudaError_t dz_gmv_launch(const GmvArgs& a, int, cudaStream_t st) {
+// Clusters of 1, 2, 4 and 8 blocks that `device` holds at once with one block
+// on an SM, then with two (a cluster stays within one GPC, so that larger ones
+// leave SMs idle). Asked once per device.
+struct GmvRoom {
+    std::atomic<bool> known{false};
+    std::atomic<int> clusters[2][4];
+};
+
+static cudaError_t gmv_room(int device, const GmvRoom** out) {
+    static GmvRoom rooms[GMV_DEVICES];
+    if (device < 0 || device >= GMV_DEVICES) return cudaErrorInvalidDevice;
+    GmvRoom& r = rooms[device];
+    if (!r.known.load(std::memory_order_acquire)) {
+        auto* k = dz_gmv_kernel<1, float, 3, 1>;
+        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, GMV_SMEM);
+        for (int two = 0; two < 2 && e == cudaSuccess; two++)
+            for (int c = 0; c < 4 && e == cudaSuccess; c++) {
+                cudaLaunchConfig_t cfg = {};
+                cfg.gridDim = dim3(8);
+                cfg.blockDim = dim3(GMV_WARPS * 32);
+                cfg.dynamicSmemBytes = two ? GMV_SMEM2 : GMV_SMEM;
+                cudaLaunchAttribute attr[1];
+                attr[0].id = cudaLaunchAttributeClusterDimension;
+                attr[0].val.clusterDim.x = 1u << c;
+                attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+                cfg.attrs = attr;
+                cfg.numAttrs = 1;
+                int n = 0;
+                e = cudaOccupancyMaxActiveClusters(&n, k, &cfg);
+                r.clusters[two][c].store(n > 0 ? n : 1, std::memory_order_relaxed);
+            }
+        if (e != cudaSuccess) return e;
+        r.known.store(true, std::memory_order_release);
+    }
+    *out = &r;
+    return cudaSuccess;
+}
+
+// How many rows a pass takes and how a tile is shared: the shape with the
+// least estimated time. False: not even one row fits. The estimate, in us on
+// one B200 (K 2048..12032, N 48..32000, 1..16 rows): four loads of activations
+// per warp take 1.9; a record 0.38 when two blocks per SM stream from HBM and
+// 0.15 + 0.15 NT + 0.02 NT GPB by its own latency; joining a cluster 0.7 and
+// 0.1 per block. 16 x 4099 x 5003: 36 us with one block to a tile, 22 with two.
+static bool gmv_plan(const GmvArgs& a, int rows, const GmvRoom& room, GmvPlan* plan) {
+    const int nd = a.type == DZ_TYPE_F32 ? 3 : 2, gpb = GMV_BLOCK / a.w.group;
+    for (rows = rows < GMV_MAX_ROWS ? rows : GMV_MAX_ROWS; rows >= 1; rows /= 2) {
+        double cost = 1e30;
+        const int nt = gmv_col_tiles(nd, rows);
+        for (int i = 0; i < 4 && (1 << i) <= a.w.nblocks; i++)
+            for (int two = 0; two < 2; two++) {
+                GmvPlan p;
+                const int c = 1 << i, fits = room.clusters[two][i].load(std::memory_order_relaxed);
+                p.rows = rows;
+                p.cluster = c;
+                p.slice = (a.w.nblocks + c - 1) / c;
+                p.clusters = fits < a.w.ntiles ? fits : a.w.ntiles;
+                p.tiles = (a.w.ntiles + p.clusters - 1) / p.clusters;
+                if (gmv_smem(a, p) > (two ? GMV_SMEM2 : GMV_SMEM)) continue;
+                const int per_batch = GMV_WARPS * 4 * (nd == 3 ? 1 : 2);
+                const double stream = 0.38 * (two + 1), own = (0.15 + 0.15 * nt + 0.02 * nt * gpb) * (two ? 1.6 : 1.0);
+                const double t = 1.9 * ((rows * p.slice + per_batch - 1) / per_batch) * (two ? 1.6 : 1.0) +
+                                 (stream > own ? stream : own) * ((p.tiles * p.slice + GMV_WARPS - 1) / GMV_WARPS) +
+                                 (c > 1 ? 0.7 + 0.1 * c : 0.0);
+                if (t < cost) {
+                    cost = t;
+                    *plan = p;
+                }
+            }
+        if (cost < 1e30) return true;
+    }
+    return false;
+}
+
+cudaError_t dz_gmv_launch(const GmvArgs& a, int device, cudaStream_t st) {
+    const GmvRoom* room;
+    const cudaError_t err = gmv_room(device, &room);
+    if (err != cudaSuccess) return err;
     GmvArgs b = a;
-    for (int m = 0; m < a.M; m += 65535) {
-        b.M = a.M - m < 65535 ? a.M - m : 65535;
+    GmvPlan plan;
+    for (int m = 0; m < a.M; m += plan.rows) {
+        if (!gmv_plan(a, a.M - m, *room, &plan)) return cudaErrorNotSupported;
         b.x = static_cast<const uint8_t*>(a.x) + (long long)m * a.ldx * type_bytes(a.type);
         b.y = static_cast<uint8_t*>(a.y) + (long long)m * a.ldy * type_bytes(a.type);
-        const dim3 grid((unsigned)a.w.ntiles, (unsigned)b.M);
-        if (a.type == DZ_TYPE_F32)
-            gmv_launch_t<float>(b, grid, st);
-        else if (a.type == DZ_TYPE_F16)
-            gmv_launch_t<__half>(b, grid, st);
+        cudaError_t e;
+        if (a.w.group == 128)
+            e = a.w.scale_f16 ? gmv_launch_n<1, __half>(b, plan, device, st) : gmv_launch_n<1, float>(b, plan, device, st);
+        else if (a.w.group == 64)
+            e = a.w.scale_f16 ? gmv_launch_n<2, __half>(b, plan, device, st) : gmv_launch_n<2, float>(b, plan, device, st);
         else
-            gmv_launch_t<__nv_bfloat16>(b, grid, st);
+            e = a.w.scale_f16 ? gmv_launch_n<4, __half>(b, plan, device, st) : gmv_launch_n<4, float>(b, plan, device, st);
+        if (e != cudaSuccess) return e;
     }
-    return cudaGetLastError();
+    return cudaSuccess;
 }
 
 }  // namespace dz
@@ -205,6 +656,13 @@ extern "C" int dz_cuda_gmatrix_create(int device, const dz_grouped_blob_t* w, dz
     m.ntiles = (m.N + GMV_TILE - 1) / GMV_TILE;
     m.nblocks = (m.K + GMV_BLOCK - 1) / GMV_BLOCK;
     m.rec_bytes = GMV_CODES + GMV_BLOCK / m.group * GMV_TILE * (m.scale_f16 ? 2 : 4);
+    GmvArgs one = {};
+    GmvPlan plan;
+    one.w = m;
+    const GmvRoom* room;
+    DZ_CUDA(gmv_room(device, &room));
+    if (!gmv_plan(one, 1, *room, &plan))
+        return fail(DZ_E_UNSUPPORTED, "gmatrix: %zu x %zu is too large for a product's shared memory", w->rows, w->cols);
     if ((long long)m.ntiles * m.nblocks > (1LL << 30)) return fail(DZ_E_UNSUPPORTED, "gmatrix: too many weights");
     auto* q = new (std::nothrow) dz_cuda_gmatrix;
     if (!q) return fail(DZ_E_NOMEM, "host allocation");
