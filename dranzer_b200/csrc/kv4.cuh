@@ -48,7 +48,7 @@ struct Kv4AttnArgs {
     long long window;
 };
 
-cudaError_t dz_kv4_append_launch(const Kv4AppendArgs& a, int type, int head_dim, cudaStream_t st);
+cudaError_t dz_kv4_append_launch(const Kv4AppendArgs& a, int type, int head_dim, int device, cudaStream_t st);
 cudaError_t dz_kv4_attn_launch(const Kv4AttnArgs& a, int type, int head_dim, int device, cudaStream_t st);
 
 }  // namespace dz
