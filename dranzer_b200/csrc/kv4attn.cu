@@ -259,6 +259,10 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT <= 2 ? 2 : 1) dz_kv4_attn_ke
         see_lo[n] = a.window ? (int)max(-1LL, pos - a.window - lo) : -1;
     }
 
+    // tiles of later positions that every pair of the block sees: rel in (all_lo, all_hi]
+    const int all_hi = (int)max(-1LL, first + j_lo - lo);
+    const int all_lo = a.window ? (int)max(-1LL, first + j_hi - a.window - lo) : -1;
+
     float m[NT], l[NT];
     float acc[NT][GR * 4][2];                // elements 64 gr + 8 g + 2 k (and 16 x that of + 1), the lane's digits
 #pragma unroll
@@ -315,7 +319,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT <= 2 ? 2 : 1) dz_kv4_attn_ke
             }
         }
         const int v0 = tile * KA_TILE;
-        const bool edge = masked || v0 + KA_TILE > count;
+        const int rel0 = v0 - nsink;
+        const bool edge = v0 + KA_TILE > count ||
+                          (masked && !(rel0 > all_lo && v0 >= nsink && rel0 + KA_TILE - 1 <= all_hi));
         uint32_t bw[NT][GR][2];              // digits of weight x value scale
         float back[NT][GR][2];               // what columns 2t, 2t + 1 count
 #pragma unroll
@@ -362,7 +368,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, NT <= 2 ? 2 : 1) dz_kv4_attn_ke
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     float s = vs[(t + 4 * i) * GR + gr];
-                    if (masked && p[i] == 0.0f) s = 0.0f;    // a token that another query sees may hold a NaN scale
+                    if (masked && edge && p[i] == 0.0f) s = 0.0f;   // another query's token may hold a NaN scale
                     w[i] = p[i] * s;
                     wtop = ka_max_nan(wtop, w[i]);
                 }
