@@ -530,15 +530,24 @@ class Model:
 
 
 class KVCache:
-    """`batch` independent ring KV caches of `capacity` tokens (dz_cuda_cache_create)."""
+    """`batch` independent ring KV caches of `capacity` tokens (dz_cuda_cache_create).
+    kv_bits=4 keeps keys and values in 4 bits, with the first `sinks` tokens
+    kept and a sliding `window` (0: what the ring holds;
+    dz_cuda_cache_create_kv4)."""
 
-    def __init__(self, model, batch, capacity=None):
+    def __init__(self, model, batch, capacity=None, kv_bits=32, sinks=0, window=0):
         self.model = model
         self.batch = batch
         self.capacity = capacity or model.desc.max_seq_len
         self.vocab = model.desc.vocab_size
         h = ctypes.c_void_p()
-        check(lib().dz_cuda_cache_create(model.handle, batch, self.capacity, ctypes.byref(h)), "cache_create")
+        if kv_bits not in (4, 32) or (kv_bits == 32 and (sinks or window)):
+            raise ValueError("kv_bits is 4 or 32; sinks and a window need 4")
+        if kv_bits == 4:
+            check(lib().dz_cuda_cache_create_kv4(model.handle, batch, self.capacity, sinks, window, ctypes.byref(h)),
+                  "cache_create_kv4")
+        else:
+            check(lib().dz_cuda_cache_create(model.handle, batch, self.capacity, ctypes.byref(h)), "cache_create")
         self.handle = h.value
 
     PATH_AUTO, PATH_LAYERED, PATH_FUSED = 0, 1, 2

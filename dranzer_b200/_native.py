@@ -153,6 +153,7 @@ SIGNATURES = {
     "dz_cuda_model_free": (None, [P]),
     "dz_cuda_model_step_bytes": (SZ, [P]),
     "dz_cuda_cache_create": (I32, [P, SZ, SZ, P]),
+    "dz_cuda_cache_create_kv4": (I32, [P, SZ, SZ, SZ, SZ, P]),
     "dz_cuda_cache_free": (None, [P]),
     "dz_cuda_cache_set_stream": (I32, [P, P]),
     "dz_cuda_cache_stream": (P, [P]),

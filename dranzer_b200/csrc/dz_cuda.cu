@@ -33,6 +33,7 @@
 #include "attn.cuh"
 #include "pfattn.cuh"
 #include "normlimbs.cuh"
+#include "kv4.cuh"
 
 using namespace dz;
 
@@ -1553,6 +1554,15 @@ struct dz_cuda_cache {
     cudaStream_t stream = nullptr;
     bool own_stream = false;
     float *keys = nullptr, *values = nullptr;  // [L][B][cap][D]
+    // 4-bit caches instead (dz_cuda_cache_create_kv4): per layer the buffers of
+    // a dz_kv4_t, and the rows that a step's (or a prefill's) products write
+    bool kv4 = false;
+    int sinks = 0, window = 0;
+    uint8_t* kv4_codes = nullptr;              // [L][keys, values][B][Hl][cap][hd / 2]
+    float* kv4_scales = nullptr;               // [L][keys, values][B][Hl][cap][hd / 64]
+    float *k_rows = nullptr, *v_rows = nullptr;   // [B][dl]
+    float *pf_k = nullptr, *pf_v = nullptr;       // [pf_rows][dl]
+    long long* origin = nullptr;               // [B] zeros: a prefill's positions
     // the K / V rings as [L * B * cap][D] fp32 tensors, box {head dim, 32}
     // (the streamed decode attention); kv_maps false: not available
     CUtensorMap tm_keys, tm_values;
@@ -1609,8 +1619,10 @@ struct dz_cuda_cache {
 static void free_prefill(dz_cuda_cache_t* c) {
     for (void* p : {(void*)c->pf_hidden, (void*)c->pf_q, (void*)c->pf_concat, (void*)c->pf_attn_raw,
                     (void*)c->pf_attn_norm, (void*)c->pf_ff, (void*)c->pf_ff_raw, (void*)c->pf_rowoff,
-                    c->pf_scratch, (void*)c->pf_ids, (void*)c->pf_lens, (void*)c->mk_buf})
+                    c->pf_scratch, (void*)c->pf_ids, (void*)c->pf_lens, (void*)c->mk_buf, (void*)c->pf_k,
+                    (void*)c->pf_v})
         cudaFree(p);
+    c->pf_k = c->pf_v = nullptr;
     c->mk_buf = nullptr;
     c->mk_cap = 0;
     c->pf_hidden = c->pf_q = c->pf_concat = c->pf_attn_raw = c->pf_attn_norm = c->pf_ff = c->pf_ff_raw = nullptr;
@@ -1658,7 +1670,8 @@ extern "C" void dz_cuda_cache_free(dz_cuda_cache_t* c) {
     delete c;
 }
 
-extern "C" int dz_cuda_cache_create(dz_cuda_model_t* m, size_t batch, size_t capacity, dz_cuda_cache_t** out) {
+static int create_cache(dz_cuda_model_t* m, size_t batch, size_t capacity, bool kv4, size_t sinks, size_t window,
+                        dz_cuda_cache_t** out) {
     if (!out) return fail(DZ_E_INVALID, "null output handle");
     *out = nullptr;
     if (!m || batch == 0 || batch > 65535 || capacity == 0 || capacity > m->desc.max_seq_len)
@@ -1670,6 +1683,9 @@ extern "C" int dz_cuda_cache_create(dz_cuda_model_t* m, size_t batch, size_t cap
     c->model = m;
     c->B = (int)batch;
     c->cap = (int)capacity;
+    c->kv4 = kv4;
+    c->sinks = (int)sinks;
+    c->window = (int)window;
     const size_t D = m->desc.embedding_dim, V = m->desc.vocab_size, Lr = m->desc.num_layers;
     const size_t B = batch;
     int rc = DZ_OK;
@@ -1679,9 +1695,18 @@ extern "C" int dz_cuda_cache_create(dz_cuda_model_t* m, size_t batch, size_t cap
         c->own_stream = true;
     }
     const size_t dl = m->dl, Fl = m->Fl;   // this rank's attention and FFN widths
-    if (!rc) rc = cache_alloc(c, (void**)&c->keys, Lr * B * capacity * dl * 4);
-    if (!rc) rc = cache_alloc(c, (void**)&c->values, Lr * B * capacity * dl * 4);
-    if (!rc) {
+    if (kv4) {
+        if (!rc) rc = cache_alloc(c, (void**)&c->kv4_codes, 2 * Lr * B * capacity * dl / 2);
+        if (!rc) rc = cache_alloc(c, (void**)&c->kv4_scales, 2 * Lr * B * capacity * dl / KV4_GROUP * 4);
+        if (!rc) rc = cache_alloc(c, (void**)&c->k_rows, B * dl * 4);
+        if (!rc) rc = cache_alloc(c, (void**)&c->v_rows, B * dl * 4);
+        if (!rc) rc = cache_alloc(c, (void**)&c->origin, B * 8);
+        if (!rc && cudaMemset(c->origin, 0, B * 8) != cudaSuccess) rc = fail(DZ_E_DEVICE, "memset");
+    } else {
+        if (!rc) rc = cache_alloc(c, (void**)&c->keys, Lr * B * capacity * dl * 4);
+        if (!rc) rc = cache_alloc(c, (void**)&c->values, Lr * B * capacity * dl * 4);
+    }
+    if (!rc && !kv4) {
         const size_t hd = D / m->desc.num_heads, rows = Lr * B * capacity;
         TensorMapEncodeFn enc = tensor_map_encoder();
         c->kv_maps = false;
@@ -1766,6 +1791,21 @@ extern "C" int dz_cuda_cache_create(dz_cuda_model_t* m, size_t batch, size_t cap
     return DZ_OK;
 }
 
+extern "C" int dz_cuda_cache_create(dz_cuda_model_t* m, size_t batch, size_t capacity, dz_cuda_cache_t** out) {
+    return create_cache(m, batch, capacity, false, 0, 0, out);
+}
+
+extern "C" int dz_cuda_cache_create_kv4(dz_cuda_model_t* m, size_t batch, size_t capacity, size_t sinks, size_t window,
+                                        dz_cuda_cache_t** out) {
+    if (out) *out = nullptr;
+    if (!m || sinks >= capacity || window > capacity - sinks)
+        return fail(DZ_E_INVALID, "4-bit cache: sinks must be below the capacity, the window at most what they leave");
+    const size_t heads = m->desc.num_heads, hd = heads ? m->desc.embedding_dim / heads : 0;
+    if ((hd != 64 && hd != 128) || hd * heads != m->desc.embedding_dim)
+        return fail(DZ_E_UNSUPPORTED, "4-bit cache: a head dimension of 64 or 128 is needed, not %zu", hd);
+    return create_cache(m, batch, capacity, true, sinks, window, out);
+}
+
 extern "C" int dz_cuda_cache_set_stream(dz_cuda_cache_t* c, void* stream) {
     if (!c) return fail(DZ_E_INVALID, "null cache");
     DeviceGuard g(c->model->device);
@@ -1815,12 +1855,64 @@ static void tp_allreduce(dz_cuda_model_t* m, float* buf, size_t count, cudaStrea
     nccl_api()->all_reduce(buf, buf, count, ncclFloat32, ncclSum, m->comm, st);
 }
 
+// Sequences s0..s0+ns-1 of a 4-bit cache's layer l.
+static Kv4Cache kv4_layer(const dz_cuda_cache_t* c, size_t l, int s0, int ns) {
+    const dz_cuda_model_t* m = c->model;
+    const size_t seq = (size_t)c->cap * m->dl, all = (size_t)c->B * seq;   // elements of a sequence, of a layer
+    Kv4Cache k;
+    k.k_codes = c->kv4_codes + (2 * l * all + s0 * seq) / 2;
+    k.v_codes = c->kv4_codes + ((2 * l + 1) * all + s0 * seq) / 2;
+    k.k_scales = c->kv4_scales + (2 * l * all + s0 * seq) / KV4_GROUP;
+    k.v_scales = c->kv4_scales + ((2 * l + 1) * all + s0 * seq) / KV4_GROUP;
+    k.batch = ns;
+    k.kv_heads = m->Hl;
+    k.capacity = c->cap;
+    k.sinks = c->sinks;
+    return k;
+}
+
+// The layer's rotation and quantization of n new tokens of every sequence,
+// and their attention. q, k, v: rows [ns x n][dl] (q rotated in place).
+static void kv4_append_attend(dz_cuda_cache_t* c, size_t l, int s0, int ns, int n, const long long* positions,
+                              long long pos_add, float* q, const float* k, const float* v, float* out) {
+    const dz_cuda_model_t* m = c->model;
+    const int dl = m->dl, hd = (int)(m->desc.embedding_dim / m->desc.num_heads);
+    Kv4AppendArgs a = {};
+    a.c = kv4_layer(c, l, s0, ns);
+    a.positions = positions;
+    a.pos_add = pos_add;
+    a.k = k;
+    a.v = v;
+    a.ldk = a.ldv = dl;
+    a.n_tokens = n;
+    if (m->rope) {
+        a.q = a.q_out = q;
+        a.ldq = a.ldqo = dl;
+        a.q_heads = m->Hl;
+        a.rope = 1;
+        dz_kv4_frequencies(10000.0, hd, a.freq);
+    }
+    dz_kv4_append_launch(a, DZ_TYPE_F32, hd, m->device, c->stream);
+    Kv4AttnArgs t = {};
+    t.c = a.c;
+    t.positions = positions;
+    t.pos_add = pos_add;
+    t.q = q;
+    t.out = out;
+    t.ldq = t.ldo = dl;
+    t.n_tokens = n;
+    t.q_heads = m->Hl;
+    t.scale = 1.0f / sqrtf((float)hd);
+    t.window = c->window;
+    dz_kv4_attn_launch(t, DZ_TYPE_F32, hd, m->device, c->stream);
+}
+
 // Launches of one layer pass over R rows and of the output head.
-static int layer_launches(const dz_cuda_model_t* m, const DevLayer& L, int R) {
+static int layer_launches(const dz_cuda_model_t* m, const DevLayer& L, int R, bool kv4 = false) {
     int n = L.fused_qkv ? qmv_launches(L.qkv, R) : qmv_launches(L.q, R) + qmv_launches(L.k, R) + qmv_launches(L.v, R);
     n += qmv_launches(L.wo, R) + qmv_launches(L.w1, R) + qmv_launches(L.w2, R);
     if (L.wg.codes) n += qmv_launches(L.wg, R);
-    return n + 3 + (m->rope ? 1 : 0) + (m->swiglu ? 1 : 0);   // attention, two norms, RoPE, SwiGLU
+    return n + 3 + (m->rope || kv4 ? 1 : 0) + (m->swiglu ? 1 : 0);   // attention, two norms, RoPE or append, SwiGLU
 }
 static int head_launches(const dz_cuda_model_t* m, int B) { return m->tied ? 1 : qmv_launches(m->head, B); }
 
@@ -1925,26 +2017,29 @@ static int enqueue_step(dz_cuda_cache_t* c, const uint32_t* tokens, long long to
     bool hidden_limbs = false;   // the previous norm wrote the limbs of the product reading c->hidden
     for (size_t l = 0; l < m->layers.size(); l++) {
         DevLayer& L = m->layers[l];
-        float* Kl = c->keys + l * (size_t)B * cap * dl;
-        float* Vl = c->values + l * (size_t)B * cap * dl;
+        // where the products write the step's K and V: ring slots, or rows for the 4-bit append
+        float* Kl = c->kv4 ? c->k_rows : c->keys + l * (size_t)B * cap * dl;
+        float* Vl = c->kv4 ? c->v_rows : c->values + l * (size_t)B * cap * dl;
+        const long long kv_ld = c->kv4 ? dl : (long long)cap * dl;
+        const int* kv_off = c->kv4 ? nullptr : c->row_off;
         if (L.fused_qkv) {
             QmvEpilogue ep = plain_epilogue(L.qkv, c->q, dl);
             ep.nseg = 3;
             ep.seg_start[0] = 0; ep.seg_start[1] = dl; ep.seg_start[2] = 2 * dl; ep.seg_start[3] = 3 * dl;
-            ep.seg_ptr[1] = Kl; ep.seg_ld[1] = (long long)cap * dl; ep.seg_row_off[1] = c->row_off;
-            ep.seg_ptr[2] = Vl; ep.seg_ld[2] = (long long)cap * dl; ep.seg_row_off[2] = c->row_off;
+            ep.seg_ptr[1] = Kl; ep.seg_ld[1] = kv_ld; ep.seg_row_off[1] = kv_off;
+            ep.seg_ptr[2] = Vl; ep.seg_ld[2] = kv_ld; ep.seg_row_off[2] = kv_off;
             launches += launch_qmv(L.qkv, c->hidden, D, B, ep, st, c->xs_scratch, c->status, hidden_limbs);
         } else {
             QmvEpilogue eq = plain_epilogue(L.q, c->q, dl);
             launches += launch_qmv(L.q, c->hidden, D, B, eq, st, c->xs_scratch, c->status);
-            QmvEpilogue ek = plain_epilogue(L.k, Kl, (long long)cap * dl);
-            ek.seg_row_off[0] = c->row_off;
+            QmvEpilogue ek = plain_epilogue(L.k, Kl, kv_ld);
+            ek.seg_row_off[0] = kv_off;
             launches += launch_qmv(L.k, c->hidden, D, B, ek, st, c->xs_scratch, c->status);
-            QmvEpilogue ev = plain_epilogue(L.v, Vl, (long long)cap * dl);
-            ev.seg_row_off[0] = c->row_off;
+            QmvEpilogue ev = plain_epilogue(L.v, Vl, kv_ld);
+            ev.seg_row_off[0] = kv_off;
             launches += launch_qmv(L.v, c->hidden, D, B, ev, st, c->xs_scratch, c->status);
         }
-        if (m->rope) {
+        if (m->rope && !c->kv4) {
             dz_rope_decode_kernel<<<B, 128, 0, st>>>(c->q, Kl, (long long)cap * dl, c->row_off, c->total, dl, hd,
                                                      m->rope_tab, m->pe_rows);
             launches++;
@@ -1956,7 +2051,11 @@ static int enqueue_step(dz_cuda_cache_t* c, const uint32_t* tokens, long long to
             ProfScope prof(DZ_KERNEL_ATTENTION, c->prof_ctx_bytes_per_layer + 8.0 * B * dl,
                            c->prof_ctx_flops_per_layer, st);
             AdArgs aa{c->q, Kl, Vl, c->start, c->ctx, c->concat, dl, cap, c->status, (int)(l * B * cap)};
-            if ((hd == 128 || hd == 64) && c->kv_maps && attn_streamed_kernel())
+            if (c->kv4) {
+                // the step's positions: total counts its token already
+                kv4_append_attend(c, l, 0, B, 1, c->total, -1, c->q, Kl, Vl, c->concat);
+                launches++;
+            } else if ((hd == 128 || hd == 64) && c->kv_maps && attn_streamed_kernel())
                 dz_attn_decode_launch(c->tm_keys, c->tm_values, aa, hd, H, B, st);
             else if (hd == 128)
                 dz_attention_decode2_kernel<4><<<dim3(H, B), ATT2_THREADS, 0, st>>>(c->q, Kl, Vl, c->start, c->ctx,
@@ -2174,7 +2273,7 @@ extern "C" int dz_cuda_select_ex(dz_cuda_cache_t* c, const dz_sampling_t* s, con
 // Whether the fused one-CTA-per-sequence kernel runs this generation.
 static bool use_seqgen(const dz_cuda_cache_t* c, const dz_sampling_t* s) {
     const dz_cuda_model_t* m = c->model;
-    if (c->path == DZ_PATH_LAYERED || !m->seq_ok) return false;
+    if (c->path == DZ_PATH_LAYERED || !m->seq_ok || c->kv4) return false;
     if (seq_smem_for(m, c->cap) > (size_t)SEQ_SMEM_LIMIT) return false;
     const bool sampled = s && s->strategy != 0 && s->temperature > 0.0f;
     if (sampled && m->desc.vocab_size > (size_t)SEL_SORT_CAP) return false;
@@ -2241,10 +2340,17 @@ static bool prefill_eligible(const dz_cuda_cache_t* c) {
     return hd == 32 || hd == 64 || hd == 128;
 }
 
+// Whether a 4-bit cache takes a prompt in one pass: no slot written twice, no
+// token of a query's window overwritten by the prompt's end.
+static bool kv4_prefill_fits(const dz_cuda_cache_t* c, size_t plen) {
+    const size_t ring = (size_t)(c->cap - c->sinks);
+    return !c->kv4 || (plen <= ring && (!c->window || (size_t)c->window + plen - 1 <= ring));
+}
+
 // Batched prefill under DZ_PREFILL_AUTO: models wide enough that their
 // projections run on the tensor-core GEMM at many rows.
 static bool use_batched_prefill(const dz_cuda_cache_t* c, size_t plen) {
-    if (plen < 2 || !prefill_eligible(c) || c->prefill == DZ_PREFILL_TOKENS) return false;
+    if (plen < 2 || !prefill_eligible(c) || !kv4_prefill_fits(c, plen) || c->prefill == DZ_PREFILL_TOKENS) return false;
     return c->prefill == DZ_PREFILL_BATCHED || c->model->desc.embedding_dim >= 512;
 }
 
@@ -2273,7 +2379,8 @@ static int ensure_prefill(dz_cuda_cache_t* c, size_t T) {
               al((void**)&c->pf_concat, rows * D * 4) && al((void**)&c->pf_attn_raw, rows * D * 4) &&
               al((void**)&c->pf_attn_norm, rows * D * 4) && al((void**)&c->pf_ff, rows * F * (m->swiglu ? 2 : 1) * 4) &&
               al((void**)&c->pf_ff_raw, rows * D * 4) && al((void**)&c->pf_rowoff, rows * 4) &&
-              al(&c->pf_scratch, scratch);
+              al(&c->pf_scratch, scratch) &&
+              (!c->kv4 || (al((void**)&c->pf_k, rows * m->dl * 4) && al((void**)&c->pf_v, rows * m->dl * 4)));
     if (!ok) {
         free_prefill(c);
         return fail(DZ_E_NOMEM, "prefill buffers for %zu rows", rows);
@@ -2299,7 +2406,7 @@ static size_t prefill_launches(const dz_cuda_cache_t* c, size_t T) {
     for (size_t g = 0; g < groups; g++) {
         const int R = (int)(std::min((size_t)c->B, (g + 1) * S) - g * S) * (int)T;
         n += 2;   // embedding, gather
-        for (const auto& L : m->layers) n += layer_launches(m, L, R);
+        for (const auto& L : m->layers) n += layer_launches(m, L, R, c->kv4);
     }
     return n;
 }
@@ -2357,26 +2464,28 @@ static int enqueue_prefill(dz_cuda_cache_t* c, const uint32_t* ids_dev, long lon
         bool hidden_limbs = false;   // the previous norm wrote the limbs of the product reading c->pf_hidden
         for (size_t l = 0; l < m->layers.size(); l++) {
             DevLayer& L = m->layers[l];
-            float* Kl = c->keys + l * (size_t)B * cap * dl + (size_t)s0 * cap * dl;
-            float* Vl = c->values + l * (size_t)B * cap * dl + (size_t)s0 * cap * dl;
+            float* Kl = c->kv4 ? c->pf_k : c->keys + l * (size_t)B * cap * dl + (size_t)s0 * cap * dl;
+            float* Vl = c->kv4 ? c->pf_v : c->values + l * (size_t)B * cap * dl + (size_t)s0 * cap * dl;
+            const long long kv_ld = c->kv4 ? dl : 0;
+            const int* kv_off = c->kv4 ? nullptr : c->pf_rowoff;
             if (L.fused_qkv) {
                 QmvEpilogue ep = plain_epilogue(L.qkv, c->pf_q, dl);
                 ep.nseg = 3;
                 ep.seg_start[0] = 0; ep.seg_start[1] = dl; ep.seg_start[2] = 2 * dl; ep.seg_start[3] = 3 * dl;
-                ep.seg_ptr[1] = Kl; ep.seg_ld[1] = 0; ep.seg_row_off[1] = c->pf_rowoff;
-                ep.seg_ptr[2] = Vl; ep.seg_ld[2] = 0; ep.seg_row_off[2] = c->pf_rowoff;
+                ep.seg_ptr[1] = Kl; ep.seg_ld[1] = kv_ld; ep.seg_row_off[1] = kv_off;
+                ep.seg_ptr[2] = Vl; ep.seg_ld[2] = kv_ld; ep.seg_row_off[2] = kv_off;
                 launches += launch_qmv(L.qkv, c->pf_hidden, D, R, ep, st, c->pf_scratch, c->status, hidden_limbs);
             } else {
                 QmvEpilogue eq = plain_epilogue(L.q, c->pf_q, dl);
                 launches += launch_qmv(L.q, c->pf_hidden, D, R, eq, st, c->pf_scratch, c->status);
-                QmvEpilogue ek = plain_epilogue(L.k, Kl, 0);
-                ek.seg_row_off[0] = c->pf_rowoff;
+                QmvEpilogue ek = plain_epilogue(L.k, Kl, kv_ld);
+                ek.seg_row_off[0] = kv_off;
                 launches += launch_qmv(L.k, c->pf_hidden, D, R, ek, st, c->pf_scratch, c->status);
-                QmvEpilogue ev = plain_epilogue(L.v, Vl, 0);
-                ev.seg_row_off[0] = c->pf_rowoff;
+                QmvEpilogue ev = plain_epilogue(L.v, Vl, kv_ld);
+                ev.seg_row_off[0] = kv_off;
                 launches += launch_qmv(L.v, c->pf_hidden, D, R, ev, st, c->pf_scratch, c->status);
             }
-            if (m->rope) {
+            if (m->rope && !c->kv4) {
                 dz_rope_prefill_kernel<<<R, 128, 0, st>>>(c->pf_q, Kl, (long long)cap * dl, T, dl, hd, m->rope_tab,
                                                           m->pe_rows);
                 launches++;
@@ -2387,7 +2496,10 @@ static int enqueue_prefill(dz_cuda_cache_t* c, const uint32_t* ids_dev, long lon
                                4.0 * ctx_pairs * hd, st);
                 const dim3 grid((unsigned)((T + PF_QT - 1) / PF_QT), (unsigned)H, (unsigned)ns);
                 const size_t smem = dz_prefill_att_smem(hd);
-                if ((!mk || (!pad && !att)) && (hd == 128 || hd == 64) && prefill_attn_tensor_cores()) {
+                if (c->kv4) {
+                    kv4_append_attend(c, l, s0, ns, T, c->origin, 0, c->pf_q, Kl, Vl, c->pf_concat);
+                    launches++;
+                } else if ((!mk || (!pad && !att)) && (hd == 128 || hd == 64) && prefill_attn_tensor_cores()) {
                     dz_pfattn_launch(c->pf_q, Kl, Vl, lens, c->pf_concat, T, dl, cap, hd, H, ns, st);
                 } else if (mk) {
                     if (hd == 128)
@@ -2517,7 +2629,7 @@ extern "C" size_t dz_cuda_generate_launches(const dz_cuda_cache_t* c, size_t ple
     if (use_seqgen(c, s)) return 2;
     const int B = (int)c->B;
     size_t step = 1 + (size_t)head_launches(m, B);   // step begin, head
-    for (const auto& L : m->layers) step += layer_launches(m, L, B);
+    for (const auto& L : m->layers) step += layer_launches(m, L, B, c->kv4);
     const size_t seeded = (s && s->strategy != 0 && s->temperature > 0.0f) ? 1 : 0;
     const size_t prefill = use_batched_prefill(c, plen) ? prefill_launches(c, plen) : plen * step;
     return seeded + 2 + prefill + n_new + (n_new ? n_new - 1 : 0) * step;   // + ring reset, history clear
@@ -2712,6 +2824,8 @@ extern "C" int dz_cuda_prefill(dz_cuda_cache_t* c, const uint32_t* ids, const ui
     if (!c || !ids || prompt_len == 0) return fail(DZ_E_INVALID, "prefill: null ids or empty prompt");
     if (prompt_len > (size_t)c->cap) return fail(DZ_E_INVALID, "prefill: prompt longer than the cache capacity");
     if (!prefill_eligible(c)) return fail(DZ_E_UNSUPPORTED, "batched prefill needs a head dimension of 32, 64 or 128");
+    if (!kv4_prefill_fits(c, prompt_len))
+        return fail(DZ_E_UNSUPPORTED, "prefill: a 4-bit cache takes prompts up to capacity - sinks (less window - 1) at once");
     const size_t B = c->B;
     std::vector<int> lv;
     if (lens) {
@@ -2759,6 +2873,7 @@ extern "C" int dz_cuda_forward_masked(dz_cuda_cache_t* c, const uint32_t* ids, s
     if (seq_len > (size_t)c->cap) return fail(DZ_E_INVALID, "forward_masked: seq_len above the cache capacity");
     if (!prefill_eligible(c))
         return fail(DZ_E_UNSUPPORTED, "the masked forward needs a head dimension of 32, 64 or 128");
+    if (c->kv4) return fail(DZ_E_UNSUPPORTED, "the masked forward needs an fp32 cache");
     const size_t B = c->B, T = seq_len;
     // the last real position of each sequence (model_forward_masked,
     // src/core/transformer.c:535-545): a padding mask with none is rejected
@@ -2857,7 +2972,9 @@ extern "C" int dz_cuda_profile_generate(dz_cuda_cache_t* c, const uint32_t* prom
     const double total_steps = (double)plen + (double)(n_new - 1);
     double mean_ctx = use_batched_prefill(c, plen) ? (double)plen + (double)n_new / 2.0 : (total_steps + 1.0) / 2.0;
     if (mean_ctx > c->cap) mean_ctx = c->cap;
-    c->prof_ctx_bytes_per_layer = 8.0 * D * mean_ctx * c->B;
+    if (c->kv4 && c->window && mean_ctx > c->window + c->sinks) mean_ctx = c->window + c->sinks;
+    // per K and V element: 4 bytes, or half a byte and a 64th of a scale
+    c->prof_ctx_bytes_per_layer = (c->kv4 ? 1.0 + 8.0 / KV4_GROUP : 8.0) * D * mean_ctx * c->B;
     c->prof_ctx_flops_per_layer = 4.0 * D * mean_ctx * c->B;
     enqueue_generate(c, prompts, plen, n_new, s, sampled ? seeds : nullptr, out);
     g_prof = nullptr;

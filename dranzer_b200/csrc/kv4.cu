@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(KV4_APPEND_WARPS * 32, 3) dz_kv4_append_kernel
         for (int i = threadIdx.x; i < cut.rows * (HD / 2); i += THREADS) {
             const int rr = i / (HD / 2), p = i % (HD / 2), w = min(row0 + rr, all_rows - 1);
             double c, s;
-            sincos((double)(a.positions[w / a.n_tokens] + w % a.n_tokens) * a.freq[p], &s, &c);
+            sincos((double)(a.positions[w / a.n_tokens] + a.pos_add + w % a.n_tokens) * a.freq[p], &s, &c);
             const int to = kv4_angle_at<HD, E>(p, a.halves);
             angles[rr][to] = make_double2(c, s);
             angles_f[rr][to] = make_float2((float)c, (float)s);
@@ -215,8 +215,8 @@ __global__ void __launch_bounds__(KV4_APPEND_WARPS * 32, 3) dz_kv4_append_kernel
     }
     if (row >= all_rows) return;
     const int b = row / a.n_tokens;
-    const long long first = a.positions[b];
-    if (first < 0) return;
+    if (a.positions[b] < 0) return;
+    const long long first = a.positions[b] + a.pos_add;
     // the lane's place in the angle table
     const int stride = a.halves ? HD / 2 / E : LPH, place = a.halves ? at % (HD / 2) / E : at / E;
 
@@ -328,6 +328,18 @@ cudaError_t dz_kv4_append_launch(const Kv4AppendArgs& a, int type, int head_dim,
     return kv4_append_h<__nv_bfloat16>(a, head_dim, sms, st);
 }
 
+void dz_kv4_frequencies(double base, size_t head_dim, double* freq) {
+    // the last ones are kept: 64 powers cost as much as a launch
+    static thread_local struct { double base, freq[64]; size_t head_dim; } last = {-1.0, {}, 0};
+    if (last.base != base || last.head_dim != head_dim) {
+        for (size_t i = 0; i < 64; i++)
+            last.freq[i] = base != 0.0 && i < head_dim / 2 ? pow(base, -2.0 * (double)i / (double)head_dim) : 0.0;
+        last.base = base;
+        last.head_dim = head_dim;
+    }
+    memcpy(freq, last.freq, sizeof(last.freq));
+}
+
 }  // namespace dz
 
 using namespace dz;
@@ -391,6 +403,7 @@ extern "C" int dz_cuda_kv4_append(const dz_kv4_t* c, const dz_kv4_append_t* p, c
     DeviceGuard g(c->device);
     if (!g.ok) return fail(DZ_E_DEVICE, "cannot select device %d", c->device);
     a.positions = (const long long*)positions;
+    a.pos_add = 0;
     a.q = p->q;
     a.k = p->k;
     a.v = p->v;
@@ -410,15 +423,7 @@ extern "C" int dz_cuda_kv4_append(const dz_kv4_t* c, const dz_kv4_append_t* p, c
     a.q_heads = (int)p->q_heads;
     a.rope = p->rope_base != 0.0;
     a.halves = p->rope_pairing == DZ_ROPE_HALVES;
-    // the last base's frequencies are kept: 64 powers cost as much as the launch
-    static thread_local struct { double base, freq[64]; size_t head_dim; } last = {0.0, {}, 0};
-    if (a.rope && (last.base != p->rope_base || last.head_dim != c->head_dim)) {
-        for (size_t i = 0; i < 64; i++)
-            last.freq[i] = i < c->head_dim / 2 ? pow(p->rope_base, -2.0 * (double)i / (double)c->head_dim) : 0.0;
-        last.base = p->rope_base;
-        last.head_dim = c->head_dim;
-    }
-    memcpy(a.freq, last.freq, sizeof(a.freq));
+    dz_kv4_frequencies(p->rope_base, c->head_dim, a.freq);
     DZ_CUDA(dz_kv4_append_launch(a, p->type, (int)c->head_dim, c->device, (cudaStream_t)stream));
     return DZ_OK;
 }
@@ -443,6 +448,7 @@ extern "C" int dz_cuda_kv4_attention(const dz_kv4_t* c, const dz_kv4_attention_t
     DeviceGuard g(c->device);
     if (!g.ok) return fail(DZ_E_DEVICE, "cannot select device %d", c->device);
     a.positions = (const long long*)positions;
+    a.pos_add = 0;
     a.q = p->q;
     a.out = p->out;
     a.ldq = (long long)p->q_stride;

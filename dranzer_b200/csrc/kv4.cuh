@@ -26,6 +26,7 @@ __device__ __forceinline__ long long kv4_slot(long long p, long long sinks, long
 struct Kv4AppendArgs {
     Kv4Cache c;
     const long long* positions;
+    long long pos_add;          // added to them (the model's caches count the step's token already)
     const void *q, *k, *v;
     void *q_out, *k_out, *v_out;
     long long ldq, ldk, ldv, ldqo, ldko, ldvo;
@@ -40,6 +41,7 @@ struct Kv4AppendArgs {
 struct Kv4AttnArgs {
     Kv4Cache c;
     const long long* positions;
+    long long pos_add;          // added to them
     const void* q;
     void* out;
     long long ldq, ldo;
@@ -47,6 +49,9 @@ struct Kv4AttnArgs {
     float scale;
     long long window;
 };
+
+// base^(-2p / head_dim) for p < head_dim / 2, the rest 0 (all 0 for base 0).
+void dz_kv4_frequencies(double base, size_t head_dim, double* freq);
 
 cudaError_t dz_kv4_append_launch(const Kv4AppendArgs& a, int type, int head_dim, int device, cudaStream_t st);
 cudaError_t dz_kv4_attn_launch(const Kv4AttnArgs& a, int type, int head_dim, int device, cudaStream_t st);

@@ -169,6 +169,20 @@ size_t dz_cuda_model_step_bytes(const dz_cuda_model_t *model);
  * (dranzer_cache_create semantics, src/include/dranzer.h:103-119). */
 int dz_cuda_cache_create(dz_cuda_model_t *model, size_t batch, size_t capacity,
                          dz_cuda_cache_t **out);
+/* The same with the keys and values in 4 bits (the layout and quantizer of
+ * dz_kv4_t, one set of rings per layer): a seventh of the fp32 bytes. The
+ * first `sinks` tokens stay visible for good, the ring of the other capacity -
+ * sinks slots holds the newest later ones, and `window` > 0 (at most capacity
+ * - sinks) hides those older than the newest `window`. Keys are rotated (RoPE
+ * models) before they are quantized. Generation runs on the layered path;
+ * BATCHED prefill attends to the quantized keys and values as decoding does,
+ * for prompts of at most capacity - sinks tokens (capacity - sinks - window +
+ * 1 with a window), longer ones go token by token (dz_cuda_prefill:
+ * DZ_E_UNSUPPORTED). DZ_E_UNSUPPORTED for head dimensions other than 64 and
+ * 128, and from dz_cuda_forward_masked on such a cache. No counterpart in the
+ * reference, whose caches are fp32. */
+int dz_cuda_cache_create_kv4(dz_cuda_model_t *model, size_t batch, size_t capacity, size_t sinks, size_t window,
+                             dz_cuda_cache_t **out);
 void dz_cuda_cache_free(dz_cuda_cache_t *cache);
 /* Use `stream` (a cudaStream_t) for all later work on this cache. */
 int dz_cuda_cache_set_stream(dz_cuda_cache_t *cache, void *stream);
