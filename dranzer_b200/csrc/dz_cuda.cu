@@ -2936,7 +2936,7 @@ extern "C" int dz_cuda_forward_masked(dz_cuda_cache_t* c, const uint32_t* ids, s
 
 extern "C" int dz_cuda_cache_set_path(dz_cuda_cache_t* c, int path) {
     if (!c || path < DZ_PATH_AUTO || path > DZ_PATH_FUSED) return fail(DZ_E_INVALID, "bad path");
-    if (path == DZ_PATH_FUSED && !c->model->seq_ok)
+    if (path == DZ_PATH_FUSED && (!c->model->seq_ok || c->kv4))
         return fail(DZ_E_UNSUPPORTED, "the fused path cannot run this model");
     DeviceGuard g(c->model->device);
     clear_graphs(c);

@@ -104,6 +104,28 @@ def test_product_special_values(gpu):
     q.close()
 
 
+def test_product_offsets_past_32_bits(gpu):
+    """Five gigabytes of records: rows and columns at both ends, some of each against the formula."""
+    k, n, group, m = 65536, 150016, 128, 3
+    g = torch.Generator("cuda").manual_seed(4)
+    low = torch.randint(0, 15, (k, n // 2), dtype=torch.uint8, device="cuda", generator=g)
+    packed = low.mul_(16).add_(torch.randint(0, 15, (k, n // 2), dtype=torch.uint8, device="cuda", generator=g))
+    scales = torch.rand(k // group, n, device="cuda", generator=g) * 0.01
+    q = gpu.GroupedWeightMatrix.from_device(scales.data_ptr(), packed.data_ptr(), k, n, group)
+    assert q.nbytes > 1 << 32
+    x = torch.randn(m, k, device="cuda", generator=g)
+    y = torch.empty(m, n, device="cuda")
+    q.matmul_async(x.data_ptr(), y.data_ptr(), m, _stream())
+    torch.cuda.synchronize()
+    pick = torch.cat([torch.arange(6), torch.arange(n // 2, n // 2 + 6), torch.arange(n - 6, n)]).cuda()
+    byte = packed[:, pick // 2].long()
+    level = torch.where(pick % 2 == 0, byte & 15, byte >> 4).double() - 7
+    w = (level * scales[:, pick].double().repeat_interleave(group, 0)).cpu().numpy()
+    ref, bound = fb.product(_np(x), w)
+    assert (np.abs(_np(y[:, pick]) - ref) <= bound + fb.rounding(ref, "f32")).all()
+    q.close()
+
+
 def test_product_refusals_on_device(gpu):
     k, n = 64, 16
     q = gpu.GroupedWeightMatrix.encode(np.ones((k, n), np.float32), 32)
@@ -462,6 +484,61 @@ def test_attention_extreme_scores(gpu):
     want = ring.rows(1, 0, 0, [50])[0].astype(np.float32)
     got = out.view(2, 128).cpu().numpy()
     assert (np.abs(got - want) <= 2.0 ** -20 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_attention_queries_of_every_size(gpu, kind):
+    """A NaN or an infinity in one query head reaches that head alone; tiny, huge and zero queries, a few large elements."""
+    rng = np.random.RandomState(13)
+    big = 3.0e4 if kind == "f16" else 1e30
+    for hq, n in ((6, 1), (4, 3)):
+        ring = Ring(gpu, 1, 2, 128, 90, 0, rng)
+        ring.scales[0][:] = 2.0 ** -3
+        q = rng.randn(n, hq, 128)
+        q[0, 1] = 0
+        q[0, 2, 5] = 100.0
+        q[0, 3] *= 1e-6
+        _check_attention(gpu, ring, kind, n, hq, 0, [80], q, 0.25)
+        q[0, 0, 77] = np.nan
+        q[n - 1, 1, 3] = -np.inf
+        q[0, 3, 9] = big
+        qt, _ = _typed(q, kind)
+        out = torch.zeros(n, hq * 128, dtype=TYPES[kind], device="cuda")
+        pos = torch.tensor([80], device="cuda")
+        ring.cache.attention(pos.data_ptr(), n, type=_dz_type(gpu, kind), q_heads=hq, q=qt.data_ptr(),
+                             out=out.data_ptr(), scale=0.25, stream_ptr=_stream())
+        torch.cuda.synchronize()
+        got = out.view(n, hq, 128)
+        assert torch.isnan(got[0, 0]).all() and torch.isnan(got[n - 1, 1]).all()
+        keep = torch.ones(n, hq, dtype=torch.bool)
+        keep[0, 0] = keep[n - 1, 1] = keep[0, 3] = False
+        assert torch.isfinite(got[keep.cuda()]).all()
+
+
+def test_cache_offsets_past_32_bits(gpu):
+    """A ring of 70 million slots: 4.5 GB of codes, the newest tokens at its far end."""
+    cap, hd, n = 70_000_000, 128, 5
+    codes = [torch.zeros(cap, hd // 2, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(cap, hd // 64, device="cuda") for _ in range(2)]
+    cache = gpu.KV4Cache(codes[0].data_ptr(), codes[1].data_ptr(), scales[0].data_ptr(), scales[1].data_ptr(), 1, 1, hd,
+                         cap, 2)
+    first = cap - n
+    pos = torch.tensor([first], device="cuda")
+    k, v, q = (torch.randn(n, hd, device="cuda") for _ in range(3))
+    held = [torch.empty(n, hd, device="cuda") for _ in range(2)]
+    cache.append(pos.data_ptr(), n, k=k.data_ptr(), v=v.data_ptr(), k_out=held[0].data_ptr(),
+                 v_out=held[1].data_ptr(), stream_ptr=_stream())
+    out = torch.empty(n, hd, device="cuda")
+    cache.attention(pos.data_ptr(), n, q_heads=1, q=q.data_ptr(), out=out.data_ptr(), window=n, stream_ptr=_stream())
+    torch.cuda.synchronize()
+    kv = [_np(t) for t in held]
+    for j in range(n):
+        # the window's older tokens and the two sinks are zeros
+        seen = [np.concatenate([np.zeros((2 + n - 1 - j, hd)), t[:j + 1]]) for t in kv]
+        tops = np.abs(seen[1]).reshape(len(seen[1]), -1, 64).max(2) / 7
+        ref, bound = fb.attend(_np(q)[j], seen[0], seen[1], hd ** -0.5, tops)
+        assert (np.abs(_np(out)[j] - ref) <= bound + fb.rounding(ref, "f32")).all(), j
+    assert int((scales[0] != 0).sum()) == 2 * n and (scales[0][-n:] != 0).all()
 
 
 def test_attention_graph_follows_positions(gpu):

@@ -197,6 +197,9 @@ def test_refusals(gpu, oracle):
     with pytest.raises(gpu.DzError) as e:
         cache.forward_masked(np.zeros((1, 4), np.uint32))
     assert e.value.status == -6
+    with pytest.raises(gpu.DzError) as e:
+        cache.set_path(cache.PATH_FUSED)
+    assert e.value.status == -6
     cache.close()
     model.close()
     narrow = make(Spec(300, 128, 4, 1, 16))
