@@ -96,15 +96,21 @@ __device__ __forceinline__ uint32_t ka_bytes(uint32_t a, uint32_t b, uint32_t c,
     return __byte_perm(__byte_perm(a, b, sel), __byte_perm(c, d, sel), 0x5410);
 }
 
-template <typename T, int HD, int ND, int NT>
+template <typename T, int HD, int ND, int NT, bool SPLIT>
 __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a,
                                                                                     int team, int cluster, int pair_blocks,
                                                                                     int units) {
     using C = KaCfg<HD>;
     constexpr int CPP = ND == 3 ? 4 : 2;     // columns of a pair
-    constexpr int PPT = 8 / CPP;             // pairs of an n-tile; lane t has columns of pair 2 t / CPP
+    // Pairs of an n-tile; lane t has columns of pair 2 t / CPP. SPLIT: where they
+    // would fill half the columns at most, the two value groups take a half
+    // each: columns 0..3 of the weights' digits belong to group 0, 4..7 to
+    // group 1, and a lane weighs the values of its columns' group alone (256 x
+    // 16 units of 640 tokens, one pair each: 69 us instead of 76).
+    constexpr int PPT = (SPLIT ? 4 : 8) / CPP;
     constexpr int PAIRS = NT * PPT;          // pairs of a block
-    constexpr int GR = C::GROUPS;
+    constexpr int GR = C::GROUPS, GA = SPLIT ? 1 : GR;   // value groups of a lane's columns
+    static_assert(!SPLIT || (NT == 1 && GR == 2), "two groups share one n-tile");
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % cluster, tw = warp % team;      // the warp's place in its team
@@ -196,7 +202,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     bool qbad[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const int pair = pair0 + n * PPT + g / CPP;
+        const int pair = pair0 + n * PPT + (SPLIT ? g % 4 : g) / CPP;
         const bool live = pair < pairs;
         const T* q = static_cast<const T*>(a.q) +
                      ((long long)b * a.n_tokens + (live ? pair / share : 0)) * a.ldq +
@@ -244,6 +250,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
         }
         qbad[n] = __any_sync(0xfu << (lane & 28), bad);
     }
+    const int tp = SPLIT ? 2 * t % 4 : 2 * t;    // the lane's first column, as pairs count them
     // ---- the score factor and the visible range of the lane's pairs
     float sfac[NT];                          // scale x log2 e (NaN for a query that holds one)
     int see_sink[NT], see_hi[NT], see_lo[NT];
@@ -252,7 +259,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     for (int n = 0; n < NT; n++) {
         const bool bad = __shfl_sync(0xffffffffu, qbad[n], 8 * t);
         sfac[n] = bad ? __int_as_float(0x7fc00000) : a.scale * 1.4426950408889634f;
-        const int pair = min(pair0 + n * PPT + 2 * t / CPP, pairs - 1);
+        const int pair = min(pair0 + n * PPT + tp / CPP, pairs - 1);
         const long long pos = first + pair / share;
         see_sink[n] = (int)min(pos, (long long)INT32_MAX);
         see_hi[n] = (int)max(-1LL, pos - lo);
@@ -264,13 +271,13 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     const int all_lo = a.window ? (int)max(-1LL, first + j_hi - a.window - lo) : -1;
 
     float m[NT], l[NT];
-    float acc[NT][GR * 4][2];                // elements 64 gr + 8 g + 2 k (and 16 x that of + 1), the lane's digits
+    float acc[NT][GA * 4][2];                // elements 64 gr + 8 g + 2 k (and 16 x that of + 1), the lane's digits
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         m[n] = -INFINITY;
         l[n] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < GR * 4; i++) acc[n][i][0] = acc[n][i][1] = 0.0f;
+        for (int i = 0; i < GA * 4; i++) acc[n][i][0] = acc[n][i][1] = 0.0f;
     }
     // the weights' digits as C columns 2t and 2t + 1 count them
     const float wd0 = ND == 3 && (t & 1) ? 65536.0f : 1.0f, wd1 = ND == 3 && (t & 1) ? 0.0f : 256.0f;
@@ -322,8 +329,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
         const int rel0 = v0 - nsink;
         const bool edge = v0 + KA_TILE > count ||
                           (masked && !(rel0 > all_lo && v0 >= nsink && rel0 + KA_TILE - 1 <= all_hi));
-        uint32_t bw[NT][GR][2];              // digits of weight x value scale
-        float back[NT][GR][2];               // what columns 2t, 2t + 1 count
+        uint32_t bw[NT][GA][2];              // digits of weight x value scale
+        float back[NT][GA][2];               // what columns 2t, 2t + 1 count
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -346,7 +353,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
                 l[n] *= c;
                 m[n] = mn;
 #pragma unroll
-                for (int i = 0; i < GR * 4; i++) {
+                for (int i = 0; i < GA * 4; i++) {
                     acc[n][i][0] *= c;
                     acc[n][i][1] *= c;
                 }
@@ -363,11 +370,11 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
             for (int i = 0; i < 8; i++)
                 p[i] = __shfl_sync(0xffffffffu, x[n][i >> 1], (t + 4 * (i & 1)) * 4 + g / 2);
 #pragma unroll
-            for (int gr = 0; gr < GR; gr++) {
+            for (int gr = 0; gr < GA; gr++) {
                 float w[8], wtop = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    float s = vs[(t + 4 * i) * GR + gr];
+                    float s = vs[(t + 4 * i) * GR + (SPLIT ? g >> 2 : gr)];
                     if (masked && edge && p[i] == 0.0f) s = 0.0f;   // another query's token may hold a NaN scale
                     w[i] = p[i] * s;
                     wtop = ka_max_nan(wtop, w[i]);
@@ -392,45 +399,73 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
             }
         }
         // values
+        int start[NT][GA][4];
 #pragma unroll
-        for (int gr = 0; gr < GR; gr++) {
-            int start[NT][4];
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
+            for (int gr = 0; gr < GA; gr++) {
                 int c[4] = {0, 0, 0, 0};     // the digits' sums over the tile
                 ka_mma_u(c, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, bw[n][gr][0], bw[n][gr][1]);
-                start[n][0] = KA_ZERO - 7 * c[0];
-                start[n][1] = KA_ZERO - 7 * c[1];
-                start[n][2] = KA_ZERO - 112 * c[0];
-                start[n][3] = KA_ZERO - 112 * c[1];
+                start[n][gr][0] = KA_ZERO - 7 * c[0];
+                start[n][gr][1] = KA_ZERO - 7 * c[1];
+                start[n][gr][2] = KA_ZERO - 112 * c[0];
+                start[n][gr][3] = KA_ZERO - 112 * c[1];
             }
-            uint32_t w[8];
+        auto codes = [&](int gr, uint32_t (&w)[8]) {     // word g of the group's eight, tokens t + 4 i
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int r = t + 4 * i;
                 const int at = HD == 128 ? ((2 * gr + (g >> 2)) ^ (t & 2)) * 16 + 4 * (g & 3) : 4 * g;
                 w[i] = *reinterpret_cast<const uint32_t*>(st + C::CODES + r * C::ROW + at);
             }
+        };
+        // Byte `byte` of the tokens: element 8 g + 2 byte in the low halves, the next one in the high halves.
+        auto multiply = [&](const uint32_t (&w)[8], int byte, int n, int gr, int (&c)[4]) {
+            const uint32_t sel = (uint32_t)byte * 0x11u + 0x40u;
+            const uint32_t b0 = ka_bytes(w[0], w[1], w[2], w[3], sel), b1 = ka_bytes(w[4], w[5], w[6], w[7], sel);
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[i] = start[n][gr][i];
+            ka_mma_u(c, b0 & LOW, b0 & HIGH, b1 & LOW, b1 & HIGH, bw[n][gr][0], bw[n][gr][1]);
+        };
+        auto add = [&](const int (&c)[4], int n, int gr, int byte) {
+            float* o = acc[n][4 * gr + byte];
+            o[0] = fmaf(__int_as_float(c[0]) - KA_ZEROF, back[n][gr][0], o[0]);
+            o[0] = fmaf(__int_as_float(c[1]) - KA_ZEROF, back[n][gr][1], o[0]);
+            o[1] = fmaf(__int_as_float(c[2]) - KA_ZEROF, back[n][gr][0], o[1]);
+            o[1] = fmaf(__int_as_float(c[3]) - KA_ZEROF, back[n][gr][1], o[1]);
+        };
+        if constexpr (SPLIT) {
+            uint32_t w0[8], w1[8];
+            codes(0, w0);
+            codes(1, w1);
 #pragma unroll
             for (int byte = 0; byte < 4; byte++) {
-                // byte `byte` of four tokens: element 8 g + 2 byte in the low halves, the next one in the high halves
-                const uint32_t sel = (uint32_t)byte * 0x11u + 0x40u;
-                const uint32_t b0 = ka_bytes(w[0], w[1], w[2], w[3], sel), b1 = ka_bytes(w[4], w[5], w[6], w[7], sel);
+                int c0[4], c1[4];
+                multiply(w0, byte, 0, 0, c0);
+                multiply(w1, byte, 0, 0, c1);
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    int c[4] = {start[n][0], start[n][1], start[n][2], start[n][3]};
-                    ka_mma_u(c, b0 & LOW, b0 & HIGH, b1 & LOW, b1 & HIGH, bw[n][gr][0], bw[n][gr][1]);
-                    float* o = acc[n][4 * gr + byte];
-                    o[0] = fmaf(__int_as_float(c[0]) - KA_ZEROF, back[n][gr][0], o[0]);
-                    o[0] = fmaf(__int_as_float(c[1]) - KA_ZEROF, back[n][gr][1], o[0]);
-                    o[1] = fmaf(__int_as_float(c[2]) - KA_ZEROF, back[n][gr][0], o[1]);
-                    o[1] = fmaf(__int_as_float(c[3]) - KA_ZEROF, back[n][gr][1], o[1]);
-                }
+                for (int i = 0; i < 4; i++) c0[i] = t < 2 ? c0[i] : c1[i];   // the lane's columns' group
+                add(c0, 0, 0, byte);
+            }
+        } else {
+#pragma unroll
+            for (int gr = 0; gr < GR; gr++) {
+                uint32_t w[8];
+                codes(gr, w);
+#pragma unroll
+                for (int byte = 0; byte < 4; byte++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        int c[4];
+                        multiply(w, byte, n, gr, c);
+                        add(c, n, gr, byte);
+                    }
             }
         }
     }
 
-    // ---- the warp's sums in units of its 2^m: lane (g, t) has elements 64 gr + 8 g .. + 7 of pair 2 t / CPP
+    // ---- the warp's sums in units of its 2^m: lane (g, t) has elements 64 gr + 8 g .. + 7 of
+    // pair tp / CPP (SPLIT: of group t / 2 alone)
     ka_wait<0>();
     __syncwarp();
 #pragma unroll
@@ -439,7 +474,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
         l[n] += __shfl_xor_sync(0xffffffffu, l[n], 8);
         l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
 #pragma unroll
-        for (int k = 0; k < GR * 4; k++) {
+        for (int k = 0; k < GA * 4; k++) {
             if (ND == 3) {
                 acc[n][k][0] += __shfl_xor_sync(0xffffffffu, acc[n][k][0], 1);
                 acc[n][k][1] += __shfl_xor_sync(0xffffffffu, acc[n][k][1], 1);
@@ -452,16 +487,17 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
                                (long long)(hk * share + p % share) * HD + d] = dz_from_float<T>(v);
     };
     const bool speaks = ND == 2 || !(t & 1);   // of two lanes with the same sums
+    const int e0 = (SPLIT ? 64 * (t >> 1) : 0) + 8 * g;
     if (team * cluster == 1) {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const int p = pair0 + n * PPT + 2 * t / CPP;
+            const int p = pair0 + n * PPT + tp / CPP;
             if (p >= pairs || !speaks) continue;
             T* o = static_cast<T*>(a.out) + ((long long)b * a.n_tokens + p / share) * a.ldo +
-                   (long long)(hk * share + p % share) * HD + 8 * g;
+                   (long long)(hk * share + p % share) * HD + e0;
             const float inv = 1.0f / l[n];
 #pragma unroll
-            for (int gr = 0; gr < GR; gr++)
+            for (int gr = 0; gr < GA; gr++)
 #pragma unroll
                 for (int k = 0; k < 8; k++) o[64 * gr + k] = dz_from_float<T>(acc[n][4 * gr + k / 2][k % 2] * inv);
         }
@@ -475,16 +511,16 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     float* so = reinterpret_cast<float*>(my);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const int pair = n * PPT + 2 * t / CPP;
+        const int pair = n * PPT + tp / CPP;
         if (!speaks) continue;
 #pragma unroll
-        for (int gr = 0; gr < GR; gr++)
+        for (int gr = 0; gr < GA; gr++)
 #pragma unroll
             for (int k = 0; k < 4; k += 2)
-                *reinterpret_cast<float4*>(so + pair * OS + 64 * gr + 8 * g + 2 * k) =
+                *reinterpret_cast<float4*>(so + pair * OS + 64 * gr + e0 + 2 * k) =
                     make_float4(acc[n][4 * gr + k][0], acc[n][4 * gr + k][1], acc[n][4 * gr + k + 1][0],
                                 acc[n][4 * gr + k + 1][1]);
-        if (g == 0) {
+        if (g == 0 && (!SPLIT || t < 2)) {
             so[PAIRS * OS + pair] = m[n];
             so[PAIRS * OS + PAIRS + pair] = l[n];
         }
@@ -544,8 +580,11 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-template <int HD, int ND, int NT> constexpr int ka_smem() {
-    constexpr int pairs = NT * (ND == 3 ? 2 : 4);
+// Pairs of a block.
+template <int ND, int NT, bool SPLIT> constexpr int ka_pairs() { return NT * (ND == 3 ? 2 : 4) / (SPLIT ? 2 : 1); }
+
+template <int HD, int ND, int NT, bool SPLIT> constexpr int ka_smem() {
+    constexpr int pairs = ka_pairs<ND, NT, SPLIT>();
     return KaCfg<HD>::RING + (pairs * HD + 2 * pairs) * 4;
 }
 
@@ -560,7 +599,7 @@ struct KaRoom {
 // visible tokens: the least number of tiles that a warp works through one
 // after the other, its start (as long as 4 tiles) and the joins (3 each) among
 // them. 256 x 16 units of 640 tokens: 76 us with a warp each, 123 with eight;
-// 16 units of 130000: 564 us with eight, 118 with 64.
+// 16 units of 130000: 564 us with eight, 118 with 64, 78 with 104.
 static void ka_shape(const KaRoom& room, long long units, long long longest, int* team, int* cluster) {
     const long long tiles = (longest + KA_TILE - 1) / KA_TILE;
     double best = 1e30;
@@ -578,10 +617,10 @@ static void ka_shape(const KaRoom& room, long long units, long long longest, int
     for (int c = 2; c <= KA_CLUSTER && (long long)(c - 1) * KA_WARPS < tiles; c++) consider(KA_WARPS, c);
 }
 
-template <typename T, int HD, int ND, int NT>
+template <typename T, int HD, int ND, int NT, bool SPLIT>
 static cudaError_t ka_launch(const Kv4AttnArgs& a, int device, cudaStream_t st) {
-    auto* k = dz_kv4_attn_kernel<T, HD, ND, NT>;
-    constexpr int smem = ka_smem<HD, ND, NT>(), pairs_per_block = NT * (ND == 3 ? 2 : 4);
+    auto* k = dz_kv4_attn_kernel<T, HD, ND, NT, SPLIT>;
+    constexpr int smem = ka_smem<HD, ND, NT, SPLIT>(), pairs_per_block = ka_pairs<ND, NT, SPLIT>();
     static KaRoom rooms[KA_DEVICES];
     if (device < 0 || device >= KA_DEVICES) return cudaErrorInvalidDevice;
     KaRoom& room = rooms[device];
@@ -627,7 +666,10 @@ static cudaError_t ka_launch(const Kv4AttnArgs& a, int device, cudaStream_t st) 
 template <typename T, int HD, int ND>
 static cudaError_t ka_launch_n(const Kv4AttnArgs& a, int device, cudaStream_t st) {
     const int pairs = a.n_tokens * (a.q_heads / a.c.kv_heads);
-    return pairs <= (ND == 3 ? 2 : 4) ? ka_launch<T, HD, ND, 1>(a, device, st) : ka_launch<T, HD, ND, 2>(a, device, st);
+    if constexpr (HD == 128)
+        if (pairs <= ka_pairs<ND, 1, true>()) return ka_launch<T, HD, ND, 1, true>(a, device, st);
+    if (pairs <= ka_pairs<ND, 1, false>()) return ka_launch<T, HD, ND, 1, false>(a, device, st);
+    return ka_launch<T, HD, ND, 2, false>(a, device, st);
 }
 
 template <typename T, int ND>
