@@ -1701,7 +1701,6 @@ static int create_cache(dz_cuda_model_t* m, size_t batch, size_t capacity, bool 
         if (!rc) rc = cache_alloc(c, (void**)&c->k_rows, B * dl * 4);
         if (!rc) rc = cache_alloc(c, (void**)&c->v_rows, B * dl * 4);
         if (!rc) rc = cache_alloc(c, (void**)&c->origin, B * 8);
-        if (!rc && cudaMemset(c->origin, 0, B * 8) != cudaSuccess) rc = fail(DZ_E_DEVICE, "memset");
     } else {
         if (!rc) rc = cache_alloc(c, (void**)&c->keys, Lr * B * capacity * dl * 4);
         if (!rc) rc = cache_alloc(c, (void**)&c->values, Lr * B * capacity * dl * 4);
@@ -1780,6 +1779,7 @@ static int create_cache(dz_cuda_model_t* m, size_t batch, size_t capacity, bool 
         cudaMemsetAsync(c->start, 0, B * 4, c->stream);
         cudaMemsetAsync(c->length, 0, B * 4, c->stream);
         cudaMemsetAsync(c->total, 0, B * 8, c->stream);
+        if (c->origin) cudaMemsetAsync(c->origin, 0, B * 8, c->stream);
         cudaMemsetAsync(c->seen, 0, B * (size_t)c->seen_words * 4, c->stream);
         if (cudaStreamSynchronize(c->stream) != cudaSuccess) rc = fail(DZ_E_DEVICE, "cache init");
     }

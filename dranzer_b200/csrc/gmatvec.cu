@@ -97,8 +97,8 @@ template <typename S> __global__ void dz_gmv_dequant_kernel(GmvMatrix w, float* 
 // sum in the tile's place, a warp that continues a tile keeps it in its own.
 // Then the parts add up in a fixed order, over warps, then over the cluster.
 //
-// Bound by HBM for large matrices: 1 x 4096 x 32000 (fp16 scales) 13.2 us per
-// call, 5.1 TB/s; by the latency of its phases for small ones: 1 x 2048 x 2048
+// Bound by HBM for large matrices: 1 x 4096 x 32000 (fp16 scales) 13.9 us per
+// call, 4.9 TB/s; by the latency of its phases for small ones: 1 x 2048 x 2048
 // 3.1 us, 8 x 2048 x 8192 (bf16) 7.5 us, 16 x 4099 x 5003 (fp16, groups of 32)
 // 16 us. The one-thread-per-column form took 157 us for the first; a barrier
 // per tile 20 us; a cluster barrier per tile 29 us.
@@ -227,8 +227,10 @@ __global__ void __launch_bounds__(GMV_WARPS * 32, NT < 3 || (NT == 3 && GPB < 4)
         pstage = pstage + 1 == GMV_STAGES ? 0 : pstage + 1;
     };
     produce();
-    // the weights are nobody's output; activations and y wait for the kernel before
-    asm volatile("griddepcontrol.launch_dependents;");
+    // The weights are nobody's output; activations and y wait for the kernel
+    // before. (Letting the next kernel start before this one ends: 13.2 against
+    // 13.9 us back to back in a graph for 1 x 4096 x 32000, but 17.4 against 13.7
+    // when calls are issued one by one about as fast as they run.)
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     // ---- activations to digits. A unit is one row's share of one block, 128

@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(KV4_APPEND_WARPS * 32, 3) dz_kv4_append_kernel
                                                                                 const __grid_constant__ Kv4AppendCut cut) {
     constexpr int E = 16 / (int)sizeof(T), LPH = HD / E, HPW = 32 / LPH;   // elements, lanes of a head, heads of a warp
     constexpr int THREADS = KV4_APPEND_WARPS * 32, ROWS = THREADS / (HD / 2);
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before ends
     __shared__ double2 angles[ROWS][HD / 2];
     __shared__ float2 angles_f[ROWS][HD / 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, at = lane % LPH * E, mine = lane / LPH;
@@ -307,8 +308,16 @@ template <typename T, int HD> static cudaError_t kv4_append_t(const Kv4AppendArg
     const long long strides = a.ldq | a.ldk | a.ldv | a.ldqo | a.ldko | a.ldvo;
     cut.wide = bases % 16 == 0 && strides * (long long)sizeof(T) % 16 == 0;
     const unsigned grid = (unsigned)((rows + cut.rows - 1) / cut.rows * cut.parts);
-    dz_kv4_append_kernel<T, HD><<<grid, KV4_APPEND_WARPS * 32, 0, st>>>(a, cut);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(KV4_APPEND_WARPS * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, dz_kv4_append_kernel<T, HD>, a, cut);
 }
 
 template <typename T> static cudaError_t kv4_append_h(const Kv4AppendArgs& a, int head_dim, int sms, cudaStream_t st) {

@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     constexpr int GR = C::GROUPS, GA = SPLIT ? 1 : GR;   // value groups of a lane's columns
     static_assert(!SPLIT || (NT == 1 && GR == 2), "two groups share one n-tile");
     extern __shared__ __align__(16) uint8_t smem[];
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before ends
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % cluster, tw = warp % team;      // the warp's place in its team
     int unit = blockIdx.x / cluster * (KA_WARPS / team) + warp / team;
@@ -631,9 +632,11 @@ static cudaError_t ka_launch(const Kv4AttnArgs& a, int device, cudaStream_t st) 
     cfg.blockDim = dim3(KA_WARPS * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     if (!room.known.load(std::memory_order_acquire)) {
         cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -659,7 +662,8 @@ static cudaError_t ka_launch(const Kv4AttnArgs& a, int device, cudaStream_t st) 
     const long long grid = (units + KA_WARPS / team - 1) / (KA_WARPS / team) * cluster;
     cfg.gridDim = dim3((unsigned)grid);
     attr[0].val.clusterDim.x = cluster;
-    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    cfg.attrs = cluster > 1 ? attr : attr + 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, k, a, team, cluster, blocks, (int)units);
 }
 
