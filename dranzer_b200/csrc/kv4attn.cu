@@ -27,23 +27,20 @@
 //
 // Bound by instruction issue: 540 per tile of 32 tokens at head dimension 128
 // and one fp32 pair, 2.5 a cycle per SM. 256 x 16 heads of 128, up to 641
-// tokens: 69 us per call, 4.9 TB/s of the 6.55 that a copy reaches. With levels
+// tokens: 67 us per call, 5.0 TB/s of the 6.55 that a copy reaches. With levels
 // widened to fp16 pairs in m16n8k16 (two fp16 parts per fp32 weight) a tile took
 // 860 instructions, most of the ALU's issue rate in widening, and the call 118
 // us.
-#include <atomic>
 #include <cmath>
 
-#include "kv4.cuh"
+#include "kv4launch.cuh"
 #include "shim.cuh"
 
 namespace dz {
 
-constexpr int KA_WARPS = 8;
-constexpr int KA_TILE = 32;     // tokens of a tile
+constexpr int KA_WARPS = KV4_WARPS;
+constexpr int KA_TILE = KV4_TILE;
 constexpr int KA_STAGES = 3;
-constexpr int KA_DEVICES = 64;  // devices whose launch state is kept
-constexpr int KA_CLUSTER = 16;            // blocks of a cluster at most
 constexpr int KA_ZERO = 0x4B400000;       // 1.5 x 2^23
 constexpr float KA_ZEROF = 12582912.0f;
 
@@ -341,7 +338,10 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
             for (int r = 0; r < 4; r++) {
                 if (ND == 3) x[n][r] += __shfl_xor_sync(0xffffffffu, x[n][r], 1);   // the pair's other digits
                 x[n][r] *= sfac[n];
-                if (edge) {
+            }
+            if (edge) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
                     const int v = v0 + r * 8 + g, rel = v - nsink;
                     const bool see = v < nsink ? v <= see_sink[n] : rel <= see_hi[n] && rel > see_lo[n];
                     if (!see || v >= count) x[n][r] = -INFINITY;
@@ -377,12 +377,13 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
             for (int gr = 0; gr < GA; gr++) {
                 float w[8], wtop = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    float s = vs[(t + 4 * i) * GR + (SPLIT ? g >> 2 : gr)];
-                    if (masked && edge && p[i] == 0.0f) s = 0.0f;   // another query's token may hold a NaN scale
-                    w[i] = p[i] * s;
-                    wtop = ka_max_nan(wtop, w[i]);
+                for (int i = 0; i < 8; i++) w[i] = p[i] * vs[(t + 4 * i) * GR + (SPLIT ? g >> 2 : gr)];
+                if (masked && edge) {        // another query's token may hold a NaN scale
+#pragma unroll
+                    for (int i = 0; i < 8; i++) w[i] = p[i] == 0.0f ? 0.0f : w[i];
                 }
+#pragma unroll
+                for (int i = 0; i < 8; i++) wtop = ka_max_nan(wtop, w[i]);
                 wtop = ka_max_nan(wtop, __shfl_xor_sync(0xffffffffu, wtop, 1));
                 wtop = ka_max_nan(wtop, __shfl_xor_sync(0xffffffffu, wtop, 2));
                 // the power of two that puts the largest in [2^22, 2^23) (or [2^14, 2^15): it may round up to
@@ -592,84 +593,15 @@ template <int HD, int ND, int NT, bool SPLIT> constexpr int ka_smem() {
     return KaCfg<HD>::RING + (pairs * HD + 2 * pairs) * 4;
 }
 
-// Clusters of 1..16 blocks of a kernel that a device holds at once (a cluster
-// stays within one GPC, so that larger ones leave SMs idle).
-struct KaRoom {
-    std::atomic<bool> known{false};
-    std::atomic<int> clusters[KA_CLUSTER + 1];
-};
-
-// Warps of a team and blocks of a cluster for `units` units of up to `longest`
-// visible tokens: the least number of tiles that a warp works through one
-// after the other, its start (as long as 4 tiles) and the joins (3 each) among
-// them. 256 x 16 units of 640 tokens: 76 us with a warp each, 123 with eight;
-// 16 units of 130000: 564 us with eight, 118 with 64, 78 with 104.
-static void ka_shape(const KaRoom& room, long long units, long long longest, int* team, int* cluster) {
-    const long long tiles = (longest + KA_TILE - 1) / KA_TILE;
-    double best = 1e30;
-    auto consider = [&](int w, int c) {
-        const long long warps = (long long)w * c, slots = (long long)room.clusters[c].load(std::memory_order_relaxed) * (KA_WARPS / w);
-        const double waves = (double)((units + slots - 1) / slots), each = (double)((tiles + warps - 1) / warps);
-        const double t = waves * (each + 4.0 + (warps > 1 ? 3.0 : 0.0) + (c > 1 ? 3.0 : 0.0));
-        if (t < best) {
-            best = t;
-            *team = w;
-            *cluster = c;
-        }
-    };
-    for (int w = 1; w <= KA_WARPS; w *= 2) consider(w, 1);
-    for (int c = 2; c <= KA_CLUSTER && (long long)(c - 1) * KA_WARPS < tiles; c++) consider(KA_WARPS, c);
-}
-
 template <typename T, int HD, int ND, int NT, bool SPLIT>
 static cudaError_t ka_launch(const Kv4AttnArgs& a, int device, cudaStream_t st) {
-    auto* k = dz_kv4_attn_kernel<T, HD, ND, NT, SPLIT>;
-    constexpr int smem = ka_smem<HD, ND, NT, SPLIT>(), pairs_per_block = ka_pairs<ND, NT, SPLIT>();
-    static KaRoom rooms[KA_DEVICES];
-    if (device < 0 || device >= KA_DEVICES) return cudaErrorInvalidDevice;
-    KaRoom& room = rooms[device];
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(KA_WARPS * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    if (!room.known.load(std::memory_order_acquire)) {
-        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        for (int c = 1; c <= KA_CLUSTER && e == cudaSuccess; c++) {
-            cfg.gridDim = dim3(c);
-            cfg.numAttrs = 1;
-            attr[0].val.clusterDim.x = c;
-            int n = 0;
-            e = cudaOccupancyMaxActiveClusters(&n, k, &cfg);
-            room.clusters[c].store(n > 0 ? n : 1, std::memory_order_relaxed);
-        }
-        if (e != cudaSuccess) return e;
-        room.known.store(true, std::memory_order_release);
-    }
-    const int pairs = a.n_tokens * (a.q_heads / a.c.kv_heads);
-    const int blocks = (pairs + pairs_per_block - 1) / pairs_per_block;
-    const long long units = (long long)a.c.batch * a.c.kv_heads * blocks;
-    const long long ring = a.c.capacity - a.c.sinks;
-    const long long longest = a.c.sinks + (a.window && a.window < ring ? a.window + a.n_tokens : ring);
-    int team, cluster;
-    ka_shape(room, units, longest, &team, &cluster);
-    const long long grid = (units + KA_WARPS / team - 1) / (KA_WARPS / team) * cluster;
-    cfg.gridDim = dim3((unsigned)grid);
-    attr[0].val.clusterDim.x = cluster;
-    cfg.attrs = cluster > 1 ? attr : attr + 1;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, k, a, team, cluster, blocks, (int)units);
+    static Kv4Room rooms[KV4_DEVICES];
+    return kv4_launch(dz_kv4_attn_kernel<T, HD, ND, NT, SPLIT>, rooms, a, ka_pairs<ND, NT, SPLIT>(),
+                      ka_smem<HD, ND, NT, SPLIT>(), device, st);
 }
 
-// One n-tile where it holds all pairs of a key head, else two. Four (a block
-// to an SM, 255 registers) took 76 against 64 us for 8 x 4 key heads of 64, 128
-// pairs each, 115 against 121 us at a head dimension of 128.
+// One n-tile where it holds all pairs of a key head, else two (more leave one
+// block to an SM).
 template <typename T, int HD, int ND>
 static cudaError_t ka_launch_n(const Kv4AttnArgs& a, int device, cudaStream_t st) {
     const int pairs = a.n_tokens * (a.q_heads / a.c.kv_heads);
@@ -679,12 +611,21 @@ static cudaError_t ka_launch_n(const Kv4AttnArgs& a, int device, cudaStream_t st
     return ka_launch<T, HD, ND, 2, false>(a, device, st);
 }
 
+// Pairs of a key head up to which tokens are the MMA's rows; above, pairs are
+// (kv4chunk.cu). Both on 8 x 4 key heads of 128 that see 4160 tokens, fp32: 4
+// pairs 21 against 22 us, 8 pairs 26 against 24, 128 pairs 218 against 105; fp16:
+// 16 pairs 27 against 32, 24 pairs 41 against 38. Of 64, fp32: 16 pairs 22 each, 24
+// pairs 34 against 25; fp16: 16 pairs 16 against 18, 128 pairs 59 against 45.
+static int ka_limit(int type, int head_dim) { return type == DZ_TYPE_F32 && head_dim == 128 ? 4 : 16; }
+
 template <typename T, int ND>
 static cudaError_t ka_launch_t(const Kv4AttnArgs& a, int head_dim, int device, cudaStream_t st) {
     return head_dim == 128 ? ka_launch_n<T, 128, ND>(a, device, st) : ka_launch_n<T, 64, ND>(a, device, st);
 }
 
 cudaError_t dz_kv4_attn_launch(const Kv4AttnArgs& a, int type, int head_dim, int device, cudaStream_t st) {
+    if ((long long)a.n_tokens * (a.q_heads / a.c.kv_heads) > ka_limit(type, head_dim))
+        return dz_kv4_chunk_launch(a, type, head_dim, device, st);
     if (type == DZ_TYPE_F32) return ka_launch_t<float, 3>(a, head_dim, device, st);
     if (type == DZ_TYPE_F16) return ka_launch_t<__half, 2>(a, head_dim, device, st);
     return ka_launch_t<__nv_bfloat16, 2>(a, head_dim, device, st);
