@@ -541,6 +541,129 @@ def test_cache_offsets_past_32_bits(gpu):
     assert int((scales[0] != 0).sum()) == 2 * n and (scales[0][-n:] != 0).all()
 
 
+# Many pairs to a key head: queries enter as fp16 parts (2^-22 of an element or finer), weights as bf16 parts
+# (2^-18 of a weight; 2^-27 for fp32), both within what fb.attend() allows for integers.
+CHUNKS = [  # batch, n, hq, hk, hd, cap, sinks, window, first positions
+    (1, 17, 1, 1, 64, 17, 0, 0, [0]),
+    (1, 1, 17, 1, 128, 1, 0, 0, [0]),
+    (2, 1, 32, 1, 64, 700, 3, 0, [5000, 31]),
+    (3, 5, 4, 1, 128, 300, 4, 32, [-1, 297, 4]),
+    (2, 3, 12, 2, 64, 2500, 0, 0, [2490, 600]),
+    (1, 6, 6, 2, 128, 5000, 2, 0, [(1 << 33) + 3]),
+    (40, 20, 2, 2, 64, 60, 4, 33, [3 * i for i in range(40)]),
+    (2, 31, 3, 3, 128, 64, 33, 1, [0, 3000]),
+    (1, 9, 10, 5, 128, 41, 0, 33, [32]),
+    (1, 16, 5, 1, 64, 400, 1, 100, [700]),
+]
+
+
+@pytest.mark.parametrize("case", CHUNKS)
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_attention_of_chunks(gpu, case, kind):
+    batch, n, hq, hk, hd, cap, sinks, window, first = case
+    rng = np.random.RandomState(cap + n)
+    ring = Ring(gpu, batch, hk, hd, cap, sinks, rng)
+    _check_attention(gpu, ring, kind, n, hq, window, first, rng.randn(batch * n, hq, hd), hd ** -0.5)
+    for old, new in zip(ring.before, ring.snapshot()):
+        np.testing.assert_array_equal(old[0], new[0])
+        np.testing.assert_array_equal(old[1], new[1])
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_chunks_with_scales_of_every_size(gpu, kind):
+    rng = np.random.RandomState(18)
+    ring = Ring(gpu, 2, 2, 128, 400, 0, rng)
+    s = ring.scales[1]
+    s.copy_(torch.from_numpy(2.0 ** rng.randint(-60, 20 if kind == "f32" else 10, s.shape).astype(np.float32)))
+    ring.scales[0][17] = 8.0
+    _check_attention(gpu, ring, kind, 9, 4, 0, [391, 300], rng.randn(18, 4, 128), 128 ** -0.5)
+
+
+def test_chunks_ignore_what_they_do_not_see(gpu):
+    """NaN scales in slots that no query of the chunk sees change nothing; one that the later queries alone see
+    reaches them alone."""
+    rng = np.random.RandomState(19)
+    n, hq = 6, 8
+    for cap, sinks, window, first in ((300, 4, 64, 5000), (300, 0, 0, 100), (64, 3, 10, 12), (140, 0, 100, 131)):
+        ring = Ring(gpu, 1, 2, 64, cap, sinks, rng)
+        q = rng.randn(n, hq, 64)
+        clean = _check_attention(gpu, ring, "f32", n, hq, window, [first], q, 0.125)
+        seen = {fb.slot(p, sinks, cap) for j in range(n)
+                for p in fb.visible(first + j, first + n - 1, sinks, cap, window)}
+        hidden = torch.tensor([h * cap + s for h in range(2) for s in range(cap) if s not in seen], device="cuda",
+                              dtype=torch.int64)
+        for which in range(2):
+            ring.scales[which][hidden] = float("nan")
+            ring.codes[which][hidden] = 0xFF
+            ring.scales[which][2 * cap:] = float("nan")
+        again = _check_attention(gpu, ring, "f32", n, hq, window, [first], q, 0.125)
+        np.testing.assert_array_equal(clean, again)
+        for which in range(2):               # the chunk's fourth token, of the second key head
+            ring.scales[which][cap + fb.slot(first + 3, sinks, cap)] = float("nan")
+            out = torch.zeros(n, hq * 64, device="cuda")
+            pos = torch.tensor([first], device="cuda")
+            qt = torch.from_numpy(q.astype(np.float32)).cuda()
+            ring.cache.attention(pos.data_ptr(), n, q_heads=hq, q=qt.data_ptr(), out=out.data_ptr(), window=window,
+                                 stream_ptr=_stream())
+            torch.cuda.synchronize()
+            got = out.view(n, hq, 64).cpu().numpy()
+            np.testing.assert_array_equal(got[:3], clean[0, :3])
+            np.testing.assert_array_equal(got[:, :4], clean[0, :, :4])
+            assert np.isnan(got[3:, 4:]).all()
+            ring.scales[which][cap + fb.slot(first + 3, sinks, cap)] = 1.0
+            clean = _check_attention(gpu, ring, "f32", n, hq, window, [first], q, 0.125)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_chunks_of_queries_of_every_size(gpu, kind):
+    rng = np.random.RandomState(23)
+    n, hq = 7, 6
+    ring = Ring(gpu, 1, 2, 128, 90, 0, rng)
+    ring.scales[0][:] = 2.0 ** -3
+    q = rng.randn(n, hq, 128)
+    q[0, 1] = 0
+    q[0, 2, 5] = 100.0
+    q[0, 3] *= 1e-6
+    clean = _check_attention(gpu, ring, kind, n, hq, 0, [80], q, 0.25)
+    q[0, 0, 77] = np.nan
+    q[n - 1, 1, 3] = -np.inf
+    q[2, 4, 9] = np.inf
+    qt, _ = _typed(q, kind)
+    out = torch.zeros(n, hq * 128, dtype=TYPES[kind], device="cuda")
+    pos = torch.tensor([80], device="cuda")
+    ring.cache.attention(pos.data_ptr(), n, type=_dz_type(gpu, kind), q_heads=hq, q=qt.data_ptr(), out=out.data_ptr(),
+                         scale=0.25, stream_ptr=_stream())
+    torch.cuda.synchronize()
+    got = _np(out).reshape(n, hq, 128)
+    bad = np.zeros((n, hq), bool)
+    bad[0, 0] = bad[n - 1, 1] = bad[2, 4] = True
+    assert np.isnan(got[bad]).all()
+    np.testing.assert_array_equal(got[~bad], clean[0][~bad])
+
+
+def test_chunk_offsets_past_32_bits(gpu):
+    """The last of 70 million slots, seen by a chunk of 20 pairs of the second key head of two."""
+    cap, hd, n = 35_000_000, 128, 5
+    codes = [torch.full((2 * cap, hd // 2), 0x77, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(2 * cap, hd // 64, device="cuda") for _ in range(2)]
+    rng = np.random.RandomState(3)
+    small = Ring(gpu, 1, 2, hd, 2 * n, 0, rng)
+    for which in range(2):
+        for h in range(2):
+            at = (h + 1) * cap - 2 * n
+            codes[which][at:at + 2 * n] = small.codes[which][h * 2 * n:(h + 1) * 2 * n]
+            scales[which][at:at + 2 * n] = small.scales[which][h * 2 * n:(h + 1) * 2 * n]
+    cache = gpu.KV4Cache(codes[0].data_ptr(), codes[1].data_ptr(), scales[0].data_ptr(), scales[1].data_ptr(), 1, 2, hd,
+                         cap, 0)
+    q = torch.from_numpy(rng.randn(n, 8, hd).astype(np.float32)).cuda()
+    out = torch.empty(n, 8 * hd, device="cuda")
+    pos = torch.tensor([cap - n], device="cuda")
+    cache.attention(pos.data_ptr(), n, q_heads=8, q=q.data_ptr(), out=out.data_ptr(), window=n, stream_ptr=_stream())
+    torch.cuda.synchronize()
+    want = _check_attention(gpu, small, "f32", n, 8, n, [n], _np(q), hd ** -0.5)
+    np.testing.assert_array_equal(_np(out).reshape(n, 8, hd), want[0])
+
+
 def test_attention_graph_follows_positions(gpu):
     """A captured append + attention is replayed as the sequences grow, the positions changed in place."""
     rng = np.random.RandomState(11)
