@@ -216,8 +216,8 @@ __global__ void __launch_bounds__(KV4_APPEND_WARPS * 32, 3) dz_kv4_append_kernel
     }
     if (row >= all_rows) return;
     const int b = row / a.n_tokens;
-    if (a.positions[b] < 0) return;
     const long long first = a.positions[b] + a.pos_add;
+    if (kv4_skips(first)) return;
     // the lane's place in the angle table
     const int stride = a.halves ? HD / 2 / E : LPH, place = a.halves ? at % (HD / 2) / E : at / E;
 
@@ -362,8 +362,8 @@ static int kv4_check(const dz_kv4_t* c, const int64_t* positions, size_t n_token
         return fail(DZ_E_UNSUPPORTED, "kv4: head dimension %zu (64 and 128 are supported)", c->head_dim);
     if (c->batch == 0 || c->batch > 65535 || c->kv_heads == 0 || c->kv_heads > 65535)
         return fail(DZ_E_INVALID, "kv4: batch and kv_heads must be 1..65535");
-    if (c->capacity == 0 || c->capacity > INT32_MAX || c->sinks >= c->capacity)
-        return fail(DZ_E_INVALID, "kv4: capacity must be 1..2^31-1 and sinks below it");
+    if (c->capacity == 0 || c->capacity > (size_t)KV4_CAPACITY || c->sinks >= c->capacity)
+        return fail(DZ_E_INVALID, "kv4: capacity must be 1..2^31-64 and sinks below it");
     if (n_tokens == 0 || n_tokens > c->capacity - c->sinks)
         return fail(DZ_E_INVALID, "kv4: n_tokens must be 1..capacity - sinks (%zu)", c->capacity - c->sinks);
     if ((((uintptr_t)c->k_codes | (uintptr_t)c->v_codes) & 15) || (((uintptr_t)c->k_scales | (uintptr_t)c->v_scales) & 7) ||

@@ -7,6 +7,8 @@
 namespace dz {
 
 constexpr int KV4_GROUP = 64;   // elements of a row that share a scale
+// Slots of a ring at most: attention counts them in 32 bits, up to two tiles past the end.
+constexpr long long KV4_CAPACITY = INT32_MAX - 63;
 
 struct Kv4Cache {
     uint8_t *k_codes, *v_codes;
@@ -22,6 +24,10 @@ __device__ __forceinline__ long long kv4_slot(long long p, long long sinks, long
     if (((r | ring) >> 32) == 0) return sinks + (long long)((uint32_t)r % (uint32_t)ring);
     return sinks + r % ring;
 }
+
+// Whether a sequence is left out: its position is negative, or one whose slot
+// arithmetic could leave 64 bits.
+__device__ __forceinline__ bool kv4_skips(long long position) { return position < 0 || position >> 62; }
 
 struct Kv4AppendArgs {
     Kv4Cache c;

@@ -120,8 +120,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     const int pb = unit % pair_blocks;
     unit /= pair_blocks;
     const int hk = unit % a.c.kv_heads, b = unit / a.c.kv_heads;
-    if (a.positions[b] < 0) return;          // the whole team, or cluster, leaves
     const long long first = a.positions[b] + a.pos_add;
+    if (kv4_skips(first)) return;   // the whole team, or cluster, leaves
     const int share = a.q_heads / a.c.kv_heads, pairs = share * a.n_tokens, pair0 = pb * PAIRS;
 
     // ---- the virtual index v = 0..count-1 runs over the sinks, then over positions lo, lo + 1, ...

@@ -123,8 +123,8 @@ __global__ void __launch_bounds__(KC_WARPS * 32, QP == 1 || HD == 64 ? 2 : 1) dz
     const int pb = unit % pair_blocks;
     unit /= pair_blocks;
     const int hk = unit % a.c.kv_heads, b = unit / a.c.kv_heads;
-    if (a.positions[b] < 0) return;          // the whole team, or cluster, leaves
     const long long first = a.positions[b] + a.pos_add;
+    if (kv4_skips(first)) return;   // the whole team, or cluster, leaves
     const int share = a.q_heads / a.c.kv_heads, pairs = share * a.n_tokens, pair0 = pb * KC_ROWS;
 
     // ---- the virtual index v = 0..count-1 runs over the sinks, then over positions lo, lo + 1, ...

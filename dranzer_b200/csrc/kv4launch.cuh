@@ -13,8 +13,8 @@ constexpr int KV4_CLUSTER = 16;   // blocks of a cluster at most
 constexpr int KV4_DEVICES = 64;   // devices whose launch state is kept
 
 // Clusters of 1..16 blocks of a kernel that a device holds at once (a cluster
-// stays within one GPC, so that larger ones leave SMs idle). Asked once per
-// kernel and device.
+// stays within one GPC, so that larger ones leave SMs idle; 0: it cannot hold
+// one). Asked once per kernel and device.
 struct Kv4Room {
     std::atomic<bool> known{false};
     std::atomic<int> clusters[KV4_CLUSTER + 1];
@@ -31,6 +31,7 @@ inline void kv4_shape(const Kv4Room& room, long long units, long long longest, i
     auto consider = [&](int w, int c) {
         const long long warps = (long long)w * c;
         const long long slots = (long long)room.clusters[c].load(std::memory_order_relaxed) * (KV4_WARPS / w);
+        if (slots <= 0) return;
         const double waves = (double)((units + slots - 1) / slots), each = (double)((tiles + warps - 1) / warps);
         const double t = waves * (each + 4.0 + (warps > 1 ? 3.0 : 0.0) + (c > 1 ? 3.0 : 0.0));
         if (t < best) {
@@ -69,7 +70,7 @@ cudaError_t kv4_launch(Kernel* kernel, Kv4Room (&rooms)[KV4_DEVICES], const Kv4A
             attr[0].val.clusterDim.x = c;
             int n = 0;
             e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
-            room.clusters[c].store(n > 0 ? n : 1, std::memory_order_relaxed);
+            room.clusters[c].store(n, std::memory_order_relaxed);
         }
         if (e != cudaSuccess) return e;
         room.known.store(true, std::memory_order_release);

@@ -124,8 +124,8 @@ int dz_cuda_matmul_grouped(const float *A, const dz_cuda_gmatrix_t *weights, flo
 /* ---- 4-bit ring caches (dz_kv4_t), on device buffers, enqueued on `stream`
  * without synchronisation; nothing is allocated. positions[batch] (device,
  * int64): the position of each sequence's first new token; a sequence with a
- * negative position is skipped and its rows are left as they were. Calls that
- * write a cache and calls that use it are ordered by the caller (one stream,
+ * negative position, or one of 2^62 or more, is skipped and its rows are left
+ * as they were. Calls that write a cache and calls that use it are ordered by the caller (one stream,
  * or events). No counterpart in the reference, whose caches are fp32. */
 
 /* For n_tokens new tokens of every sequence: queries and keys normed per head

@@ -96,7 +96,7 @@ typedef struct {
  * value = scale * (code - 7). head_dim is 64 or 128. Position p of a sequence
  * lives in slot p while p < sinks (the first tokens, which stay), else in slot
  * sinks + (p - sinks) % (capacity - sinks): the newest capacity - sinks later
- * positions are retained. sinks < capacity. Code buffers start on 16-byte
+ * positions are retained. sinks < capacity <= 2^31 - 64. Code buffers start on 16-byte
  * boundaries, scale buffers on 8-byte ones; k and v buffers do not overlap. */
 typedef struct {
     int device;

@@ -141,6 +141,16 @@ def test_kv4_attention_refuses(dz, change):
     assert st == INVALID and _native.last_error()[1]
 
 
+def test_kv4_refuses_capacities_past_32_bit_counts(dz):
+    """The kernels count slots in 32 bits up to two tiles of 32 past the last."""
+    from dranzer_b200 import _native
+    L = _native.lib()
+    for capacity in ((1 << 31) - 1, (1 << 31) - 63):
+        c = _cache(capacity=capacity)
+        assert L.dz_cuda_kv4_append(ctypes.byref(c), ctypes.byref(_append()), 4096, 1, None) == INVALID
+        assert L.dz_cuda_kv4_attention(ctypes.byref(c), ctypes.byref(_attention()), 4096, 1, None) == INVALID
+
+
 def test_kv4_refuses_token_counts(dz):
     from dranzer_b200 import _native
     L = _native.lib()

@@ -664,6 +664,26 @@ def test_chunk_offsets_past_32_bits(gpu):
     np.testing.assert_array_equal(_np(out).reshape(n, 8, hd), want[0])
 
 
+@pytest.mark.parametrize("n", [1, 9])
+def test_positions_that_are_skipped(gpu, n):
+    """Negative positions and those of 2^62 and more: neither the cache nor any output row is touched."""
+    skipped = [-1, -(1 << 63), 1 << 62, (1 << 63) - 1, (1 << 62) + 12345]
+    ring = Ring(gpu, len(skipped), 2, 64, 40, 3, np.random.RandomState(5))
+    pos = torch.tensor(skipped, dtype=torch.int64, device="cuda")
+    rows = len(skipped) * n
+    x = torch.ones(rows, 4 * 64, device="cuda")
+    out = [torch.full((rows, 4 * 64), 9.0, device="cuda") for _ in range(2)]
+    ring.cache.append(pos.data_ptr(), n, q_heads=4, q=x.data_ptr(), k=x.data_ptr(), v=x.data_ptr(), q_stride=256,
+                      k_stride=256, v_stride=256, q_out=out[0].data_ptr(), rope_base=1e4, stream_ptr=_stream())
+    ring.cache.attention(pos.data_ptr(), n, q_heads=4, q=x.data_ptr(), out=out[1].data_ptr(), window=20,
+                         stream_ptr=_stream())
+    torch.cuda.synchronize()
+    assert all((t == 9.0).all() for t in out)
+    for old, new in zip(ring.before, ring.snapshot()):
+        np.testing.assert_array_equal(old[0], new[0])
+        np.testing.assert_array_equal(old[1], new[1])
+
+
 def test_attention_graph_follows_positions(gpu):
     """A captured append + attention is replayed as the sequences grow, the positions changed in place."""
     rng = np.random.RandomState(11)
