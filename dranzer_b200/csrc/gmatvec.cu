@@ -5,6 +5,7 @@
 #include <atomic>
 #include <cmath>
 #include <new>
+#include <type_traits>
 
 #include "gmatvec.cuh"
 #include "shim.cuh"
@@ -75,21 +76,28 @@ template <typename S> __global__ void dz_gmv_dequant_kernel(GmvMatrix w, float* 
 
 // ------------------------------------------------------------------ product
 //
-// Integer formulation. Each 128 consecutive activations of a row (one block of
-// the layout) are scaled by a power of two, rounded to integers X and cut into
-// ND balanced base-256 digits (X = 65536 top + 256 mid + low for ND = 3).
-// Digits and levels meet in the 8-bit integer MMA, whose sums over one scale
-// group are exact (16 x 7 x 128 x 128 < 2^22); B column ND m + d is digit d of
-// row m. An accumulator starts at the bits of 1.5 x 2^23, whose step is 1, so
-// that its bits read as a float are 1.5 x 2^23 plus the sum: one subtraction
-// converts it. Group sums times scale and times the power of two add up in
-// fp32. fp32 activations take three digits, the largest of a block in [2^22,
-// 2^23): 2^-23 of it at most is lost. fp16 and bf16 ones take two, the largest
-// in [2^14, 2^15): about 2^-15 of it at most is lost, a sixteenth of fp16's own
-// rounding of that element; two digits make a third fewer MMAs and bytes.
+// Every activation keeps its own precision, whatever stands beside it, in one of
+// two forms; sums are fp32 from a scale group on.
+//
+// Several rows: the 16-bit MMA (m16n8k16) with fp32 sums, whose products are
+// exact. Levels -7..7 are exact in fp16 and bf16, fp16 and bf16 activations enter
+// as they are, and an fp32 one as three bf16 parts of eight bits each, a column
+// of B each (P m + p is part p of row m). Widening costs most of the
+// instructions: a nibble xor-ed into the low mantissa bits of 1032 (fp16; the next
+// nibble too, as 16 times it) or of 136 / 1024 (bf16, whose step there is 1 / 1024)
+// adds it, one subtraction (or fma) leaves the level.
+//
+// One row: the 8-bit integer MMA (m16n8k32), which takes a quarter of that
+// widening. The block's 128 activations are scaled by a power of two that puts
+// the largest in [2^21, 2^22) and cut into 8 balanced base-256 digits, one for
+// each column of B: three of the integer part, three of the next 23 bits, two
+// of the next 15. What lies 2^-60 below the largest is lost. Digit sums over a
+// scale group are exact (16 x 7 x 128 x 128 < 2^22): an accumulator starts at the
+// bits of 1.5 x 2^23, whose step is 1, so that its bits read as a float are
+// 1.5 x 2^23 plus the sum. Times scale and digit weight they add up in fp32.
 //
 // Work. A cluster of 1 to 8 blocks takes a contiguous range of tiles; its
-// blocks take a share of the rows of W each (so that each converts only its
+// blocks take a share of the rows of W each (so that each stages only its
 // share of the activations), and a block's eight warps equal contiguous
 // ranges of its (tile, block) records, whatever tile borders lie inside. A
 // warp streams its records through its own ring of cp.async stages and meets
@@ -97,10 +105,13 @@ template <typename S> __global__ void dz_gmv_dequant_kernel(GmvMatrix w, float* 
 // sum in the tile's place, a warp that continues a tile keeps it in its own.
 // Then the parts add up in a fixed order, over warps, then over the cluster.
 //
-// Bound by HBM for large matrices: 1 x 4096 x 32000 (fp16 scales) 13.9 us per
-// call, 4.9 TB/s; by the latency of its phases for small ones: 1 x 2048 x 2048
-// 3.2 us, 8 x 2048 x 8192 (bf16) 7.7 us, 16 x 4099 x 5003 (fp16, groups of 32)
-// 16.2 us. The one-thread-per-column form took 157 us for the first; a barrier
+// On one B200, per call: 1 x 4096 x 32000 (fp32, fp16 scales) 14.5 us, 4.7 TB/s, bound by
+// HBM while records stream; 1 x 2048 x 2048 3.4 us, the latency of its phases; 8 x
+// 2048 x 8192 (bf16) 6.0 us and 16 x 4099 x 5003 (fp16, groups of 32) 12.8 us, staging
+// and widening. One row through the 16-bit MMA took 17.1 us for the first. With
+// digits for all rows (three of fp32, two of 16 bits, against a block's largest
+// element) they took 14.0, 3.2, 7.7 and 16.4 us, and lost the small elements beside
+// large ones. The one-thread-per-column form took 157 us for the first; a barrier
 // per tile 20 us; a cluster barrier per tile 29 us.
 
 constexpr int GMV_DEVICES = 64;         // devices whose launch state is kept
@@ -109,10 +120,13 @@ constexpr int GMV_SMEM2 = 113 * 1024 - 128;// and if two are to fit an SM
 constexpr int GMV_WARPS = 8;
 constexpr int GMV_STAGES = 4;
 constexpr int GMV_MAX_ROWS = 16;        // rows of one pass
+constexpr int GMV_DIGITS = 8;           // of an activation of a single row
 constexpr int GMV_ZERO = 0x4B400000;    // 1.5 x 2^23
+constexpr float GMV_ZEROF = 12582912.0f;
 
 struct GmvPlan {
     int rows;         // rows of this launch
+    int digits;       // whether its one row goes as digits
     int cluster;      // blocks that share a tile
     int clusters;     // clusters of the grid
     int slice;        // records of a tile that a block has, at most
@@ -124,6 +138,67 @@ __device__ __forceinline__ void gmv_mma(int (&d)[4], uint32_t a0, uint32_t a1, u
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
 }
+__device__ __forceinline__ void gmv_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void gmv_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// (w & mask) ^ base in one instruction: both constants stay in registers.
+__device__ __forceinline__ uint32_t gmv_mask_xor(uint32_t w, uint32_t mask, uint32_t base) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(y) : "r"(w), "r"(mask), "r"(base));
+    return y;
+}
+
+// Levels of a word's rows 0, 2 (first) and 1, 3 (second) for i = 0, of rows 4, 6
+// and 5, 7 for i = 1, as pairs of the MMA's type. A nibble is the level's two's
+// complement: its top bit flipped, it is the level + 8.
+__device__ __forceinline__ uint32_t gmv_level_low(uint32_t w) {
+    const uint32_t x = gmv_mask_xor(w, 0x000F000Fu, 0x64086408u);
+    const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6408)));   // 1032
+    return *reinterpret_cast<const uint32_t*>(&a);
+}
+__device__ __forceinline__ uint32_t gmv_level_high(uint32_t w) {
+    const uint32_t x = gmv_mask_xor(w, 0x00F000F0u, 0x64806480u);
+    const __half2 a = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x2C00)),    // 1/16
+                              __half2half2(__ushort_as_half(0xD480)));                                          // -72
+    return *reinterpret_cast<const uint32_t*>(&a);
+}
+__device__ __forceinline__ uint32_t gmv_level_bf16(uint32_t w) {   // level / 1024
+    const uint32_t x = gmv_mask_xor(w, 0x000F000Fu, 0x3E083E08u);
+    const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x),
+                                     __bfloat162bfloat162(__ushort_as_bfloat16(0x3E08)));                  // 136 / 1024
+    return *reinterpret_cast<const uint32_t*>(&a);
+}
+__device__ __forceinline__ void gmv_levels(uint32_t w, int i, uint32_t& first, uint32_t& second, __half) {
+    first = i ? gmv_level_low(w) : gmv_level_high(w);
+    second = i ? gmv_level_low(w >> 8) : gmv_level_high(w >> 8);
+}
+__device__ __forceinline__ void gmv_levels(uint32_t w, int i, uint32_t& first, uint32_t& second, __nv_bfloat16) {
+    first = gmv_level_bf16(i ? w : w >> 4);
+    second = gmv_level_bf16(i ? w >> 8 : w >> 12);
+}
+
+// What an activation type takes in the MMA, and in how many columns of a row.
+// UNIT: what a result's sums are counted in. bf16 levels are a 1024th, so that a
+// group's sum (at most 7 x 128 of its largest activation) stays in fp32's range
+// before its scale takes it back.
+template <typename T> struct GmvType {
+    using Mma = T;
+    static constexpr int PARTS = 1;
+    static constexpr float UNIT = std::is_same<T, __half>::value ? 1.0f : 1024.0f;
+};
+template <> struct GmvType<float> {
+    using Mma = __nv_bfloat16;
+    static constexpr int PARTS = 3;
+    static constexpr float UNIT = 1024.0f;
+};
 
 // E consecutive activations (16 bytes: 4 fp32 or 8 of 16 bits) from element k
 // of a row of K, zero past the end. wide: rows start on 16-byte boundaries.
@@ -138,7 +213,6 @@ template <int E> __device__ __forceinline__ uint4 gmv_load(const void* x, long l
         q.w = k + 3 < K ? p[3] : 0u;
         return q;
     }
-    // (aligned 16-byte loads around the 16 bytes and a shift: more code, 0.2 to 1.5 us more per call)
     const uint16_t* p = static_cast<const uint16_t*>(x) + row + k;
     if (wide && k + E <= K) return *reinterpret_cast<const uint4*>(p);
     uint32_t h[8];
@@ -151,10 +225,67 @@ template <int E> __device__ __forceinline__ uint4 gmv_load(const void* x, long l
     return q;
 }
 
-__device__ __forceinline__ void gmv_store(void* y, int type, long long at, float v) {
-    if (type == DZ_TYPE_F32) static_cast<float*>(y)[at] = v;
-    else if (type == DZ_TYPE_F16) static_cast<__half*>(y)[at] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
+// Stages 16 bytes of a row's activations in its columns, `stride` bytes apart,
+// eight elements in the order 0 2 1 3 4 6 5 7 of gmv_levels. x + 0 x turns an
+// infinity into a NaN, so that the whole row reads NaN also where its level is
+// not 0 (as fp32's parts do: infinity less infinity).
+template <typename T2> __device__ __forceinline__ void gmv_stage16(uint8_t* to, const uint4& q, T2 zero) {
+    uint32_t w[4] = {__byte_perm(q.x, q.y, 0x5410), __byte_perm(q.x, q.y, 0x7632), __byte_perm(q.z, q.w, 0x5410),
+                     __byte_perm(q.z, q.w, 0x7632)};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const T2 v = *reinterpret_cast<const T2*>(&w[i]), r = __hfma2(v, zero, v);
+        w[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void gmv_stage(uint8_t* to, int, const uint4& q, __half) {
+    gmv_stage16(to, q, __half2half2(__ushort_as_half(0)));
+}
+__device__ __forceinline__ void gmv_stage(uint8_t* to, int, const uint4& q, __nv_bfloat16) {
+    gmv_stage16(to, q, __bfloat162bfloat162(__ushort_as_bfloat16(0)));
+}
+// An fp32 value is the sum of the upper halves of x, of what is left of it and of
+// what is left then: eight of its 24 bits each, without a rounding (but for bits
+// below 2^-133).
+__device__ __forceinline__ void gmv_stage(uint8_t* to, int stride, const uint4& q, float) {
+    float r[4] = {__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z), __uint_as_float(q.w)};
+#pragma unroll
+    for (int p = 0; p < 3; p++) {
+        uint2 w;
+        w.x = __byte_perm(__float_as_uint(r[0]), __float_as_uint(r[2]), 0x7632);
+        w.y = __byte_perm(__float_as_uint(r[1]), __float_as_uint(r[3]), 0x7632);
+        *reinterpret_cast<uint2*>(to + p * stride) = w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) r[i] -= __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
+    }
+}
+
+// Digits of four consecutive activations, `stride` bytes apart; f is the block's power of two.
+__device__ __forceinline__ void gmv_stage_digits(uint8_t* to, int stride, const float (&v)[4], float f) {
+    uint32_t y[3][4];         // an integer's digits in its low bytes, those below the top one + 128
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float a = fmaf(v[i], f, GMV_ZEROF), r = fmaf(v[i], f, GMV_ZEROF - a);
+        const float b = fmaf(r, 8388608.0f, GMV_ZEROF), u = fmaf(r, 8388608.0f, GMV_ZEROF - b);
+        const float c = fmaf(u, 32768.0f, GMV_ZEROF);
+        // 0x40 of byte 2 belongs to 1.5 x 2^23: 0xC0 more takes it out
+        y[0][i] = __float_as_uint(a) + 0x00C08080u;
+        y[1][i] = __float_as_uint(b) + 0x00C08080u;
+        y[2][i] = __float_as_uint(c) + 0x80u;
+    }
+#pragma unroll
+    for (int d = 0; d < GMV_DIGITS; d++) {
+        const uint32_t(&z)[4] = y[d / 3], sel = (uint32_t)(d % 3) | (uint32_t)(4 + d % 3) << 4;
+        const uint32_t flip = d % 3 == 2 || d == 7 ? 0u : 0x80808080u;
+        *reinterpret_cast<uint32_t*>(to + d * stride) =
+            __byte_perm(__byte_perm(z[0], z[1], sel), __byte_perm(z[2], z[3], sel), 0x5410) ^ flip;
+    }
+}
+// What digit d counts in units of the block's power: 2^-4 for the levels' factor 16 taken back.
+__device__ __forceinline__ float gmv_digit_weight(int d) {
+    const int e = d < 3 ? 8 * d - 4 : d < 6 ? 8 * (d - 3) - 27 : 8 * (d - 6) - 42;
+    return __int_as_float((127 + e) << 23);
 }
 
 // Where share i of n things among `of` begins: shares differ by at most one.
@@ -163,34 +294,43 @@ __device__ __forceinline__ int gmv_share(unsigned n, unsigned i, unsigned of) {
     return (int)(q * i + r * i / of);
 }
 
-// Shared memory: the rings (over them, at a tile's end, nothing), the digit
-// columns, the digits' weights, a warp's tile in accumulator order, the parts.
-template <int ND, int NT> struct GmvSmem {
-    static constexpr int LD = 8 * NT + 1;                    // floats between the columns of W in a warp's tile
+// Shared memory: the rings, the columns of activations (or digits and their
+// weights), a warp's tile in accumulator order, the parts.
+template <int P, int NT> struct GmvSmem {   // NT 0: one row as digits
+    static constexpr int TILES = NT ? NT : 1;
+    static constexpr int LD = 8 * TILES + 1;                 // floats between the columns of W in a warp's tile
     static constexpr int TILE = (GMV_TILE * LD + 3) / 4 * 4;
     static __host__ __device__ int ring(int rec) { return GMV_WARPS * GMV_STAGES * rec; }
-    static __host__ __device__ int stride(int slice) { return slice * GMV_BLOCK + 32; }   // bytes between digit columns
-    static __host__ __device__ int digits(int rows, int slice) { return ND * rows * stride(slice); }
+    // bytes between columns: what neighbours read of a piece (64 bytes, 32 of digits) falls into different banks
+    static __host__ __device__ int stride(int slice) { return NT ? slice * GMV_BLOCK * 2 + 64 : slice * GMV_BLOCK + 32; }
+    static __host__ __device__ int columns(int rows, int slice) {
+        return NT ? P * rows * stride(slice) : GMV_DIGITS * stride(slice) + slice * GMV_DIGITS * 4;
+    }
     static __host__ __device__ int total(int rec, const GmvPlan& p) {
-        return ring(rec) + digits(p.rows, p.slice) + p.slice * 8 * NT * 4 + GMV_WARPS * TILE * 4 +
-               (p.tiles + GMV_WARPS) * GMV_TILE * p.rows * 4;
+        return ring(rec) + columns(p.rows, p.slice) + GMV_WARPS * TILE * 4 + (p.tiles + GMV_WARPS) * GMV_TILE * p.rows * 4;
     }
 };
 
-template <int GPB, typename S, int ND, int NT>   // scale groups of a block, scale type, digits, column tiles of 8
-__global__ void __launch_bounds__(GMV_WARPS * 32, NT < 3 || (NT == 3 && GPB < 4) ? 2 : 1) dz_gmv_kernel(const __grid_constant__ GmvArgs a,
-                                                                                const __grid_constant__ GmvPlan plan) {
-    using L = GmvSmem<ND, NT>;
+// Blocks of an instantiation that an SM is to hold: its registers would not let
+// more tiles or groups share it without spills.
+constexpr int gmv_blocks(int nt, int gpb) { return nt < 3 || (nt == 3 && gpb == 1) ? 2 : 1; }
+
+template <int GPB, typename S, typename T, int NT>   // scale groups of a block, scale and activation type, column tiles of 8
+__global__ void __launch_bounds__(GMV_WARPS * 32, gmv_blocks(NT, GPB)) dz_gmv_kernel(
+    const __grid_constant__ GmvArgs a, const __grid_constant__ GmvPlan plan) {
+    using Mma = typename GmvType<T>::Mma;
+    constexpr int P = GmvType<T>::PARTS, E = 16 / (int)sizeof(T), COLS = NT ? NT : 1;
+    using L = GmvSmem<P, NT>;
     constexpr int REC = GMV_CODES + GPB * GMV_TILE * (int)sizeof(S), CHUNKS = REC / 16;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int head_tile[GMV_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % plan.cluster, who = blockIdx.x / plan.cluster;
     const int M = plan.rows, stride = L::stride(plan.slice);
-    uint8_t* digits = smem + L::ring(REC);
-    float* fx = reinterpret_cast<float*>(digits + L::digits(M, plan.slice));   // [record of the slice][8 NT]
-    float* mine = fx + plan.slice * 8 * NT + warp * L::TILE;
-    float* parts = fx + plan.slice * 8 * NT + GMV_WARPS * L::TILE;             // [tile][M][32]
+    uint8_t* columns = smem + L::ring(REC);
+    float* fx = reinterpret_cast<float*>(columns + GMV_DIGITS * stride);       // digits' weights [record of the slice][digit]
+    float* mine = reinterpret_cast<float*>(columns + L::columns(M, plan.slice)) + warp * L::TILE;
+    float* parts = mine + (GMV_WARPS - warp) * L::TILE;                        // [tile][M][32]
     float* heads = parts + plan.tiles * GMV_TILE * M;                          // [warp][M][32]
 
     // (32-bit divisions only: a 64-bit one costs some hundred cycles before the first load)
@@ -234,106 +374,90 @@ __global__ void __launch_bounds__(GMV_WARPS * 32, NT < 3 || (NT == 3 && GPB < 4)
     // when calls are issued one by one about as fast as they run.)
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- activations to digits. A unit is one row's share of one block, 128
-    // elements: 16 bytes a lane, so a warp takes one (fp32) or two (16 bits) at
-    // a time; four such loads go out ahead of the rest of the ring (behind it
-    // they would wait for the weights) and four more while the last are worked on
-    {
-        constexpr int E = ND == 3 ? 4 : 8, UNITS = E / 4, AHEAD = 4;
-        const bool wide = (((uintptr_t)a.x | (uintptr_t)(a.ldx * (16 / E))) & 15) == 0;
-        const int le = UNITS == 1 ? lane : lane & 15;
-        int m = 0, kx = warp * UNITS + (UNITS == 1 ? 0 : lane >> 4);   // this lane's units: every 8 UNITS-th of M x nb
-        while (kx >= nb) { kx -= nb; m++; }
-        uint4 raw[2][AHEAD];
-        int um[2][AHEAD], uk[2][AHEAD];
-        auto fetch = [&](uint4 (&r)[AHEAD], int (&rm)[AHEAD], int (&rk)[AHEAD]) {
+    // ---- activations to columns, 16 bytes at a time; the first four loads of a
+    // thread go out ahead of the rest of the ring (behind it they would wait for
+    // the weights), four more while the last are worked on
+    constexpr int AHEAD = 4, THREADS = GMV_WARPS * 32, PER = GMV_BLOCK / E;   // chunks of a block
+    const bool wide = (((uintptr_t)a.x | (uintptr_t)(a.ldx * (int)sizeof(T))) & 15) == 0;
+    const int per = nb * PER;                          // of a row
+    int m = 0, c = threadIdx.x;
+    while (c >= per) { c -= per; m++; }
+    uint4 raw[2][AHEAD];
+    int at[2][AHEAD];                                  // row and chunk; -1: none
+    auto fetch = [&](uint4 (&r)[AHEAD], int (&to)[AHEAD]) {
 #pragma unroll
-            for (int u = 0; u < AHEAD; u++) {
-                rm[u] = m;
-                rk[u] = kx;
-                r[u] = make_uint4(0, 0, 0, 0);
-                if (m < M) {
-                    r[u] = gmv_load<E>(a.x, (long long)m * a.ldx, (kb0 + kx) * GMV_BLOCK + E * le, a.w.K, wide);
-                    kx += GMV_WARPS * UNITS;
-                    while (kx >= nb) { kx -= nb; m++; }
-                }
+        for (int u = 0; u < AHEAD; u++) {
+            to[u] = -1;
+            if (m < M) {
+                to[u] = NT ? P * m * stride + c * E * 2 : c;
+                r[u] = gmv_load<E>(a.x, (long long)m * a.ldx, kb0 * GMV_BLOCK + c * E, a.w.K, wide);
+                c += THREADS;
+                while (c >= per) { c -= per; m++; }
             }
-        };
-        auto work = [&](const uint4 (&r)[AHEAD], const int (&rm)[AHEAD], const int (&rk)[AHEAD]) {
+        }
+    };
+    auto work = [&](const uint4 (&r)[AHEAD], const int (&to)[AHEAD]) {
+        if constexpr (NT > 0) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++)
+                if (to[u] >= 0) gmv_stage(columns + to[u], stride, r[u], T());
+        } else {
+            // a block's chunks lie in neighbouring lanes of one warp, all of them there or none
             unsigned top[AHEAD];             // bits of the largest magnitude: above 0x7f7fffff it is not finite
             float v[AHEAD][E];
 #pragma unroll
             for (int u = 0; u < AHEAD; u++) {
                 const uint32_t q[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
-                const bool f16 = a.type == DZ_TYPE_F16;
                 top[u] = 0;
-                if (E == 8) {                // the largest magnitudes of the low and high halves, then of both
-#pragma unroll
-                    for (int j = 0; j < 4; j++) top[u] = __vmaxu2(top[u], q[j] & 0x7fff7fffu);
-                    top[u] = max(top[u] & 0xffffu, top[u] >> 16);
-                    top[u] = f16 ? __float_as_uint(__half2float(__ushort_as_half((unsigned short)top[u]))) : top[u] << 16;
-                }
 #pragma unroll
                 for (int j = 0; j < E; j++) {
-                    if (E == 4) v[u][j] = __uint_as_float(q[j]);
-                    else if (f16) v[u][j] = __half2float(__ushort_as_half((unsigned short)(q[j / 2] >> 16 * (j & 1))));
-                    else v[u][j] = __uint_as_float(j & 1 ? q[j / 2] & 0xffff0000u : q[j / 2] << 16);
-                    if (E == 4) top[u] = max(top[u], __float_as_uint(v[u][j]) & 0x7fffffffu);
+                    if (E == 4) v[u][j] = __uint_as_float(q[j % 4]);
+                    else if (std::is_same<T, __half>::value)
+                        v[u][j] = __half2float(__ushort_as_half((unsigned short)(q[j / 2 % 4] >> 16 * (j & 1))));
+                    else v[u][j] = __uint_as_float(j & 1 ? q[j / 2 % 4] & 0xffff0000u : q[j / 2 % 4] << 16);
+                    top[u] = max(top[u], __float_as_uint(v[u][j]) & 0x7fffffffu);
                 }
-                top[u] = __reduce_max_sync(UNITS == 1 ? 0xffffffffu : lane < 16 ? 0xffffu : 0xffff0000u, top[u]);
+                if (to[u] < 0) top[u] = 0;
+                top[u] = __reduce_max_sync(PER == 32 ? 0xffffffffu : lane < 16 ? 0xffffu : 0xffff0000u, top[u]);
             }
 #pragma unroll
             for (int u = 0; u < AHEAD; u++) {
-                // the power stays a normal float: a block below 2^-104 keeps fewer bits
-                constexpr int BITS = ND == 3 ? 22 : 14;
-                constexpr float LIMIT = ND == 3 ? 8355711.0f : 32639.0f;   // the top digit must stay below 128
-                int s = min(127 + BITS - (int)(top[u] >> 23), 126);
-                if (__uint_as_float(top[u]) * __int_as_float((127 + s) << 23) > LIMIT) s--;
+                if (to[u] < 0) continue;
+                // the power stays a normal float: of a block below 2^-105 bits under 2^-164 are lost
+                const int s = min(127 + 21 - (int)(top[u] >> 23), 126);
                 const float f = __int_as_float((127 + s) << 23);
-                // X + 0x8080 (0x80): its bytes less 128 are the lower digits, its last byte the top one. Of two
-                // digits, X rounds where 1.5 x 2^23 is added (a conversion each instead: 8.0 against 7.7 us for 8 x 2048 x 8192)
-                uint32_t y[E];
 #pragma unroll
-                for (int j = 0; j < E; j++)
-                    y[j] = ND == 3 ? (uint32_t)(__float2int_rn(v[u][j] * f) + 0x8080)
-                                   : __float_as_uint(fmaf(v[u][j], f, 12582912.0f + 128.0f));
-                if (rm[u] >= M) continue;
-                uint8_t* to = digits + ND * rm[u] * stride + rk[u] * GMV_BLOCK + E * le;
-#pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const uint32_t sel = (uint32_t)d | (uint32_t)(4 + d) << 4, flip = d < ND - 1 ? 0x80808080u : 0u;
-#pragma unroll
-                    for (int j = 0; j < E; j += 4)
-                        *reinterpret_cast<uint32_t*>(to + d * stride + j) =
-                            __byte_perm(__byte_perm(y[j], y[j + 1], sel), __byte_perm(y[j + 2], y[j + 3], sel), 0x5410) ^ flip;
+                for (int j = 0; j < E; j += 4) {
+                    const float z[4] = {v[u][j], v[u][j + 1], v[u][j + 2], v[u][j + 3]};
+                    gmv_stage_digits(columns + to[u] * E + j, stride, z, f);
                 }
-                if (le < ND) {   // the digit's weight, the levels' factor 16 taken back
-                    const float back = __int_as_float((127 - s) << 23) * (le == 0 ? 0.0625f : le == 1 ? 16.0f : 4096.0f);
-                    fx[rk[u] * 8 * NT + ND * rm[u] + le] = top[u] > 0x7f7fffffu ? __int_as_float(0x7fc00000) : back;
-                }
+                const int d = to[u] % PER;
+                if (d < GMV_DIGITS)
+                    fx[to[u] / PER * GMV_DIGITS + d] = top[u] > 0x7f7fffffu ? __int_as_float(0x7fc00000)
+                                                                           : __int_as_float((127 - s) << 23) * gmv_digit_weight(d);
             }
-        };
-        fetch(raw[0], um[0], uk[0]);
-#pragma unroll
-        for (int i = 0; i < GMV_STAGES - 2; i++) produce();
-        // both lane halves go round until neither has a unit left
-        while (__any_sync(0xffffffffu, um[0][0] < M)) {
-            fetch(raw[1], um[1], uk[1]);
-            work(raw[0], um[0], uk[0]);
-            if (!__any_sync(0xffffffffu, um[1][0] < M)) break;
-            fetch(raw[0], um[0], uk[0]);
-            work(raw[1], um[1], uk[1]);
         }
+    };
+    fetch(raw[0], at[0]);
+#pragma unroll
+    for (int i = 0; i < GMV_STAGES - 2; i++) produce();
+    while (__any_sync(0xffffffffu, at[0][0] >= 0)) {
+        fetch(raw[1], at[1]);
+        work(raw[0], at[0]);
+        if (!__any_sync(0xffffffffu, at[1][0] >= 0)) break;
+        fetch(raw[0], at[0]);
+        work(raw[1], at[1]);
     }
     __syncthreads();
 
     // ---- records
-    const uint8_t* col[NT];   // this lane's digit columns (columns past ND M read the last one; nobody reads their sums)
+    const uint8_t* col[COLS]; // this lane's columns (those past P M read the last one; nobody reads their sums)
 #pragma unroll
-    for (int n = 0; n < NT; n++) col[n] = digits + min(n * 8 + g, ND * M - 1) * stride + 8 * t;
-    float out[NT][8];         // columns g, g + 8 (0..3), g + 16, g + 24 (4..7) of W by columns 2t, 2t + 1 of B
+    for (int n = 0; n < COLS; n++)
+        col[n] = NT ? columns + min(n * 8 + g, P * M - 1) * stride + 16 * t : columns + g * stride + 8 * t;
+    float out[COLS][8];       // columns g, g + 8 (0..3), g + 16, g + 24 (4..7) of W by columns 2t, 2t + 1 of B
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+    for (int n = 0; n < COLS; n++)
 #pragma unroll
         for (int r = 0; r < 8; r++) out[n][r] = 0.0f;
     bool head = kb != 0 && r0 < r1;   // the first tile is another warp's to begin
@@ -346,48 +470,72 @@ __global__ void __launch_bounds__(GMV_WARPS * 32, NT < 3 || (NT == 3 && GPB < 4)
         const uint8_t* st = my + cstage * REC;
         cstage = cstage + 1 == GMV_STAGES ? 0 : cstage + 1;
         const S* scale = reinterpret_cast<const S*>(st + GMV_CODES) + g;
-        float part[NT][8];
+        float part[8];
 #pragma unroll
         for (int gi = 0; gi < GPB; gi++) {
-            int acc[NT][2][4];
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int q = 0; q < 8; q++) acc[n][q >> 2][q & 3] = GMV_ZERO;
-#pragma unroll
-            for (int k = gi * (4 / GPB); k < (gi + 1) * (4 / GPB); k++) {   // 32 rows each
-                const uint4 w = *reinterpret_cast<const uint4*>(st + k * 512 + lane * 16);
-                uint2 b[NT];
-#pragma unroll
-                for (int n = 0; n < NT; n++) b[n] = *reinterpret_cast<const uint2*>(col[n] + kb * GMV_BLOCK + k * 32);
-                constexpr uint32_t HIGH = 0xF0F0F0F0u;
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    gmv_mma(acc[n][0], w.x & HIGH, w.y & HIGH, (w.x << 4) & HIGH, (w.y << 4) & HIGH, b[n]);
-                    gmv_mma(acc[n][1], w.z & HIGH, w.w & HIGH, (w.z << 4) & HIGH, (w.w << 4) & HIGH, b[n]);
-                }
-            }
             float s[4];
 #pragma unroll
             for (int q = 0; q < 4; q++) s[q] = dz_to_float(scale[gi * GMV_TILE + 8 * q]);
+            if constexpr (NT == 0) {
+                int acc[2][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+                for (int q = 0; q < 8; q++) acc[q >> 2][q & 3] = GMV_ZERO;
+#pragma unroll
+                for (int k = gi * (4 / GPB); k < (gi + 1) * (4 / GPB); k++) {   // 32 rows each
+                    const uint4 w = *reinterpret_cast<const uint4*>(st + k * 512 + lane * 16);
+                    const uint2 b = *reinterpret_cast<const uint2*>(col[0] + kb * GMV_BLOCK + k * 32);
+                    constexpr uint32_t HIGH = 0xF0F0F0F0u;
+                    gmv_mma(acc[0], w.x & HIGH, w.y & HIGH, (w.x << 4) & HIGH, (w.y << 4) & HIGH, b);
+                    gmv_mma(acc[1], w.z & HIGH, w.w & HIGH, (w.z << 4) & HIGH, (w.w << 4) & HIGH, b);
+                }
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
-                    const float v = __int_as_float(acc[n][q >> 2][q & 3]) - 12582912.0f;
-                    part[n][q] = gi ? fmaf(v, s[q >> 1], part[n][q]) : v * s[q >> 1];
+                    const float v = __int_as_float(acc[q >> 2][q & 3]) - GMV_ZEROF;
+                    part[q] = gi ? fmaf(v, s[q >> 1], part[q]) : v * s[q >> 1];
                 }
+            } else {
+                float acc[COLS][2][4];
+#pragma unroll
+                for (int n = 0; n < COLS; n++)
+#pragma unroll
+                    for (int q = 0; q < 8; q++) acc[n][q >> 2][q & 3] = 0.0f;
+#pragma unroll
+                for (int k = gi * (4 / GPB); k < (gi + 1) * (4 / GPB); k++) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(st + k * 512 + lane * 16);
+                    uint4 b[COLS];
+#pragma unroll
+                    for (int n = 0; n < COLS; n++)
+                        b[n] = *reinterpret_cast<const uint4*>(col[n] + (kb * GMV_BLOCK + k * 32) * 2);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        uint32_t f0[4], f1[4];   // columns g, g + 8; g + 16, g + 24
+                        gmv_levels(w.x, i, f0[0], f0[2], Mma());
+                        gmv_levels(w.y, i, f0[1], f0[3], Mma());
+                        gmv_levels(w.z, i, f1[0], f1[2], Mma());
+                        gmv_levels(w.w, i, f1[1], f1[3], Mma());
+#pragma unroll
+                        for (int n = 0; n < COLS; n++) {
+                            const uint32_t b0 = i ? b[n].z : b[n].x, b1 = i ? b[n].w : b[n].y;
+                            gmv_mma(acc[n][0], f0, b0, b1, Mma());
+                            gmv_mma(acc[n][1], f1, b0, b1, Mma());
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < COLS; n++)
+#pragma unroll
+                    for (int q = 0; q < 8; q++) out[n][q] = fmaf(acc[n][q >> 2][q & 3], s[q >> 1], out[n][q]);
+            }
         }
+        if constexpr (NT == 0) {
+            const float2 f = *reinterpret_cast<const float2*>(fx + kb * GMV_DIGITS + 2 * t);
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const float2 f = *reinterpret_cast<const float2*>(fx + kb * 8 * NT + 8 * n + 2 * t);
-#pragma unroll
-            for (int q = 0; q < 8; q++) out[n][q] = fmaf(part[n][q], q & 1 ? f.y : f.x, out[n][q]);
+            for (int q = 0; q < 8; q++) out[0][q] = fmaf(part[q], q & 1 ? f.y : f.x, out[0][q]);
         }
         if (++kb < nb && r + 1 < r1) continue;
-        // the tile ends, or the warp's range does: add the digits, keep the part
+        // the tile ends, or the warp's range does: add a row's parts or digits, the smallest first, keep the sum
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < COLS; n++)
 #pragma unroll
             for (int q = 0; q < 8; q++) {
                 mine[(g + 8 * (q >> 1)) * L::LD + 8 * n + 2 * t + (q & 1)] = out[n][q];
@@ -397,8 +545,11 @@ __global__ void __launch_bounds__(GMV_WARPS * 32, NT < 3 || (NT == 3 && GPB < 4)
         float* to = head ? heads + warp * GMV_TILE * M : parts + ti * GMV_TILE * M;
 #pragma unroll 4
         for (int m = 0; m < M; m++) {
-            const float* p = mine + lane * L::LD + ND * m;
-            to[m * GMV_TILE + lane] = ND == 3 ? p[0] + p[1] + p[2] : p[0] + p[1];
+            const float* p = mine + lane * L::LD + P * m;
+            if (NT == 0)
+                to[lane] = ((((p[6] + p[7]) + p[3]) + p[4]) + p[5]) + ((p[0] + p[1]) + p[2]);
+            else
+                to[m * GMV_TILE + lane] = P == 3 ? (p[2] + p[1]) + p[0] : p[0];
         }
         __syncwarp();
         head = false;
@@ -433,25 +584,26 @@ __global__ void __launch_bounds__(GMV_WARPS * 32, NT < 3 || (NT == 3 && GPB < 4)
                 s += v;
             }
         }
-        if (n < a.w.N) gmv_store(a.y, a.type, (long long)m * a.ldy + n, s);
+        if (n < a.w.N) static_cast<T*>(a.y)[(long long)m * a.ldy + n] = dz_from_float<T>(NT ? s * GmvType<T>::UNIT : s);
     }
     // no block leaves while another may still read its shared memory
     if (plan.cluster > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-template <int GPB, typename S, int ND, int NT>
+template <int GPB, typename S, typename T, int NT>
 static cudaError_t gmv_launch_t(const GmvArgs& a, const GmvPlan& plan, int device, cudaStream_t st) {
-    auto* k = dz_gmv_kernel<GPB, S, ND, NT>;
+    auto* k = dz_gmv_kernel<GPB, S, T, NT>;
     static std::atomic<bool> ready[GMV_DEVICES];
     if (device >= GMV_DEVICES || !ready[device].load(std::memory_order_relaxed)) {
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, GMV_SMEM);
+        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, GMV_SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         if (device < GMV_DEVICES) ready[device].store(true, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(plan.clusters * plan.cluster));
     cfg.blockDim = dim3(GMV_WARPS * 32);
-    cfg.dynamicSmemBytes = (size_t)GmvSmem<ND, NT>::total(a.w.rec_bytes, plan);
+    cfg.dynamicSmemBytes = (size_t)GmvSmem<GmvType<T>::PARTS, NT>::total(a.w.rec_bytes, plan);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -464,49 +616,48 @@ static cudaError_t gmv_launch_t(const GmvArgs& a, const GmvPlan& plan, int devic
     return cudaLaunchKernelEx(&cfg, k, a, plan);
 }
 
-// Column tiles of 8 for `rows` rows: the instantiations below.
-static int gmv_col_tiles(int nd, int rows) {
-    const int n = (nd * rows + 7) / 8;
-    return n <= 3 ? n : nd == 3 ? 6 : 4;
+// Columns of B that a row takes, and column tiles of 8 for `rows` rows: the instantiations below.
+static int gmv_parts(int type) { return type == DZ_TYPE_F32 ? GmvType<float>::PARTS : 1; }
+static int gmv_col_tiles(int parts, int rows) {
+    const int n = (parts * rows + 7) / 8;
+    return n <= 3 ? n : 6;
 }
 
 template <int GPB, typename S>
 static cudaError_t gmv_launch_n(const GmvArgs& a, const GmvPlan& plan, int device, cudaStream_t st) {
-    if (a.type == DZ_TYPE_F32) {
-        switch (gmv_col_tiles(3, plan.rows)) {
-        case 1: return gmv_launch_t<GPB, S, 3, 1>(a, plan, device, st);
-        case 2: return gmv_launch_t<GPB, S, 3, 2>(a, plan, device, st);
-        case 3: return gmv_launch_t<GPB, S, 3, 3>(a, plan, device, st);
-        default: return gmv_launch_t<GPB, S, 3, 6>(a, plan, device, st);
-        }
-    }
-    switch (gmv_col_tiles(2, plan.rows)) {
-    case 1: return gmv_launch_t<GPB, S, 2, 1>(a, plan, device, st);
-    case 2: return gmv_launch_t<GPB, S, 2, 2>(a, plan, device, st);
-    case 3: return gmv_launch_t<GPB, S, 2, 3>(a, plan, device, st);
-    default: return gmv_launch_t<GPB, S, 2, 4>(a, plan, device, st);
-    }
+    const int n = gmv_col_tiles(gmv_parts(a.type), plan.rows);
+    if (plan.digits)
+        return a.type == DZ_TYPE_F32   ? gmv_launch_t<GPB, S, float, 0>(a, plan, device, st)
+               : a.type == DZ_TYPE_F16 ? gmv_launch_t<GPB, S, __half, 0>(a, plan, device, st)
+                                       : gmv_launch_t<GPB, S, __nv_bfloat16, 0>(a, plan, device, st);
+    if (a.type == DZ_TYPE_F32)
+        return n == 1   ? gmv_launch_t<GPB, S, float, 1>(a, plan, device, st)
+               : n == 2 ? gmv_launch_t<GPB, S, float, 2>(a, plan, device, st)
+               : n == 3 ? gmv_launch_t<GPB, S, float, 3>(a, plan, device, st)
+                        : gmv_launch_t<GPB, S, float, 6>(a, plan, device, st);
+    if (a.type == DZ_TYPE_F16)
+        return n == 1 ? gmv_launch_t<GPB, S, __half, 1>(a, plan, device, st) : gmv_launch_t<GPB, S, __half, 2>(a, plan, device, st);
+    return n == 1 ? gmv_launch_t<GPB, S, __nv_bfloat16, 1>(a, plan, device, st)
+                  : gmv_launch_t<GPB, S, __nv_bfloat16, 2>(a, plan, device, st);
 }
 
 static int gmv_smem(const GmvArgs& a, const GmvPlan& p) {
-    const int nd = a.type == DZ_TYPE_F32 ? 3 : 2, nt = gmv_col_tiles(nd, p.rows), rec = a.w.rec_bytes;
-    if (nd == 3)
+    const int parts = gmv_parts(a.type), nt = gmv_col_tiles(parts, p.rows), rec = a.w.rec_bytes;
+    if (p.digits) return GmvSmem<1, 0>::total(rec, p);
+    if (parts == 3)
         return nt == 1   ? GmvSmem<3, 1>::total(rec, p)
                : nt == 2 ? GmvSmem<3, 2>::total(rec, p)
                : nt == 3 ? GmvSmem<3, 3>::total(rec, p)
                          : GmvSmem<3, 6>::total(rec, p);
-    return nt == 1   ? GmvSmem<2, 1>::total(rec, p)
-           : nt == 2 ? GmvSmem<2, 2>::total(rec, p)
-           : nt == 3 ? GmvSmem<2, 3>::total(rec, p)
-                     : GmvSmem<2, 4>::total(rec, p);
+    return nt == 1 ? GmvSmem<1, 1>::total(rec, p) : GmvSmem<1, 2>::total(rec, p);
 }
 
-// Clusters of 1, 2, 4 and 8 blocks that `device` holds at once with one block
-// on an SM, then with two (a cluster stays within one GPC, so that larger ones
-// leave SMs idle). Asked once per device.
+// Clusters of 1, 2, 4, 8 and 16 blocks that `device` holds at once with one
+// block on an SM, then with two (a cluster stays within one GPC, so that larger
+// ones leave SMs idle). Asked once per device.
 struct GmvRoom {
     std::atomic<bool> known{false};
-    std::atomic<int> clusters[2][4];
+    std::atomic<int> clusters[2][5];
 };
 
 static cudaError_t gmv_room(int device, const GmvRoom** out) {
@@ -514,12 +665,13 @@ static cudaError_t gmv_room(int device, const GmvRoom** out) {
     if (device < 0 || device >= GMV_DEVICES) return cudaErrorInvalidDevice;
     GmvRoom& r = rooms[device];
     if (!r.known.load(std::memory_order_acquire)) {
-        auto* k = dz_gmv_kernel<1, float, 3, 1>;
+        auto* k = dz_gmv_kernel<1, float, float, 0>;
         cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, GMV_SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         for (int two = 0; two < 2 && e == cudaSuccess; two++)
-            for (int c = 0; c < 4 && e == cudaSuccess; c++) {
+            for (int c = 0; c < 5 && e == cudaSuccess; c++) {
                 cudaLaunchConfig_t cfg = {};
-                cfg.gridDim = dim3(8);
+                cfg.gridDim = dim3(16);
                 cfg.blockDim = dim3(GMV_WARPS * 32);
                 cfg.dynamicSmemBytes = two ? GMV_SMEM2 : GMV_SMEM;
                 cudaLaunchAttribute attr[1];
@@ -539,39 +691,49 @@ static cudaError_t gmv_room(int device, const GmvRoom** out) {
     return cudaSuccess;
 }
 
-// How many rows a pass takes and how a tile is shared: the shape with the
-// least estimated time. False: not even one row fits. The estimate, in us on
-// one B200 (K 2048..12032, N 48..32000, 1..16 rows): four loads of activations
-// per warp take 1.9; a record 0.38 when two blocks per SM stream from HBM and
-// 0.15 + 0.15 NT + 0.02 NT GPB by its own latency; joining a cluster 0.7 and
-// 0.1 per block. 16 x 4099 x 5003: 36 us with one block to a tile, 22 with two.
-static bool gmv_plan(const GmvArgs& a, int rows, const GmvRoom& room, GmvPlan* plan) {
-    const int nd = a.type == DZ_TYPE_F32 ? 3 : 2, gpb = GMV_BLOCK / a.w.group;
-    for (rows = rows < GMV_MAX_ROWS ? rows : GMV_MAX_ROWS; rows >= 1; rows /= 2) {
-        double cost = 1e30;
-        const int nt = gmv_col_tiles(nd, rows);
-        for (int i = 0; i < 4 && (1 << i) <= a.w.nblocks; i++)
-            for (int two = 0; two < 2; two++) {
-                GmvPlan p;
-                const int c = 1 << i, fits = room.clusters[two][i].load(std::memory_order_relaxed);
-                p.rows = rows;
-                p.cluster = c;
-                p.slice = (a.w.nblocks + c - 1) / c;
-                p.clusters = fits < a.w.ntiles ? fits : a.w.ntiles;
-                p.tiles = (a.w.ntiles + p.clusters - 1) / p.clusters;
-                if (gmv_smem(a, p) > (two ? GMV_SMEM2 : GMV_SMEM)) continue;
-                const int per_batch = GMV_WARPS * 4 * (nd == 3 ? 1 : 2);
-                const double stream = 0.38 * (two + 1), own = (0.15 + 0.15 * nt + 0.02 * nt * gpb) * (two ? 1.6 : 1.0);
-                const double t = 1.9 * ((rows * p.slice + per_batch - 1) / per_batch) * (two ? 1.6 : 1.0) +
-                                 (stream > own ? stream : own) * ((p.tiles * p.slice + GMV_WARPS - 1) / GMV_WARPS) +
-                                 (c > 1 ? 0.7 + 0.1 * c : 0.0);
-                if (t < cost) {
-                    cost = t;
-                    *plan = p;
-                }
+// How a tile is shared: the shape with the least estimated time. False: none
+// holds the rows' activations. The estimate, in us on one B200 (K 256..12032, N
+// 48..32000, 1..16 rows): four loads of activations by every thread 0.9 (16 bits:
+// 0.6), from the third time on 0.6 more, whose latency nothing hides; a record
+// 0.38 when all SMs stream from HBM, and by its own latency 0.3 + 0.15 NT + 0.02
+// NT GPB; a cluster's join 1.0, 0.16 per block and what each reads of the others.
+// 16 x 4096 x 4096 in fp32: 33 us with one block to a tile, 20 with two, 17 with
+// four, 14 with eight; 2 x 4096 x 4096: 5.8, 6.2, 6.2 and 6.7 us.
+static bool gmv_plan_as(const GmvArgs& a, int rows, int digits, const GmvRoom& room, GmvPlan* plan) {
+    const int parts = gmv_parts(a.type), gpb = GMV_BLOCK / a.w.group, nt = digits ? 0 : gmv_col_tiles(parts, rows);
+    double cost = 1e30;
+    for (int i = 0; i < 5 && (1 << i) <= a.w.nblocks; i++) {
+        if (i == 4 && cost < 1e30) break;              // 16 blocks only where 8 cannot hold their rows' activations
+        for (int two = 0; two < gmv_blocks(nt, gpb); two++) {
+            GmvPlan p;
+            const int c = 1 << i, fits = room.clusters[two][i].load(std::memory_order_relaxed);
+            p.rows = rows;
+            p.digits = digits;
+            p.cluster = c;
+            p.slice = (a.w.nblocks + c - 1) / c;
+            p.clusters = fits < a.w.ntiles ? fits : a.w.ntiles;
+            p.tiles = (a.w.ntiles + p.clusters - 1) / p.clusters;
+            if (gmv_smem(a, p) > (two ? GMV_SMEM2 : GMV_SMEM)) continue;
+            const int per_batch = GMV_WARPS * (parts == 3 ? 4 : 8), batches = (rows * p.slice + per_batch - 1) / per_batch;
+            const double stage = (parts == 3 ? 0.9 : 0.6) * batches + 0.6 * (batches > 2 ? batches - 2 : 0);
+            const double stream = 0.38 * (two + 1), own = (0.3 + 0.15 * nt + 0.02 * nt * gpb) * (two ? 1.6 : 1.0);
+            const double t = stage * (two ? 1.6 : 1.0) +
+                             (stream > own ? stream : own) * ((p.tiles * p.slice + GMV_WARPS - 1) / GMV_WARPS) +
+                             (c > 1 ? 1.0 + 0.16 * c + 0.0125 * p.tiles * rows : 0.0);
+            if (t < cost) {
+                cost = t;
+                *plan = p;
             }
-        if (cost < 1e30) return true;
+        }
     }
+    return cost < 1e30;
+}
+
+// How many rows a pass takes, and how: half as many where no shape holds them.
+static bool gmv_plan(const GmvArgs& a, int rows, const GmvRoom& room, GmvPlan* plan) {
+    if (rows == 1 && gmv_plan_as(a, 1, 1, room, plan)) return true;
+    for (rows = rows < GMV_MAX_ROWS ? rows : GMV_MAX_ROWS; rows >= 1; rows /= 2)
+        if (gmv_plan_as(a, rows, 0, room, plan)) return true;
     return false;
 }
 

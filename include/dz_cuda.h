@@ -110,11 +110,13 @@ size_t dz_cuda_gmatrix_bytes(const dz_cuda_gmatrix_t *matrix);
 int dz_cuda_gmatrix_unpack(const dz_cuda_gmatrix_t *matrix, float *dst);
 /* C (m x n) = A (m x k) . W on device buffers, enqueued on `stream` (a
  * cudaStream_t) without synchronisation. A and C have element type `type` and
- * row strides lda >= k, ldc >= n in elements; they must not overlap. Each
- * activation is held to 2^-22 (fp32) or 2^-14 (fp16, bf16) of the largest of
- * its 128 consecutive ones, sums are fp32, one rounding to `type` at the end;
- * a row that holds an infinity or a NaN reads NaN. Meant for few rows (16 at a time
- * pass over the weights). Nothing is allocated and the handle holds no
+ * row strides lda >= k, ldc >= n in elements; they must not overlap.
+ * Activations enter with their own precision, whatever stands beside them (what
+ * lies 2^-60 below the largest of 128 consecutive ones may be lost), their
+ * products with the levels are exact, sums are fp32, one rounding to `type` at
+ * the end; a row that holds an infinity or a NaN reads NaN. The order of the
+ * sums depends on m. Meant for few rows (16 at a time pass over the weights).
+ * Nothing is allocated and the handle holds no
  * scratch: calls on one matrix may overlap, and a call may be captured. */
 int dz_cuda_matmul_grouped_async(const void *A_dev, size_t lda, const dz_cuda_gmatrix_t *weights, void *C_dev,
                                  size_t ldc, size_t m, size_t k, int type, void *stream);
