@@ -115,23 +115,8 @@ template <typename S> __global__ void dz_gmv_dequant_kernel(GmvMatrix w, float* 
 // per tile 20 us; a cluster barrier per tile 29 us.
 
 constexpr int GMV_DEVICES = 64;         // devices whose launch state is kept
-constexpr int GMV_SMEM = 227 * 1024 - 128;// shared memory a block may have
-constexpr int GMV_SMEM2 = 113 * 1024 - 128;// and if two are to fit an SM
-constexpr int GMV_WARPS = 8;
-constexpr int GMV_STAGES = 4;
-constexpr int GMV_MAX_ROWS = 16;        // rows of one pass
-constexpr int GMV_DIGITS = 8;           // of an activation of a single row
 constexpr int GMV_ZERO = 0x4B400000;    // 1.5 x 2^23
 constexpr float GMV_ZEROF = 12582912.0f;
-
-struct GmvPlan {
-    int rows;         // rows of this launch
-    int digits;       // whether its one row goes as digits
-    int cluster;      // blocks that share a tile
-    int clusters;     // clusters of the grid
-    int slice;        // records of a tile that a block has, at most
-    int tiles;        // tiles of a cluster, at most
-};
 
 __device__ __forceinline__ void gmv_mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -293,27 +278,6 @@ __device__ __forceinline__ int gmv_share(unsigned n, unsigned i, unsigned of) {
     const unsigned q = n / of, r = n - q * of;
     return (int)(q * i + r * i / of);
 }
-
-// Shared memory: the rings, the columns of activations (or digits and their
-// weights), a warp's tile in accumulator order, the parts.
-template <int P, int NT> struct GmvSmem {   // NT 0: one row as digits
-    static constexpr int TILES = NT ? NT : 1;
-    static constexpr int LD = 8 * TILES + 1;                 // floats between the columns of W in a warp's tile
-    static constexpr int TILE = (GMV_TILE * LD + 3) / 4 * 4;
-    static __host__ __device__ int ring(int rec) { return GMV_WARPS * GMV_STAGES * rec; }
-    // bytes between columns: what neighbours read of a piece (64 bytes, 32 of digits) falls into different banks
-    static __host__ __device__ int stride(int slice) { return NT ? slice * GMV_BLOCK * 2 + 64 : slice * GMV_BLOCK + 32; }
-    static __host__ __device__ int columns(int rows, int slice) {
-        return NT ? P * rows * stride(slice) : GMV_DIGITS * stride(slice) + slice * GMV_DIGITS * 4;
-    }
-    static __host__ __device__ int total(int rec, const GmvPlan& p) {
-        return ring(rec) + columns(p.rows, p.slice) + GMV_WARPS * TILE * 4 + (p.tiles + GMV_WARPS) * GMV_TILE * p.rows * 4;
-    }
-};
-
-// Blocks of an instantiation that an SM is to hold: its registers would not let
-// more tiles or groups share it without spills.
-constexpr int gmv_blocks(int nt, int gpb) { return nt < 3 || (nt == 3 && gpb == 1) ? 2 : 1; }
 
 template <int GPB, typename S, typename T, int NT>   // scale groups of a block, scale and activation type, column tiles of 8
 __global__ void __launch_bounds__(GMV_WARPS * 32, gmv_blocks(NT, GPB)) dz_gmv_kernel(
@@ -616,16 +580,9 @@ static cudaError_t gmv_launch_t(const GmvArgs& a, const GmvPlan& plan, int devic
     return cudaLaunchKernelEx(&cfg, k, a, plan);
 }
 
-// Columns of B that a row takes, and column tiles of 8 for `rows` rows: the instantiations below.
-static int gmv_parts(int type) { return type == DZ_TYPE_F32 ? GmvType<float>::PARTS : 1; }
-static int gmv_col_tiles(int parts, int rows) {
-    const int n = (parts * rows + 7) / 8;
-    return n <= 3 ? n : 6;
-}
-
 template <int GPB, typename S>
 static cudaError_t gmv_launch_n(const GmvArgs& a, const GmvPlan& plan, int device, cudaStream_t st) {
-    const int n = gmv_col_tiles(gmv_parts(a.type), plan.rows);
+    const int n = gmv_col_tiles(a.type == DZ_TYPE_F32 ? GmvType<float>::PARTS : 1, plan.rows);
     if (plan.digits)
         return a.type == DZ_TYPE_F32   ? gmv_launch_t<GPB, S, float, 0>(a, plan, device, st)
                : a.type == DZ_TYPE_F16 ? gmv_launch_t<GPB, S, __half, 0>(a, plan, device, st)
@@ -640,25 +597,6 @@ static cudaError_t gmv_launch_n(const GmvArgs& a, const GmvPlan& plan, int devic
     return n == 1 ? gmv_launch_t<GPB, S, __nv_bfloat16, 1>(a, plan, device, st)
                   : gmv_launch_t<GPB, S, __nv_bfloat16, 2>(a, plan, device, st);
 }
-
-static int gmv_smem(const GmvArgs& a, const GmvPlan& p) {
-    const int parts = gmv_parts(a.type), nt = gmv_col_tiles(parts, p.rows), rec = a.w.rec_bytes;
-    if (p.digits) return GmvSmem<1, 0>::total(rec, p);
-    if (parts == 3)
-        return nt == 1   ? GmvSmem<3, 1>::total(rec, p)
-               : nt == 2 ? GmvSmem<3, 2>::total(rec, p)
-               : nt == 3 ? GmvSmem<3, 3>::total(rec, p)
-                         : GmvSmem<3, 6>::total(rec, p);
-    return nt == 1 ? GmvSmem<1, 1>::total(rec, p) : GmvSmem<1, 2>::total(rec, p);
-}
-
-// Clusters of 1, 2, 4, 8 and 16 blocks that `device` holds at once with one
-// block on an SM, then with two (a cluster stays within one GPC, so that larger
-// ones leave SMs idle). Asked once per device.
-struct GmvRoom {
-    std::atomic<bool> known{false};
-    std::atomic<int> clusters[2][5];
-};
 
 static cudaError_t gmv_room(int device, const GmvRoom** out) {
     static GmvRoom rooms[GMV_DEVICES];
@@ -682,7 +620,7 @@ static cudaError_t gmv_room(int device, const GmvRoom** out) {
                 cfg.numAttrs = 1;
                 int n = 0;
                 e = cudaOccupancyMaxActiveClusters(&n, k, &cfg);
-                r.clusters[two][c].store(n > 0 ? n : 1, std::memory_order_relaxed);
+                r.clusters[two][c].store(n, std::memory_order_relaxed);
             }
         if (e != cudaSuccess) return e;
         r.known.store(true, std::memory_order_release);
@@ -691,50 +629,8 @@ static cudaError_t gmv_room(int device, const GmvRoom** out) {
     return cudaSuccess;
 }
 
-// How a tile is shared: the shape with the least estimated time. False: none
-// holds the rows' activations. The estimate, in us on one B200 (K 256..12032, N
-// 48..32000, 1..16 rows): four loads of activations by every thread 0.9 (16 bits:
-// 0.6), from the third time on 0.6 more, whose latency nothing hides; a record
-// 0.38 when all SMs stream from HBM, and by its own latency 0.3 + 0.15 NT + 0.02
-// NT GPB; a cluster's join 1.0, 0.16 per block and what each reads of the others.
-// 16 x 4096 x 4096 in fp32: 33 us with one block to a tile, 20 with two, 17 with
-// four, 14 with eight; 2 x 4096 x 4096: 5.8, 6.2, 6.2 and 6.7 us.
-static bool gmv_plan_as(const GmvArgs& a, int rows, int digits, const GmvRoom& room, GmvPlan* plan) {
-    const int parts = gmv_parts(a.type), gpb = GMV_BLOCK / a.w.group, nt = digits ? 0 : gmv_col_tiles(parts, rows);
-    double cost = 1e30;
-    for (int i = 0; i < 5 && (1 << i) <= a.w.nblocks; i++) {
-        if (i == 4 && cost < 1e30) break;              // 16 blocks only where 8 cannot hold their rows' activations
-        for (int two = 0; two < gmv_blocks(nt, gpb); two++) {
-            GmvPlan p;
-            const int c = 1 << i, fits = room.clusters[two][i].load(std::memory_order_relaxed);
-            p.rows = rows;
-            p.digits = digits;
-            p.cluster = c;
-            p.slice = (a.w.nblocks + c - 1) / c;
-            p.clusters = fits < a.w.ntiles ? fits : a.w.ntiles;
-            p.tiles = (a.w.ntiles + p.clusters - 1) / p.clusters;
-            if (gmv_smem(a, p) > (two ? GMV_SMEM2 : GMV_SMEM)) continue;
-            const int per_batch = GMV_WARPS * (parts == 3 ? 4 : 8), batches = (rows * p.slice + per_batch - 1) / per_batch;
-            const double stage = (parts == 3 ? 0.9 : 0.6) * batches + 0.6 * (batches > 2 ? batches - 2 : 0);
-            const double stream = 0.38 * (two + 1), own = (0.3 + 0.15 * nt + 0.02 * nt * gpb) * (two ? 1.6 : 1.0);
-            const double t = stage * (two ? 1.6 : 1.0) +
-                             (stream > own ? stream : own) * ((p.tiles * p.slice + GMV_WARPS - 1) / GMV_WARPS) +
-                             (c > 1 ? 1.0 + 0.16 * c + 0.0125 * p.tiles * rows : 0.0);
-            if (t < cost) {
-                cost = t;
-                *plan = p;
-            }
-        }
-    }
-    return cost < 1e30;
-}
-
-// How many rows a pass takes, and how: half as many where no shape holds them.
-static bool gmv_plan(const GmvArgs& a, int rows, const GmvRoom& room, GmvPlan* plan) {
-    if (rows == 1 && gmv_plan_as(a, 1, 1, room, plan)) return true;
-    for (rows = rows < GMV_MAX_ROWS ? rows : GMV_MAX_ROWS; rows >= 1; rows /= 2)
-        if (gmv_plan_as(a, rows, 0, room, plan)) return true;
-    return false;
+static GmvShape gmv_shape(const GmvMatrix& w, int type) {
+    return GmvShape{w.ntiles, w.nblocks, w.group, w.rec_bytes, type == DZ_TYPE_F32 ? GmvType<float>::PARTS : 1};
 }
 
 cudaError_t dz_gmv_launch(const GmvArgs& a, int device, cudaStream_t st) {
@@ -743,8 +639,9 @@ cudaError_t dz_gmv_launch(const GmvArgs& a, int device, cudaStream_t st) {
     if (err != cudaSuccess) return err;
     GmvArgs b = a;
     GmvPlan plan;
+    const GmvShape shape = gmv_shape(a.w, a.type);
     for (int m = 0; m < a.M; m += plan.rows) {
-        if (!gmv_plan(a, a.M - m, *room, &plan)) return cudaErrorNotSupported;
+        if (!gmv_plan(shape, a.M - m, *room, &plan)) return cudaErrorNotSupported;
         b.x = static_cast<const uint8_t*>(a.x) + (long long)m * a.ldx * type_bytes(a.type);
         b.y = static_cast<uint8_t*>(a.y) + (long long)m * a.ldy * type_bytes(a.type);
         cudaError_t e;
@@ -836,12 +733,10 @@ extern "C" int dz_cuda_gmatrix_create(int device, const dz_grouped_blob_t* w, dz
     m.ntiles = (m.N + GMV_TILE - 1) / GMV_TILE;
     m.nblocks = (m.K + GMV_BLOCK - 1) / GMV_BLOCK;
     m.rec_bytes = GMV_CODES + GMV_BLOCK / m.group * GMV_TILE * (m.scale_f16 ? 2 : 4);
-    GmvArgs one = {};
     GmvPlan plan;
-    one.w = m;
     const GmvRoom* room;
     DZ_CUDA(gmv_room(device, &room));
-    if (!gmv_plan(one, 1, *room, &plan))
+    if (!gmv_plan(gmv_shape(m, DZ_TYPE_F32), 1, *room, &plan))
         return fail(DZ_E_UNSUPPORTED, "gmatrix: %zu x %zu is too large for a product's shared memory", w->rows, w->cols);
     if ((long long)m.ntiles * m.nblocks > (1LL << 30)) return fail(DZ_E_UNSUPPORTED, "gmatrix: too many weights");
     auto* q = new (std::nothrow) dz_cuda_gmatrix;

@@ -15,11 +15,9 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
-namespace dz {
+#include "gmvplan.h"
 
-constexpr int GMV_TILE = 32;     // columns of a tile
-constexpr int GMV_BLOCK = 128;   // rows of a block
-constexpr int GMV_CODES = GMV_TILE * GMV_BLOCK / 2;
+namespace dz {
 
 struct GmvMatrix {
     uint8_t* rec = nullptr;      // [ntiles][nblocks] records
