@@ -1,8 +1,8 @@
 // Attention over the 4-bit ring caches (kv4.cuh), in a translation unit of its
 // own.
 //
-// A unit is one (sequence, key head) and up to 4 NT (fp32: 2 NT) of its (query
-// token, query head) pairs. Its visible tokens go in tiles of 32 to a team of
+// A unit is one (sequence, key head) and up to 2 NT of its (query token, query
+// head) pairs. Its visible tokens go in tiles of 32 to a team of
 // 1, 2, 4 or 8 warps in turn, or to the warps of a cluster of 2 to 16 blocks;
 // each warp keeps its own softmax state and the states join in shared memory,
 // then across the cluster. A warp's start and its part in a join cost as much
@@ -12,22 +12,28 @@
 // 64-element group are exact. Codes are its A operand as they are, unsigned
 // bytes holding code or 16 x code, so that one or two logic operations widen
 // four of them; the 7 that a code stands above its level is taken off by the
-// value that an accumulator starts at. B columns are digits of base 256:
-//   scores   A = 16 tokens x 32 elements of K, B = the query's balanced digits.
-//            Its elements are integers after a power of two per 64-element
-//            group. Group sums times the token's scale add up in fp32.
+// value that an accumulator starts at. B columns are balanced digits of base 256:
+//   scores   A = 16 tokens x 32 elements of K, B = the query's digits. Its
+//            elements are integers after a power of two per 64-element group.
+//            Group sums times the token's scale add up in fp32.
 //   values   A = 16 elements of V^T x 32 tokens, B = the digits of weight x
-//            value scale, integers after a power of two per tile and group.
-//            Tile sums add up in fp32.
-// fp32 takes three digits: 2^-23 of the group's largest element, or of the
-// tile's largest weight x scale, is lost at most; fp16 and bf16 take two, 2^-15
-// of either, well below their outputs' rounding. A pair takes 4 (fp32, one of them
-// idle) or 2 columns of the 8. An accumulator starts at the bits of 1.5 x 2^23
+//            value scale (of either sign), integers after a power of two per
+//            tile and group. Tile sums add up in fp32.
+// A pair takes 4 of the 8 columns: three digits of a query (half a step is at most
+// 1 / (2 x 4177855) of the group's largest element), four of a weight (2^-30 of the
+// tile's largest weight x scale). An accumulator starts at the bits of 1.5 x 2^23
 // (less the 7s): its bits read as a float are 1.5 x 2^23 plus the sum.
 //
-// Bound by instruction issue: 540 per tile of 32 tokens at head dimension 128
-// and one fp32 pair, 2.5 a cycle per SM. 256 x 16 heads of 128, up to 641
-// tokens: 67 us per call, 5.0 TB/s of the 6.55 that a copy reaches. With levels
+// 3 or 4 pairs of 16-bit types (FV) take their values in the 16-bit MMA: weight x
+// scale in two bf16 parts (2^-17 of itself), two columns for a pair, levels widened
+// to bf16 and summed in the accumulators over all tiles. 2 x 8 key heads of 128, 4
+// queries each, 130k tokens: 103 us, 155 with digits in two n-tiles. (Two digits
+// for queries and weights of 16-bit types took 76 us, and lost small elements
+// and small weights beside large ones.)
+//
+// Bound by instruction issue: 550 per tile of 32 tokens at head dimension 128
+// and one pair, 2.5 a cycle per SM. 256 x 16 heads of 128, up to 641
+// tokens: 68 us per call, 4.9 TB/s of the 6.55 that a copy reaches. With levels
 // widened to fp16 pairs in m16n8k16 (two fp16 parts per fp32 weight) a tile took
 // 860 instructions, most of the ALU's issue rate in widening, and the call 118
 // us.
@@ -64,16 +70,10 @@ template <int BYTES> __device__ __forceinline__ void ka_copy_small(uint32_t dst,
 __device__ __forceinline__ void ka_commit() { asm volatile("cp.async.commit_group;"); }
 template <int N> __device__ __forceinline__ void ka_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N)); }
 
-// A unsigned; B signed (the query's digits) or unsigned (the weights').
-__device__ __forceinline__ void ka_mma_s(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+// A unsigned, B signed.
+__device__ __forceinline__ void ka_mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void ka_mma_u(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -91,17 +91,35 @@ __device__ __forceinline__ float ka_max_nan(float a, float b) {
     return y;
 }
 
+__device__ __forceinline__ void ka_mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Levels of the nibbles at bits 0 and 16 of w as a bf16 pair: or-ed into 128,
+// whose step is 1, a nibble adds itself; 135 less is the level. (lop3: both
+// constants stay in registers, one instruction.)
+__device__ __forceinline__ uint32_t ka_level(uint32_t w) {
+    uint32_t x;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w), "r"(0x000F000Fu), "r"(0x43004300u));
+    const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x),
+                                     __bfloat162bfloat162(__ushort_as_bfloat16(0x4307)));
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
+
 // Byte d of four words (sel = d | (4 + d) << 4).
 __device__ __forceinline__ uint32_t ka_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t sel) {
     return __byte_perm(__byte_perm(a, b, sel), __byte_perm(c, d, sel), 0x5410);
 }
 
-template <typename T, int HD, int ND, int NT, bool SPLIT>
+template <typename T, int HD, int NT, bool SPLIT, bool FV>
 __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a,
                                                                                     int team, int cluster, int pair_blocks,
                                                                                     int units) {
     using C = KaCfg<HD>;
-    constexpr int CPP = ND == 3 ? 4 : 2;     // columns of a pair
+    constexpr int CPP = 4;                   // columns of a pair
     // Pairs of an n-tile; lane t has columns of pair 2 t / CPP. SPLIT: where they
     // would fill half the columns at most, the two value groups take a half
     // each: columns 0..3 of the weights' digits belong to group 0, 4..7 to
@@ -111,6 +129,11 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     constexpr int PAIRS = NT * PPT;          // pairs of a block
     constexpr int GR = C::GROUPS, GA = SPLIT ? 1 : GR;   // value groups of a lane's columns
     static_assert(!SPLIT || (NT == 1 && GR == 2), "two groups share one n-tile");
+    // FV: values in the 16-bit MMA, one n-tile for 4 pairs. The scores' two n-tiles
+    // hold pairs 2 c and 2 c + 1 in column block c, so that lane t ends up with
+    // pair t alone: one softmax state a lane.
+    static_assert(!FV || (NT == 2 && !SPLIT), "the four lanes of a row have a pair each");
+    constexpr int SN = FV ? 1 : NT;          // softmax states of a lane
     extern __shared__ __align__(16) uint8_t smem[];
     asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before ends
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -203,7 +226,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     bool qbad[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const int pair = pair0 + n * PPT + (SPLIT ? g % 4 : g) / CPP;
+        const int pair = pair0 + (FV ? 2 * (g / CPP) + n : n * PPT + (SPLIT ? g % 4 : g) / CPP);
         const bool live = pair < pairs;
         const T* q = static_cast<const T*>(a.q) +
                      ((long long)b * a.n_tokens + (live ? pair / share : 0)) * a.ldq +
@@ -220,15 +243,14 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            constexpr int BITS = ND == 3 ? 22 : 14;
-            constexpr float LIMIT = ND == 3 ? 8355711.0f : 32639.0f;   // the top digit must stay below 128
-            int e = min(127 + BITS - (int)(__float_as_uint(top) >> 23), 126);
+            constexpr float LIMIT = 8355711.0f;   // the top digit must stay below 128
+            int e = min(127 + 22 - (int)(__float_as_uint(top) >> 23), 126);
             if (top * __int_as_float((127 + e) << 23) > LIMIT) e--;
             const float f = __int_as_float((127 + e) << 23);
             uint32_t y[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++) y[i] = (uint32_t)(__float2int_rn(x[i] * f) + (ND == 3 ? 0x8080 : 0x80));
-            const uint32_t flip = g % CPP < ND - 1 ? 0x80808080u : 0u, keep = g % CPP < ND ? ~0u : 0u;
+            for (int i = 0; i < 16; i++) y[i] = (uint32_t)(__float2int_rn(x[i] * f) + 0x8080);
+            const uint32_t flip = g % CPP < 2 ? 0x80808080u : 0u, keep = g % CPP < 3 ? ~0u : 0u;
             int sum = 0;
 #pragma unroll
             for (int h = 0; h < 2; h++)
@@ -252,15 +274,21 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
         qbad[n] = __any_sync(0xfu << (lane & 28), bad);
     }
     const int tp = SPLIT ? 2 * t % 4 : 2 * t;    // the lane's first column, as pairs count them
+    auto lane_pair = [&](int n) { return FV ? t : n * PPT + tp / CPP; };   // of the block's
     // ---- the score factor and the visible range of the lane's pairs
-    float sfac[NT];                          // scale x log2 e (NaN for a query that holds one)
-    int see_sink[NT], see_hi[NT], see_lo[NT];
+    float sfac[SN];                          // scale x log2 e (NaN for a query that holds one)
+    int see_sink[SN], see_hi[SN], see_lo[SN];
     const bool masked = a.n_tokens > 1;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const bool bad = __shfl_sync(0xffffffffu, qbad[n], 8 * t);
+    for (int n = 0; n < SN; n++) {
+        // (columns 2t of the n-tile are lane 8 t's; of FV's pair t, n-tile t % 2's block t / 2, lane 16 (t / 2)'s)
+        bool bad = __shfl_sync(0xffffffffu, qbad[n], FV ? 16 * (t >> 1) : 8 * t);
+        if constexpr (FV) {
+            const bool odd = __shfl_sync(0xffffffffu, qbad[1], 16 * (t >> 1));
+            bad = t & 1 ? odd : bad;
+        }
         sfac[n] = bad ? __int_as_float(0x7fc00000) : a.scale * 1.4426950408889634f;
-        const int pair = min(pair0 + n * PPT + tp / CPP, pairs - 1);
+        const int pair = min(pair0 + lane_pair(n), pairs - 1);
         const long long pos = first + pair / share;
         see_sink[n] = (int)min(pos, (long long)INT32_MAX);
         see_hi[n] = (int)max(-1LL, pos - lo);
@@ -271,17 +299,22 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     const int all_hi = (int)max(-1LL, first + j_lo - lo);
     const int all_lo = a.window ? (int)max(-1LL, first + j_hi - a.window - lo) : -1;
 
-    float m[NT], l[NT];
-    float acc[NT][GA * 4][2];                // elements 64 gr + 8 g + 2 k (and 16 x that of + 1), the lane's digits
+    float m[SN], l[SN];
+    // elements 64 gr + 8 g + 2 k (and 16 x that of + 1), the lane's digits; FV: two parts of each of the two
+    constexpr int AW = FV ? 4 : 2;
+    float acc[SN][GA * 4][AW];
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
+    for (int n = 0; n < SN; n++) {
         m[n] = -INFINITY;
         l[n] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < GA * 4; i++) acc[n][i][0] = acc[n][i][1] = 0.0f;
+        for (int i = 0; i < GA * 4; i++)
+#pragma unroll
+            for (int j = 0; j < AW; j++) acc[n][i][j] = 0.0f;
     }
     // the weights' digits as C columns 2t and 2t + 1 count them
-    const float wd0 = ND == 3 && (t & 1) ? 65536.0f : 1.0f, wd1 = ND == 3 && (t & 1) ? 0.0f : 256.0f;
+    const float wd0 = t & 1 ? 65536.0f : 1.0f, wd1 = t & 1 ? 16777216.0f : 256.0f;
+    const uint32_t wflip = g % CPP < 3 ? 0x80808080u : 0u;
 
     int stage = 0, next = KA_STAGES - 1;
     for (int tile = tile0; tile < ntiles; tile += step) {
@@ -315,9 +348,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     int c[4] = {zero[n][gr][0], zero[n][gr][1], zero[n][gr][0], zero[n][gr][1]};
-                    ka_mma_s(c, (w0.x << 4) & HIGH, (w1.x << 4) & HIGH, (w0.y << 4) & HIGH, (w1.y << 4) & HIGH,
+                    ka_mma(c, (w0.x << 4) & HIGH, (w1.x << 4) & HIGH, (w0.y << 4) & HIGH, (w1.y << 4) & HIGH,
                              qd[n][gr][0][0], qd[n][gr][0][1]);
-                    ka_mma_s(c, w0.x & HIGH, w1.x & HIGH, w0.y & HIGH, w1.y & HIGH, qd[n][gr][1][0], qd[n][gr][1][1]);
+                    ka_mma(c, w0.x & HIGH, w1.x & HIGH, w0.y & HIGH, w1.y & HIGH, qd[n][gr][1][0], qd[n][gr][1][1]);
                     const float u0 = qw[n][gr][0], u1 = qw[n][gr][1];
                     const float s0 = fmaf(__int_as_float(c[1]) - KA_ZEROF, u1, (__int_as_float(c[0]) - KA_ZEROF) * u0);
                     const float s1 = fmaf(__int_as_float(c[3]) - KA_ZEROF, u1, (__int_as_float(c[2]) - KA_ZEROF) * u0);
@@ -330,13 +363,22 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
         const int rel0 = v0 - nsink;
         const bool edge = v0 + KA_TILE > count ||
                           (masked && !(rel0 > all_lo && v0 >= nsink && rel0 + KA_TILE - 1 <= all_hi));
-        uint32_t bw[NT][GA][2];              // digits of weight x value scale
-        float back[NT][GA][2];               // what columns 2t, 2t + 1 count
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
+        uint32_t bw[SN][GA][2];              // digits of weight x value scale (of either sign)
+        uint32_t wb[GA][4];                  // FV: a part of them, tokens t + 8 i and t + 8 i + 4
+        float back[SN][GA][2];               // what columns 2t, 2t + 1 count
+        if constexpr (FV) {
+            // even lanes have digits 0 and 1 of both n-tiles' pairs, odd ones 2 and 3: even take the first n-tile's others
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                if (ND == 3) x[n][r] += __shfl_xor_sync(0xffffffffu, x[n][r], 1);   // the pair's other digits
+                const float other = __shfl_xor_sync(0xffffffffu, t & 1 ? x[0][r] : x[1][r], 1);
+                x[0][r] = (t & 1 ? x[1][r] : x[0][r]) + other;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < SN; n++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                if constexpr (!FV) x[n][r] += __shfl_xor_sync(0xffffffffu, x[n][r], 1);   // the pair's other digits
                 x[n][r] *= sfac[n];
             }
             if (edge) {
@@ -357,10 +399,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
                 l[n] *= c;
                 m[n] = mn;
 #pragma unroll
-                for (int i = 0; i < GA * 4; i++) {
-                    acc[n][i][0] *= c;
-                    acc[n][i][1] *= c;
-                }
+                for (int i = 0; i < GA * 4; i++)
+#pragma unroll
+                    for (int j = 0; j < AW; j++) acc[n][i][j] *= c;
             }
             const float ref = m[n] == -INFINITY ? 0.0f : m[n];
 #pragma unroll
@@ -382,40 +423,38 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
 #pragma unroll
                     for (int i = 0; i < 8; i++) w[i] = p[i] == 0.0f ? 0.0f : w[i];
                 }
+                if constexpr (FV) {          // column g is part g % 2 of pair g / 2: the weight in bf16, or what is left of it
 #pragma unroll
-                for (int i = 0; i < 8; i++) wtop = ka_max_nan(wtop, w[i]);
-                wtop = ka_max_nan(wtop, __shfl_xor_sync(0xffffffffu, wtop, 1));
-                wtop = ka_max_nan(wtop, __shfl_xor_sync(0xffffffffu, wtop, 2));
-                // the power of two that puts the largest in [2^22, 2^23) (or [2^14, 2^15): it may round up to
-                // the next power, which has to fit the digits); 2^23 added, the float's low bytes are the
-                // integer. Below 2^-102 the weights fade out.
-                constexpr uint32_t TOP = ND == 3 ? 22 : 14;
-                const uint32_t e = max(__float_as_uint(wtop) & 0x7F800000u, 25u << 23);
-                const float f = __uint_as_float(((254u + TOP) << 23) - e);
-                uint32_t y[8];
+                    for (int i = 0; i < 8; i += 2) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(w[i], w[i + 1]);
+                        const uint32_t hi = *reinterpret_cast<const uint32_t*>(&h);
+                        const __nv_bfloat162 r = __floats2bfloat162_rn(w[i] - __uint_as_float(hi << 16),
+                                                                       w[i + 1] - __uint_as_float(hi & 0xffff0000u));
+                        wb[gr][i / 2] = g & 1 ? *reinterpret_cast<const uint32_t*>(&r) : hi;
+                    }
+                } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = __float_as_uint(fmaf(w[i], f, 8388608.0f));
-                bw[n][gr][0] = ka_bytes(y[0], y[1], y[2], y[3], dsel);
-                bw[n][gr][1] = ka_bytes(y[4], y[5], y[6], y[7], dsel);
-                // its inverse, NaN where a weight is not finite
-                const float inv = fmaf(wtop, 0.0f, __uint_as_float(e - (TOP << 23)));
-                back[n][gr][0] = __shfl_sync(0xffffffffu, inv, 8 * t) * wd0;
-                back[n][gr][1] = __shfl_sync(0xffffffffu, inv, 8 * t + 4) * wd1;
+                    for (int i = 0; i < 8; i++) wtop = ka_max_nan(wtop, fabsf(w[i]));
+                    wtop = ka_max_nan(wtop, __shfl_xor_sync(0xffffffffu, wtop, 1));
+                    wtop = ka_max_nan(wtop, __shfl_xor_sync(0xffffffffu, wtop, 2));
+                    // the power of two that puts the largest in [2^29, 2^30); 0x808080 added, the lower bytes less
+                    // 128 are the lower digits, the last byte the top one. Below 2^-97 the weights fade out.
+                    constexpr uint32_t TOP = 29;
+                    const uint32_t e = max(__float_as_uint(wtop) & 0x7F800000u, 30u << 23);
+                    const float f = __uint_as_float(((254u + TOP) << 23) - e);
+                    uint32_t y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) y[i] = (uint32_t)__float2int_rn(w[i] * f) + 0x808080u;
+                    bw[n][gr][0] = ka_bytes(y[0], y[1], y[2], y[3], dsel) ^ wflip;
+                    bw[n][gr][1] = ka_bytes(y[4], y[5], y[6], y[7], dsel) ^ wflip;
+                    // its inverse, NaN where a weight is not finite
+                    const float inv = fmaf(wtop, 0.0f, __uint_as_float(e - (TOP << 23)));
+                    back[n][gr][0] = __shfl_sync(0xffffffffu, inv, 8 * t) * wd0;
+                    back[n][gr][1] = __shfl_sync(0xffffffffu, inv, 8 * t + 4) * wd1;
+                }
             }
         }
-        // values
-        int start[NT][GA][4];
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int gr = 0; gr < GA; gr++) {
-                int c[4] = {0, 0, 0, 0};     // the digits' sums over the tile
-                ka_mma_u(c, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, bw[n][gr][0], bw[n][gr][1]);
-                start[n][gr][0] = KA_ZERO - 7 * c[0];
-                start[n][gr][1] = KA_ZERO - 7 * c[1];
-                start[n][gr][2] = KA_ZERO - 112 * c[0];
-                start[n][gr][3] = KA_ZERO - 112 * c[1];
-            }
+        // ---- values
         auto codes = [&](int gr, uint32_t (&w)[8]) {     // word g of the group's eight, tokens t + 4 i
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -424,47 +463,79 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
                 w[i] = *reinterpret_cast<const uint32_t*>(st + C::CODES + r * C::ROW + at);
             }
         };
-        // Byte `byte` of the tokens: element 8 g + 2 byte in the low halves, the next one in the high halves.
-        auto multiply = [&](const uint32_t (&w)[8], int byte, int n, int gr, int (&c)[4]) {
-            const uint32_t sel = (uint32_t)byte * 0x11u + 0x40u;
-            const uint32_t b0 = ka_bytes(w[0], w[1], w[2], w[3], sel), b1 = ka_bytes(w[4], w[5], w[6], w[7], sel);
-#pragma unroll
-            for (int i = 0; i < 4; i++) c[i] = start[n][gr][i];
-            ka_mma_u(c, b0 & LOW, b0 & HIGH, b1 & LOW, b1 & HIGH, bw[n][gr][0], bw[n][gr][1]);
-        };
-        auto add = [&](const int (&c)[4], int n, int gr, int byte) {
-            float* o = acc[n][4 * gr + byte];
-            o[0] = fmaf(__int_as_float(c[0]) - KA_ZEROF, back[n][gr][0], o[0]);
-            o[0] = fmaf(__int_as_float(c[1]) - KA_ZEROF, back[n][gr][1], o[0]);
-            o[1] = fmaf(__int_as_float(c[2]) - KA_ZEROF, back[n][gr][0], o[1]);
-            o[1] = fmaf(__int_as_float(c[3]) - KA_ZEROF, back[n][gr][1], o[1]);
-        };
-        if constexpr (SPLIT) {
-            uint32_t w0[8], w1[8];
-            codes(0, w0);
-            codes(1, w1);
-#pragma unroll
-            for (int byte = 0; byte < 4; byte++) {
-                int c0[4], c1[4];
-                multiply(w0, byte, 0, 0, c0);
-                multiply(w1, byte, 0, 0, c1);
-#pragma unroll
-                for (int i = 0; i < 4; i++) c0[i] = t < 2 ? c0[i] : c1[i];   // the lane's columns' group
-                add(c0, 0, 0, byte);
-            }
-        } else {
+        if constexpr (FV) {
+            // rows g and g + 8 of an A operand are elements 8 g + 2 byte and + 1, its columns tokens t + 16 s + 4 i
 #pragma unroll
             for (int gr = 0; gr < GR; gr++) {
                 uint32_t w[8];
                 codes(gr, w);
 #pragma unroll
-                for (int byte = 0; byte < 4; byte++)
+                for (int byte = 0; byte < 4; byte++) {
+                    const uint32_t sel = (uint32_t)byte * 0x11u | (uint32_t)(4 + byte) * 0x1100u;
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        int c[4];
-                        multiply(w, byte, n, gr, c);
-                        add(c, n, gr, byte);
+                    for (int s = 0; s < 2; s++) {
+                        const uint32_t u = __byte_perm(w[4 * s], w[4 * s + 1], sel);
+                        const uint32_t v = __byte_perm(w[4 * s + 2], w[4 * s + 3], sel);
+                        ka_mma_bf16(acc[0][4 * gr + byte], ka_level(u), ka_level(u >> 4), ka_level(v), ka_level(v >> 4),
+                                    wb[gr][2 * s], wb[gr][2 * s + 1]);
                     }
+                }
+            }
+        } else {
+            int start[SN][GA][4];
+#pragma unroll
+            for (int n = 0; n < SN; n++)
+#pragma unroll
+                for (int gr = 0; gr < GA; gr++) {
+                    int c[4] = {0, 0, 0, 0};     // the digits' sums over the tile
+                    ka_mma(c, 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, bw[n][gr][0], bw[n][gr][1]);
+                    start[n][gr][0] = KA_ZERO - 7 * c[0];
+                    start[n][gr][1] = KA_ZERO - 7 * c[1];
+                    start[n][gr][2] = KA_ZERO - 112 * c[0];
+                    start[n][gr][3] = KA_ZERO - 112 * c[1];
+                }
+            // Byte `byte` of the tokens: element 8 g + 2 byte in the low halves, the next one in the high halves.
+            auto multiply = [&](const uint32_t (&w)[8], int byte, int n, int gr, int (&c)[4]) {
+                const uint32_t sel = (uint32_t)byte * 0x11u + 0x40u;
+                const uint32_t b0 = ka_bytes(w[0], w[1], w[2], w[3], sel), b1 = ka_bytes(w[4], w[5], w[6], w[7], sel);
+#pragma unroll
+                for (int i = 0; i < 4; i++) c[i] = start[n][gr][i];
+                ka_mma(c, b0 & LOW, b0 & HIGH, b1 & LOW, b1 & HIGH, bw[n][gr][0], bw[n][gr][1]);
+            };
+            auto add = [&](const int (&c)[4], int n, int gr, int byte) {
+                float* o = acc[n][4 * gr + byte];
+                o[0] = fmaf(__int_as_float(c[0]) - KA_ZEROF, back[n][gr][0], o[0]);
+                o[0] = fmaf(__int_as_float(c[1]) - KA_ZEROF, back[n][gr][1], o[0]);
+                o[1] = fmaf(__int_as_float(c[2]) - KA_ZEROF, back[n][gr][0], o[1]);
+                o[1] = fmaf(__int_as_float(c[3]) - KA_ZEROF, back[n][gr][1], o[1]);
+            };
+            if constexpr (SPLIT) {
+                uint32_t w0[8], w1[8];
+                codes(0, w0);
+                codes(1, w1);
+#pragma unroll
+                for (int byte = 0; byte < 4; byte++) {
+                    int c0[4], c1[4];
+                    multiply(w0, byte, 0, 0, c0);
+                    multiply(w1, byte, 0, 0, c1);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) c0[i] = t < 2 ? c0[i] : c1[i];   // the lane's columns' group
+                    add(c0, 0, 0, byte);
+                }
+            } else {
+#pragma unroll
+                for (int gr = 0; gr < GR; gr++) {
+                    uint32_t w[8];
+                    codes(gr, w);
+#pragma unroll
+                    for (int byte = 0; byte < 4; byte++)
+#pragma unroll
+                        for (int n = 0; n < SN; n++) {
+                            int c[4];
+                            multiply(w, byte, n, gr, c);
+                            add(c, n, gr, byte);
+                        }
+                }
             }
         }
     }
@@ -474,29 +545,32 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     ka_wait<0>();
     __syncwarp();
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
+    for (int n = 0; n < SN; n++) {
         l[n] += __shfl_xor_sync(0xffffffffu, l[n], 4);
         l[n] += __shfl_xor_sync(0xffffffffu, l[n], 8);
         l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
 #pragma unroll
         for (int k = 0; k < GA * 4; k++) {
-            if (ND == 3) {
+            if constexpr (FV) {
+                acc[n][k][0] += acc[n][k][1];
+                acc[n][k][1] = acc[n][k][2] + acc[n][k][3];
+            } else {
                 acc[n][k][0] += __shfl_xor_sync(0xffffffffu, acc[n][k][0], 1);
                 acc[n][k][1] += __shfl_xor_sync(0xffffffffu, acc[n][k][1], 1);
+                acc[n][k][1] *= 0.0625f;
             }
-            acc[n][k][1] *= 0.0625f;
         }
     }
     auto store_out = [&](int p, int d, float v) {
         static_cast<T*>(a.out)[((long long)b * a.n_tokens + p / share) * a.ldo +
                                (long long)(hk * share + p % share) * HD + d] = dz_from_float<T>(v);
     };
-    const bool speaks = ND == 2 || !(t & 1);   // of two lanes with the same sums
+    const bool speaks = FV || !(t & 1);        // of two lanes with the same sums
     const int e0 = (SPLIT ? 64 * (t >> 1) : 0) + 8 * g;
     if (team * cluster == 1) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int p = pair0 + n * PPT + tp / CPP;
+        for (int n = 0; n < SN; n++) {
+            const int p = pair0 + lane_pair(n);
             if (p >= pairs || !speaks) continue;
             T* o = static_cast<T*>(a.out) + ((long long)b * a.n_tokens + p / share) * a.ldo +
                    (long long)(hk * share + p % share) * HD + e0;
@@ -515,8 +589,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
     static_assert(PAIRS * OS + 2 * PAIRS <= MINE, "a warp's part of the join lies over its ring");
     float* so = reinterpret_cast<float*>(my);
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int pair = n * PPT + tp / CPP;
+    for (int n = 0; n < SN; n++) {
+        const int pair = lane_pair(n);
         if (!speaks) continue;
 #pragma unroll
         for (int gr = 0; gr < GA; gr++)
@@ -586,49 +660,47 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
 }
 
 // Pairs of a block.
-template <int ND, int NT, bool SPLIT> constexpr int ka_pairs() { return NT * (ND == 3 ? 2 : 4) / (SPLIT ? 2 : 1); }
+template <int NT, bool SPLIT> constexpr int ka_pairs() { return NT * 2 / (SPLIT ? 2 : 1); }
 
-template <int HD, int ND, int NT, bool SPLIT> constexpr int ka_smem() {
-    constexpr int pairs = ka_pairs<ND, NT, SPLIT>();
+template <int HD, int NT, bool SPLIT> constexpr int ka_smem() {
+    constexpr int pairs = ka_pairs<NT, SPLIT>();
     return KaCfg<HD>::RING + (pairs * HD + 2 * pairs) * 4;
 }
 
-template <typename T, int HD, int ND, int NT, bool SPLIT>
+template <typename T, int HD, int NT, bool SPLIT, bool FV>
 static cudaError_t ka_launch(const Kv4AttnArgs& a, int device, cudaStream_t st) {
     static Kv4Room rooms[KV4_DEVICES];
-    return kv4_launch(dz_kv4_attn_kernel<T, HD, ND, NT, SPLIT>, rooms, a, ka_pairs<ND, NT, SPLIT>(),
-                      ka_smem<HD, ND, NT, SPLIT>(), device, st);
+    return kv4_launch(dz_kv4_attn_kernel<T, HD, NT, SPLIT, FV>, rooms, a, ka_pairs<NT, SPLIT>(), ka_smem<HD, NT, SPLIT>(), device,
+                      st);
 }
 
 // One n-tile where it holds all pairs of a key head, else two (more leave one
 // block to an SM).
-template <typename T, int HD, int ND>
-static cudaError_t ka_launch_n(const Kv4AttnArgs& a, int device, cudaStream_t st) {
+template <typename T, int HD> static cudaError_t ka_launch_n(const Kv4AttnArgs& a, int device, cudaStream_t st) {
     const int pairs = a.n_tokens * (a.q_heads / a.c.kv_heads);
     if constexpr (HD == 128)
-        if (pairs <= ka_pairs<ND, 1, true>()) return ka_launch<T, HD, ND, 1, true>(a, device, st);
-    if (pairs <= ka_pairs<ND, 1, false>()) return ka_launch<T, HD, ND, 1, false>(a, device, st);
-    return ka_launch<T, HD, ND, 2, false>(a, device, st);
+        if (pairs <= ka_pairs<1, true>()) return ka_launch<T, HD, 1, true, false>(a, device, st);
+    if (pairs <= ka_pairs<1, false>()) return ka_launch<T, HD, 1, false, false>(a, device, st);
+    return ka_launch<T, HD, 2, false, sizeof(T) == 2>(a, device, st);
 }
 
 // Pairs of a key head up to which tokens are the MMA's rows; above, pairs are
 // (kv4chunk.cu). Both on 8 x 4 key heads of 128 that see 4160 tokens, fp32: 4
-// pairs 21 against 22 us, 8 pairs 26 against 24, 128 pairs 218 against 105; fp16:
-// 16 pairs 27 against 32, 24 pairs 41 against 38. Of 64, fp32: 16 pairs 22 each, 24
-// pairs 34 against 25; fp16: 16 pairs 16 against 18, 128 pairs 59 against 45.
+// pairs 22 us each, 8 pairs 27 against 24; fp16: 4 pairs 18 against 25, 8 pairs 21
+// against 27, 16 pairs 30 against 32, 24 pairs 47 against 38. Of 64, fp32: 8 pairs
+// 16 against 19, 16 pairs 23 against 22; fp16: 8 pairs 13 against 16, 16 pairs 18 each.
 static int ka_limit(int type, int head_dim) { return type == DZ_TYPE_F32 && head_dim == 128 ? 4 : 16; }
 
-template <typename T, int ND>
-static cudaError_t ka_launch_t(const Kv4AttnArgs& a, int head_dim, int device, cudaStream_t st) {
-    return head_dim == 128 ? ka_launch_n<T, 128, ND>(a, device, st) : ka_launch_n<T, 64, ND>(a, device, st);
+template <typename T> static cudaError_t ka_launch_t(const Kv4AttnArgs& a, int head_dim, int device, cudaStream_t st) {
+    return head_dim == 128 ? ka_launch_n<T, 128>(a, device, st) : ka_launch_n<T, 64>(a, device, st);
 }
 
 cudaError_t dz_kv4_attn_launch(const Kv4AttnArgs& a, int type, int head_dim, int device, cudaStream_t st) {
     if ((long long)a.n_tokens * (a.q_heads / a.c.kv_heads) > ka_limit(type, head_dim))
         return dz_kv4_chunk_launch(a, type, head_dim, device, st);
-    if (type == DZ_TYPE_F32) return ka_launch_t<float, 3>(a, head_dim, device, st);
-    if (type == DZ_TYPE_F16) return ka_launch_t<__half, 2>(a, head_dim, device, st);
-    return ka_launch_t<__nv_bfloat16, 2>(a, head_dim, device, st);
+    if (type == DZ_TYPE_F32) return ka_launch_t<float>(a, head_dim, device, st);
+    if (type == DZ_TYPE_F16) return ka_launch_t<__half>(a, head_dim, device, st);
+    return ka_launch_t<__nv_bfloat16>(a, head_dim, device, st);
 }
 
 }  // namespace dz

@@ -93,7 +93,8 @@ typedef struct {
  *   codes  [batch][kv_heads][capacity][head_dim / 2] bytes, element e of a row
  *          in the low half of byte e / 2 when e is even, else in its high half
  *   scales [batch][kv_heads][capacity][head_dim / 64] fp32, one per 64 elements
- * value = scale * (code - 7). head_dim is 64 or 128. Position p of a sequence
+ * value = scale * (code - 7), the scale of either sign (a NaN marks 64 elements
+ * that hold none). head_dim is 64 or 128. Position p of a sequence
  * lives in slot p while p < sinks (the first tokens, which stay), else in slot
  * sinks + (p - sinks) % (capacity - sinks): the newest capacity - sinks later
  * positions are retained. sinks < capacity <= 2^31 - 64. Code buffers start on 16-byte

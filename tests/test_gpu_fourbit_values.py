@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import _fourbit as fb
-from test_gpu_fourbit import TYPES, _dz_type, _np, _stream, _typed
+from test_gpu_fourbit import Ring, TYPES, _dz_type, _np, _stream, _typed
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +122,88 @@ def test_products_of_the_longest_rows(gpu):
         ref = xv @ values
         assert (np.abs(got - ref) <= product_bound(xv, values, 32) + fb.rounding(ref, kind)).all(), kind
     q.close()
+
+
+# ----------------------------------------------------------------- attention
+
+PAIRS = [(1, 2, 2), (1, 4, 2), (1, 4, 1), (2, 4, 1), (2, 8, 1), (9, 4, 1)]   # tokens, heads, key heads: both kernels
+
+
+def attend_bound(q, k, v, scale, v_scales, kind, p):
+    """What an evaluation with fp32 sums may lose. A query's element is held to
+    2^-30 of the largest of its 64, or to 2^-22 = 4 u of its own size; a score is
+    the sum of hd / 16 additions of 16 products whose 17 terms may each be off by 2
+    u of the largest, and a dozen roundings. A weight is off by twice its score's
+    error, by the exponential's 2^-21, by 2^-17 (fp16 and bf16: two bf16 parts) or
+    2^-26 of itself or by 2^-30 of the largest in its tile of 32 tokens, all within
+    31 places of it, times a level of at most 7. Values add up in at most 6 such
+    additions of 16 per 32 tokens, and joins in n / 16 + 64 roundings."""
+    n, hd = k.shape
+    tops = np.abs(q).reshape(-1, fb.GROUP).max(1)
+    held = (np.abs(k).reshape(n, -1, fb.GROUP).sum(2) @ tops).max() * 2.0 ** -30
+    score = abs(scale) * ((34 * hd / 16 + 16) * fb.U * (np.abs(k) @ np.abs(q)).max() + held)
+    w = np.pad(p * np.abs(v_scales).max(1), 31)
+    near = np.lib.stride_tricks.sliding_window_view(w, 63).max(1)
+    own = 2.0 ** -26 if kind == "f32" else 2.0 ** -17
+    sums = (n / 16 + 64 + 6 * 34 * (n / 32 + 1)) * fb.U
+    return (2 * score + 2.0 ** -21 + own + sums) * (p @ np.abs(v)) + 7 * 2.0 ** -30 * near.sum()
+
+
+def _attend(gpu, ring, kind, n, hq, first, q, scale, window=0):
+    """Runs attention and compares every output with the formula; returns the outputs."""
+    qt, qv = _typed(q, kind)
+    out = torch.full((ring.batch * n, hq * ring.hd), 9.0, dtype=TYPES[kind], device="cuda")
+    pos = torch.tensor(first, dtype=torch.int64, device="cuda")
+    ring.cache.attention(pos.data_ptr(), n, type=_dz_type(gpu, kind), q_heads=hq, q=qt.data_ptr(), out=out.data_ptr(),
+                         scale=scale, window=window, stream_ptr=_stream())
+    torch.cuda.synchronize()
+    got = _np(out).reshape(ring.batch, n, hq, ring.hd)
+    qv = qv.reshape(ring.batch, n, hq, ring.hd)
+    for b, f in enumerate(first):
+        for h in range(hq):
+            kv = [ring.rows(w, b, h * ring.heads // hq, list(range(ring.cap))) for w in range(2)]
+            vs = ring.scale_rows(1, b, h * ring.heads // hq, list(range(ring.cap)))
+            for j in range(n):
+                slots = [fb.slot(p, ring.sinks, ring.cap)
+                         for p in fb.visible(f + j, f + n - 1, ring.sinks, ring.cap, window)]
+                k, v = (x[slots] for x in kv)
+                e = scale * (k @ qv[b, j, h])
+                e = np.exp(e - e.max())
+                ref = (e / e.sum()) @ v
+                bound = attend_bound(qv[b, j, h], k, v, scale, vs[slots], kind, e / e.sum())
+                err = np.abs(got[b, j, h] - ref) - 1.001 * fb.rounding(ref, kind)
+                assert (err <= bound).all(), (b, j, h, (err / bound).max())
+    return got
+
+
+@pytest.mark.parametrize("n,hq,hk", PAIRS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_attention_with_scales_of_both_signs(gpu, n, hq, hk, hd, kind):
+    """A scale's sign is the caller's: value = scale * (code - 7) for keys and values."""
+    rng = np.random.RandomState(31 + n + hd)
+    ring = Ring(gpu, 2, hk, hd, 150, 3, rng)
+    for s in ring.scales:
+        s.mul_(torch.from_numpy(rng.choice([-1.0, 1.0], s.shape).astype(np.float32)).cuda())
+    _attend(gpu, ring, kind, n, hq, [140, 4321], rng.randn(2 * n, hq, hd), hd ** -0.5)
+    ring.scales[1].abs_().neg_()
+    _attend(gpu, ring, kind, n, hq, [77, 30], rng.randn(2 * n, hq, hd), hd ** -0.5, window=100)
+
+
+@pytest.mark.parametrize("n,hq,hk", PAIRS)
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_attention_beside_a_token_that_takes_all_weight(gpu, n, hq, hk, kind):
+    """The first token takes all weight but 2^-12 or so and holds level 0 in half of the elements: there
+    the others alone make the result, most of all those of its own tile."""
+    rng = np.random.RandomState(41 + n)
+    hd, count = 128, 40
+    ring = Ring(gpu, 1, hk, hd, 60, 0, rng)
+    q = rng.choice([-1.0, 1.0], hd)
+    for h in range(hk):
+        at = h * ring.cap
+        level = (7 + 7 * q).astype(np.uint8)                  # key: +-7 along the query
+        ring.codes[0][at] = torch.from_numpy(level[0::2] | level[1::2] << 4).cuda()
+        ring.scales[0][at] = 0.25
+        ring.codes[1][at] = ring.codes[1][at] & 0xF0 | 7      # value: even elements level 0
+        ring.scales[0][at + 1:at + ring.cap] = 2.0 ** -10
+    _attend(gpu, ring, kind, n, hq, [count - n], np.broadcast_to(q, (n, hq, hd)), 0.04)
