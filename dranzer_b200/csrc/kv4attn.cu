@@ -19,10 +19,10 @@
 //   values   A = 16 elements of V^T x 32 tokens, B = the digits of weight x
 //            value scale (of either sign), integers after a power of two per
 //            tile and group. Tile sums add up in fp32.
-// A pair takes 4 of the 8 columns: three digits of a query (half a step is at most
-// 1 / (2 x 4177855) of the group's largest element), four of a weight (2^-30 of the
-// tile's largest weight x scale). An accumulator starts at the bits of 1.5 x 2^23
-// (less the 7s): its bits read as a float are 1.5 x 2^23 plus the sum.
+// A pair takes 4 of the 8 columns. Half a step is at most 2^-30 of the group's
+// largest element, or of the tile's largest weight x scale: 16-bit queries are
+// exact but for what lies below that. An accumulator starts at the bits of 1.5 x
+// 2^23 (less the 7s): its bits read as a float are 1.5 x 2^23 plus the sum.
 //
 // 3 or 4 pairs of 16-bit types (FV) take their values in the 16-bit MMA: weight x
 // scale in two bf16 parts (2^-17 of itself), two columns for a pair, levels widened
@@ -243,27 +243,26 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            constexpr float LIMIT = 8355711.0f;   // the top digit must stay below 128
-            int e = min(127 + 22 - (int)(__float_as_uint(top) >> 23), 126);
-            if (top * __int_as_float((127 + e) << 23) > LIMIT) e--;
+            // the power of two that puts the largest in [2^29, 2^30)
+            const int e = min(127 + 29 - (int)(__float_as_uint(top) >> 23), 126);
             const float f = __int_as_float((127 + e) << 23);
             uint32_t y[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++) y[i] = (uint32_t)(__float2int_rn(x[i] * f) + 0x8080);
-            const uint32_t flip = g % CPP < 2 ? 0x80808080u : 0u, keep = g % CPP < 3 ? ~0u : 0u;
+            for (int i = 0; i < 16; i++) y[i] = (uint32_t)__float2int_rn(x[i] * f) + 0x808080u;
+            const uint32_t flip = g % CPP < 3 ? 0x80808080u : 0u;   // the lower digits' 128 taken off
             int sum = 0;
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     const uint32_t* z = y + 8 * j + h;
-                    qd[n][gr][h][j] = (ka_bytes(z[0], z[2], z[4], z[6], dsel) ^ flip) & keep;
+                    qd[n][gr][h][j] = ka_bytes(z[0], z[2], z[4], z[6], dsel) ^ flip;
                     sum = __dp4a((int)qd[n][gr][h][j], 0x01010101, sum);
                 }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             const int start0 = KA_ZERO - 112 * sum;
-            const float digit = g % CPP == 0 ? 0.0625f : g % CPP == 1 ? 16.0f : g % CPP == 2 ? 4096.0f : 0.0f;
+            const float digit = g % CPP == 0 ? 0.0625f : g % CPP == 1 ? 16.0f : g % CPP == 2 ? 4096.0f : 1048576.0f;
             const float weight = digit * __int_as_float((127 - e) << 23);
 #pragma unroll
             for (int i = 0; i < 2; i++) {

@@ -149,7 +149,8 @@ int dz_cuda_kv4_append(const dz_kv4_t *cache, const dz_kv4_append_t *args, const
  * window, window + n_tokens - 1 <= capacity - sinks is asked (so that no
  * query has lost a token of its window), and n_tokens <= capacity - sinks
  * always. Scores, softmax statistics and sums are fp32, scales of either sign. A
- * query's element is held to 2^-22 of the largest of its 64, a softmax weight x
+ * query's element is held to 2^-30 of the largest of its 64 or to 2^-22 of itself
+ * (fp16, bf16: to 2^-30 of the largest of its head), a softmax weight x
  * value scale to 2^-26 (fp16, bf16: 2^-17) of itself or to 2^-30 of the largest in
  * its tile of 32 tokens. out must not overlap q or the cache. */
 int dz_cuda_kv4_attention(const dz_kv4_t *cache, const dz_kv4_attention_t *args, const int64_t *positions,

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import _fourbit as fb
+from _fourbit import GROUP
 from test_gpu_fourbit import Ring, TYPES, _dz_type, _np, _stream, _typed
 
 pytestmark = pytest.mark.gpu
@@ -139,8 +140,8 @@ def attend_bound(q, k, v, scale, v_scales, kind, p):
     31 places of it, times a level of at most 7. Values add up in at most 6 such
     additions of 16 per 32 tokens, and joins in n / 16 + 64 roundings."""
     n, hd = k.shape
-    tops = np.abs(q).reshape(-1, fb.GROUP).max(1)
-    held = (np.abs(k).reshape(n, -1, fb.GROUP).sum(2) @ tops).max() * 2.0 ** -30
+    tops = np.abs(q).reshape(-1, GROUP).max(1)
+    held = (np.abs(k).reshape(n, -1, GROUP).sum(2) @ tops).max() * 2.0 ** -30
     score = abs(scale) * ((34 * hd / 16 + 16) * fb.U * (np.abs(k) @ np.abs(q)).max() + held)
     w = np.pad(p * np.abs(v_scales).max(1), 31)
     near = np.lib.stride_tricks.sliding_window_view(w, 63).max(1)
@@ -207,3 +208,21 @@ def test_attention_beside_a_token_that_takes_all_weight(gpu, n, hq, hk, kind):
         ring.codes[1][at] = ring.codes[1][at] & 0xF0 | 7      # value: even elements level 0
         ring.scales[0][at + 1:at + ring.cap] = 2.0 ** -10
     _attend(gpu, ring, kind, n, hq, [count - n], np.broadcast_to(q, (n, hq, hd)), 0.04)
+
+
+@pytest.mark.parametrize("n,hq,hk", PAIRS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_attention_of_queries_with_large_elements(gpu, n, hq, hk, hd, kind):
+    """Every 64 elements of a query hold one 2^12 to 2^15 above the rest, at which all keys hold level 0: the
+    others alone make the scores, as precisely with few pairs to a key head as with many."""
+    rng = np.random.RandomState(51 + n + hd)
+    ring = Ring(gpu, 2, hk, hd, 150, 3, rng)
+    large = np.arange(rng.randint(GROUP), hd, GROUP)
+    for e in large:
+        codes = ring.codes[0][:, e // 2]
+        codes.copy_(codes & 0xF0 | 7 if e % 2 == 0 else codes & 0x0F | 0x70)
+    for top in (12, 15):
+        q = rng.randn(2 * n, hq, hd) * (0.5 if kind == "f16" else 1)
+        q[..., large] = 2.0 ** top * rng.uniform(0.6, 0.95, (2 * n, hq, large.size))
+        _attend(gpu, ring, kind, n, hq, [140, 4321], q, 0.25)
