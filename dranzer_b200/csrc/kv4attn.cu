@@ -685,17 +685,18 @@ template <typename T, int HD> static cudaError_t ka_launch_n(const Kv4AttnArgs& 
 
 // Pairs of a key head up to which tokens are the MMA's rows; above, pairs are
 // (kv4chunk.cu). Both on 8 x 4 key heads of 128 that see 4160 tokens, fp32: 4
-// pairs 22 us each, 8 pairs 27 against 24; fp16: 4 pairs 18 against 25, 8 pairs 21
-// against 27, 16 pairs 30 against 32, 24 pairs 47 against 38. Of 64, fp32: 8 pairs
-// 16 against 19, 16 pairs 23 against 22; fp16: 8 pairs 13 against 16, 16 pairs 18 each.
-static int ka_limit(int type, int head_dim) { return type == DZ_TYPE_F32 && head_dim == 128 ? 4 : 16; }
+// pairs 22 us each, 8 pairs 27 against 24; fp16: 4 pairs 18 against 17, 8 pairs 21
+// against 19 (2 x 8 key heads, 130k tokens, bf16: 4 pairs 103 against 165, 8 pairs 155
+// against 167), 16 pairs 30 against 22. Of 64, fp32: 8 pairs 16 against 19, 16 pairs
+// 23 against 21; fp16: 8 pairs 13 against 15, 16 pairs 18 against 17.
+static int ka_limit(int head_dim) { return head_dim == 128 ? 4 : 8; }
 
 template <typename T> static cudaError_t ka_launch_t(const Kv4AttnArgs& a, int head_dim, int device, cudaStream_t st) {
     return head_dim == 128 ? ka_launch_n<T, 128>(a, device, st) : ka_launch_n<T, 64>(a, device, st);
 }
 
 cudaError_t dz_kv4_attn_launch(const Kv4AttnArgs& a, int type, int head_dim, int device, cudaStream_t st) {
-    if ((long long)a.n_tokens * (a.q_heads / a.c.kv_heads) > ka_limit(type, head_dim))
+    if ((long long)a.n_tokens * (a.q_heads / a.c.kv_heads) > ka_limit(head_dim))
         return dz_kv4_chunk_launch(a, type, head_dim, device, st);
     if (type == DZ_TYPE_F32) return ka_launch_t<float>(a, head_dim, device, st);
     if (type == DZ_TYPE_F16) return ka_launch_t<__half>(a, head_dim, device, st);
