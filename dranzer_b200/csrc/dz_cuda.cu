@@ -1558,6 +1558,7 @@ struct dz_cuda_cache {
     // a dz_kv4_t, and the rows that a step's (or a prefill's) products write
     bool kv4 = false;
     int sinks = 0, window = 0;
+    cudaError_t kv4_error = cudaSuccess;       // of the first launch since take_kv4_error that failed
     uint8_t* kv4_codes = nullptr;              // [L][keys, values][B][Hl][cap][hd / 2]
     float* kv4_scales = nullptr;               // [L][keys, values][B][Hl][cap][hd / 64]
     float *k_rows = nullptr, *v_rows = nullptr;   // [B][dl]
@@ -1871,8 +1872,17 @@ static Kv4Cache kv4_layer(const dz_cuda_cache_t* c, size_t l, int s0, int ns) {
     return k;
 }
 
+// What the 4-bit launches enqueued since the last call came to: their launchers
+// may refuse before anything reaches the runtime's last error.
+static cudaError_t take_kv4_error(dz_cuda_cache_t* c) {
+    const cudaError_t e = c->kv4_error;
+    c->kv4_error = cudaSuccess;
+    return e;
+}
+
 // The layer's rotation and quantization of n new tokens of every sequence,
-// and their attention. q, k, v: rows [ns x n][dl] (q rotated in place).
+// and their attention. q, k, v: rows [ns x n][dl] (q rotated in place). A
+// failed launch is kept in c->kv4_error, and nothing is enqueued after it.
 static void kv4_append_attend(dz_cuda_cache_t* c, size_t l, int s0, int ns, int n, const long long* positions,
                               long long pos_add, float* q, const float* k, const float* v, float* out) {
     const dz_cuda_model_t* m = c->model;
@@ -1892,7 +1902,7 @@ static void kv4_append_attend(dz_cuda_cache_t* c, size_t l, int s0, int ns, int 
         a.rope = 1;
         dz_kv4_frequencies(10000.0, hd, a.freq);
     }
-    dz_kv4_append_launch(a, DZ_TYPE_F32, hd, m->device, c->stream);
+    if (c->kv4_error == cudaSuccess) c->kv4_error = dz_kv4_append_launch(a, DZ_TYPE_F32, hd, m->device, c->stream);
     Kv4AttnArgs t = {};
     t.c = a.c;
     t.positions = positions;
@@ -1904,7 +1914,7 @@ static void kv4_append_attend(dz_cuda_cache_t* c, size_t l, int s0, int ns, int 
     t.q_heads = m->Hl;
     t.scale = 1.0f / sqrtf((float)hd);
     t.window = c->window;
-    dz_kv4_attn_launch(t, DZ_TYPE_F32, hd, m->device, c->stream);
+    if (c->kv4_error == cudaSuccess) c->kv4_error = dz_kv4_attn_launch(t, DZ_TYPE_F32, hd, m->device, c->stream);
 }
 
 // Launches of one layer pass over R rows and of the output head.
@@ -2198,6 +2208,9 @@ extern "C" int dz_cuda_forward_tokens(dz_cuda_cache_t* c, const uint32_t* token_
         DZ_CUDA(cudaStreamBeginCapture(c->stream, cudaStreamCaptureModeThreadLocal));
         enqueue_step(c, c->tok, 1);
         cudaError_t e = cudaStreamEndCapture(c->stream, &graph);
+        const cudaError_t kv4 = take_kv4_error(c);
+        if (e == cudaSuccess && kv4 != cudaSuccess) cudaGraphDestroy(graph);   // it lacks the launches that failed
+        DZ_CUDA(kv4);
         if (e != cudaSuccess) return fail(DZ_E_DEVICE, "capture: %s", cudaGetErrorString(e));
         e = cudaGraphInstantiate(&c->step_graph, graph, 0);
         cudaGraphDestroy(graph);
@@ -2665,6 +2678,7 @@ static int generate_async(dz_cuda_cache_t* c, const uint32_t* prompts, size_t pl
     if (dz_cuda_generate_launches(c, plen, n_new, s) > GRAPH_MAX_LAUNCHES) {
         // jobs this long launch directly: a graph of this many nodes costs more to build than it saves
         enqueue_generate(c, prompts, plen, n_new, s, sampled ? seeds : nullptr, out, ctl);
+        DZ_CUDA(take_kv4_error(c));
         DZ_CUDA(cudaGetLastError());
         return DZ_OK;
     }
@@ -2674,6 +2688,9 @@ static int generate_async(dz_cuda_cache_t* c, const uint32_t* prompts, size_t pl
         DZ_CUDA(cudaStreamBeginCapture(c->stream, cudaStreamCaptureModeThreadLocal));
         enqueue_generate(c, prompts, plen, n_new, s, sampled ? seeds : nullptr, out, ctl);
         cudaError_t e = cudaStreamEndCapture(c->stream, &graph);
+        const cudaError_t kv4 = take_kv4_error(c);
+        if (e == cudaSuccess && kv4 != cudaSuccess) cudaGraphDestroy(graph);
+        DZ_CUDA(kv4);
         if (e != cudaSuccess) return fail(DZ_E_DEVICE, "capture: %s", cudaGetErrorString(e));
         cudaGraphExec_t exec;
         e = cudaGraphInstantiate(&exec, graph, 0);
@@ -2855,6 +2872,7 @@ extern "C" int dz_cuda_prefill(dz_cuda_cache_t* c, const uint32_t* ids, const ui
         c->seen, c->seen_words, nullptr);
     c->seen_valid = true;
     enqueue_prefill(c, c->pf_ids, (long long)prompt_len, (int)prompt_len, lens ? c->pf_lens : nullptr);
+    DZ_CUDA(take_kv4_error(c));
     DZ_CUDA(cudaGetLastError());
     if (logits_out)
         DZ_CUDA(cudaMemcpyAsync(logits_out, c->logits, B * c->model->desc.vocab_size * 4, cudaMemcpyDeviceToHost,
@@ -2978,7 +2996,8 @@ extern "C" int dz_cuda_profile_generate(dz_cuda_cache_t* c, const uint32_t* prom
     c->prof_ctx_flops_per_layer = 4.0 * D * mean_ctx * c->B;
     enqueue_generate(c, prompts, plen, n_new, s, sampled ? seeds : nullptr, out);
     g_prof = nullptr;
-    cudaError_t e = cudaStreamSynchronize(c->stream);
+    cudaError_t e = take_kv4_error(c);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
     for (size_t k = 0; k < n_stats; k++) {
         stats[k].kind = (uint32_t)k;
         stats[k].launches = 0;

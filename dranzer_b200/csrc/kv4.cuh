@@ -59,9 +59,9 @@ struct Kv4AttnArgs {
 // base^(-2p / head_dim) for p < head_dim / 2, the rest 0 (all 0 for base 0).
 void dz_kv4_frequencies(double base, size_t head_dim, double* freq);
 
-cudaError_t dz_kv4_append_launch(const Kv4AppendArgs& a, int type, int head_dim, int device, cudaStream_t st);
+[[nodiscard]] cudaError_t dz_kv4_append_launch(const Kv4AppendArgs& a, int type, int head_dim, int device, cudaStream_t st);
 // Picks the kernel: kv4attn.cu for few pairs to a key head, kv4chunk.cu for many.
-cudaError_t dz_kv4_chunk_launch(const Kv4AttnArgs& a, int type, int head_dim, int device, cudaStream_t st);
-cudaError_t dz_kv4_attn_launch(const Kv4AttnArgs& a, int type, int head_dim, int device, cudaStream_t st);
+[[nodiscard]] cudaError_t dz_kv4_chunk_launch(const Kv4AttnArgs& a, int type, int head_dim, int device, cudaStream_t st);
+[[nodiscard]] cudaError_t dz_kv4_attn_launch(const Kv4AttnArgs& a, int type, int head_dim, int device, cudaStream_t st);
 
 }  // namespace dz
