@@ -640,18 +640,26 @@ cudaError_t dz_gmv_launch(const GmvArgs& a, int device, cudaStream_t st) {
     GmvArgs b = a;
     GmvPlan plan;
     const GmvShape shape = gmv_shape(a.w, a.type);
-    for (int m = 0; m < a.M; m += plan.rows) {
-        if (!gmv_plan(shape, a.M - m, *room, &plan)) return cudaErrorNotSupported;
-        b.x = static_cast<const uint8_t*>(a.x) + (long long)m * a.ldx * type_bytes(a.type);
-        b.y = static_cast<uint8_t*>(a.y) + (long long)m * a.ldy * type_bytes(a.type);
-        cudaError_t e;
-        if (a.w.group == 128)
-            e = a.w.scale_f16 ? gmv_launch_n<1, __half>(b, plan, device, st) : gmv_launch_n<1, float>(b, plan, device, st);
-        else if (a.w.group == 64)
-            e = a.w.scale_f16 ? gmv_launch_n<2, __half>(b, plan, device, st) : gmv_launch_n<2, float>(b, plan, device, st);
-        else
-            e = a.w.scale_f16 ? gmv_launch_n<4, __half>(b, plan, device, st) : gmv_launch_n<4, float>(b, plan, device, st);
-        if (e != cudaSuccess) return e;
+    const int bytes = (int)type_bytes(a.type);
+    for (int tile = 0, tiles; tile < a.w.ntiles; tile += tiles) {   // all of them at once but for the widest matrices
+        tiles = gmv_plan_tiles(shape, a.w.ntiles - tile, a.M, *room, &plan);
+        if (!tiles) return cudaErrorNotSupported;
+        b.w.rec = a.w.rec + (long long)tile * a.w.nblocks * a.w.rec_bytes;
+        b.w.ntiles = tiles;
+        b.w.N = a.w.N - tile * GMV_TILE;
+        for (int m = 0; m < a.M; m += plan.rows) {
+            if (m && !gmv_plan(gmv_shape(b.w, a.type), a.M - m, *room, &plan)) return cudaErrorNotSupported;
+            b.x = static_cast<const uint8_t*>(a.x) + (long long)m * a.ldx * bytes;
+            b.y = static_cast<uint8_t*>(a.y) + ((long long)m * a.ldy + (long long)tile * GMV_TILE) * bytes;
+            cudaError_t e;
+            if (a.w.group == 128)
+                e = a.w.scale_f16 ? gmv_launch_n<1, __half>(b, plan, device, st) : gmv_launch_n<1, float>(b, plan, device, st);
+            else if (a.w.group == 64)
+                e = a.w.scale_f16 ? gmv_launch_n<2, __half>(b, plan, device, st) : gmv_launch_n<2, float>(b, plan, device, st);
+            else
+                e = a.w.scale_f16 ? gmv_launch_n<4, __half>(b, plan, device, st) : gmv_launch_n<4, float>(b, plan, device, st);
+            if (e != cudaSuccess) return e;
+        }
     }
     return cudaSuccess;
 }
@@ -665,7 +673,7 @@ struct dz_cuda_gmatrix {
     GmvMatrix m;
 };
 
-// K and N up to 2^24 and at most 2^31 records keep the kernels' indexes in range.
+// K and N up to 2^24 and at most 2^30 records keep the kernels' indexes in range.
 constexpr size_t GMV_MAX_DIM = (size_t)1 << 24;
 
 static int gmv_check(const dz_grouped_blob_t* w) {
@@ -736,9 +744,9 @@ extern "C" int dz_cuda_gmatrix_create(int device, const dz_grouped_blob_t* w, dz
     GmvPlan plan;
     const GmvRoom* room;
     DZ_CUDA(gmv_room(device, &room));
-    if (!gmv_plan(gmv_shape(m, DZ_TYPE_F32), 1, *room, &plan))
-        return fail(DZ_E_UNSUPPORTED, "gmatrix: %zu x %zu is too large for a product's shared memory", w->rows, w->cols);
     if ((long long)m.ntiles * m.nblocks > (1LL << 30)) return fail(DZ_E_UNSUPPORTED, "gmatrix: too many weights");
+    if (!gmv_plan_tiles(gmv_shape(m, DZ_TYPE_F32), 1, 1, *room, &plan))
+        return fail(DZ_E_UNSUPPORTED, "gmatrix: %zu rows are too many for a product's shared memory", w->rows);
     auto* q = new (std::nothrow) dz_cuda_gmatrix;
     if (!q) return fail(DZ_E_NOMEM, "host allocation");
     cudaStream_t st = nullptr;

@@ -131,4 +131,13 @@ inline bool gmv_plan(const GmvShape& a, int rows, const GmvRoom& room, GmvPlan* 
     return false;
 }
 
+// The tiles that one launch takes of the matrix's last `tiles` (their sums lie in
+// shared memory), and its plan; 0: not even one.
+inline int gmv_plan_tiles(const GmvShape& a, int tiles, int rows, const GmvRoom& room, GmvPlan* plan) {
+    GmvShape s = a;
+    for (s.ntiles = tiles; s.ntiles >= 1; s.ntiles /= 2)
+        if (gmv_plan(s, rows, room, plan)) return s.ntiles;
+    return 0;
+}
+
 }  // namespace dz

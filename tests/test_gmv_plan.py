@@ -25,7 +25,11 @@ int main() {
             }
         GmvShape s{(int)((n + 31) / 32), (int)((k + 127) / 128), group, GMV_CODES + 128 / group * 32 * sb, parts};
         GmvPlan p{};
-        const bool ok = gmv_plan(s, (int)rows, room, &p);
+        int ok = gmv_plan(s, (int)rows, room, &p);
+        if (!ok) {
+            const int tiles = gmv_plan_tiles(s, s.ntiles, (int)rows, room, &p);
+            ok = -tiles;   // the first launch of several takes so many
+        }
         printf("%d %d %d %d %d %d %d %d\n", ok, p.rows, p.digits, p.cluster, p.clusters, p.slice, p.tiles,
                ok ? gmv_smem(s, p) : 0);
     }
@@ -77,7 +81,7 @@ def test_clusters_that_the_device_cannot_hold_are_not_chosen(plan, most):
     keep = [1 << i <= most for i in range(5)] * 2
     room = [v if k else 0 for v, k in zip([20, 10, 5, 2, 1, 40, 20, 10, 4, 2], keep)]
     for c, p in zip(CASES, plan([(c, room) for c in CASES])):
-        if p["ok"]:
+        if p["ok"] > 0:
             assert p["cluster"] <= most
             _check(c, room, p)
         else:
@@ -87,3 +91,25 @@ def test_clusters_that_the_device_cannot_hold_are_not_chosen(plan, most):
 
 def test_a_device_that_holds_no_block_has_no_plan(plan):
     assert not plan([((1, 4096, 4096, 128, 4, 3), [0] * 10)])[0]["ok"]
+
+
+def test_wide_matrices_go_in_several_launches(plan):
+    """Tiles whose sums do not fit shared memory beside long rows; the first launch's plan holds its share."""
+    cases = [(rows, k, n, group, 4, parts) for rows in (1, 16) for k, n in ((100000, 300000), (200000, 200000), (64, 1 << 24),
+             (4096, 1 << 24)) for group in (32, 128) for parts in (1, 3)]
+    for c, p in zip(cases, plan([(c, FULL) for c in cases])):
+        assert p["ok"] != 0, c
+        if p["ok"] < 0:
+            assert -p["ok"] < -(-c[2] // 32)
+            _check((c[0], c[1], -p["ok"] * 32), FULL, p)
+        else:
+            _check(c, FULL, p)
+
+
+def test_the_longest_rows(plan):
+    """Rows of 348000 (what three digits of fp32 fitted) and more still have a plan, of any type and group."""
+    cases = [(rows, 350000, 64, group, sb, parts) for rows in (1, 2, 16) for group in (32, 64, 128) for sb in (2, 4)
+             for parts in (1, 3)]
+    for c, p in zip(cases, plan([(c, FULL) for c in cases])):
+        assert p["ok"] > 0, c
+        _check(c, FULL, p)

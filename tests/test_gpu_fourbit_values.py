@@ -125,6 +125,29 @@ def test_products_of_the_longest_rows(gpu):
     q.close()
 
 
+def test_product_in_several_launches(gpu):
+    """K so long and N so wide that a launch takes a range of the columns; strided rows, guard columns."""
+    rng = np.random.RandomState(25)
+    k, n, m, group = 360000, 20011, 2, 32
+    codes = torch.randint(0, 15, (k * n // 2 + 1,), dtype=torch.uint8, device="cuda")
+    codes.mul_(16).add_(torch.randint(0, 15, codes.shape, dtype=torch.uint8, device="cuda"))
+    scales = torch.rand(-(-k // group), n, device="cuda") * 0.01
+    q = gpu.GroupedWeightMatrix.from_device(scales.data_ptr(), codes.data_ptr(), k, n, group)
+    x = torch.from_numpy(rng.randn(m, k + 3).astype(np.float32)).cuda()
+    y = torch.full((m, n + 5), 9.0, device="cuda")
+    q.matmul_async(x.data_ptr(), y.data_ptr(), m, _stream(), lda=k + 3, ldc=n + 5)
+    torch.cuda.synchronize()
+    assert (y[:, n:] == 9.0).all()
+    pick = torch.cat([torch.arange(0, n, 997), torch.arange(n - 40, n)]).cuda()
+    at = torch.arange(k, device="cuda")[:, None] * n + pick
+    byte = codes[at // 2].long()
+    w = (torch.where(at % 2 == 0, byte & 15, byte >> 4).double() - 7) * scales[:, pick].double().repeat_interleave(group, 0)[:k]
+    w, xv = w.cpu().numpy(), _np(x[:, :k])
+    ref = xv @ w
+    assert (np.abs(_np(y[:, pick]) - ref) <= product_bound(xv, w, group) + fb.rounding(ref, "f32")).all()
+    q.close()
+
+
 # ----------------------------------------------------------------- attention
 
 PAIRS = [(1, 2, 2), (1, 4, 2), (1, 4, 1), (2, 4, 1), (2, 8, 1), (9, 4, 1)]   # tokens, heads, key heads: both kernels
