@@ -690,23 +690,30 @@ static int gmv_check(const dz_grouped_blob_t* w) {
     return DZ_OK;
 }
 
-// Lays w out into m->rec on the current device; the staging copies live here.
-static int gmv_fill(const dz_grouped_blob_t* w, GmvMatrix* m, cudaStream_t st, uint8_t** codes, uint8_t** scales,
-                    int** bad) {
+// Lays w out into m->rec on `device`, the current one; the staging copies live here.
+static int gmv_fill(const dz_grouped_blob_t* w, GmvMatrix* m, int device, cudaStream_t st, uint8_t** codes,
+                    uint8_t** scales, int** bad) {
     const size_t sb = w->scale_count * (m->scale_f16 ? 2 : 4);
     const long long recs = (long long)m->ntiles * m->nblocks;
     DZ_CUDA(cudaMalloc(&m->rec, (size_t)recs * m->rec_bytes));
     DZ_CUDA(cudaMalloc(codes, w->packed_size));
     DZ_CUDA(cudaMalloc(scales, sb));
     DZ_CUDA(cudaMalloc(bad, 4));
-    // sources in device memory may still be written by any stream
+    // sources in device memory may still be written by any stream of theirs
+    bool waited = false;
     for (const void* src : {(const void*)w->packed, w->scales}) {
         cudaPointerAttributes at;
-        if (cudaPointerGetAttributes(&at, src) != cudaSuccess)
+        if (cudaPointerGetAttributes(&at, src) != cudaSuccess) {
             (void)cudaGetLastError();
-        else if (at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged) {
+            continue;
+        }
+        if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) continue;
+        if (!waited) DZ_CUDA(cudaDeviceSynchronize());
+        waited = true;
+        if (at.device != device) {
+            DeviceGuard other(at.device);
+            if (!other.ok) return fail(DZ_E_DEVICE, "cannot select device %d", at.device);
             DZ_CUDA(cudaDeviceSynchronize());
-            break;
         }
     }
     DZ_CUDA(cudaMemcpyAsync(*codes, w->packed, w->packed_size, cudaMemcpyDefault, st));
@@ -754,7 +761,7 @@ extern "C" int dz_cuda_gmatrix_create(int device, const dz_grouped_blob_t* w, dz
     int* bad = nullptr;
     if (cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) != cudaSuccess)
         rc = fail(DZ_E_DEVICE, "stream creation failed");
-    if (!rc) rc = gmv_fill(w, &m, st, &codes, &scales, &bad);
+    if (!rc) rc = gmv_fill(w, &m, device, st, &codes, &scales, &bad);
     cudaFree(codes);
     cudaFree(scales);
     cudaFree(bad);

@@ -101,7 +101,8 @@ typedef struct dz_cuda_gmatrix dz_cuda_gmatrix_t;
 /* Lays the matrix out on `device`; `packed` and `scales` may be host or device
  * memory and are copied. DZ_E_INVALID for a code of 15, a scale that is
  * negative or not finite, or sizes that do not belong together. Synchronous;
- * for sources in device memory it first waits for all work on `device`. */
+ * for sources in device memory it first waits for all work on `device` and on
+ * the device that holds them. */
 int dz_cuda_gmatrix_create(int device, const dz_grouped_blob_t *weights, dz_cuda_gmatrix_t **out);
 void dz_cuda_gmatrix_free(dz_cuda_gmatrix_t *matrix);
 /* Device bytes of codes + scales a product streams. */

@@ -148,6 +148,26 @@ def test_product_in_several_launches(gpu):
     q.close()
 
 
+def test_matrix_from_codes_that_another_device_still_writes(gpu):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two devices")
+    k, n, group = 4096, 4096, 128
+    rng = np.random.RandomState(26)
+    s, p = gpu.quantize_pack_grouped(rng.randn(k, n).astype(np.float32), group)
+    with torch.cuda.device(1):
+        ps, pp = torch.from_numpy(s).pin_memory(), torch.from_numpy(p).pin_memory()
+        a = torch.randn(8192, 8192, device="cuda:1")
+        ds, dp = torch.zeros(s.shape, device="cuda:1"), torch.zeros(p.shape, dtype=torch.uint8, device="cuda:1")
+        torch.cuda.synchronize()
+        for _ in range(20):
+            a = a @ a * 1e-4
+        ds.copy_(ps, non_blocking=True)
+        dp.copy_(pp, non_blocking=True)
+    q = gpu.GroupedWeightMatrix.from_device(ds.data_ptr(), dp.data_ptr(), k, n, group)
+    np.testing.assert_array_equal(q.unpack(), fb.dequant(s, p, k, n, group).astype(np.float32))
+    q.close()
+
+
 # ----------------------------------------------------------------- attention
 
 PAIRS = [(1, 2, 2), (1, 4, 2), (1, 4, 1), (2, 4, 1), (2, 8, 1), (9, 4, 1)]   # tokens, heads, key heads: both kernels
