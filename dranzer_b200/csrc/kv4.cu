@@ -354,7 +354,7 @@ void dz_kv4_frequencies(double base, size_t head_dim, double* freq) {
 using namespace dz;
 
 // The limits keep every index of a launch in range: rows x heads below 2^31
-// warps, one cache buffer below 2^62 bytes.
+// warps, one cache buffer of at most 2^62 bytes.
 static int kv4_check(const dz_kv4_t* c, const int64_t* positions, size_t n_tokens, Kv4Cache* out) {
     if (!c || !c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales || !positions)
         return fail(DZ_E_INVALID, "kv4: null argument");
@@ -364,6 +364,9 @@ static int kv4_check(const dz_kv4_t* c, const int64_t* positions, size_t n_token
         return fail(DZ_E_INVALID, "kv4: batch and kv_heads must be 1..65535");
     if (c->capacity == 0 || c->capacity > (size_t)KV4_CAPACITY || c->sinks >= c->capacity)
         return fail(DZ_E_INVALID, "kv4: capacity must be 1..2^31-64 and sinks below it");
+    if (c->capacity > ((size_t)1 << 62) / (c->batch * c->kv_heads * (c->head_dim / 2)))
+        return fail(DZ_E_INVALID, "kv4: a buffer of %zu x %zu rings of %zu rows is above 2^62 bytes", c->batch, c->kv_heads,
+                    c->capacity);
     if (n_tokens == 0 || n_tokens > c->capacity - c->sinks)
         return fail(DZ_E_INVALID, "kv4: n_tokens must be 1..capacity - sinks (%zu)", c->capacity - c->sinks);
     if ((((uintptr_t)c->k_codes | (uintptr_t)c->v_codes) & 15) || (((uintptr_t)c->k_scales | (uintptr_t)c->v_scales) & 7) ||
@@ -375,7 +378,7 @@ static int kv4_check(const dz_kv4_t* c, const int64_t* positions, size_t n_token
 }
 
 // A typed row-strided operand: base aligned to its type, rows that hold their
-// heads (or a single row), offsets in range.
+// heads, offsets in range.
 static int kv4_rows(const char* what, const void* base, size_t stride, size_t heads, size_t head_dim, int type) {
     if (!base) return fail(DZ_E_INVALID, "kv4: %s is null", what);
     if ((uintptr_t)base % type_bytes(type)) return fail(DZ_E_INVALID, "kv4: %s is not aligned to its type", what);
