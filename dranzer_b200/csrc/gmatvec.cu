@@ -690,6 +690,12 @@ static int gmv_check(const dz_grouped_blob_t* w) {
     return DZ_OK;
 }
 
+// A failed call's status; its error is not left for a later call to find.
+static int gmv_fail(const char* what, cudaError_t e) {
+    (void)cudaGetLastError();
+    return fail(e == cudaErrorMemoryAllocation ? DZ_E_NOMEM : DZ_E_DEVICE, "%s: %s", what, cudaGetErrorString(e));
+}
+
 // Lays w out into m->rec on `device`, the current one; the staging copies live here.
 static int gmv_fill(const dz_grouped_blob_t* w, GmvMatrix* m, int device, cudaStream_t st, uint8_t** codes,
                     uint8_t** scales, int** bad) {
@@ -759,8 +765,8 @@ extern "C" int dz_cuda_gmatrix_create(int device, const dz_grouped_blob_t* w, dz
     cudaStream_t st = nullptr;
     uint8_t *codes = nullptr, *scales = nullptr;
     int* bad = nullptr;
-    if (cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) != cudaSuccess)
-        rc = fail(DZ_E_DEVICE, "stream creation failed");
+    const cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+    if (e != cudaSuccess) rc = gmv_fail("gmatrix: stream creation", e);
     if (!rc) rc = gmv_fill(w, &m, device, st, &codes, &scales, &bad);
     cudaFree(codes);
     cudaFree(scales);
@@ -791,6 +797,7 @@ extern "C" size_t dz_cuda_gmatrix_bytes(const dz_cuda_gmatrix_t* q) {
 extern "C" int dz_cuda_gmatrix_unpack(const dz_cuda_gmatrix_t* q, float* dst) {
     if (!q || !dst) return fail(DZ_E_INVALID, "null argument");
     DeviceGuard g(q->device);
+    if (!g.ok) return fail(DZ_E_DEVICE, "cannot select device %d", q->device);
     const long long total = (long long)q->m.K * q->m.N;
     float* d = nullptr;
     DZ_CUDA(cudaMalloc(&d, total * 4));
@@ -802,8 +809,7 @@ extern "C" int dz_cuda_gmatrix_unpack(const dz_cuda_gmatrix_t* q, float* dst) {
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) e = cudaMemcpy(dst, d, total * 4, cudaMemcpyDeviceToHost);
     cudaFree(d);
-    if (e != cudaSuccess) return fail(DZ_E_DEVICE, "unpack: %s", cudaGetErrorString(e));
-    return DZ_OK;
+    return e == cudaSuccess ? DZ_OK : gmv_fail("unpack", e);
 }
 
 extern "C" int dz_cuda_matmul_grouped_async(const void* A, size_t lda, const dz_cuda_gmatrix_t* q, void* C, size_t ldc,
@@ -834,20 +840,17 @@ extern "C" int dz_cuda_matmul_grouped(const float* A, const dz_cuda_gmatrix_t* q
     if (!q || !A || !C || m == 0 || m > (1u << 24) || k != (size_t)q->m.K)
         return fail(DZ_E_INVALID, "matmul_grouped: bad arguments (k must equal the matrix rows)");
     DeviceGuard g(q->device);
+    if (!g.ok) return fail(DZ_E_DEVICE, "cannot select device %d", q->device);
     const size_t n = (size_t)q->m.N;
     float *dA = nullptr, *dC = nullptr;
-    DZ_CUDA(cudaMalloc(&dA, m * k * 4));
-    if (cudaMalloc(&dC, m * n * 4) != cudaSuccess) {
-        cudaFree(dA);
-        return fail(DZ_E_NOMEM, "device allocation");
-    }
-    cudaError_t e = cudaMemcpy(dA, A, m * k * 4, cudaMemcpyHostToDevice);
+    cudaError_t e = cudaMalloc(&dA, m * k * 4);
+    if (e == cudaSuccess) e = cudaMalloc(&dC, m * n * 4);
+    if (e == cudaSuccess) e = cudaMemcpy(dA, A, m * k * 4, cudaMemcpyHostToDevice);
     int rc = DZ_OK;
     if (e == cudaSuccess) rc = dz_cuda_matmul_grouped_async(dA, k, q, dC, n, m, k, DZ_TYPE_F32, nullptr);
     if (e == cudaSuccess && rc == DZ_OK) e = cudaMemcpy(C, dC, m * n * 4, cudaMemcpyDeviceToHost);
     cudaFree(dA);
     cudaFree(dC);
     if (rc) return rc;
-    if (e != cudaSuccess) return fail(DZ_E_DEVICE, "matmul_grouped: %s", cudaGetErrorString(e));
-    return DZ_OK;
+    return e == cudaSuccess ? DZ_OK : gmv_fail("matmul_grouped", e);
 }

@@ -168,6 +168,20 @@ def test_matrix_from_codes_that_another_device_still_writes(gpu):
     q.close()
 
 
+def test_an_allocation_that_fails_leaves_no_error_behind(gpu):
+    """A product whose result no device holds is refused, and the next call does not find its error."""
+    L = gpu.lib()
+    k, n, m = 1, 100000, 1 << 24
+    q = gpu.GroupedWeightMatrix.encode(np.ones((k, n), np.float32), 32)
+    a = np.ones((m, k), np.float32)
+    assert L.dz_cuda_matmul_grouped(a.ctypes.data, q.handle, a.ctypes.data, m, k) == -5     # a 6 TB result: not enough memory
+    again = gpu.GroupedWeightMatrix.encode(np.ones((40, 8), np.float32), 32)
+    assert (again.unpack() == 1).all()
+    assert np.abs(again.matmul(np.ones((2, 40), np.float32)) - 40).max() < 1e-4
+    again.close()
+    q.close()
+
+
 # ----------------------------------------------------------------- attention
 
 PAIRS = [(1, 2, 2), (1, 4, 2), (1, 4, 1), (2, 4, 1), (2, 8, 1), (9, 4, 1)]   # tokens, heads, key heads: both kernels
