@@ -380,12 +380,16 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
                 if constexpr (!FV) x[n][r] += __shfl_xor_sync(0xffffffffu, x[n][r], 1);   // the pair's other digits
                 x[n][r] *= sfac[n];
             }
+            unsigned hidden = 0;
             if (edge) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int v = v0 + r * 8 + g, rel = v - nsink;
                     const bool see = v < nsink ? v <= see_sink[n] : rel <= see_hi[n] && rel > see_lo[n];
-                    if (!see || v >= count) x[n][r] = -INFINITY;
+                    if (!see || v >= count) {
+                        x[n][r] = -INFINITY;
+                        hidden |= 1u << r;
+                    }
                 }
             }
             float top = fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3]));
@@ -408,6 +412,13 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
                 x[n][r] = ka_exp2(x[n][r] - ref);
                 l[n] += x[n][r];
             }
+            // another query's token may hold a NaN scale: its weight is marked by its sign, and makes no product
+            // (a token that is seen and whose weight is 0 makes one: its NaN counts)
+            if (masked && edge) {
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (hidden >> r & 1) x[n][r] = -0.0f;
+            }
             // the weights in B layout: tokens t + 4 i, column g
             float p[8];
 #pragma unroll
@@ -418,9 +429,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 2) dz_kv4_attn_kernel(const __g
                 float w[8], wtop = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) w[i] = p[i] * vs[(t + 4 * i) * GR + (SPLIT ? g >> 2 : gr)];
-                if (masked && edge) {        // another query's token may hold a NaN scale
+                if (masked && edge) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) w[i] = p[i] == 0.0f ? 0.0f : w[i];
+                    for (int i = 0; i < 8; i++) w[i] = __float_as_uint(p[i]) == 0x80000000u ? 0.0f : w[i];
                 }
                 if constexpr (FV) {          // column g is part g % 2 of pair g / 2: the weight in bf16, or what is left of it
 #pragma unroll

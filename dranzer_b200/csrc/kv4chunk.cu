@@ -319,6 +319,7 @@ __global__ void __launch_bounds__(KC_WARPS * 32, HD == 64 ? 2 : 1) dz_kv4_chunk_
         // ---- softmax: rows g (h = 0) and g + 8
         bool grows = false;
         float top[2];
+        unsigned hidden = 0;
         if (edge) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -327,6 +328,7 @@ __global__ void __launch_bounds__(KC_WARPS * 32, HD == 64 ? 2 : 1) dz_kv4_chunk_
                     const int h = c >> 1, v = v0 + 8 * i + t + 4 * (c & 1), rel = v - nsink;
                     const bool see = v < nsink ? v <= see_sink[h] : rel <= see_hi[h] && rel > see_lo[h];
                     x[i][c] = see && v < count ? x[i][c] * sfac[h] : -INFINITY;
+                    if (!see || v >= count) hidden |= 1u << (4 * i + c);
                 }
         } else {
 #pragma unroll
@@ -368,6 +370,15 @@ __global__ void __launch_bounds__(KC_WARPS * 32, HD == 64 ? 2 : 1) dz_kv4_chunk_
                     l[h] += y;
                 }
         }
+        // a token that another row sees may hold a NaN scale: its weight is marked by its sign, and makes no product
+        // (a token that is seen and whose weight is 0 makes one: its NaN counts)
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    if (hidden >> (4 * i + c) & 1) x[i][c] = -0.0f;
+        }
         // ---- values: 16 tokens (two n-tiles of scores) at a time
 #pragma unroll
         for (int gr = 0; gr < GR; gr++)
@@ -383,12 +394,12 @@ __global__ void __launch_bounds__(KC_WARPS * 32, HD == 64 ? 2 : 1) dz_kv4_chunk_
                         ws[i][0][c] = x[2 * j + i][c] * s;
                         ws[i][1][c] = x[2 * j + i][2 + c] * s;
                     }
-                if (edge) {                  // a token that another row sees may hold a NaN scale
+                if (edge) {
 #pragma unroll
                     for (int i = 0; i < 2; i++)
 #pragma unroll
                         for (int c = 0; c < 4; c++)
-                            if (x[2 * j + i][c] == 0.0f) ws[i][c >> 1][c & 1] = 0.0f;
+                            if (__float_as_uint(x[2 * j + i][c]) == 0x80000000u) ws[i][c >> 1][c & 1] = 0.0f;
                 }
                 uint32_t wa[WP][4];
 #pragma unroll
