@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(KV4_APPEND_WARPS * 32, 3) dz_kv4_append_kernel
                     n = 1.0f;
                 }
 #pragma unroll
-                for (int i = 0; i < E; i++) x[i] = gain[i] * x[i] * n;
+                for (int i = 0; i < E; i++) x[i] = gain[i] * (x[i] * n);   // x n is about 1: gains of any size
             }
             if (a.rope) kv4_rotate<HD>(x, a.halves, lane, at, [&](int i) { return turn[i]; });
             store(out + h * HD, x);

@@ -7,7 +7,7 @@ import torch
 
 import _fourbit as fb
 from _fourbit import GROUP
-from test_gpu_fourbit import Ring, TYPES, _dz_type, _np, _stream, _typed
+from test_gpu_fourbit import Ring, TYPES, _append, _dz_type, _np, _stream, _typed
 
 pytestmark = pytest.mark.gpu
 
@@ -180,6 +180,29 @@ def test_an_allocation_that_fails_leaves_no_error_behind(gpu):
     assert np.abs(again.matmul(np.ones((2, 40), np.float32)) - 40).max() < 1e-4
     again.close()
     q.close()
+
+
+# -------------------------------------------------------------------- append
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("halves", [False, True])
+def test_append_norms_with_gains_of_every_size(gpu, hd, halves):
+    """Rows of 1e-12 to 1e17 normed to 1, times gains of 1e-25 to 1e25: neither product leaves fp32's range on the way."""
+    rng = np.random.RandomState(27)
+    ring = Ring(gpu, 6, 1, hd, 4, 0, rng)
+    pos = torch.tensor([0, 1, 2, 3, 100, 7], device="cuda")
+    for size in (1e25, 1.0, 1e-25):
+        x = (rng.randn(6, 1, hd) * np.array([1e-12, 1e-6, 1.0, 1e6, 1e12, 1e17]).reshape(6, 1, 1)).astype(np.float32)
+        gain = (size * (1 + 0.2 * rng.randn(hd))).astype(np.float32)
+        t = torch.from_numpy(x).cuda()
+        q, k, _ = _append(gpu, ring, "f32", pos, 1, 1, t, t, t, (gain, gain), 1e4, halves, eps=0.0)
+        want, mag = fb.norm_rotate(x, gain, 0.0, _np(pos), 1e4, halves)
+        got = _np(q).reshape(want.shape)
+        # about a dozen fp32 roundings of a norm (its sum is a tree) and three of a rotation
+        assert (np.abs(got - want) <= 2.0 ** -20 * mag + fb.rounding(want, "f32")).all(), size
+        held = _np(k).reshape(want.shape)
+        step = np.abs(want).reshape(6, -1, GROUP).max(2).repeat(GROUP, 1).reshape(want.shape) / 7
+        assert (np.abs(held - want) <= step * (0.5 + 2.0 ** -17)).all(), size
 
 
 # ----------------------------------------------------------------- attention
