@@ -27,13 +27,13 @@
 // 3 or 4 pairs of 16-bit types (FV) take their values in the 16-bit MMA: weight x
 // scale in two bf16 parts (2^-17 of itself), two columns for a pair, levels widened
 // to bf16 and summed in the accumulators over all tiles. 2 x 8 key heads of 128, 4
-// queries each, 130k tokens: 103 us, 155 with digits in two n-tiles. (Two digits
+// queries each, 130k tokens: 104 us, 155 with digits in two n-tiles. (Two digits
 // for queries and weights of 16-bit types took 76 us, and lost small elements
 // and small weights beside large ones.)
 //
-// Bound by instruction issue: 550 per tile of 32 tokens at head dimension 128
+// Bound by instruction issue: 540 per tile of 32 tokens at head dimension 128
 // and one pair, 2.5 a cycle per SM. 256 x 16 heads of 128, up to 641
-// tokens: 68 us per call, 4.9 TB/s of the 6.55 that a copy reaches. With levels
+// tokens: 69 us per call, 4.9 TB/s of the 6.55 that a copy reaches. With levels
 // widened to fp16 pairs in m16n8k16 (two fp16 parts per fp32 weight) a tile took
 // 860 instructions, most of the ALU's issue rate in widening, and the call 118
 // us.
@@ -697,7 +697,7 @@ template <typename T, int HD> static cudaError_t ka_launch_n(const Kv4AttnArgs& 
 // Pairs of a key head up to which tokens are the MMA's rows; above, pairs are
 // (kv4chunk.cu). Both on 8 x 4 key heads of 128 that see 4160 tokens, fp32: 4
 // pairs 22 us each, 8 pairs 27 against 24; fp16: 4 pairs 18 against 17, 8 pairs 21
-// against 19 (2 x 8 key heads, 130k tokens, bf16: 4 pairs 103 against 165, 8 pairs 155
+// against 19 (2 x 8 key heads, 130k tokens, bf16: 4 pairs 104 against 165, 8 pairs 155
 // against 167), 16 pairs 30 against 22. Of 64, fp32: 8 pairs 16 against 19, 16 pairs
 // 23 against 21; fp16: 8 pairs 13 against 15, 16 pairs 18 against 17.
 static int ka_limit(int head_dim) { return head_dim == 128 ? 4 : 8; }

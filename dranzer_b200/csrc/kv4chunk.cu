@@ -5,7 +5,7 @@
 // A unit is one (sequence, key head) and 16 of its pairs, which are the rows of
 // mma.m16n8k16; tokens are its columns, so the score accumulators become the
 // weights' A operand in place and the codes are widened once for 16 pairs
-// (kv4attn.cu has tokens as rows and at most 8 pairs to a block, for decoding).
+// (kv4attn.cu has tokens as rows and at most 4 pairs to a unit, for decoding).
 // Visible tokens go in tiles of 32 to a team of warps or a cluster of blocks,
 // as there.
 //
@@ -19,10 +19,10 @@
 //            for fp32 (2^-27), two for 16-bit types (2^-18). B = levels of V.
 // Sums, maxima and joins are fp32.
 //
-// Bound by instruction issue (2.3 a cycle per SM; the 16-bit MMAs take a
-// quarter of the tensor pipe). On one B200, against kv4attn.cu's kernel: 8 x 4 key
-// heads of 64, 16 tokens of 8 heads each over 4160 tokens, fp16, 45 us (59), fp32
-// 56 us (113); key heads of 128, fp32, 105 us (218).
+// Bound by instruction issue (2.2 a cycle per SM; the 16-bit MMAs take a
+// third of the tensor pipe). On one B200, against kv4attn.cu's kernel: 8 x 4 key
+// heads of 64, 16 tokens of 8 heads each over 4160 tokens, fp16, 42 us (91), fp32
+// 56 us (122); key heads of 128, fp16, 77 us (162), fp32 98 us (230).
 #include <cmath>
 
 #include "kv4launch.cuh"
