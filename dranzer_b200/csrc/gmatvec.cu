@@ -96,7 +96,7 @@ template <typename S> __global__ void dz_gmv_dequant_kernel(GmvMatrix w, float* 
 // bits of 1.5 x 2^23, whose step is 1, so that its bits read as a float are
 // 1.5 x 2^23 plus the sum. Times scale and digit weight they add up in fp32.
 //
-// Work. A cluster of 1 to 8 blocks takes a contiguous range of tiles; its
+// Work. A cluster of 1 to 8 blocks (16 for the longest rows) takes a contiguous range of tiles; its
 // blocks take a share of the rows of W each (so that each stages only its
 // share of the activations), and a block's eight warps equal contiguous
 // ranges of its (tile, block) records, whatever tile borders lie inside. A
@@ -173,7 +173,7 @@ __device__ __forceinline__ void gmv_levels(uint32_t w, int i, uint32_t& first, u
 // What an activation type takes in the MMA, and in how many columns of a row.
 // UNIT: what a result's sums are counted in. bf16 levels are a 1024th, so that a
 // group's sum (at most 7 x 128 of its largest activation) stays in fp32's range
-// before its scale takes it back.
+// before its scale takes it back (results below 2^-116 lose bits to it).
 template <typename T> struct GmvType {
     using Mma = T;
     static constexpr int PARTS = 1;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(GMV_WARPS * 32, gmv_blocks(NT, GPB)) dz_gmv_ke
 #pragma unroll
             for (int u = 0; u < AHEAD; u++) {
                 if (to[u] < 0) continue;
-                // the power stays a normal float: of a block below 2^-105 bits under 2^-164 are lost
+                // the power stays a normal float; of a block below 2^-86, digits that count less than 2^-149 are lost
                 const int s = min(127 + 21 - (int)(top[u] >> 23), 126);
                 const float f = __int_as_float((127 + s) << 23);
 #pragma unroll

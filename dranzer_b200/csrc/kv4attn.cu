@@ -24,7 +24,7 @@
 // exact but for what lies below that. An accumulator starts at the bits of 1.5 x
 // 2^23 (less the 7s): its bits read as a float are 1.5 x 2^23 plus the sum.
 //
-// 3 or 4 pairs of 16-bit types (FV) take their values in the 16-bit MMA: weight x
+// Units of 3 or 4 pairs of 16-bit types (FV) take their values in the 16-bit MMA: weight x
 // scale in two bf16 parts (2^-17 of itself), two columns for a pair, levels widened
 // to bf16 and summed in the accumulators over all tiles. 2 x 8 key heads of 128, 4
 // queries each, 130k tokens: 104 us, 155 with digits in two n-tiles. (Two digits

@@ -113,12 +113,12 @@ int dz_cuda_gmatrix_unpack(const dz_cuda_gmatrix_t *matrix, float *dst);
  * cudaStream_t) without synchronisation. A and C have element type `type` and
  * row strides lda >= k, ldc >= n in elements; they must not overlap.
  * Activations enter with their own precision, whatever stands beside them (what
- * lies 2^-60 below the largest of 128 consecutive ones may be lost), their
- * products with the levels are exact, sums are fp32, one rounding to `type` at
- * the end; a row that holds an infinity or a NaN reads NaN. The order of the
- * sums depends on m. Meant for few rows (16 at a time pass over the weights).
- * Nothing is allocated and the handle holds no
- * scratch: calls on one matrix may overlap, and a call may be captured. */
+ * lies 2^-60 below the largest of 128 consecutive ones may be lost, and so may
+ * what is next to fp32's smallest numbers), their products with the levels are
+ * exact, sums are fp32, one rounding to `type` at the end; a row that holds an
+ * infinity or a NaN reads NaN. The order of the sums depends on m. Meant for few
+ * rows (16 at a time pass over the weights). Nothing is allocated and the handle
+ * holds no scratch: calls on one matrix may overlap, and a call may be captured. */
 int dz_cuda_matmul_grouped_async(const void *A_dev, size_t lda, const dz_cuda_gmatrix_t *weights, void *C_dev,
                                  size_t ldc, size_t m, size_t k, int type, void *stream);
 /* The same on contiguous fp32 host buffers, synchronous. */
@@ -153,7 +153,9 @@ int dz_cuda_kv4_append(const dz_kv4_t *cache, const dz_kv4_append_t *args, const
  * query's element is held to 2^-30 of the largest of its 64 or to 2^-22 of itself
  * (fp16, bf16: to 2^-30 of the largest of its head), a softmax weight x
  * value scale to 2^-26 (fp16, bf16: 2^-17) of itself or to 2^-30 of the largest in
- * its tile of 32 tokens. out must not overlap q or the cache. */
+ * its tile of 32 tokens (or to 2^-127). A token that is seen makes a NaN of its
+ * output where its value is one, whatever its weight. out must not overlap q or
+ * the cache. */
 int dz_cuda_kv4_attention(const dz_kv4_t *cache, const dz_kv4_attention_t *args, const int64_t *positions,
                           size_t n_tokens, void *stream);
 
