@@ -9,6 +9,10 @@ include/dz_host.h and include/dz_cuda.h (dranzer_b200/libdz_cuda.so):
   quantize_pack_grouped,
   GroupedWeightMatrix, KV4Cache        none: 4-bit weights with group scales, the
                                        4-bit ring cache and its attention
+  norm_q8, KV8Cache,
+  QuantizedWeightMatrix.matmul_q8_async
+                                       none: rows in 8 bits and products of them, the
+                                       8-bit paged cache and its attention
   Bundle (code-retaining loader),
   save_quantized_bundle                src/include/core/bundle.h:52-85
   Model, KVCache.forward_tokens        model_forward_token, src/core/transformer.c:755
@@ -23,7 +27,8 @@ import ctypes
 import numpy as np
 
 from ._native import (DzBundleInfo, DzBundleMeta, DzError, DzGenerationControls, DzGenerationResult, DzGroupedBlob,
-                      DzKv4, DzKv4Append, DzKv4Attention, DzModelDesc, DzSampling, DzTensorBlob, check, lib)
+                      DzKv4, DzKv4Append, DzKv4Attention, DzKv8, DzKv8Attention, DzModelDesc, DzNormQ8, DzSampling,
+                      DzTensorBlob, check, lib)
 
 __all__ = ["GRAN_TENSOR", "GRAN_ROW", "GRAN_COLUMN", "GREEDY", "TOPK", "TOPP", "STREAM_INIT",
            "STREAM_DROPOUT", "STREAM_SAMPLING", "STREAM_TESTING", "DzError", "available",
@@ -31,7 +36,7 @@ __all__ = ["GRAN_TENSOR", "GRAN_ROW", "GRAN_COLUMN", "GREEDY", "TOPK", "TOPP", "
            "quantized_packed_size", "quantize_pack", "quantize_unpack", "quantized_slice", "positional_encoding", "fnv1a",
            "QuantizedWeightMatrix", "matmul_quantized_weight", "Bundle", "save_quantized_bundle",
            "TYPE_F32", "TYPE_F16", "TYPE_BF16", "quantize_pack_grouped", "quantize_unpack_grouped",
-           "GroupedWeightMatrix", "KV4Cache", "minimal_tokenizer", "model_tensor_layout", "Sampling", "Controls", "Model", "KVCache"]
+           "GroupedWeightMatrix", "KV4Cache", "norm_q8", "KV8Cache", "minimal_tokenizer", "model_tensor_layout", "Sampling", "Controls", "Model", "KVCache"]
 
 GRAN_TENSOR, GRAN_ROW, GRAN_COLUMN = 0, 1, 2
 GREEDY, TOPK, TOPP = 0, 1, 2
@@ -214,6 +219,17 @@ class QuantizedWeightMatrix:
         check(lib().dz_cuda_matmul_quantized_async(a_ptr, self.handle, c_ptr, m, self.rows, stream_ptr),
               "matmul_quantized_async")
 
+    def matmul_q8_async(self, codes_ptr, scales_ptr, c_ptr, m, stream_ptr=None, type=TYPE_F32, lda=None, ldc=None,
+                        bias_ptr=None):
+        """C = (rows in 8 bits with a scale each) . W + bias on device buffers
+        (dz_cuda_matmul_q8_async): codes int8 with row stride lda (None: the
+        rows of W rounded up to 16), C of element type `type`."""
+        status = lib().dz_cuda_matmul_q8_async(codes_ptr, -(-self.rows // 16) * 16 if lda is None else lda, scales_ptr,
+                                               self.handle, bias_ptr, c_ptr, self.cols if ldc is None else ldc, m,
+                                               self.rows, type, stream_ptr)
+        if status:
+            check(status, "matmul_q8_async")
+
     def close(self):
         if getattr(self, "handle", None):
             lib().dz_cuda_qmatrix_free(self.handle)
@@ -362,6 +378,69 @@ class KV4Cache:
         status = lib().dz_cuda_kv4_attention(self._ref, ctypes.byref(a), positions, n_tokens, stream_ptr)
         if status:
             check(status, "kv4_attention")
+
+
+# --------------------------------------------------- 8-bit rows and caches
+
+def norm_q8(rows, width, *, x, codes, scales, type=TYPE_F32, x_stride=None, residual=None, residual_stride=None,
+            sum_out=None, sum_stride=None, gain=None, norm=True, eps=1e-6, codes_stride=None, device=0, stream_ptr=None):
+    """Residual addition, root-mean-square norm (norm=False: none) and rows in 8
+    bits with a scale each (dz_cuda_norm_q8). Operands are device addresses,
+    strides in elements (None: contiguous; of codes: the width rounded up to 16,
+    as matmul_q8_async takes them)."""
+    a = DzNormQ8(device, type, x, width if x_stride is None else x_stride, residual,
+                 width if residual_stride is None else residual_stride, sum_out,
+                 width if sum_stride is None else sum_stride, gain, 1 if norm else 0, eps, codes,
+                 -(-width // 16) * 16 if codes_stride is None else codes_stride, scales)
+    status = lib().dz_cuda_norm_q8(ctypes.byref(a), rows, width, stream_ptr)
+    if status:
+        check(status, "norm_q8")
+
+
+class KV8Cache:
+    """8-bit caches of one layer on a pool of pages (dz_kv8_t) over device
+    buffers that the caller owns: codes [pages, kv_heads, page, head_dim] int8,
+    scales [pages, kv_heads] float32, table [batch, table_pages] int32, given as
+    addresses. Positions are a device int64 [batch] array (negative: skip the
+    sequence); operands are device addresses, rows [batch * n_tokens], strides
+    in elements (None: contiguous)."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales, pages, page, kv_heads, head_dim, table, batch, table_pages,
+                 device=0):
+        self.pages, self.page, self.kv_heads, self.head_dim = pages, page, kv_heads, head_dim
+        self.batch, self.table_pages, self.device = batch, table_pages, device
+        self.c = DzKv8(device, k_codes, v_codes, k_scales, v_scales, pages, page, kv_heads, head_dim, table, batch,
+                       table_pages)
+        self._ref = ctypes.byref(self.c)
+
+    def append(self, positions, n_tokens, *, type=TYPE_F32, q_heads=0, q=None, k=None, v=None, q_stride=None,
+               k_stride=None, v_stride=None, q_out=None, q_out_stride=None, k_out=None, v_out=None,
+               k_out_stride=None, v_out_stride=None, q_gain=None, k_gain=None, eps=1e-6, rope_base=0.0,
+               halves=False, stream_ptr=None):
+        """Norm and rotate q and k per head, quantize k and v into their pages
+        (dz_cuda_kv8_append)."""
+        wq, wk = q_heads * self.head_dim, self.kv_heads * self.head_dim
+        a = DzKv4Append(type, q_heads, q, k, v, wq if q_stride is None else q_stride,
+                        wk if k_stride is None else k_stride, wk if v_stride is None else v_stride, q_out,
+                        wq if q_out_stride is None else q_out_stride, k_out, v_out,
+                        wk if k_out_stride is None else k_out_stride, wk if v_out_stride is None else v_out_stride,
+                        q_gain, k_gain, eps, rope_base, 1 if halves else 0)
+        status = lib().dz_cuda_kv8_append(self._ref, ctypes.byref(a), positions, n_tokens, stream_ptr)
+        if status:
+            check(status, "kv8_append")
+
+    def attention(self, positions, n_tokens, *, type=TYPE_F32, q_heads, q, out, q_stride=None, out_stride=None,
+                  scale=None, window=0, longest=0, stream_ptr=None):
+        """Attention of the n_tokens newest queries of every sequence
+        (dz_cuda_kv8_attention); scale None: 1 / sqrt(head_dim). longest, where
+        known, shapes the launch and changes no result."""
+        w = q_heads * self.head_dim
+        a = DzKv8Attention(type, q_heads, q, w if q_stride is None else q_stride, out,
+                           w if out_stride is None else out_stride,
+                           self.head_dim ** -0.5 if scale is None else scale, window, longest)
+        status = lib().dz_cuda_kv8_attention(self._ref, ctypes.byref(a), positions, n_tokens, stream_ptr)
+        if status:
+            check(status, "kv8_attention")
 
 
 # -------------------------------------------------------------------- bundles

@@ -99,6 +99,22 @@ class DzKv4Attention(ctypes.Structure):
                 ("scale", F32), ("window", SZ)]
 
 
+class DzNormQ8(ctypes.Structure):
+    _fields_ = [("device", I32), ("type", I32), ("x", P), ("x_stride", SZ), ("residual", P), ("residual_stride", SZ),
+                ("sum_out", P), ("sum_stride", SZ), ("gain", P), ("norm", I32), ("eps", F64), ("codes", P),
+                ("codes_stride", SZ), ("scales", P)]
+
+
+class DzKv8(ctypes.Structure):
+    _fields_ = [("device", I32), ("k_codes", P), ("v_codes", P), ("k_scales", P), ("v_scales", P), ("pages", SZ),
+                ("page", SZ), ("kv_heads", SZ), ("head_dim", SZ), ("table", P), ("batch", SZ), ("table_pages", SZ)]
+
+
+class DzKv8Attention(ctypes.Structure):
+    _fields_ = [("type", I32), ("q_heads", SZ), ("q", P), ("q_stride", SZ), ("out", P), ("out_stride", SZ),
+                ("scale", F32), ("window", SZ), ("longest", SZ)]
+
+
 # name -> (restype, argtypes); every exported symbol of include/dz_host.h and include/dz_cuda.h
 SIGNATURES = {
     # dz_host.h
@@ -149,6 +165,10 @@ SIGNATURES = {
     "dz_cuda_matmul_grouped_async": (I32, [P, SZ, P, P, SZ, SZ, SZ, I32, P]),
     "dz_cuda_kv4_append": (I32, [P, P, P, SZ, P]),
     "dz_cuda_kv4_attention": (I32, [P, P, P, SZ, P]),
+    "dz_cuda_norm_q8": (I32, [P, SZ, SZ, P]),
+    "dz_cuda_matmul_q8_async": (I32, [P, SZ, P, P, P, P, SZ, SZ, SZ, I32, P]),
+    "dz_cuda_kv8_append": (I32, [P, P, P, SZ, P]),
+    "dz_cuda_kv8_attention": (I32, [P, P, P, SZ, P]),
     "dz_cuda_model_create": (I32, [P, P, SZ, I32, P]),
     "dz_cuda_model_free": (None, [P]),
     "dz_cuda_model_step_bytes": (SZ, [P]),

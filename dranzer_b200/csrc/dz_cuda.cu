@@ -26,6 +26,7 @@
 #include "qmma.cuh"
 #include "select.cuh"
 #include "prefill.cuh"
+#include "qlevels.cuh"
 #include "seqgen.cuh"
 #include "umma.cuh"
 #include "qmvi.cuh"
@@ -912,6 +913,20 @@ struct dz_cuda_qmatrix {
     size_t scratch_bytes = 0;
     int* status = nullptr;              // device word: a weight-copy wait gave up
 };
+
+void dz::dz_qmatrix_levels(const dz_cuda_qmatrix_t* q, QLevels* out) {
+    *out = QLevels{q->device, q->m.K, q->m.N, q->m.gran, q->m.kn, q->m.col_scale, q->m.tm_kn};
+}
+
+bool dz::dz_encode_u8_map(CUtensorMap* tm, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                          const uint32_t* box) {
+    cuuint64_t d[5], s[5];
+    for (int i = 0; i < rank; i++) {
+        d[i] = dims[i];
+        s[i] = i + 1 < rank ? strides[i] : 0;
+    }
+    return encode_u8_map(tm, const_cast<void*>(base), rank, d, s, box);
+}
 
 static int qmatrix_scratch(dz_cuda_qmatrix_t* q, int M) {
     const size_t need = qmv_scratch_bytes(q->m, M);

@@ -159,6 +159,65 @@ int dz_cuda_kv4_append(const dz_kv4_t *cache, const dz_kv4_append_t *args, const
 int dz_cuda_kv4_attention(const dz_kv4_t *cache, const dz_kv4_attention_t *args, const int64_t *positions,
                           size_t n_tokens, void *stream);
 
+/* ---- 8-bit activations and caches, on device buffers, enqueued on `stream`
+ * without synchronisation; nothing is allocated. No counterpart in the
+ * reference, whose activations and caches are fp32. */
+
+/* Rows in 8 bits with a scale each, what dz_cuda_matmul_q8_async takes. For
+ * every row: h = x + residual rounded to `type` (x without a residual), u =
+ * fp32(gain * h), P the largest |u|, code = round_half_away(fp32(u * fp32(127 /
+ * P))), scale = P / 127, with the norm P / sqrt(mean(h^2) + eps) / 127, so that
+ * scale * code stands for u over the root mean square of h. Where P < 2^-100, u
+ * and P are taken times 2^100 for the codes. A row of zeros has codes and scale
+ * 0; one whose u holds an infinity or a NaN has codes 0 and the scale NaN.
+ * sum_out may be x or residual itself (same pointer and stride); otherwise
+ * outputs overlap no input. */
+int dz_cuda_norm_q8(const dz_norm_q8_t *args, size_t rows, size_t width, void *stream);
+
+/* C (m x n) = a_scales[m] * col_scale[n] * sum_k A[m][k] level[k][n] + bias[n]
+ * for a quantized matrix of 4 or 8 bits with column scales or one scale
+ * (DZ_E_UNSUPPORTED for row scales, and for matrices of more than 131072 rows):
+ * A int8 with row stride lda >= k, a multiple of 16, on a 16-byte boundary;
+ * what a row holds past k does not matter. bias fp32 or NULL. C has element type `type` and row
+ * stride ldc >= n in elements, and overlaps nothing else. Sums are exact, the
+ * rest fp32 with one rounding to `type`. The handle holds no scratch for it:
+ * calls on one matrix may overlap, and a call may be captured. */
+int dz_cuda_matmul_q8_async(const int8_t *A_dev, size_t lda, const float *a_scales_dev,
+                            const dz_cuda_qmatrix_t *weights, const float *bias_dev, void *C_dev, size_t ldc, size_t m,
+                            size_t k, int type, void *stream);
+
+/* 8-bit caches (dz_kv8_t). positions[batch] (device, int64): the position of
+ * each sequence's first new token; a sequence with a negative position, or one
+ * of 2^62 or more, is skipped and its rows are left as they were. Calls that
+ * write a cache and calls that use it are ordered by the caller (one stream, or
+ * events).
+ *
+ * For n_tokens new tokens of every sequence: queries and keys normed per head
+ * and rotated as dz_cuda_kv4_append does, queries written to q_out, keys and
+ * values quantized into their pages. The scale S of a page and head whose first
+ * token is new becomes fp32(peak / 127) over its new rows; where the page holds
+ * earlier tokens, S stays unless that is larger, and when it grows, the earlier
+ * tokens' codes become round_half_away(fp32(code * fp32(old S / S))). New codes
+ * are clamp(round_half_away(fp32(x * fp32(1 / S))), -127, 127), x rounded to
+ * fp32 once. New rows that hold an infinity or a NaN make S a NaN, which it
+ * stays until the page is begun anew. k_out and v_out rows of tokens that no
+ * page holds are left as they were. An output row may be its own input row
+ * (same pointer and stride); otherwise outputs overlap no input. */
+int dz_cuda_kv8_append(const dz_kv8_t *cache, const dz_kv8_append_t *args, const int64_t *positions, size_t n_tokens,
+                       void *stream);
+
+/* softmax(scale * q . k) . v over the cache for the n_tokens queries of every
+ * sequence, whose own keys have been appended (positions as in that append):
+ * the query at position i sees position p <= i where the table names a page,
+ * and with a window p > i - window. A query that sees nothing reads 0. Scores,
+ * softmax statistics and sums are fp32. An fp32 or bf16 query's element is held
+ * to 2^-22 of itself or to 2^-38 of the largest of its head, a softmax weight to
+ * 2^-22 of itself or 2^-39 of the largest. A token that is seen makes a NaN of
+ * its output where its page's scale is one, whatever its weight. out must not
+ * overlap q or the cache. */
+int dz_cuda_kv8_attention(const dz_kv8_t *cache, const dz_kv8_attention_t *args, const int64_t *positions,
+                          size_t n_tokens, void *stream);
+
 /* ---- Model: the parameters of a v2/v3 bundle kept as codes on the device.
  * `tensors` are the n blobs of model_param_tensors() order
  * (src/core/model_params.c:39-103), as dz_bundle_tensors() returns them; they are

@@ -37,8 +37,8 @@ enum { DZ_GRAN_TENSOR = 0, DZ_GRAN_ROW = 1, DZ_GRAN_COLUMN = 2 };
 /* Parameter kinds, src/include/core/model_params.h:20-38. */
 enum { DZ_KIND_PROJECTION = 0, DZ_KIND_EMBEDDING = 1, DZ_KIND_BIAS = 2, DZ_KIND_NORM = 3 };
 
-/* Element type of the activations of the 4-bit operators (and of the scales of
- * a group-scaled matrix). No counterpart in the reference, which is fp32. */
+/* Element type of the activations of the 4-bit and 8-bit operators (and of the
+ * scales of a group-scaled matrix). No counterpart in the reference, which is fp32. */
 enum { DZ_TYPE_F32 = 0, DZ_TYPE_F16 = 1, DZ_TYPE_BF16 = 2 };
 
 /* Model shape: the six bundle header dimensions (src/core/bundle.c:452-458)
@@ -146,6 +146,71 @@ typedef struct {
     float scale;           /* scores are scale * (q . k) */
     size_t window;         /* 0: every retained token; else the newest `window` and the sinks */
 } dz_kv4_attention_t;
+
+/* One call of dz_cuda_norm_q8: rows of `width` elements, element e of row r at
+ * base[r * stride + e] (strides in elements, no alignment asked). */
+typedef struct {
+    int device;
+    int type;                /* DZ_TYPE_* of x, residual and sum_out */
+    const void *x;
+    size_t x_stride;
+    const void *residual;    /* added to x, or NULL */
+    size_t residual_stride;
+    void *sum_out;           /* x + residual rounded to `type`, or NULL */
+    size_t sum_stride;
+    const float *gain;       /* [width], or NULL: 1 */
+    int norm;                /* 1: the root-mean-square norm, 0: the rows as they are */
+    double eps;
+    int8_t *codes;           /* row r at codes + r * codes_stride */
+    size_t codes_stride;
+    float *scales;           /* [rows] */
+} dz_norm_q8_t;
+
+/* Keys and values of `batch` sequences of one layer in 8 bits, on a pool of
+ * pages that the sequences share: device buffers that the caller owns.
+ *   codes  [pages][kv_heads][page][head_dim] int8, -127..127
+ *   scales [pages][kv_heads] fp32, one per page and head (a NaN marks a page that
+ *          holds no values)
+ *   table  [batch][table_pages] int32: the page that holds the tokens [j * page,
+ *          (j + 1) * page) of sequence b is table[b * table_pages + j]
+ * value = scale * code. `page` is 32 or 64 tokens, head_dim 64 or 128. An entry
+ * outside 0..pages-1 names no page: tokens there are neither stored nor seen,
+ * nor are those at table_pages * page and after. Several entries may name one
+ * page for attention (sequences that share a prefix); an append writes to every
+ * page that its new tokens fall in, which then has to be named once. table_pages
+ * * page <= 2^31 - 64. Code buffers start on 16-byte boundaries; k and v
+ * buffers do not overlap. */
+typedef struct {
+    int device;
+    int8_t *k_codes;
+    int8_t *v_codes;
+    float *k_scales;
+    float *v_scales;
+    size_t pages;
+    size_t page;
+    size_t kv_heads;
+    size_t head_dim;
+    const int32_t *table;
+    size_t batch;
+    size_t table_pages;
+} dz_kv8_t;
+
+/* One call of dz_cuda_kv8_append: the fields of a 4-bit cache's. */
+typedef dz_kv4_append_t dz_kv8_append_t;
+
+/* One call of dz_cuda_kv8_attention. */
+typedef struct {
+    int type;              /* DZ_TYPE_* of q and out */
+    size_t q_heads;        /* a multiple of kv_heads: q_heads / kv_heads share a key head */
+    const void *q;
+    size_t q_stride;
+    void *out;
+    size_t out_stride;
+    float scale;           /* scores are scale * (q . k) */
+    size_t window;         /* 0: every token; else the newest `window` */
+    size_t longest;        /* 0, or a hint: about the most tokens that a sequence holds. It
+                            * shapes the launch, results hold whatever it is */
+} dz_kv8_attention_t;
 
 #ifdef __cplusplus
 }
