@@ -8,26 +8,10 @@
 
 #include <atomic>
 
+#include "q8matmul.cuh"
 #include "qlevels.cuh"
-#include "shim.cuh"
 
 namespace dz {
-
-struct Q8MatArgs {
-    const int8_t* a;
-    long long lda;
-    const float* a_scales;
-    const int8_t* levels;
-    const float* col_scale;
-    const float* bias;
-    void* c;
-    long long ldc;
-    int M, N, K, nkb;
-};
-
-template <typename T> __device__ __forceinline__ T q8_finish(int sum, float a_scale, float col_scale, float bias) {
-    return dz_from_float<T>(fmaf((float)sum * a_scale, col_scale, bias));
-}
 
 // ------------------------------------------------------------- few rows
 //
@@ -168,7 +152,6 @@ __global__ void __launch_bounds__(Q8V_WARPS * 32, 2) dz_q8mv_kernel(const __grid
     }
 }
 
-constexpr int Q8_DEVICES = 64;
 constexpr int Q8V_SMEM = 96 * 1024;          // staged rows of a block, two blocks to an SM
 
 template <typename T, int G, bool STAGED> static cudaError_t q8mv_g(const Q8MatArgs& a, int device, int sms, cudaStream_t st) {
@@ -222,7 +205,7 @@ extern "C" int dz_cuda_matmul_q8_async(const int8_t* A, size_t lda, const float*
     if (w.gran == DZ_GRAN_ROW) return fail(DZ_E_UNSUPPORTED, "matmul_q8: row scales do not factor out of 8-bit rows");
     if (!w.levels) return fail(DZ_E_UNSUPPORTED, "matmul_q8: matrices of more than 131072 rows are not supported");
     if (((uintptr_t)A | lda) & 15) return fail(DZ_E_INVALID, "matmul_q8: rows must start on 16-byte boundaries");
-    if (lda < k || lda > (1ull << 40) || ldc < (size_t)w.N || ldc > (1ull << 40))
+    if (lda < k || lda >= (1ull << 40) || ldc < (size_t)w.N || ldc > (1ull << 40))
         return fail(DZ_E_INVALID, "matmul_q8: row strides must hold k (%zu) and n (%d) elements", k, w.N);
     if ((((uintptr_t)a_scales | (uintptr_t)bias) & 3) || (uintptr_t)C % type_bytes(type))
         return fail(DZ_E_INVALID, "matmul_q8: scales, bias or output are not aligned to their type");
@@ -248,6 +231,8 @@ extern "C" int dz_cuda_matmul_q8_async(const int8_t* A, size_t lda, const float*
     a.N = w.N;
     a.K = w.K;
     a.nkb = (w.K + 127) / 128;
-    DZ_CUDA(q8mv_launch(a, type, w.device, sms, (cudaStream_t)stream));
+    // few rows go through the matrix at the rate of its bytes either way; the MMAs of registers take 8 rows each time
+    cudaStream_t st = (cudaStream_t)stream;
+    DZ_CUDA(m <= 16 ? q8mv_launch(a, type, w.device, sms, st) : dz_q8gemm_launch(a, w.map, type, w.device, sms, st));
     return DZ_OK;
 }
