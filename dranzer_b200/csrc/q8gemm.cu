@@ -223,11 +223,278 @@ static cudaError_t q8gemm_t(const Q8MatArgs& a, const CUtensorMap& levels, int d
     return cudaLaunchKernelEx(&cfg, kernel, levels, rows, a, parts);
 }
 
+// ------------------------------------------------- many rows: pairs of SMs
+//
+// Two blocks of a cluster share a tile of 256 columns x 256 rows
+// (cta_group::2): each loads 128 columns of levels and half of the rows, 32 KB
+// for 256 x 128 x 128 products of its own, where a block alone would load 48.
+// The pairs stay and take tiles in turn. Two accumulators fill the tensor
+// memory, so that four warps of each block write a tile while the next one's
+// MMAs run. The first block of a pair issues the MMAs for both; its `full`
+// barriers count both blocks' bytes, commits arrive at both blocks' barriers.
+
+constexpr int Q8P_THREADS = 192;                 // warp 0 copies, warp 1 MMAs, warps 2..5 outputs
+constexpr int Q8P_TILE = 256;
+constexpr uint32_t Q8P_STAGE = 2 * 128 * 128;
+constexpr int Q8P_STAGES = 6;
+constexpr size_t Q8P_SMEM = (size_t)Q8P_STAGES * Q8P_STAGE + 1024 + 256;
+constexpr int Q8P_BAND = 8;                      // tiles of rows that neighbouring pairs share columns over
+
+__device__ __forceinline__ uint32_t q8p_at_leader(const void* p) {       // the same place in the pair's first block
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(dz_smem_addr(p)));
+    return r;
+}
+__device__ __forceinline__ void q8p_tma_4d(void* dst, const CUtensorMap* tm, int c2, int c3, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %3, %4}], "
+        "[%5];" ::"r"(dz_smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(0), "r"(c2), "r"(c3), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void q8p_tma_2d(void* dst, const CUtensorMap* tm, int c0, int c1, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dz_smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void q8p_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+    const uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(256 >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives at `bar` of both blocks once every MMA issued so far has completed.
+__device__ __forceinline__ void q8p_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     dz_smem_addr(bar)),
+                 "h"((unsigned short)3)
+                 : "memory");
+}
+// dz_mbar_wait for barriers that the other block arrives at.
+__device__ __forceinline__ bool q8p_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(dz_smem_addr(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool q8p_wait(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+    for (int i = 0; i < 4; i++)
+        if (q8p_test(bar, parity)) return true;
+    const uint64_t t0 = dz_global_ns();
+    for (unsigned i = 0;; i++) {
+        if (q8p_test(bar, parity)) return true;
+        if ((i & 255u) == 255u && dz_global_ns() - t0 > 1000000000ull) return false;
+    }
+}
+
+// Tile i of the grid: bands of Q8P_BAND tiles of rows, columns in turn within a
+// band, so that the pairs at work at a time share both operands in L2.
+__device__ __forceinline__ void q8p_place(int i, int ntiles, int mtiles, int* n, int* m) {
+    const int band = i / (Q8P_BAND * ntiles), within = i - band * Q8P_BAND * ntiles;
+    const int high = min(Q8P_BAND, mtiles - band * Q8P_BAND);
+    *n = within / high;
+    *m = band * Q8P_BAND + within % high;
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q8P_THREADS, 1)
+    dz_q8pair_kernel(const __grid_constant__ CUtensorMap tm_levels, const __grid_constant__ CUtensorMap tm_rows,
+                     const __grid_constant__ Q8MatArgs a, int ntiles, int mtiles) {
+    extern __shared__ __align__(1024) uint8_t q8g_raw[];
+    uint8_t* sm = q8g_raw + ((1024u - (dz_smem_addr(q8g_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + (size_t)Q8P_STAGES * Q8P_STAGE);   // used in the first block
+    uint64_t* empty = full + Q8P_STAGES;
+    uint64_t* done = empty + Q8P_STAGES;         // [2] an accumulator is complete
+    uint64_t* drained = done + 2;                // [2] and has been read by both blocks; used in the first block
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
+    volatile int* failed = reinterpret_cast<int*>(tmem_slot + 1);
+    int* issued = reinterpret_cast<int*>(tmem_slot + 2);         // stages copied, consumed
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)(blockIdx.x & 1u), pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+    const int tiles = ntiles * mtiles;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Q8P_STAGES; s++) {
+            dz_mbar_init(&full[s]);
+            dz_mbar_init(&empty[s]);
+        }
+        for (int i = 0; i < 2; i++) {
+            dz_mbar_init(&done[i]);
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 8;" ::"r"(dz_smem_addr(&drained[i])) : "memory");   // warps
+        }
+        *failed = 0;
+        issued[0] = issued[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dz_smem_addr(tmem_slot)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    ug_fence_before();
+    __syncthreads();
+    cg::this_cluster().sync();                   // both blocks' barriers are ready
+    ug_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    if (warp == 0) {
+        if (lane == 0) {
+            int step = 0;                        // stages since the start
+            bool ok = true, waited = false;
+            for (int i = pair; i < tiles && ok; i += pairs) {
+                int tn, tm;
+                q8p_place(i, ntiles, mtiles, &tn, &tm);
+                for (int kb = 0; kb < a.nkb; kb++, step++) {
+                    const int s = step % Q8P_STAGES;
+                    if (step >= Q8P_STAGES && !q8p_wait(&empty[s], (uint32_t)((step / Q8P_STAGES - 1) & 1))) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* to = sm + (size_t)s * Q8P_STAGE;
+                    const uint32_t bar = q8p_at_leader(&full[s]);
+                    if (rank == 0) dz_mbar_expect_tx(&full[s], 2 * Q8P_STAGE);
+                    q8p_tma_4d(to, &tm_levels, kb, tn * 2 + rank, bar);
+                    if (!waited) {               // the levels are no kernel's output, the rows are
+                        asm volatile("griddepcontrol.wait;" ::: "memory");
+                        waited = true;
+                    }
+                    q8p_tma_2d(to + Q8G_A_BYTES, &tm_rows, kb * 128, tm * Q8P_TILE + rank * 128, bar);
+                }
+            }
+            if (!ok) *failed = 1;
+            issued[0] = step;
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int step = 0, turn = 0;
+            bool ok = true;
+            for (int i = pair; i < tiles && ok; i += pairs, turn++) {
+                const int b = turn & 1;
+                if (turn >= 2 && !q8p_wait(&drained[b], (uint32_t)((turn / 2 - 1) & 1))) {
+                    ok = false;
+                    break;
+                }
+                ug_fence_after();
+                for (int kb = 0; kb < a.nkb; kb++, step++) {
+                    const int s = step % Q8P_STAGES;
+                    if (!q8p_wait(&full[s], (uint32_t)((step / Q8P_STAGES) & 1))) {
+                        ok = false;
+                        break;
+                    }
+                    ug_fence_after();
+                    const uint32_t at = dz_smem_addr(sm + (size_t)s * Q8P_STAGE);
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++)
+                        q8p_mma(tmem + (uint32_t)(b * 256), ug_desc_kmajor(at + kk * 32),
+                                ug_desc_kmajor(at + Q8G_A_BYTES + kk * 32), (kb > 0 || kk > 0) ? 1u : 0u);
+                    q8p_commit(&empty[s]);
+                }
+                if (ok) q8p_commit(&done[b]);
+            }
+            if (!ok) *failed = 1;
+            issued[1] = step;
+        }
+        __syncwarp();
+    } else {
+        asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows' scales
+        const int quarter = warp & 3;            // a warp reads the lanes of its number modulo 4
+        int turn = 0;
+        T* c = static_cast<T*>(a.c);
+        for (int i = pair; i < tiles; i += pairs, turn++) {
+            const int b = turn & 1;
+            int tn, tm;
+            q8p_place(i, ntiles, mtiles, &tn, &tm);
+            const int n = tn * Q8P_TILE + rank * 128 + quarter * 32 + lane, m0 = tm * Q8P_TILE;
+            const float scale = n < a.N ? a.col_scale[n] : 0.0f, bias = n < a.N && a.bias ? a.bias[n] : 0.0f;
+            const bool ok = q8p_wait(&done[b], (uint32_t)((turn / 2) & 1));
+            if (!ok && lane == 0) *failed = 1;
+            ug_fence_after();
+            for (int c0 = 0; c0 < Q8P_TILE && m0 + c0 < a.M; c0 += 32) {
+                const float own = m0 + c0 + lane < a.M ? a.a_scales[m0 + c0 + lane] : 0.0f;
+                int32_t v[32];
+                ug_tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 256 + c0), v);
+                T* to = c + (long long)(m0 + c0) * a.ldc + n;
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    const float row = __shfl_sync(0xffffffffu, own, j);
+                    if (n < a.N && m0 + c0 + j < a.M)
+                        to[j * a.ldc] = ok ? q8_finish<T>(v[j], row, scale, bias) : dz_from_float<T>(__int_as_float(0x7fc00000));
+                }
+            }
+            ug_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(q8p_at_leader(&drained[b]))
+                             : "memory");
+            }
+            if (!ok) {                           // the tiles left read NaN
+                for (i += pairs; i < tiles; i += pairs) {
+                    q8p_place(i, ntiles, mtiles, &tn, &tm);
+                    const int nn = tn * Q8P_TILE + rank * 128 + quarter * 32 + lane;
+                    for (int m = tm * Q8P_TILE; m < min(a.M, (tm + 1) * Q8P_TILE); m++)
+                        if (nn < a.N) c[m * a.ldc + nn] = dz_from_float<T>(__int_as_float(0x7fc00000));
+                }
+                break;
+            }
+        }
+    }
+    // copies and MMAs in flight end, in both blocks, before shared memory and tensor memory are released
+    ug_fence_before();
+    __syncthreads();
+    cg::this_cluster().sync();
+    if (rank == 0 && threadIdx.x == 0 && issued[1] < issued[0])
+        for (int s = issued[1]; s < issued[0]; s++)
+            if (!q8p_wait(&full[s % Q8P_STAGES], (uint32_t)((s / Q8P_STAGES) & 1))) break;
+    __syncthreads();
+    cg::this_cluster().sync();
+    if (warp == 1) {
+        ug_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <typename T> static cudaError_t q8pair_t(const Q8MatArgs& a, const CUtensorMap& levels, int device, int sms, cudaStream_t st) {
+    static std::atomic<bool> ready[Q8_DEVICES];
+    const auto kernel = dz_q8pair_kernel<T>;
+    if (!ready[device].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Q8P_SMEM);
+        if (e != cudaSuccess) return e;
+        ready[device].store(true, std::memory_order_release);
+    }
+    CUtensorMap rows;
+    const uint64_t dims[2] = {(uint64_t)a.K, (uint64_t)a.M}, strides[1] = {(uint64_t)a.lda};
+    const uint32_t box[2] = {128, 128};
+    if (!dz_encode_u8_map(&rows, a.a, 2, dims, strides, box)) return cudaErrorInvalidValue;
+    const int ntiles = (a.N + Q8P_TILE - 1) / Q8P_TILE, mtiles = (a.M + Q8P_TILE - 1) / Q8P_TILE;
+    const long long tiles = (long long)ntiles * mtiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * (tiles < sms / 2 ? tiles : sms / 2)));
+    cfg.blockDim = dim3(Q8P_THREADS);
+    cfg.dynamicSmemBytes = Q8P_SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, levels, rows, a, ntiles, mtiles);
+}
+
 template <typename T> static cudaError_t q8gemm_n(const Q8MatArgs& a, const CUtensorMap& levels, int device, int sms, cudaStream_t st) {
     if (a.M <= 32) return q8gemm_t<T, 32>(a, levels, device, sms, st);
     if (a.M <= 64) return q8gemm_t<T, 64>(a, levels, device, sms, st);
     if (a.M <= 128) return q8gemm_t<T, 128>(a, levels, device, sms, st);
-    return q8gemm_t<T, 256>(a, levels, device, sms, st);
+    if (a.M <= 256) return q8gemm_t<T, 256>(a, levels, device, sms, st);
+    return q8pair_t<T>(a, levels, device, sms, st);
 }
 
 cudaError_t dz_q8gemm_launch(const Q8MatArgs& a, const CUtensorMap& levels, int type, int device, int sms, cudaStream_t st) {
