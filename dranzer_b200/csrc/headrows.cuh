@@ -1,5 +1,5 @@
-// The norm and the rotation of a head that the lanes of a warp share, for the
-// appends to 4-bit and 8-bit caches.
+// The norm of a head that the lanes of a warp share, for the appends to 4-bit
+// and 8-bit caches.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -31,39 +31,6 @@ template <int LPH, int E, typename A> __device__ __forceinline__ A kv4_square_su
 #pragma unroll
     for (int off = LPH / 2; off >= 1; off >>= 1) s += __shfl_xor_sync(mask, s, off);
     return s;
-}
-
-__device__ __forceinline__ float kv4_signed(float v, bool minus) {
-    return __uint_as_float(__float_as_uint(v) ^ (minus ? 0x80000000u : 0u));
-}
-__device__ __forceinline__ double kv4_signed(double v, bool minus) {
-    return __hiloint2double(__double2hiint(v) ^ (minus ? (int)0x80000000 : 0), __double2loint(v));
-}
-
-// Rotates a head's E elements of this lane, element `at` first; angle(i) gives
-// cosine and sine of the lane's i-th pair.
-template <int HD, int E, typename A, typename F>
-__device__ __forceinline__ void kv4_rotate(A (&x)[E], bool halves, int lane, int at, F angle) {
-    constexpr int LPH = HD / E;
-    if (halves) {
-        // element e pairs with e + HD / 2, which the lane half a head away holds at the same index:
-        // x cos - other sin in the first half, x cos + other sin in the second
-        const unsigned mask = kv4_mask<LPH>(lane);
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            const auto q = angle(i);
-            const A other = kv4_signed(__shfl_xor_sync(mask, x[i], LPH / 2), at < HD / 2);
-            x[i] = x[i] * (A)q.x + other * (A)q.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < E; i += 2) {
-            const auto q = angle(i / 2);
-            const A u = x[i], v = x[i + 1];
-            x[i] = u * (A)q.x - v * (A)q.y;
-            x[i + 1] = u * (A)q.y + v * (A)q.x;
-        }
-    }
 }
 
 }  // namespace dz

@@ -38,6 +38,39 @@ template <int HD, int E> __device__ __forceinline__ int kv4_angle_at(int p, bool
     return p % own * (HD / 2 / own) + p / own;
 }
 
+__device__ __forceinline__ float kv4_signed(float v, bool minus) {
+    return __uint_as_float(__float_as_uint(v) ^ (minus ? 0x80000000u : 0u));
+}
+__device__ __forceinline__ double kv4_signed(double v, bool minus) {
+    return __hiloint2double(__double2hiint(v) ^ (minus ? (int)0x80000000 : 0), __double2loint(v));
+}
+
+// Rotates a head's E elements of this lane, element `at` first; angle(i) gives
+// cosine and sine of the lane's i-th pair.
+template <int HD, int E, typename A, typename F>
+__device__ __forceinline__ void kv4_rotate(A (&x)[E], bool halves, int lane, int at, F angle) {
+    constexpr int LPH = HD / E;
+    if (halves) {
+        // element e pairs with e + HD / 2, which the lane half a head away holds at the same index:
+        // x cos - other sin in the first half, x cos + other sin in the second
+        const unsigned mask = kv4_mask<LPH>(lane);
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            const auto q = angle(i);
+            const A other = kv4_signed(__shfl_xor_sync(mask, x[i], LPH / 2), at < HD / 2);
+            x[i] = x[i] * (A)q.x + other * (A)q.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; i += 2) {
+            const auto q = angle(i / 2);
+            const A u = x[i], v = x[i + 1];
+            x[i] = u * (A)q.x - v * (A)q.y;
+            x[i + 1] = u * (A)q.y + v * (A)q.x;
+        }
+    }
+}
+
 // Quantizes the lane's elements of a row and writes their codes (and the
 // group's scale) at cache row `row`; x becomes the values that they stand for.
 template <int HD, int E>

@@ -11,13 +11,21 @@
 
 namespace dz {
 
-// A block takes the new tokens of one sequence that fall in one page, and a
-// share of their heads: keys, values, queries. A head's rows go to a team of 1
-// to 8 warps, at most eight rows to a warp, a row over the lanes of a warp; a
-// key or value head is held in registers until the team knows its peak, so that
-// the page's scale needs no second pass over memory. The rows' angles are
-// computed once per block: sine and cosine of every 16th row in 64 bits, the
-// rows between by turning on by one token's angle (15 roundings of 2^-53).
+// A lane holds eight elements of a row in two quads that contain both elements
+// of each pair of the rotation: element 8 l of 8 side by side, or 4 l of 4 of
+// each half. Eight or sixteen lanes have a row, a warp four or two rows (or
+// heads of one row).
+//
+// Many tokens: a block takes the new tokens of one sequence that fall in one
+// page, and a share of their heads: keys, values, queries. A head's rows go to a
+// team of 1 to 8 warps, eight rows to a warp at most; a key or value head is
+// held in registers until the team knows its peak, so that the page's scale
+// needs no second pass over memory. The rows' angles are computed once per
+// block: sine and cosine of every 16th row in 64 bits, the rows between by
+// turning on by one token's angle (15 roundings of 2^-53).
+//
+// One token: a block takes a share of a row's heads, a warp two or four heads
+// at a time.
 //
 // Queries are normed and rotated in fp32. Keys are in 64 bits up to one
 // rounding to fp32, because the codes that follow round values next to a border
@@ -29,48 +37,40 @@ constexpr int KV8_TURN = 16;       // rows between angles that are computed afre
 
 struct Kv8AppendCut {
     int runs;                      // pages that a sequence's new tokens can touch
-    int parts;                     // blocks that share a run's heads
+    int parts;                     // blocks that share a run's (a row's) heads
     int team;                      // warps of a head
-    int wide;                      // every row of every operand is aligned to a lane's elements
-    int table_rows;                // rows of the angle table
+    int wide;                      // every row of every operand is aligned to a quad
 };
 
-template <typename T, int E> union Kv8Lane {     // a lane's elements of a row
-    T e[E];
+template <typename T> union Kv8Quad {
+    T e[4];
     uint2 w2;
     uint4 w4;
-    unsigned w1;
-    __device__ Kv8Lane() {}
+    __device__ Kv8Quad() {}
 };
 
-template <typename T, int E> __device__ __forceinline__ void kv8_load(const T* in, bool wide, Kv8Lane<T, E>& to) {
-    constexpr int B = E * (int)sizeof(T);
+template <typename T> __device__ __forceinline__ void kv8_load(const T* in, bool wide, Kv8Quad<T>& to) {
     if (!wide) {
 #pragma unroll
-        for (int i = 0; i < E; i++) to.e[i] = in[i];
-    } else if (B == 16) {
+        for (int i = 0; i < 4; i++) to.e[i] = in[i];
+    } else if (sizeof(T) == 4) {
         to.w4 = *reinterpret_cast<const uint4*>(in);
-    } else if (B == 8) {
-        to.w2 = *reinterpret_cast<const uint2*>(in);
     } else {
-        to.w1 = *reinterpret_cast<const unsigned*>(in);
+        to.w2 = *reinterpret_cast<const uint2*>(in);
     }
 }
 
-template <typename T, int E> __device__ __forceinline__ void kv8_store(T* out, bool wide, const float (&x)[E]) {
-    constexpr int B = E * (int)sizeof(T);
-    Kv8Lane<T, E> io;
+template <typename T> __device__ __forceinline__ void kv8_store(T* out, bool wide, const float* x) {
+    Kv8Quad<T> io;
 #pragma unroll
-    for (int i = 0; i < E; i++) io.e[i] = dz_from_float<T>(x[i]);
+    for (int i = 0; i < 4; i++) io.e[i] = dz_from_float<T>(x[i]);
     if (!wide) {
 #pragma unroll
-        for (int i = 0; i < E; i++) out[i] = io.e[i];
-    } else if (B == 16) {
+        for (int i = 0; i < 4; i++) out[i] = io.e[i];
+    } else if (sizeof(T) == 4) {
         *reinterpret_cast<uint4*>(out) = io.w4;
-    } else if (B == 8) {
-        *reinterpret_cast<uint2*>(out) = io.w2;
     } else {
-        *reinterpret_cast<unsigned*>(out) = io.w1;
+        *reinterpret_cast<uint2*>(out) = io.w2;
     }
 }
 
@@ -79,31 +79,157 @@ __device__ __forceinline__ int kv8_round(float v) {
     const float r = __fadd_rn(v, copysignf(0.5f, v));
     return __float2int_rz(fminf(fmaxf(r, -127.0f), 127.0f)) & (v != v ? 0 : -1);
 }
+// The same for |v| <= 127 and two roundings.
+__device__ __forceinline__ unsigned kv8_round_held(float v) {
+    return (unsigned)__float2int_rz(__fadd_rn(v, copysignf(0.5f, v))) & 0xffu;
+}
+
+// Turns the lane's four pairs by their angles.
+template <typename A, typename C> __device__ __forceinline__ void kv8_rotate(A (&x)[8], bool halves, const C (&turn)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const A c = turn[i].x, s = turn[i].y;
+        if (halves) {
+            const A u = x[i], v = x[i + 4];
+            x[i] = u * c - v * s;
+            x[i + 4] = u * s + v * c;
+        } else {
+            const A u = x[2 * i], v = x[2 * i + 1];
+            x[2 * i] = u * c - v * s;
+            x[2 * i + 1] = u * s + v * c;
+        }
+    }
+}
+
+// A query's eight elements normed and rotated in fp32.
+template <int HD>
+__device__ __forceinline__ void kv8_query(float (&x)[8], const float (&gain)[8], const float2 (&turn)[4], const Kv8AppendArgs& a) {
+    if (a.q_gain) {
+        const float s = kv4_square_sum<HD / 8>(x, 0xffffffffu);
+        float n = kv4_rsqrt(s * (1.0f / HD) + (float)a.eps);
+        if (__any_sync(0xffffffffu, !(s > 1e-25f && s < 1e37f))) {   // squares that leave fp32's range
+            double y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = (double)x[i];
+            const double m = kv4_rsqrt(kv4_square_sum<HD / 8>(y, 0xffffffffu) / HD + a.eps);
+            if (!(s > 1e-25f && s < 1e37f)) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = (float)(y[i] * m);
+                n = 1.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = gain[i] * (x[i] * n);   // x n is about 1: gains of any size
+    }
+    if (a.rope) kv8_rotate(x, a.halves, turn);
+}
+
+// A key's eight elements, in 64 bits up to the last rounding; `at` its quads'
+// elements, turn(i) the angle of its i-th pair.
+template <int HD, typename F>
+__device__ __forceinline__ void kv8_key(float (&x)[8], const int (&at)[2], F turn, const Kv8AppendArgs& a) {
+    if (!a.k_gain && !a.rope) return;
+    double y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = (double)x[i];
+    if (a.k_gain) {
+        const double n = kv4_rsqrt(kv4_square_sum<HD / 8>(y, 0xffffffffu) / HD + a.eps);
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = (double)a.k_gain[at[i / 4] + i % 4] * y[i] * n;
+    }
+    if (a.rope) {
+        const double2 by[4] = {turn(0), turn(1), turn(2), turn(3)};
+        kv8_rotate(y, a.halves, by);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = (float)y[i];
+}
+
+__device__ __forceinline__ unsigned kv8_top(const float (&x)[8]) {
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    return top;
+}
+
+// The scale of a page's head from the new rows' largest magnitude (as bits;
+// above 0x7f7fffff it is not finite) and the scale of the rows before them.
+struct Kv8Scale {
+    float scale, inverse;
+    bool empty, plain;         // codes are 0; the inverse is finite and the codes need no clamp
+};
+__device__ __forceinline__ Kv8Scale kv8_scale(unsigned top, float old) {
+    Kv8Scale s;
+    const bool poisoned = top > 0x7f7fffffu || old != old;
+    s.scale = poisoned ? __int_as_float(0x7fc00000) : fmaxf(old, __fdiv_rn(__uint_as_float(top), 127.0f));
+    s.inverse = __fdiv_rn(1.0f, s.scale);
+    s.empty = poisoned || s.scale == 0.0f;
+    s.plain = s.scale >= 0x1p-120f;          // a peak's quotient rounds well there
+    return s;
+}
+
+// Codes of a lane's elements to the row at `to`; x becomes what they stand for.
+__device__ __forceinline__ void kv8_codes(float (&x)[8], const Kv8Scale& s, int8_t* to, const int (&at)[2]) {
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+        unsigned word = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float v = __fmul_rn(x[4 * q + i], s.inverse);
+            const unsigned c = s.empty ? 0u : s.plain ? kv8_round_held(v) : (unsigned)kv8_round(v) & 0xffu;
+            word |= c << (8 * i);
+            x[4 * q + i] = (float)(int)(int8_t)c * s.scale;
+        }
+        *reinterpret_cast<unsigned*>(to + at[q]) = word;
+    }
+}
+
+// The codes of a page's first `rows` rows after its scale went from `old` to
+// `scale`: thread `me` of `count`.
+template <int HD> __device__ __forceinline__ void kv8_rescale(int8_t* codes, int rows, float old, float scale, int me, int count) {
+    const float ratio = __fdiv_rn(old, scale);
+    for (int i = me; i < rows * (HD / 16); i += count) {
+        uint4* at = reinterpret_cast<uint4*>(codes) + i;
+        uint4 v = *at;
+        unsigned* w = reinterpret_cast<unsigned*>(&v);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            unsigned n = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                n |= ((unsigned)kv8_round(__fmul_rn((float)(int)(int8_t)(w[q] >> (8 * e)), ratio)) & 0xffu) << (8 * e);
+            w[q] = n;
+        }
+        *at = v;
+    }
+}
+
+// Where the angle of pair p of a row lies: the i-th pairs of a row's lanes side by side.
+template <int HD> __device__ __forceinline__ int kv8_angle_at(int p) { return p % 4 * (HD / 8) + p / 4; }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(KV8_WARPS * 32) dz_kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a,
-                                                                      const __grid_constant__ Kv8AppendCut cut) {
-    constexpr int E = HD / 32, P = HD / 2;
-    extern __shared__ __align__(16) uint8_t kv8_smem[];
-    double2* angles = reinterpret_cast<double2*>(kv8_smem);                        // [rows][P]
-    float2* angles_f = reinterpret_cast<float2*>(angles + cut.table_rows * P);     // [rows][P]
+__global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a,
+                                                                         const __grid_constant__ Kv8AppendCut cut) {
+    constexpr int LANES = HD / 8, SLOTS = 32 / LANES, R = KV8_ROWS / SLOTS, P = HD / 2;
+    extern __shared__ __align__(16) double2 kv8_angles[];                          // [rows][P]
     __shared__ unsigned tops[2][KV8_WARPS];
     asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before ends
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, at = lane * E;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, slot = lane / LANES;
+    const int at[2] = {a.halves ? l * 4 : l * 8, a.halves ? P + l * 4 : l * 8 + 4};
     int where = blockIdx.x;
     const int part = where % cut.parts;
     where /= cut.parts;
     const int run = where % cut.runs, b = where / cut.runs;
     const long long first = a.positions[b];
     if (kv8_skips(first)) return;
-    // this block's tokens: lo..hi-1 of the call's, all in page `slot` of the sequence
-    const long long slot = first / a.c.page + run, start = slot * a.c.page;
+    // this block's tokens: lo..hi-1 of the call's, all in page `j` of the sequence
+    const long long j = first / a.c.page + run, start = j * a.c.page;
     const int lo = (int)max(0LL, start - first), hi = (int)min((long long)a.n_tokens, start + a.c.page - first);
     if (lo >= hi) return;
     const int rows = hi - lo, offset = (int)(first + lo - start);     // rows of the page before them
-    int where_page = -1;
-    if (slot < a.c.table_pages) where_page = a.c.table[(long long)b * a.c.table_pages + slot];
-    const bool held = (unsigned)where_page < (unsigned)a.c.pages;
+    int page = -1;
+    if (j < a.c.table_pages) page = a.c.table[(long long)b * a.c.table_pages + j];
+    const bool held = (unsigned)page < (unsigned)a.c.pages;
     if (a.rope) {
         for (int i = threadIdx.x; i < P * ((rows + KV8_TURN - 1) / KV8_TURN); i += KV8_WARPS * 32) {
             const int p = i % P, r0 = i / P * KV8_TURN, r1 = min(r0 + KV8_TURN, rows);
@@ -111,8 +237,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) dz_kv8_append_kernel(const __g
             sincos((double)(first + lo + r0) * a.freq[p], &s, &c);
             sincos(a.freq[p], &s1, &c1);
             for (int r = r0; r < r1; r++) {
-                angles[r * P + p] = make_double2(c, s);
-                angles_f[r * P + p] = make_float2((float)c, (float)s);
+                kv8_angles[r * P + kv8_angle_at<HD>(p)] = make_double2(c, s);
                 const double next = c * c1 - s * s1;
                 s = s * c1 + c * s1;
                 c = next;
@@ -121,97 +246,52 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) dz_kv8_append_kernel(const __g
         __syncthreads();
     }
     const int team = cut.team, mine = warp / team, rank = warp % team, teams = KV8_WARPS / team;
-    const int step = cut.parts * teams;
+    const int step = cut.parts * teams, heads = 2 * a.c.kv_heads + a.q_heads;
     const long long row0 = (long long)b * a.n_tokens + lo;
-    // the lane's pair i of a row: (2p, 2p + 1), or element e with e + HD / 2
-    const int pair0 = a.halves ? at % P : at / 2;
-    int parity = 0;
-    for (int item = part * teams + mine; item < 2 * a.c.kv_heads + a.q_heads; item += step) {
-        if (item >= 2 * a.c.kv_heads) {      // a query head
-            const int h = item - 2 * a.c.kv_heads;
-            const T* in = static_cast<const T*>(a.q) + row0 * a.ldq + h * HD + at;
-            T* out = static_cast<T*>(a.q_out) + row0 * a.ldqo + h * HD + at;
-            float gain[E];
+    // the warp's rows: SLOTS at a time, those of the team in turn
+    auto row_of = [&](int i) { return (i * team + rank) * SLOTS + slot; };
+    auto load = [&](int item, Kv8Quad<T> (&io)[R][2]) {
+        if (item >= heads) return;
+        const bool key = item < a.c.kv_heads, value = !key && item < 2 * a.c.kv_heads;
+        const T* in = static_cast<const T*>(key ? a.k : value ? a.v : a.q);
+        const long long ld = key ? a.ldk : value ? a.ldv : a.ldq;
+        in += row0 * ld + (key ? item : value ? item - a.c.kv_heads : item - 2 * a.c.kv_heads) * HD;
 #pragma unroll
-            for (int i = 0; i < E; i++) gain[i] = a.q_gain ? a.q_gain[at + i] : 1.0f;
-            Kv8Lane<T, E> io[KV8_ROWS];
-#pragma unroll
-            for (int j = 0; j < KV8_ROWS; j++) {
-                const int r = rank + j * team;
-                if (r < rows) kv8_load<T, E>(in + r * a.ldq, cut.wide, io[j]);
+        for (int i = 0; i < R; i++) {
+            const int r = row_of(i);
+            if (r < rows) {
+                kv8_load(in + r * ld + at[0], cut.wide, io[i][0]);
+                kv8_load(in + r * ld + at[1], cut.wide, io[i][1]);
             }
-#pragma unroll
-            for (int j = 0; j < KV8_ROWS; j++) {
-                const int r = rank + j * team;
-                if (r >= rows) break;
-                float x[E];
-#pragma unroll
-                for (int i = 0; i < E; i++) x[i] = dz_to_float(io[j].e[i]);
-                if (a.q_gain) {
-                    const float s = kv4_square_sum<32>(x, 0xffffffffu);
-                    float n = kv4_rsqrt(s * (1.0f / HD) + (float)a.eps);
-                    if (!(s > 1e-25f && s < 1e37f)) {   // squares that leave fp32's range
-                        double y[E];
-#pragma unroll
-                        for (int i = 0; i < E; i++) y[i] = (double)x[i];
-                        const double m = kv4_square_sum<32>(y, 0xffffffffu) / HD + a.eps;
-#pragma unroll
-                        for (int i = 0; i < E; i++) x[i] = (float)(y[i] * kv4_rsqrt(m));
-                        n = 1.0f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < E; i++) x[i] = gain[i] * (x[i] * n);   // x n is about 1: gains of any size
-                }
-                if (a.rope) kv4_rotate<HD>(x, a.halves, lane, at, [&](int i) { return angles_f[r * P + pair0 + i]; });
-                kv8_store<T, E>(out + r * a.ldqo, cut.wide, x);
-            }
-            continue;
         }
+    };
+    int item = part * teams + mine, parity = 0;
+    Kv8Quad<T> next[R][2];
+    load(item, next);
+    float x[R][8];
+    auto take = [&] {                        // the item's elements, and the next one's loads
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[i][e] = row_of(i) < rows ? dz_to_float(next[i][e / 4].e[e % 4]) : 0.0f;
+        load(item + step, next);
+    };
+    for (; item < 2 * a.c.kv_heads; item += step) {
+        take();
+        if (!held) continue;                 // the whole block alike
         const bool key = item < a.c.kv_heads;
         const int h = key ? item : item - a.c.kv_heads;
-        const long long ld = key ? a.ldk : a.ldv;
-        const T* in = static_cast<const T*>(key ? a.k : a.v) + row0 * ld + h * HD + at;
-        if (!held) continue;                 // the whole block alike
-        float x[KV8_ROWS][E];
-        unsigned top = 0;                    // bits of the largest magnitude; above 0x7f7fffff it is not finite
-        {
-            Kv8Lane<T, E> io[KV8_ROWS];
+        unsigned top = 0;
 #pragma unroll
-            for (int j = 0; j < KV8_ROWS; j++) {
-                const int r = rank + j * team;
-                if (r < rows) kv8_load<T, E>(in + r * ld, cut.wide, io[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < KV8_ROWS; j++) {
-                const int r = rank + j * team;
-                if (r < rows) {
-#pragma unroll
-                    for (int i = 0; i < E; i++) x[j][i] = dz_to_float(io[j].e[i]);
-                    if (key && (a.k_gain || a.rope)) {
-                        double y[E];
-#pragma unroll
-                        for (int i = 0; i < E; i++) y[i] = (double)x[j][i];
-                        if (a.k_gain) {
-                            const double n = kv4_rsqrt(kv4_square_sum<32>(y, 0xffffffffu) / HD + a.eps);
-#pragma unroll
-                            for (int i = 0; i < E; i++) y[i] = (double)a.k_gain[at + i] * y[i] * n;
-                        }
-                        if (a.rope)
-                            kv4_rotate<HD>(y, a.halves, lane, at, [&](int i) { return angles[r * P + pair0 + i]; });
-#pragma unroll
-                        for (int i = 0; i < E; i++) x[j][i] = (float)y[i];
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < E; i++) x[j][i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < E; i++) top = max(top, __float_as_uint(x[j][i]) & 0x7fffffffu);
-            }
+        for (int i = 0; i < R; i++) {
+            const int r = min(row_of(i), rows - 1);
+            if (key && (i * team + rank) * SLOTS < rows)                 // the warp alike
+                kv8_key<HD>(x[i], at, [&](int p) { return kv8_angles[r * P + p * LANES + l]; }, a);
+            if (row_of(i) < rows) top = max(top, kv8_top(x[i]));
         }
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const long long place = (long long)where_page * a.c.kv_heads + h;      // the page's head
+        const long long place = (long long)page * a.c.kv_heads + h;      // the page's head
         float* scales = key ? a.c.k_scales : a.c.v_scales;
         const float old = offset ? scales[place] : 0.0f;
         if (team > 1) {                      // the team's peak
@@ -222,52 +302,139 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) dz_kv8_append_kernel(const __g
         } else {
             __syncwarp();
         }
-        const bool poisoned = top > 0x7f7fffffu || old != old;
-        const float fresh = __fdiv_rn(__uint_as_float(top), 127.0f);
-        const float scale = poisoned ? __int_as_float(0x7fc00000) : fmaxf(old, fresh);
-        const float inverse = __fdiv_rn(1.0f, scale);
+        const Kv8Scale s = kv8_scale(top, old);
         int8_t* codes = (key ? a.c.k_codes : a.c.v_codes) + place * (a.c.page * HD);
-        if (scale > old && offset) {         // the earlier rows take the larger scale
-            const float ratio = __fdiv_rn(old, scale);
-            for (int i = rank * 32 + lane; i < offset * (HD / 16); i += team * 32) {
-                uint4* word = reinterpret_cast<uint4*>(codes) + i;
-                uint4 v = *word;
-                unsigned* w = reinterpret_cast<unsigned*>(&v);
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    unsigned n = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int c = (int)(int8_t)(w[q] >> (8 * e));
-                        n |= ((unsigned)kv8_round(__fmul_rn((float)c, ratio)) & 0xffu) << (8 * e);
-                    }
-                    w[q] = n;
-                }
-                *word = v;
-            }
-        }
-        if (rank == 0 && lane == 0) scales[place] = scale;
+        if (offset && s.scale > old) kv8_rescale<HD>(codes, offset, old, s.scale, rank * 32 + lane, team * 32);
+        if (rank == 0 && lane == 0) scales[place] = s.scale;
         T* out = static_cast<T*>(key ? a.k_out : a.v_out);
         const long long ldo = key ? a.ldko : a.ldvo;
-        if (out) out += row0 * ldo + h * HD + at;
+        if (out) out += row0 * ldo + h * HD;
 #pragma unroll
-        for (int j = 0; j < KV8_ROWS; j++) {
-            const int r = rank + j * team;
-            if (r >= rows) break;
-            unsigned word = 0;
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                // zeros where the scale's inverse is not finite: 0 * inf is a NaN, and rounds to 0
-                const int c = poisoned || scale == 0.0f ? 0 : kv8_round(__fmul_rn(x[j][i], inverse));
-                word |= ((unsigned)c & 0xffu) << (8 * i);
-                x[j][i] = (float)c * scale;
+        for (int i = 0; i < R; i++) {
+            const int r = row_of(i);
+            if (r >= rows) continue;
+            kv8_codes(x[i], s, codes + (offset + r) * HD, at);
+            if (out) {
+                kv8_store(out + r * ldo + at[0], cut.wide, x[i]);
+                kv8_store(out + r * ldo + at[1], cut.wide, x[i] + 4);
             }
-            int8_t* to = codes + (offset + r) * HD + at;
-            if (E == 4)
-                *reinterpret_cast<unsigned*>(to) = word;
-            else
-                *reinterpret_cast<unsigned short*>(to) = (unsigned short)word;
-            if (out) kv8_store<T, E>(out + r * ldo, cut.wide, x[j]);
+        }
+    }
+    if (item >= heads) return;
+    float gain[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) gain[i] = a.q_gain ? a.q_gain[at[i / 4] + i % 4] : 1.0f;
+    for (; item < heads; item += step) {
+        take();
+        T* out = static_cast<T*>(a.q_out) + row0 * a.ldqo + (item - 2 * a.c.kv_heads) * HD;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            if ((i * team + rank) * SLOTS >= rows) break;                // the warp alike
+            const int r = row_of(i);
+            float2 turn[4];
+#pragma unroll
+            for (int p = 0; p < 4; p++)
+                if (a.rope) {
+                    const double2 d = kv8_angles[min(r, rows - 1) * P + p * LANES + l];
+                    turn[p] = make_float2((float)d.x, (float)d.y);
+                }
+            kv8_query<HD>(x[i], gain, turn, a);
+            if (r < rows) {
+                kv8_store(out + r * a.ldqo + at[0], cut.wide, x[i]);
+                kv8_store(out + r * a.ldqo + at[1], cut.wide, x[i] + 4);
+            }
+        }
+    }
+}
+
+// One new token of every sequence.
+template <typename T, int HD>
+__global__ void __launch_bounds__(KV8_WARPS * 32, 4) dz_kv8_append_one_kernel(const __grid_constant__ Kv8AppendArgs a,
+                                                                             const __grid_constant__ Kv8AppendCut cut) {
+    constexpr int LANES = HD / 8, SLOTS = 32 / LANES, P = HD / 2;
+    __shared__ double2 angles[P];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, slot = lane / LANES;
+    const int at[2] = {a.halves ? l * 4 : l * 8, a.halves ? P + l * 4 : l * 8 + 4};
+    const int b = blockIdx.x / (unsigned)cut.parts, part = blockIdx.x % (unsigned)cut.parts;
+    const long long pos = a.positions[b];
+    const int nk = (a.c.kv_heads + SLOTS - 1) / SLOTS, nq = (a.q_heads + SLOTS - 1) / SLOTS;    // items
+    const int step = cut.parts * KV8_WARPS;
+    Kv8Quad<T> next[2];
+    auto load = [&](int item) {              // keys, then values, then queries
+        const bool key = item < nk, value = !key && item < 2 * nk;
+        const int h = (key ? item : value ? item - nk : item - 2 * nk) * SLOTS + slot;
+        if (item >= 2 * nk + nq || h >= (key || value ? a.c.kv_heads : a.q_heads)) return;
+        const T* in = static_cast<const T*>(key ? a.k : value ? a.v : a.q) + b * (key ? a.ldk : value ? a.ldv : a.ldq) + h * HD;
+        kv8_load(in + at[0], cut.wide, next[0]);
+        kv8_load(in + at[1], cut.wide, next[1]);
+    };
+    int item = part * KV8_WARPS + warp;
+    load(item);
+    if (kv8_skips(pos)) return;
+    const long long j = pos / a.c.page;
+    const int offset = (int)(pos - j * a.c.page);        // rows of the page before the token's
+    int page = -1;
+    if (j < a.c.table_pages) page = a.c.table[(long long)b * a.c.table_pages + j];
+    const bool held = (unsigned)page < (unsigned)a.c.pages;
+    if (a.rope) {
+        if (threadIdx.x < P) {
+            double c, s;
+            sincos((double)pos * a.freq[threadIdx.x], &s, &c);
+            angles[kv8_angle_at<HD>(threadIdx.x)] = make_double2(c, s);
+        }
+        __syncthreads();
+    }
+    float x[8];
+    auto take = [&](bool valid) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = valid ? dz_to_float(next[e / 4].e[e % 4]) : 0.0f;
+        load(item + step);
+    };
+    for (; item < 2 * nk; item += step) {
+        const bool key = item < nk;
+        const int h = (key ? item : item - nk) * SLOTS + slot;
+        const bool valid = h < a.c.kv_heads;
+        take(valid);
+        if (!held) continue;
+        const long long place = (long long)page * a.c.kv_heads + (valid ? h : 0);
+        float* scales = key ? a.c.k_scales : a.c.v_scales;
+        const float old = offset ? scales[place] : 0.0f;
+        if (key) kv8_key<HD>(x, at, [&](int p) { return angles[p * LANES + l]; }, a);
+        unsigned top = kv8_top(x);
+#pragma unroll
+        for (int off = LANES / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if (!valid) continue;
+        const Kv8Scale s = kv8_scale(top, old);
+        int8_t* codes = (key ? a.c.k_codes : a.c.v_codes) + place * (a.c.page * HD);
+        if (offset && s.scale > old) kv8_rescale<HD>(codes, offset, old, s.scale, l, LANES);
+        if (l == 0) scales[place] = s.scale;
+        kv8_codes(x, s, codes + offset * HD, at);
+        T* out = static_cast<T*>(key ? a.k_out : a.v_out);
+        if (out) {
+            out += b * (key ? a.ldko : a.ldvo) + h * HD;
+            kv8_store(out + at[0], cut.wide, x);
+            kv8_store(out + at[1], cut.wide, x + 4);
+        }
+    }
+    float gain[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) gain[i] = a.q_gain ? a.q_gain[at[i / 4] + i % 4] : 1.0f;
+    for (; item < 2 * nk + nq; item += step) {
+        const int h = (item - 2 * nk) * SLOTS + slot;
+        take(h < a.q_heads);
+        float2 turn[4];
+#pragma unroll
+        for (int p = 0; p < 4; p++)
+            if (a.rope) {
+                const double2 d = angles[p * LANES + l];
+                turn[p] = make_float2((float)d.x, (float)d.y);
+            }
+        kv8_query<HD>(x, gain, turn, a);
+        if (h < a.q_heads) {
+            T* out = static_cast<T*>(a.q_out) + b * a.ldqo + h * HD;
+            kv8_store(out + at[0], cut.wide, x);
+            kv8_store(out + at[1], cut.wide, x + 4);
         }
     }
 }
@@ -276,37 +443,44 @@ constexpr int KV8_DEVICES = 64;
 
 template <typename T, int HD> static cudaError_t kv8_append_t(const Kv8AppendArgs& a, int device, int sms, cudaStream_t st) {
     static std::atomic<bool> ready[KV8_DEVICES];
-    constexpr int most = 64 * (HD / 2) * (int)(sizeof(double2) + sizeof(float2));
-    if (!ready[device].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(dz_kv8_append_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        if (e != cudaSuccess) return e;
-        ready[device].store(true, std::memory_order_release);
-    }
-    Kv8AppendCut cut;
     const int rows = a.n_tokens < a.c.page ? a.n_tokens : a.c.page;          // of a block at most
-    cut.runs = (int)(((long long)a.n_tokens + a.c.page - 2) / a.c.page) + 1;
-    for (cut.team = 1; cut.team * KV8_ROWS < rows;) cut.team *= 2;
-    // four blocks to an SM, as far as there are heads for their teams
-    const long long blocks = (long long)a.c.batch * cut.runs, teams = KV8_WARPS / cut.team;
-    const long long heads = (2 * a.c.kv_heads + a.q_heads + teams - 1) / teams;
-    long long parts = (4LL * sms + blocks - 1) / blocks;
-    cut.parts = (int)(parts < heads ? parts : heads);
-    constexpr int B = HD / 32 * (int)sizeof(T);
+    Kv8AppendCut cut;
     const uintptr_t bases = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out | (uintptr_t)a.k_out |
                             (uintptr_t)a.v_out;
     const long long strides = a.ldq | a.ldk | a.ldv | a.ldqo | a.ldko | a.ldvo;
-    cut.wide = bases % B == 0 && strides * (long long)sizeof(T) % B == 0;
-    cut.table_rows = a.rope ? rows : 0;
+    cut.wide = bases % (4 * sizeof(T)) == 0 && strides % 4 == 0;
+    long long blocks = a.c.batch, most;                  // most: blocks that have heads for their warps
+    if (a.n_tokens == 1) {
+        constexpr int SLOTS = 256 / HD;
+        cut.runs = cut.team = 1;
+        most = (2 * ((a.c.kv_heads + SLOTS - 1) / SLOTS) + (a.q_heads + SLOTS - 1) / SLOTS + KV8_WARPS - 1) / KV8_WARPS;
+    } else {
+        cut.runs = (int)(((long long)a.n_tokens + a.c.page - 2) / a.c.page) + 1;
+        blocks *= cut.runs;
+        for (cut.team = 1; cut.team * KV8_ROWS < rows;) cut.team *= 2;
+        const int teams = KV8_WARPS / cut.team;
+        most = (2 * a.c.kv_heads + a.q_heads + teams - 1) / teams;
+    }
+    // four blocks to an SM, as far as there are heads
+    const long long parts = (4LL * sms + blocks - 1) / blocks;
+    cut.parts = (int)(parts < most ? parts : most);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(blocks * cut.parts));
     cfg.blockDim = dim3(KV8_WARPS * 32);
-    cfg.dynamicSmemBytes = (size_t)cut.table_rows * (HD / 2) * (sizeof(double2) + sizeof(float2));
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if (a.n_tokens == 1) return cudaLaunchKernelEx(&cfg, dz_kv8_append_one_kernel<T, HD>, a, cut);
+    constexpr int most_smem = 64 * (HD / 2) * (int)sizeof(double2);
+    if (!ready[device].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(dz_kv8_append_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
+        if (e != cudaSuccess) return e;
+        ready[device].store(true, std::memory_order_release);
+    }
+    cfg.dynamicSmemBytes = a.rope ? (size_t)rows * (HD / 2) * sizeof(double2) : 0;
     return cudaLaunchKernelEx(&cfg, dz_kv8_append_kernel<T, HD>, a, cut);
 }
 

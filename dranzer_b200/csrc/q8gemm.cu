@@ -229,15 +229,16 @@ static cudaError_t q8gemm_t(const Q8MatArgs& a, const CUtensorMap& levels, int d
 // (cta_group::2): each loads 128 columns of levels and half of the rows, 32 KB
 // for 256 x 128 x 128 products of its own, where a block alone would load 48.
 // The pairs stay and take tiles in turn. Two accumulators fill the tensor
-// memory, so that four warps of each block write a tile while the next one's
-// MMAs run. The first block of a pair issues the MMAs for both; its `full`
+// memory, so that eight warps of each block write a tile while the next one's
+// MMAs run (four took 250 us for 4096 x 4096 x 16384, the MMAs waiting). The first block of a pair issues the MMAs for both; its `full`
 // barriers count both blocks' bytes, commits arrive at both blocks' barriers.
 
-constexpr int Q8P_THREADS = 192;                 // warp 0 copies, warp 1 MMAs, warps 2..5 outputs
+constexpr int Q8P_WRITERS = 8;
+constexpr int Q8P_THREADS = 64 + Q8P_WRITERS * 32;   // warp 0 copies, warp 1 MMAs, the others outputs
 constexpr int Q8P_TILE = 256;
 constexpr uint32_t Q8P_STAGE = 2 * 128 * 128;
 constexpr int Q8P_STAGES = 6;
-constexpr size_t Q8P_SMEM = (size_t)Q8P_STAGES * Q8P_STAGE + 1024 + 256;
+constexpr size_t Q8P_SMEM = (size_t)Q8P_STAGES * Q8P_STAGE + 1024 + 256 + 2 * Q8P_TILE * sizeof(float);
 constexpr int Q8P_BAND = 8;                      // tiles of rows that neighbouring pairs share columns over
 
 __device__ __forceinline__ uint32_t q8p_at_leader(const void* p) {       // the same place in the pair's first block
@@ -318,6 +319,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q8P_THREADS, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
     volatile int* failed = reinterpret_cast<int*>(tmem_slot + 1);
     int* issued = reinterpret_cast<int*>(tmem_slot + 2);         // stages copied, consumed
+    float* scales = reinterpret_cast<float*>(sm + (size_t)Q8P_STAGES * Q8P_STAGE + 256);   // [2][256] of the rows
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x & 1u), pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
     const int tiles = ntiles * mtiles;
@@ -328,7 +330,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q8P_THREADS, 1)
         }
         for (int i = 0; i < 2; i++) {
             dz_mbar_init(&done[i]);
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 8;" ::"r"(dz_smem_addr(&drained[i])) : "memory");   // warps
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(dz_smem_addr(&drained[i])), "r"(2 * Q8P_WRITERS)
+                         : "memory");            // their writers
         }
         *failed = 0;
         issued[0] = issued[1] = 0;
@@ -406,44 +409,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q8P_THREADS, 1)
         __syncwarp();
     } else {
         asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows' scales
-        const int quarter = warp & 3;            // a warp reads the lanes of its number modulo 4
+        // a warp reads the lanes of its number modulo 4: 32 columns, and half of the rows
+        const int quarter = warp & 3, half = (warp - 2) / 4 * (Q8P_TILE / 2), thread = (int)threadIdx.x - 64;
+        const T nothing = dz_from_float<T>(__int_as_float(0x7fc00000));
         int turn = 0;
-        T* c = static_cast<T*>(a.c);
+        bool ok = true;
         for (int i = pair; i < tiles; i += pairs, turn++) {
             const int b = turn & 1;
             int tn, tm;
             q8p_place(i, ntiles, mtiles, &tn, &tm);
             const int n = tn * Q8P_TILE + rank * 128 + quarter * 32 + lane, m0 = tm * Q8P_TILE;
             const float scale = n < a.N ? a.col_scale[n] : 0.0f, bias = n < a.N && a.bias ? a.bias[n] : 0.0f;
-            const bool ok = q8p_wait(&done[b], (uint32_t)((turn / 2) & 1));
-            if (!ok && lane == 0) *failed = 1;
+            float* row_scales = scales + b * Q8P_TILE;
+            row_scales[thread] = m0 + thread < a.M ? a.a_scales[m0 + thread] : 0.0f;
+            asm volatile("bar.sync 1, %0;" ::"n"(Q8P_WRITERS * 32) : "memory");
+            if (ok && !q8p_wait(&done[b], (uint32_t)((turn / 2) & 1))) {
+                ok = false;                      // this tile and those after it read NaN
+                *failed = 1;
+            }
             ug_fence_after();
-            for (int c0 = 0; c0 < Q8P_TILE && m0 + c0 < a.M; c0 += 32) {
-                const float own = m0 + c0 + lane < a.M ? a.a_scales[m0 + c0 + lane] : 0.0f;
+            for (int c0 = half; c0 < half + Q8P_TILE / 2 && m0 + c0 < a.M; c0 += 32) {
                 int32_t v[32];
                 ug_tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 256 + c0), v);
-                T* to = c + (long long)(m0 + c0) * a.ldc + n;
+                T* to = static_cast<T*>(a.c) + (long long)(m0 + c0) * a.ldc + n;
+                const int rows = min(32, a.M - m0 - c0);
+                if (n < a.N) {
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    const float row = __shfl_sync(0xffffffffu, own, j);
-                    if (n < a.N && m0 + c0 + j < a.M)
-                        to[j * a.ldc] = ok ? q8_finish<T>(v[j], row, scale, bias) : dz_from_float<T>(__int_as_float(0x7fc00000));
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 r = *reinterpret_cast<const float4*>(row_scales + c0 + j);
+                        const float y[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            if (j + e < rows) *to = ok ? q8_finish<T>(v[j + e], y[e], scale, bias) : nothing;
+                            to += a.ldc;
+                        }
+                    }
                 }
+                __syncwarp();
             }
             ug_fence_before();
             __syncwarp();
             if (lane == 0) {
                 asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(q8p_at_leader(&drained[b]))
                              : "memory");
-            }
-            if (!ok) {                           // the tiles left read NaN
-                for (i += pairs; i < tiles; i += pairs) {
-                    q8p_place(i, ntiles, mtiles, &tn, &tm);
-                    const int nn = tn * Q8P_TILE + rank * 128 + quarter * 32 + lane;
-                    for (int m = tm * Q8P_TILE; m < min(a.M, (tm + 1) * Q8P_TILE); m++)
-                        if (nn < a.N) c[m * a.ldc + nn] = dz_from_float<T>(__int_as_float(0x7fc00000));
-                }
-                break;
             }
         }
     }
