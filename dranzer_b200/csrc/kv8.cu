@@ -18,7 +18,7 @@ namespace dz {
 //
 // Many tokens: a block takes the new tokens of one sequence that fall in one
 // page, and a share of their heads: keys, values, queries. A head's rows go to a
-// team of 1 to 8 warps, eight rows to a warp at most; a key or value head is
+// team of 1 to 16 warps, four rows to a warp at most; a key or value head is
 // held in registers until the team knows its peak, so that the page's scale
 // needs no second pass over memory. The rows' angles are computed once per
 // block: sine and cosine of every 16th row in 64 bits, the rows between by
@@ -31,15 +31,16 @@ namespace dz {
 // rounding to fp32, because the codes that follow round values next to a border
 // and two summation orders would otherwise give different codes.
 
-constexpr int KV8_WARPS = 8;
-constexpr int KV8_ROWS = 8;        // rows of a warp
+constexpr int KV8_WARPS = 16;      // warps of a block, many tokens
+constexpr int KV8_ROWS = 4;        // rows of a warp
+constexpr int KV8_ONE_WARPS = 8;   // warps of a block, one token
 constexpr int KV8_TURN = 16;       // rows between angles that are computed afresh
 
 struct Kv8AppendCut {
     int runs;                      // pages that a sequence's new tokens can touch
     int parts;                     // blocks that share a run's (a row's) heads
     int team;                      // warps of a head
-    int wide;                      // every row of every operand is aligned to a quad
+    int table_rows;                // rows of the angle tables
 };
 
 template <typename T> union Kv8Quad {
@@ -49,8 +50,8 @@ template <typename T> union Kv8Quad {
     __device__ Kv8Quad() {}
 };
 
-template <typename T> __device__ __forceinline__ void kv8_load(const T* in, bool wide, Kv8Quad<T>& to) {
-    if (!wide) {
+template <bool WIDE, typename T> __device__ __forceinline__ void kv8_load(const T* in, Kv8Quad<T>& to) {
+    if (!WIDE) {
 #pragma unroll
         for (int i = 0; i < 4; i++) to.e[i] = in[i];
     } else if (sizeof(T) == 4) {
@@ -60,11 +61,11 @@ template <typename T> __device__ __forceinline__ void kv8_load(const T* in, bool
     }
 }
 
-template <typename T> __device__ __forceinline__ void kv8_store(T* out, bool wide, const float* x) {
+template <bool WIDE, typename T> __device__ __forceinline__ void kv8_store(T* out, const float* x) {
     Kv8Quad<T> io;
 #pragma unroll
     for (int i = 0; i < 4; i++) io.e[i] = dz_from_float<T>(x[i]);
-    if (!wide) {
+    if (!WIDE) {
 #pragma unroll
         for (int i = 0; i < 4; i++) out[i] = io.e[i];
     } else if (sizeof(T) == 4) {
@@ -80,9 +81,7 @@ __device__ __forceinline__ int kv8_round(float v) {
     return __float2int_rz(fminf(fmaxf(r, -127.0f), 127.0f)) & (v != v ? 0 : -1);
 }
 // The same for |v| <= 127 and two roundings.
-__device__ __forceinline__ unsigned kv8_round_held(float v) {
-    return (unsigned)__float2int_rz(__fadd_rn(v, copysignf(0.5f, v))) & 0xffu;
-}
+__device__ __forceinline__ int kv8_round_held(float v) { return __float2int_rz(__fadd_rn(v, copysignf(0.5f, v))); }
 
 // Turns the lane's four pairs by their angles.
 template <typename A, typename C> __device__ __forceinline__ void kv8_rotate(A (&x)[8], bool halves, const C (&turn)[4]) {
@@ -124,10 +123,10 @@ __device__ __forceinline__ void kv8_query(float (&x)[8], const float (&gain)[8],
     if (a.rope) kv8_rotate(x, a.halves, turn);
 }
 
-// A key's eight elements, in 64 bits up to the last rounding; `at` its quads'
-// elements, turn(i) the angle of its i-th pair.
+// A key's eight elements, in 64 bits up to the last rounding; turn(i) is the
+// angle of its i-th pair.
 template <int HD, typename F>
-__device__ __forceinline__ void kv8_key(float (&x)[8], const int (&at)[2], F turn, const Kv8AppendArgs& a) {
+__device__ __forceinline__ void kv8_key(float (&x)[8], const float (&gain)[8], F turn, const Kv8AppendArgs& a) {
     if (!a.k_gain && !a.rope) return;
     double y[8];
 #pragma unroll
@@ -135,7 +134,7 @@ __device__ __forceinline__ void kv8_key(float (&x)[8], const int (&at)[2], F tur
     if (a.k_gain) {
         const double n = kv4_rsqrt(kv4_square_sum<HD / 8>(y, 0xffffffffu) / HD + a.eps);
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = (double)a.k_gain[at[i / 4] + i % 4] * y[i] * n;
+        for (int i = 0; i < 8; i++) y[i] = (double)gain[i] * y[i] * n;
     }
     if (a.rope) {
         const double2 by[4] = {turn(0), turn(1), turn(2), turn(3)};
@@ -156,7 +155,7 @@ __device__ __forceinline__ unsigned kv8_top(const float (&x)[8]) {
 // above 0x7f7fffff it is not finite) and the scale of the rows before them.
 struct Kv8Scale {
     float scale, inverse;
-    bool empty, plain;         // codes are 0; the inverse is finite and the codes need no clamp
+    bool empty, plain;         // codes are 0; the codes need no clamp (not empty, and the inverse is finite)
 };
 __device__ __forceinline__ Kv8Scale kv8_scale(unsigned top, float old) {
     Kv8Scale s;
@@ -164,23 +163,27 @@ __device__ __forceinline__ Kv8Scale kv8_scale(unsigned top, float old) {
     s.scale = poisoned ? __int_as_float(0x7fc00000) : fmaxf(old, __fdiv_rn(__uint_as_float(top), 127.0f));
     s.inverse = __fdiv_rn(1.0f, s.scale);
     s.empty = poisoned || s.scale == 0.0f;
-    s.plain = s.scale >= 0x1p-120f;          // a peak's quotient rounds well there
+    s.plain = s.scale >= 0x1p-120f;          // a peak's quotient rounds well there; false for a NaN
     return s;
 }
 
-// Codes of a lane's elements to the row at `to`; x becomes what they stand for.
-__device__ __forceinline__ void kv8_codes(float (&x)[8], const Kv8Scale& s, int8_t* to, const int (&at)[2]) {
+// Codes of a lane's elements to the row at `to`; where `values` are wanted, x
+// becomes what they stand for.
+__device__ __forceinline__ void kv8_codes(float (&x)[8], const Kv8Scale& s, int8_t* to, const int (&at)[2], bool values) {
 #pragma unroll
     for (int q = 0; q < 2; q++) {
-        unsigned word = 0;
+        int c[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float v = __fmul_rn(x[4 * q + i], s.inverse);
-            const unsigned c = s.empty ? 0u : s.plain ? kv8_round_held(v) : (unsigned)kv8_round(v) & 0xffu;
-            word |= c << (8 * i);
-            x[4 * q + i] = (float)(int)(int8_t)c * s.scale;
+            c[i] = s.plain ? kv8_round_held(v) : s.empty ? 0 : kv8_round(v);
         }
-        *reinterpret_cast<unsigned*>(to + at[q]) = word;
+        *reinterpret_cast<unsigned*>(to + at[q]) = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        if (values) {
+            // 2^23 + 2^22 + c, less 2^23 + 2^22
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[4 * q + i] = (__int_as_float(0x4B400000 + c[i]) - 12582912.0f) * s.scale;
+        }
     }
 }
 
@@ -207,11 +210,12 @@ template <int HD> __device__ __forceinline__ void kv8_rescale(int8_t* codes, int
 // Where the angle of pair p of a row lies: the i-th pairs of a row's lanes side by side.
 template <int HD> __device__ __forceinline__ int kv8_angle_at(int p) { return p % 4 * (HD / 8) + p / 4; }
 
-template <typename T, int HD>
+template <typename T, int HD, bool WIDE>     // every row of every operand is aligned to a quad
 __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a,
                                                                          const __grid_constant__ Kv8AppendCut cut) {
     constexpr int LANES = HD / 8, SLOTS = 32 / LANES, R = KV8_ROWS / SLOTS, P = HD / 2;
-    extern __shared__ __align__(16) double2 kv8_angles[];                          // [rows][P]
+    extern __shared__ __align__(16) double2 kv8_angles[];                          // [rows][P], then the same in fp32
+    float2* kv8_angles_f = reinterpret_cast<float2*>(kv8_angles + cut.table_rows * P);
     __shared__ unsigned tops[2][KV8_WARPS];
     asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before ends
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, slot = lane / LANES;
@@ -238,6 +242,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
             sincos(a.freq[p], &s1, &c1);
             for (int r = r0; r < r1; r++) {
                 kv8_angles[r * P + kv8_angle_at<HD>(p)] = make_double2(c, s);
+                kv8_angles_f[r * P + kv8_angle_at<HD>(p)] = make_float2((float)c, (float)s);
                 const double next = c * c1 - s * s1;
                 s = s * c1 + c * s1;
                 c = next;
@@ -246,25 +251,30 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
         __syncthreads();
     }
     const int team = cut.team, mine = warp / team, rank = warp % team, teams = KV8_WARPS / team;
-    const int step = cut.parts * teams, heads = 2 * a.c.kv_heads + a.q_heads;
+    const int step = cut.parts * teams, heads = 2 * a.c.kv_heads;
     const long long row0 = (long long)b * a.n_tokens + lo;
     // the warp's rows: SLOTS at a time, those of the team in turn
     auto row_of = [&](int i) { return (i * team + rank) * SLOTS + slot; };
     auto load = [&](int item, Kv8Quad<T> (&io)[R][2]) {
         if (item >= heads) return;
-        const bool key = item < a.c.kv_heads, value = !key && item < 2 * a.c.kv_heads;
-        const T* in = static_cast<const T*>(key ? a.k : value ? a.v : a.q);
-        const long long ld = key ? a.ldk : value ? a.ldv : a.ldq;
-        in += row0 * ld + (key ? item : value ? item - a.c.kv_heads : item - 2 * a.c.kv_heads) * HD;
+        const bool key = item < a.c.kv_heads;
+        const long long ld = key ? a.ldk : a.ldv;
+        const T* in = static_cast<const T*>(key ? a.k : a.v) + row0 * ld + (key ? item : item - a.c.kv_heads) * HD;
 #pragma unroll
         for (int i = 0; i < R; i++) {
             const int r = row_of(i);
             if (r < rows) {
-                kv8_load(in + r * ld + at[0], cut.wide, io[i][0]);
-                kv8_load(in + r * ld + at[1], cut.wide, io[i][1]);
+                kv8_load<WIDE>(in + r * ld + at[0], io[i][0]);
+                kv8_load<WIDE>(in + r * ld + at[1], io[i][1]);
             }
         }
     };
+    float gain[8];
+    auto gains = [&](const float* g) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) gain[i] = g ? g[at[i / 4] + i % 4] : 1.0f;
+    };
+    gains(a.k_gain);
     int item = part * teams + mine, parity = 0;
     Kv8Quad<T> next[R][2];
     load(item, next);
@@ -276,7 +286,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
             for (int e = 0; e < 8; e++) x[i][e] = row_of(i) < rows ? dz_to_float(next[i][e / 4].e[e % 4]) : 0.0f;
         load(item + step, next);
     };
-    for (; item < 2 * a.c.kv_heads; item += step) {
+    for (; item < heads; item += step) {
         take();
         if (!held) continue;                 // the whole block alike
         const bool key = item < a.c.kv_heads;
@@ -286,7 +296,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
         for (int i = 0; i < R; i++) {
             const int r = min(row_of(i), rows - 1);
             if (key && (i * team + rank) * SLOTS < rows)                 // the warp alike
-                kv8_key<HD>(x[i], at, [&](int p) { return kv8_angles[r * P + p * LANES + l]; }, a);
+                kv8_key<HD>(x[i], gain, [&](int p) { return kv8_angles[r * P + p * LANES + l]; }, a);
             if (row_of(i) < rows) top = max(top, kv8_top(x[i]));
         }
 #pragma unroll
@@ -313,43 +323,61 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
         for (int i = 0; i < R; i++) {
             const int r = row_of(i);
             if (r >= rows) continue;
-            kv8_codes(x[i], s, codes + (offset + r) * HD, at);
+            kv8_codes(x[i], s, codes + (offset + r) * HD, at, out != nullptr);
             if (out) {
-                kv8_store(out + r * ldo + at[0], cut.wide, x[i]);
-                kv8_store(out + r * ldo + at[1], cut.wide, x[i] + 4);
+                kv8_store<WIDE>(out + r * ldo + at[0], x[i]);
+                kv8_store<WIDE>(out + r * ldo + at[1], x[i] + 4);
             }
         }
     }
-    if (item >= heads) return;
-    float gain[8];
+    // queries: a warp takes SLOTS rows at a time, whose angles and gains stay in registers, and this block's heads in
+    // turn, AHEAD of them in flight (two took 57 us of 8000 rows' 115, 16 KB in flight on an SM)
+    constexpr int AHEAD = 8 / (int)sizeof(T);
+    const int h0 = a.q_heads * part / cut.parts, h1 = a.q_heads * (part + 1) / cut.parts;
+    if (h0 == h1) return;
+    gains(a.q_gain);
+    for (int set = warp; set * SLOTS < rows; set += KV8_WARPS) {
+        const int r = set * SLOTS + slot;
+        const bool valid = r < rows;
+        float2 turn[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) gain[i] = a.q_gain ? a.q_gain[at[i / 4] + i % 4] : 1.0f;
-    for (; item < heads; item += step) {
-        take();
-        T* out = static_cast<T*>(a.q_out) + row0 * a.ldqo + (item - 2 * a.c.kv_heads) * HD;
+        for (int p = 0; p < 4; p++)
+            if (a.rope) turn[p] = kv8_angles_f[min(r, rows - 1) * P + p * LANES + l];
+        const T* in = static_cast<const T*>(a.q) + (row0 + r) * a.ldq + h0 * HD + at[0];
+        T* out = static_cast<T*>(a.q_out) + (row0 + r) * a.ldqo + h0 * HD + at[0];
+        const int quad = at[1] - at[0];
+        Kv8Quad<T> ring[AHEAD][2];
+        auto fetch = [&](int h, Kv8Quad<T> (&io)[2]) {
+            if (valid && h < h1) {
+                kv8_load<WIDE>(in, io[0]);
+                kv8_load<WIDE>(in + quad, io[1]);
+            }
+            in += HD;
+        };
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-            if ((i * team + rank) * SLOTS >= rows) break;                // the warp alike
-            const int r = row_of(i);
-            float2 turn[4];
+        for (int k = 0; k < AHEAD; k++) fetch(h0 + k, ring[k]);
+        for (int h = h0; h < h1; h += AHEAD) {
 #pragma unroll
-            for (int p = 0; p < 4; p++)
-                if (a.rope) {
-                    const double2 d = kv8_angles[min(r, rows - 1) * P + p * LANES + l];
-                    turn[p] = make_float2((float)d.x, (float)d.y);
+            for (int k = 0; k < AHEAD; k++) {
+                if (h + k >= h1) break;      // the warp alike
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = valid ? dz_to_float(ring[k][e / 4].e[e % 4]) : 0.0f;
+                fetch(h + k + AHEAD, ring[k]);
+                kv8_query<HD>(y, gain, turn, a);
+                if (valid) {
+                    kv8_store<WIDE>(out, y);
+                    kv8_store<WIDE>(out + quad, y + 4);
                 }
-            kv8_query<HD>(x[i], gain, turn, a);
-            if (r < rows) {
-                kv8_store(out + r * a.ldqo + at[0], cut.wide, x[i]);
-                kv8_store(out + r * a.ldqo + at[1], cut.wide, x[i] + 4);
+                out += HD;
             }
         }
     }
 }
 
 // One new token of every sequence.
-template <typename T, int HD>
-__global__ void __launch_bounds__(KV8_WARPS * 32, 4) dz_kv8_append_one_kernel(const __grid_constant__ Kv8AppendArgs a,
+template <typename T, int HD, bool WIDE>
+__global__ void __launch_bounds__(KV8_ONE_WARPS * 32, 4) dz_kv8_append_one_kernel(const __grid_constant__ Kv8AppendArgs a,
                                                                              const __grid_constant__ Kv8AppendCut cut) {
     constexpr int LANES = HD / 8, SLOTS = 32 / LANES, P = HD / 2;
     __shared__ double2 angles[P];
@@ -359,17 +387,17 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 4) dz_kv8_append_one_kernel(co
     const int b = blockIdx.x / (unsigned)cut.parts, part = blockIdx.x % (unsigned)cut.parts;
     const long long pos = a.positions[b];
     const int nk = (a.c.kv_heads + SLOTS - 1) / SLOTS, nq = (a.q_heads + SLOTS - 1) / SLOTS;    // items
-    const int step = cut.parts * KV8_WARPS;
+    const int step = cut.parts * KV8_ONE_WARPS;
     Kv8Quad<T> next[2];
     auto load = [&](int item) {              // keys, then values, then queries
         const bool key = item < nk, value = !key && item < 2 * nk;
         const int h = (key ? item : value ? item - nk : item - 2 * nk) * SLOTS + slot;
         if (item >= 2 * nk + nq || h >= (key || value ? a.c.kv_heads : a.q_heads)) return;
         const T* in = static_cast<const T*>(key ? a.k : value ? a.v : a.q) + b * (key ? a.ldk : value ? a.ldv : a.ldq) + h * HD;
-        kv8_load(in + at[0], cut.wide, next[0]);
-        kv8_load(in + at[1], cut.wide, next[1]);
+        kv8_load<WIDE>(in + at[0], next[0]);
+        kv8_load<WIDE>(in + at[1], next[1]);
     };
-    int item = part * KV8_WARPS + warp;
+    int item = part * KV8_ONE_WARPS + warp;
     load(item);
     if (kv8_skips(pos)) return;
     const long long j = pos / a.c.page;
@@ -385,7 +413,12 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 4) dz_kv8_append_one_kernel(co
         }
         __syncthreads();
     }
-    float x[8];
+    float x[8], gain[8];
+    auto gains = [&](const float* g) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) gain[i] = g ? g[at[i / 4] + i % 4] : 1.0f;
+    };
+    if (item < nk) gains(a.k_gain);
     auto take = [&](bool valid) {
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = valid ? dz_to_float(next[e / 4].e[e % 4]) : 0.0f;
@@ -400,7 +433,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 4) dz_kv8_append_one_kernel(co
         const long long place = (long long)page * a.c.kv_heads + (valid ? h : 0);
         float* scales = key ? a.c.k_scales : a.c.v_scales;
         const float old = offset ? scales[place] : 0.0f;
-        if (key) kv8_key<HD>(x, at, [&](int p) { return angles[p * LANES + l]; }, a);
+        if (key) kv8_key<HD>(x, gain, [&](int p) { return angles[p * LANES + l]; }, a);
         unsigned top = kv8_top(x);
 #pragma unroll
         for (int off = LANES / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
@@ -409,17 +442,15 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 4) dz_kv8_append_one_kernel(co
         int8_t* codes = (key ? a.c.k_codes : a.c.v_codes) + place * (a.c.page * HD);
         if (offset && s.scale > old) kv8_rescale<HD>(codes, offset, old, s.scale, l, LANES);
         if (l == 0) scales[place] = s.scale;
-        kv8_codes(x, s, codes + offset * HD, at);
         T* out = static_cast<T*>(key ? a.k_out : a.v_out);
+        kv8_codes(x, s, codes + offset * HD, at, out != nullptr);
         if (out) {
             out += b * (key ? a.ldko : a.ldvo) + h * HD;
-            kv8_store(out + at[0], cut.wide, x);
-            kv8_store(out + at[1], cut.wide, x + 4);
+            kv8_store<WIDE>(out + at[0], x);
+            kv8_store<WIDE>(out + at[1], x + 4);
         }
     }
-    float gain[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) gain[i] = a.q_gain ? a.q_gain[at[i / 4] + i % 4] : 1.0f;
+    if (item < 2 * nk + nq) gains(a.q_gain);
     for (; item < 2 * nk + nq; item += step) {
         const int h = (item - 2 * nk) * SLOTS + slot;
         take(h < a.q_heads);
@@ -433,59 +464,63 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 4) dz_kv8_append_one_kernel(co
         kv8_query<HD>(x, gain, turn, a);
         if (h < a.q_heads) {
             T* out = static_cast<T*>(a.q_out) + b * a.ldqo + h * HD;
-            kv8_store(out + at[0], cut.wide, x);
-            kv8_store(out + at[1], cut.wide, x + 4);
+            kv8_store<WIDE>(out + at[0], x);
+            kv8_store<WIDE>(out + at[1], x + 4);
         }
     }
 }
 
 constexpr int KV8_DEVICES = 64;
 
-template <typename T, int HD> static cudaError_t kv8_append_t(const Kv8AppendArgs& a, int device, int sms, cudaStream_t st) {
+template <typename T, int HD, bool WIDE> static cudaError_t kv8_append_t(const Kv8AppendArgs& a, int device, int sms, cudaStream_t st) {
     static std::atomic<bool> ready[KV8_DEVICES];
     const int rows = a.n_tokens < a.c.page ? a.n_tokens : a.c.page;          // of a block at most
     Kv8AppendCut cut;
-    const uintptr_t bases = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out | (uintptr_t)a.k_out |
-                            (uintptr_t)a.v_out;
-    const long long strides = a.ldq | a.ldk | a.ldv | a.ldqo | a.ldko | a.ldvo;
-    cut.wide = bases % (4 * sizeof(T)) == 0 && strides % 4 == 0;
+    cut.table_rows = a.rope ? rows : 0;
     long long blocks = a.c.batch, most;                  // most: blocks that have heads for their warps
     if (a.n_tokens == 1) {
         constexpr int SLOTS = 256 / HD;
         cut.runs = cut.team = 1;
-        most = (2 * ((a.c.kv_heads + SLOTS - 1) / SLOTS) + (a.q_heads + SLOTS - 1) / SLOTS + KV8_WARPS - 1) / KV8_WARPS;
+        most = (2 * ((a.c.kv_heads + SLOTS - 1) / SLOTS) + (a.q_heads + SLOTS - 1) / SLOTS + KV8_ONE_WARPS - 1) / KV8_ONE_WARPS;
     } else {
         cut.runs = (int)(((long long)a.n_tokens + a.c.page - 2) / a.c.page) + 1;
         blocks *= cut.runs;
         for (cut.team = 1; cut.team * KV8_ROWS < rows;) cut.team *= 2;
         const int teams = KV8_WARPS / cut.team;
-        most = (2 * a.c.kv_heads + a.q_heads + teams - 1) / teams;
+        most = (2 * a.c.kv_heads + teams - 1) / teams;
+        if (most < a.q_heads) most = a.q_heads;
     }
-    // four blocks to an SM, as far as there are heads
-    const long long parts = (4LL * sms + blocks - 1) / blocks;
-    cut.parts = (int)(parts < most ? parts : most);
+    // as many blocks as the SMs hold at once (four, two of many tokens), as far as there are heads: a part of a wave
+    // more cost 8000 rows a third of their time
+    const long long parts = (a.n_tokens == 1 ? 4LL : 2LL) * sms / blocks;
+    cut.parts = (int)(parts < 1 ? 1 : parts < most ? parts : most);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(blocks * cut.parts));
-    cfg.blockDim = dim3(KV8_WARPS * 32);
+    cfg.blockDim = dim3((a.n_tokens == 1 ? KV8_ONE_WARPS : KV8_WARPS) * 32);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (a.n_tokens == 1) return cudaLaunchKernelEx(&cfg, dz_kv8_append_one_kernel<T, HD>, a, cut);
-    constexpr int most_smem = 64 * (HD / 2) * (int)sizeof(double2);
+    if (a.n_tokens == 1) return cudaLaunchKernelEx(&cfg, dz_kv8_append_one_kernel<T, HD, WIDE>, a, cut);
+    constexpr int most_smem = 64 * (HD / 2) * (int)(sizeof(double2) + sizeof(float2));
     if (!ready[device].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(dz_kv8_append_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
+        const cudaError_t e = cudaFuncSetAttribute(dz_kv8_append_kernel<T, HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
         if (e != cudaSuccess) return e;
         ready[device].store(true, std::memory_order_release);
     }
-    cfg.dynamicSmemBytes = a.rope ? (size_t)rows * (HD / 2) * sizeof(double2) : 0;
-    return cudaLaunchKernelEx(&cfg, dz_kv8_append_kernel<T, HD>, a, cut);
+    cfg.dynamicSmemBytes = (size_t)cut.table_rows * (HD / 2) * (sizeof(double2) + sizeof(float2));
+    return cudaLaunchKernelEx(&cfg, dz_kv8_append_kernel<T, HD, WIDE>, a, cut);
 }
 
 template <typename T> static cudaError_t kv8_append_h(const Kv8AppendArgs& a, int head_dim, int device, int sms, cudaStream_t st) {
-    return head_dim == 128 ? kv8_append_t<T, 128>(a, device, sms, st) : kv8_append_t<T, 64>(a, device, sms, st);
+    const uintptr_t bases = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out | (uintptr_t)a.k_out |
+                            (uintptr_t)a.v_out;
+    const long long strides = a.ldq | a.ldk | a.ldv | a.ldqo | a.ldko | a.ldvo;
+    if (bases % (4 * sizeof(T)) == 0 && strides % 4 == 0)
+        return head_dim == 128 ? kv8_append_t<T, 128, true>(a, device, sms, st) : kv8_append_t<T, 64, true>(a, device, sms, st);
+    return head_dim == 128 ? kv8_append_t<T, 128, false>(a, device, sms, st) : kv8_append_t<T, 64, false>(a, device, sms, st);
 }
 
 cudaError_t dz_kv8_append_launch(const Kv8AppendArgs& a, int type, int head_dim, int device, cudaStream_t st) {
