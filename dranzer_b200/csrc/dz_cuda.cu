@@ -115,15 +115,17 @@ static TensorMapEncodeFn tensor_map_encoder() {
     return fn;
 }
 
-// A 128 x 128-byte tiled uint8 TMA map with the 128-byte swizzle over a
-// tensor of `rank` dims (dims[0] innermost, strides in bytes for dims 1..).
+// A tiled uint8 TMA map with the 128-byte swizzle (64 where the box's rows are
+// that long) over a tensor of `rank` dims (dims[0] innermost, strides in bytes
+// for dims 1..).
 static bool encode_u8_map(CUtensorMap* tm, void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
                           const cuuint32_t* box) {
     TensorMapEncodeFn enc = tensor_map_encoder();
     if (!enc) return false;
     const cuuint32_t es[5] = {1, 1, 1, 1, 1};
     return enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank, base, dims, strides, box, es,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -2,21 +2,27 @@
 // the newest queries of every sequence, with fp32 sums and running statistics.
 //
 // A unit is one (sequence, key head) and up to 8 NT pairs (query token, query
-// head). Tokens are the rows of the 16-bit MMAs (m16n8k16) of the scores, pairs
-// their columns; elements of the head are the rows of those of the sums, pairs
-// again their columns, so that few pairs leave few columns idle. Warps take
+// head). Tokens are the rows of the 8-bit integer MMAs (m16n8k32) of the scores,
+// pairs their columns; elements of the head are the rows of the 16-bit MMAs
+// (m16n8k16) of the sums, pairs again their columns, so that few pairs leave few
+// columns idle. Warps take
 // tiles of 32 tokens of a unit in turn, a tile lying in one page, so that one
-// scale for keys and one for values serve a whole tile. A lane loads 16 bytes
-// of a token at a time straight into the MMAs' operands (elements and tokens
-// may come in any order as long as the other operand follows it), without
-// shared memory; the weights turn from the scores' result into the sums'
-// operand by movmatrix. Codes become fp16 exactly, two at a time, by setting
-// the exponent of 1024 above the byte and subtracting 1024 + 128.
+// scale for keys and one for values serve a whole tile. Its keys and its values
+// come by TMA, each a box of 32 rows into a slot of the warp's own ring, three
+// or four of them ahead (loads into registers left no room for enough of them:
+// 231 us where this takes less). They
+// are read as MMA operands by ldmatrix: keys as they are, values turned in units
+// of two elements, so that a register holds two elements of two tokens; the
+// weights turn from the scores' result into the sums' operand by movmatrix.
 //
-// Queries are fp16 as they are, bf16 times a power of two of their row (its
-// largest element in [2^13, 2^14)), fp32 the same in two fp16 parts; weights
-// are taken times 2^15 in two fp16 parts. Scores of a tile take the page's key
-// scale, the sums of a tile its value scale, both in fp32.
+// Keys enter as their codes. A query is counted in steps of 2^-30 of a power of
+// two above its largest element and cut into four balanced base-256 digits, so
+// that products and sums are exact and nothing is widened (with keys widened to
+// fp16, as values are, a tile took 831 instructions). Values become fp16
+// exactly, two at a time, by setting the exponent of 1024 above the byte and
+// subtracting 1024 + 128; weights are taken times 2^15 in two fp16 parts. Scores
+// of a tile take the page's key scale, the sums of a tile its value scale, both
+// in fp32.
 //
 // Few units of long contexts go to clusters of blocks, many to a warp each
 // (kv8_shape); the parts (maximum, sum of weights, sums) join at the end in
@@ -25,8 +31,10 @@
 #include <cooperative_groups.h>
 #include <type_traits>
 
+#include "async.cuh"
 #include "dz_types.h"
 #include "kv8.cuh"
+#include "qlevels.cuh"
 #include "shim.cuh"
 
 namespace dz {
@@ -36,9 +44,6 @@ namespace cg = cooperative_groups;
 constexpr int KV8_TILE = 32;       // tokens that a warp takes at a time
 constexpr int KV8_CLUSTER = 16;    // blocks of a cluster at most
 constexpr int KV8_DEVICES = 64;    // devices whose launch state is kept
-// Warps of a block: as many as their registers let an SM hold in one block.
-template <int NT> struct Kv8Warps { static constexpr int N = NT == 1 ? 12 : 8; };
-
 __device__ __forceinline__ void kv8_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -54,24 +59,48 @@ __device__ __forceinline__ void kv8_mma_first(float (&d)[4], const uint32_t (&a)
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-__device__ __forceinline__ uint4 kv8_ld16(const int8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 kv8_ld8(const int8_t* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
+template <bool FIRST>                // the first product of a sum: no registers to clear
+__device__ __forceinline__ void kv8_imma(int (&d)[4], const uint32_t (&a)[4], uint2 b) {
+    if (FIRST)
+        asm volatile(
+            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0));
+    else asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 
-// Bytes 2h and 2h + 1 of `biased` (code + 128) as two fp16 codes.
-template <int H> __device__ __forceinline__ uint32_t kv8_widen(uint32_t biased) {
-    const uint32_t x = __byte_perm(biased, 0x64646464u, H ? 0x4342 : 0x4140);
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));      // 1152
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), off);
+// A box of 32 tokens' codes of a page's head.
+__device__ __forceinline__ void kv8_copy(void* dst, const CUtensorMap* tm, int row, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dz_smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(0), "r"(row), "r"(page), "r"(dz_smem_addr(bar))
+        : "memory");
+}
+
+// Four 8 x 8 matrices of 16-bit units from shared memory, lane l giving the
+// address of row l % 8 of matrix l / 8.
+__device__ __forceinline__ void kv8_matrices(uint32_t (&d)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void kv8_matrices_turned(uint32_t (&d)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(at)
+                 : "memory");
+}
+
+// The codes in bytes 0 and 2 (1 and 3) of x as two fp16.
+template <bool ODD> __device__ __forceinline__ uint32_t kv8_widen(uint32_t x) {
+    uint32_t biased;             // (x & bytes) ^ base, 1024 + 128 + code; one instruction, both constants in registers
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(biased) : "r"(ODD ? x >> 8 : x), "r"(0x00ff00ffu), "r"(0x64806480u));
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&y);
 }
 
@@ -93,24 +122,44 @@ __device__ __forceinline__ uint32_t kv8_turn(uint32_t x) {
     return y;
 }
 
-// Parts of a 16-bit query's element: one, of an fp32 one's: two.
-template <typename T> struct Kv8Parts { static constexpr int N = 1; };
-template <> struct Kv8Parts<float> { static constexpr int N = 2; };
+// A block: as many warps as the SM's registers and shared memory hold, and the
+// shared memory of one: its ring, which its sums overlay at the end, its
+// queries as operands, maximum, weights and whether anything was seen of each
+// pair, and the ring's barriers.
+template <int HD, int NT> struct Kv8Block {
+    static constexpr int WARPS = NT > 1 ? 8 : HD == 64 ? 16 : 12;
+    static constexpr int SLOTS = HD == 128 && NT == 1 ? 3 : 4, SLOT = KV8_TILE * HD, PAIRS = 8 * NT;
+    static constexpr int RING = SLOTS * SLOT > PAIRS * HD * 4 ? SLOTS * SLOT : PAIRS * HD * 4;
+    static constexpr int QUERIES = PAIRS * HD * 4, STATS = PAIRS * 12;
+    static constexpr int SMEM = 1024 + WARPS * (RING + QUERIES + STATS + SLOTS * 8);
+    static_assert(SMEM <= 227 * 1024, "the shared memory of a block");
+};
 
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(Kv8Warps<NT>::N * 32, 1)
-    dz_kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a, int team, int cluster, int blocks, int units) {
-    constexpr int PARTS = Kv8Parts<T>::N, PAIRS = 8 * NT, WARPS = Kv8Warps<NT>::N;
-    constexpr int STEPS = HD / 16;           // score MMAs over a head's elements, each of 4 bytes a lane and token
+__global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
+    dz_kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, int team, int cluster, int blocks, int units) {
+    using B = Kv8Block<HD, NT>;
+    constexpr int PAIRS = B::PAIRS, WARPS = B::WARPS, SLOTS = B::SLOTS;
+    constexpr int STEPS = HD / 32;           // score MMAs over a head's elements
     constexpr int TILES = HD / 16;           // sum MMAs over a head's elements
-    constexpr int COLS = HD / 8;             // a lane's elements of a token's value
-    extern __shared__ __align__(16) float kv8_join[];                 // [warps][PAIRS][HD], then
-    float2* stats = reinterpret_cast<float2*>(kv8_join + WARPS * PAIRS * HD);       // [warps][PAIRS] maximum, weights
-    int* seens = reinterpret_cast<int*>(stats + WARPS * PAIRS);                     // [warps][PAIRS]
-    // [warps][PARTS][NT][STEPS][32 lanes]: queries as B operands; registers for them would leave too few for the rest
-    uint2* queries = reinterpret_cast<uint2*>(seens + WARPS * PAIRS);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    extern __shared__ __align__(1024) uint8_t kv8_raw[];
+    uint8_t* sm = kv8_raw + ((1024u - (dz_smem_addr(kv8_raw) & 1023u)) & 1023u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float* join = reinterpret_cast<float*>(sm);                       // [warps][RING / 4]: [PAIRS][HD]
+    uint2* queries = reinterpret_cast<uint2*>(sm + WARPS * B::RING);  // [warps][NT][STEPS][4 digits][32 lanes]
+    float2* stats = reinterpret_cast<float2*>(sm + WARPS * (B::RING + B::QUERIES));     // [warps][PAIRS] maximum, weights
+    uint64_t* bars = reinterpret_cast<uint64_t*>(stats + WARPS * PAIRS);                // [warps][SLOTS]
+    int* seens = reinterpret_cast<int*>(bars + WARPS * SLOTS);                          // [warps][PAIRS]
+    uint8_t* ring = sm + warp * B::RING;
+    uint64_t* bar = bars + warp * SLOTS;
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) dz_mbar_init(&bar[i]);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int rank = cluster > 1 ? (int)(blockIdx.x % (unsigned)cluster) : 0;
     const int unit = cluster > 1 ? blockIdx.x / cluster : blockIdx.x * (WARPS / team) + warp / team;
     const int warps = team * cluster, me = cluster > 1 ? rank * WARPS + warp : warp % team;
@@ -126,7 +175,7 @@ __global__ void __launch_bounds__(Kv8Warps<NT>::N * 32, 1)
         first = a.positions[b];
         if (kv8_skips(first)) rows = 0;
     }
-    float o[TILES][NT][4];                   // elements COLS g + 2 i (0, 1) and + 1 (2, 3) of pairs 2 t, 2 t + 1
+    float o[TILES][NT][4];                   // elements 16 i + 2 g (0, 1) and + 1 (2, 3) of pairs 2 t, 2 t + 1
 #pragma unroll
     for (int i = 0; i < TILES; i++)
 #pragma unroll
@@ -159,148 +208,170 @@ __global__ void __launch_bounds__(Kv8Warps<NT>::N * 32, 1)
                 low[n][e] = low_of(8 * n + 2 * t + e);
             }
         const int high_all = high_of(0), low_all = low_of(rows - 1);  // a tile within them is seen by every pair
-        // queries as B operands: step s takes elements 64 (s / 4) + 16 t + 4 (s % 4) + 0..3 of pair 8 n + g
-        uint2* qb = queries + (threadIdx.x >> 5) * (PARTS * NT * STEPS * 32) + lane;
+        const int32_t* table = a.c.table + (long long)b * a.c.table_pages;
+        const int shift = a.c.page == 64 ? 6 : 5;
+        const int from = low_of(0), to = min(high_of(rows - 1), (int)reach - 1);
+        const int t_first = from >> 5, t_last = to < from ? -1 : to >> 5;                 // tiles
+        // the warp's tiles that have a page, in turn: this one and the two after it, looked up one ahead
+        int at = t_first + me - warps, raw = t_first + me <= t_last ? table[(t_first + me) >> (shift - 5)] : -1;
+        int tile[3], page[3];
+        auto look = [&](int& tile_out, int& page_out) {
+            page_out = -1;
+            while (at + warps <= t_last) {
+                at += warps;
+                tile_out = at;
+                page_out = (unsigned)raw < (unsigned)a.c.pages ? raw : -1;
+                raw = at + warps <= t_last ? table[(at + warps) >> (shift - 5)] : -1;
+                if (page_out >= 0) break;
+            }
+        };
+        unsigned flying = 0, parity = 0;     // slots that are being filled; their barriers' phases
+        auto copy = [&](int slot, bool keys, int which) {
+            if (page[which] < 0) return;
+            if (lane == 0) {
+                dz_mbar_expect_tx(&bar[slot], B::SLOT);
+                kv8_copy(ring + slot * B::SLOT, keys ? &tm_k : &tm_v,
+                         h * a.c.page + (shift == 6 ? (tile[which] & 1) * KV8_TILE : 0), page[which], &bar[slot]);
+            }
+            flying |= 1u << slot;
+        };
+        auto arrived = [&](int slot) {
+            const bool ok = dz_mbar_wait(&bar[slot], parity >> slot & 1u);
+            parity ^= 1u << slot;
+            flying &= ~(1u << slot);
+            return ok;
+        };
+#pragma unroll
+        for (int i = 0; i < 3; i++) look(tile[i], page[i]);
+        copy(0, true, 0);
+        copy(1, false, 0);
+        copy(2, true, 1);
+        if (SLOTS == 4) copy(3, false, 1);
+        const float *k_scales = a.c.k_scales + h, *v_scales = a.c.v_scales + h;
+        auto scale_of = [&](const float* scales) { return page[0] >= 0 ? scales[(long long)page[0] * a.c.kv_heads] : 0.0f; };
+        float k_scale = scale_of(k_scales), v_scale = scale_of(v_scales);
+        // queries as B operands: step s takes elements 32 s + 4 t + 0..3 and 16 further on of pair 8 n + g
+        uint2* qb = queries + warp * (NT * STEPS * 4 * 32) + lane;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const int r = min(r0 + 8 * n + g, pairs - 1);
             const T* q = static_cast<const T*>(a.q) + ((long long)b * a.n_tokens + r / share) * a.ldq +
-                         (h * share + r % share) * HD + 16 * t;
+                         (h * share + r % share) * HD + 4 * t;
             float peak = 0.0f;
             bool bad = false;
 #pragma unroll
-            for (int s = 0; s < STEPS; s++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float x = dz_to_float(q[64 * (s / 4) + 4 * (s % 4) + e]);
-                    peak = fmaxf(peak, fabsf(x));
-                    bad |= !(fabsf(x) <= 3.402823466e38f);
-                }
-            float up = 1.0f, own = a.scale * 1.4426950408889634f;
-            if (!std::is_same<T, __half>::value) {
-                peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
-                peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-                // 2^e that takes the largest to [2^13, 2^14), within fp32
-                const int e = peak > 0.0f ? min(max(13 - (int)((__float_as_uint(peak) >> 23) & 255) + 127, -126), 126) : 0;
-                up = __uint_as_float((unsigned)(e + 127) << 23);
-                own *= __uint_as_float((unsigned)(127 - e) << 23);
+            for (int e = 0; e < HD / 4; e++) {
+                const float x = dz_to_float(q[16 * (e / 4) + e % 4]);
+                peak = fmaxf(peak, fabsf(x));
+                bad |= !(fabsf(x) <= 3.402823466e38f);
             }
+            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
             bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 1);
             bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 2);
+            // 2^e that takes the largest to [2^29, 2^30), in two factors within fp32
+            const int e = peak > 0.0f ? 29 - (int)((__float_as_uint(peak) >> 23) & 255) + 127 : 0;
+            const int e0 = min(max(e, -126), 126), e1 = e - e0;
+            const float up0 = __uint_as_float((unsigned)(e0 + 127) << 23), up1 = __uint_as_float((unsigned)(e1 + 127) << 23);
+            float own = a.scale * 1.4426950408889634f * __uint_as_float((unsigned)(127 - e0) << 23) *
+                        __uint_as_float((unsigned)(127 - e1) << 23);
             if (bad) own = __int_as_float(0x7fc00000);
             factor[n][0] = __shfl_sync(0xffffffffu, own, 8 * t);      // of pair 2 t, which lanes 8 t.. hold
             factor[n][1] = __shfl_sync(0xffffffffu, own, 8 * t + 4);
 #pragma unroll
             for (int s = 0; s < STEPS; s++) {
-                uint32_t part[PARTS][2];
+                unsigned word[8];            // an element's four digits: the carries of 128 a digit, taken off again
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    const T* x = q + 64 * (s / 4) + 4 * (s % 4) + 2 * w;
-                    const float u = dz_to_float(x[0]) * up, v = dz_to_float(x[1]) * up;
-                    const uint32_t hi = kv8_half2(u, v);
-                    part[0][w] = hi;
-                    if (PARTS == 2) {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                        part[PARTS - 1][w] = kv8_half2(u - f.x, v - f.y);
-                    }
+                for (int i = 0; i < 8; i++) {
+                    const float x = dz_to_float(q[32 * s + 16 * (i / 4) + i % 4]);
+                    word[i] = ((unsigned)(bad ? 0 : __float2int_rn(x * up0 * up1)) + 0x80808080u) ^ 0x80808080u;
                 }
 #pragma unroll
-                for (int p = 0; p < PARTS; p++) qb[((p * NT + n) * STEPS + s) * 32] = make_uint2(part[p][0], part[p][1]);
+                for (int d = 0; d < 4; d++) {                    // digit d of four elements side by side
+                    const unsigned pick = (unsigned)(d | (d + 4) << 4);
+                    uint2 v;
+                    v.x = __byte_perm(__byte_perm(word[0], word[1], pick), __byte_perm(word[2], word[3], pick), 0x5410);
+                    v.y = __byte_perm(__byte_perm(word[4], word[5], pick), __byte_perm(word[6], word[7], pick), 0x5410);
+                    qb[((n * STEPS + s) * 4 + d) * 32] = v;
+                }
             }
         }
-        const int32_t* table = a.c.table + (long long)b * a.c.table_pages;
-        const int shift = a.c.page == 64 ? 6 : 5;
-        const int from = low_of(0), to = min(high_of(rows - 1), (int)reach - 1);
-        const int t_first = from >> 5, t_last = to < from ? -1 : to >> 5;                 // tiles
-        auto page_of = [&](int tile) {
-            const int p = tile <= t_last ? table[tile >> (shift - 5)] : -1;
-            return (unsigned)p < (unsigned)a.c.pages ? p : -1;
-        };
-        // where the tile's codes start, elements from the start of a code buffer
-        auto place_of = [&](int page, int tile) {
-            return ((long long)page * a.c.kv_heads + h) * (a.c.page * HD) + (shift == 6 ? (tile & 1) * (32 * HD) : 0);
-        };
-        uint32_t k[4][STEPS];                // the next tile's keys: token 8 i + g, 4 bytes a step
-        auto load_k = [&](int page, int tile) {
-            if (page < 0) return;
-            const int8_t* p = a.c.k_codes + place_of(page, tile) + g * HD + t * 16;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int s = 0; s < STEPS / 4; s++)
-                    *reinterpret_cast<uint4*>(&k[i][4 * s]) = kv8_ld16(p + i * (8 * HD) + s * 64);
-        };
-        int tile = t_first + me;
-        int page = page_of(tile), next = page_of(tile + warps);
-        load_k(page, tile);
-        for (; tile <= t_last; tile += warps) {
-            const int here = page;
-            page = next;
-            next = page_of(tile + 2 * warps);
-            if (here < 0) {
-                load_k(page, tile + warps);
-                continue;
-            }
-            const float k_scale = a.c.k_scales[(long long)here * a.c.kv_heads + h];
-            const float v_scale = a.c.v_scales[(long long)here * a.c.kv_heads + h];
+        __syncwarp();
+        // the row that the lane addresses in a slot, whose 16-byte chunks are swizzled: of keys tokens 0..15 by 2 chunks, of
+        // values tokens 0..31
+        const int row = lane & 7, turn = HD == 128 ? row : row >> 1;
+        const int k_at = (row + (lane & 8)) * HD + ((lane >> 4 ^ turn) * 16), v_at = lane * HD + turn * 16;
+        bool ok = true;
+        int slot = 0;
+        while (page[0] >= 0) {
+            const int p0 = tile[0] * KV8_TILE;
+            if (!arrived(slot)) ok = false;
+            const uint32_t keys = dz_smem_addr(ring + slot * B::SLOT) + k_at;
             float s[2][NT][4];               // tokens 16 i + g (0, 1) and + 8 (2, 3), pairs 2 t, 2 t + 1
+            constexpr int TOGETHER = NT == 1 ? 2 : 1;            // MMA rows of tokens at a time, by registers
 #pragma unroll
-            for (int e = 0; e < STEPS; e++) {
-                uint2 q[PARTS][NT];
+            for (int i0 = 0; i0 < 2; i0 += TOGETHER) {
+                int sums[TOGETHER][NT][4][4];
 #pragma unroll
-                for (int p = 0; p < PARTS; p++)
+                for (int e = 0; e < STEPS; e++) {
+                    uint32_t k[TOGETHER][4];
 #pragma unroll
-                    for (int n = 0; n < NT; n++) q[p][n] = qb[((p * NT + n) * STEPS + e) * 32];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint32_t u = k[2 * i][e] ^ 0x80808080u, w = k[2 * i + 1][e] ^ 0x80808080u;
-                    const uint32_t ka[4] = {kv8_widen<0>(u), kv8_widen<0>(w), kv8_widen<1>(u), kv8_widen<1>(w)};
+                    for (int i = 0; i < TOGETHER; i++) kv8_matrices(k[i], (keys ^ 32 * e) + (i0 + i) * (16 * HD));
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int p = 0; p < PARTS; p++) {
-                            if (e == 0 && p == 0)
-                                kv8_mma_first(s[i][n], ka, q[p][n].x, q[p][n].y);
-                            else
-                                kv8_mma(s[i][n], ka, q[p][n].x, q[p][n].y);
+                        for (int d = 0; d < 4; d++) {
+                            const uint2 q = qb[((n * STEPS + e) * 4 + d) * 32];
+#pragma unroll
+                            for (int i = 0; i < TOGETHER; i++) {
+                                if (e == 0)
+                                    kv8_imma<true>(sums[i][n][d], k[i], q);
+                                else
+                                    kv8_imma<false>(sums[i][n][d], k[i], q);
+                            }
                         }
                 }
+#pragma unroll
+                for (int i = 0; i < TOGETHER; i++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++)              // below 2^29 each
+                            s[i0 + i][n][c] = fmaf((float)(sums[i][n][3][c] * 256 + sums[i][n][2][c]), 65536.0f,
+                                                   (float)(sums[i][n][1][c] * 256 + sums[i][n][0][c]));
             }
-            // values: tokens 16 s + 2 t, + 1, + 8, + 9, elements COLS g .. COLS g + COLS - 1
-            uint32_t v[2][4][COLS / 4];
-            const int8_t* pv = a.c.v_codes + place_of(here, tile) + 2 * t * HD + g * COLS;
+            __syncwarp();                    // the keys' slot is free: the next copy but two
+            if (SLOTS == 3)
+                copy(slot, false, 1);
+            else
+                copy(slot, true, 2);
+            // scores are f times the dot products, f > 0: the products' signs turned where the scales' are not alike, and a
+            // least f, so that hidden tokens stay at -inf
+            if ((k_scale < 0.0f) != (a.scale < 0.0f)) {
 #pragma unroll
-            for (int s = 0; s < 2; s++)
+                for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int8_t* p = pv + (16 * s + (i & 1) + (i >> 1) * 8) * HD;
-                    if (COLS == 16)
-                        *reinterpret_cast<uint4*>(&v[s][i][0]) = kv8_ld16(p);
-                    else
-                        *reinterpret_cast<uint2*>(&v[s][i][0]) = kv8_ld8(p);
-                }
-            const int p0 = tile * KV8_TILE;
-            const bool whole = p0 + KV8_TILE - 1 <= high_all && p0 >= low_all;
-            float less[NT][2], shrink[NT][2], vs[NT][2];
-            bool grown = false;
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) s[i][n][c] = -s[i][n][c];
+            }
+            float f[NT][2], vs[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    // scores are f times the dot products, f >= 0 (their signs turned where it is not)
-                    float f = k_scale * factor[n][e];
-                    if (f < 0.0f) {
-                        f = -f;
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            s[i][n][e] = -s[i][n][e];
-                            s[i][n][2 + e] = -s[i][n][2 + e];
-                        }
-                    }
+                    f[n][e] = fabsf(k_scale * factor[n][e]);
+                    f[n][e] = f[n][e] == 0.0f ? 1.17549435e-38f : f[n][e];
                     vs[n][e] = v_scale;
-                    if (whole) {
-                        seen[n][e] = 1;
-                    } else {                 // value scale 0 where the pair sees nothing of the tile
+                }
+            if (p0 + KV8_TILE - 1 <= high_all && p0 >= low_all) {      // every pair sees the whole tile
+#pragma unroll
+                for (int n = 0; n < NT; n++) seen[n][0] = seen[n][1] = 1;
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
                         int any = 0;
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
@@ -312,40 +383,46 @@ __global__ void __launch_bounds__(Kv8Warps<NT>::N * 32, 1)
                         any |= __shfl_xor_sync(0xffffffffu, any, 4);
                         any |= __shfl_xor_sync(0xffffffffu, any, 8);
                         any |= __shfl_xor_sync(0xffffffffu, any, 16);
-                        if (!any) f = vs[n][e] = 0.0f;
+                        if (!any) {          // whatever the scales are
+                            f[n][e] = 1.17549435e-38f;
+                            vs[n][e] = 0.0f;
+                        }
                         seen[n][e] |= any;
                     }
-                    f = f == 0.0f ? 1.17549435e-38f : f;       // hidden tokens stay at -inf
+            }
+            float shrink[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
                     float m = fmaxf(fmaxf(s[0][n][e], s[0][n][2 + e]), fmaxf(s[1][n][e], s[1][n][2 + e]));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    m = fmaxf(top[n][e], m * f);
-                    less[n][e] = (m == -INFINITY ? 0.0f : m) - 15.0f;            // weights times 2^15
+                    m = fmaxf(top[n][e], m * f[n][e]);
+                    const float less = 15.0f - (m == -INFINITY ? 0.0f : m);      // weights times 2^15
                     shrink[n][e] = top[n][e] == m ? 1.0f : kv8_exp2(top[n][e] - m);
-                    grown |= shrink[n][e] != 1.0f;
                     top[n][e] = m;
                     float w = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 2; i++)
 #pragma unroll
                         for (int j = 0; j < 2; j++) {
-                            s[i][n][2 * j + e] = kv8_exp2(fmaf(s[i][n][2 * j + e], f, -less[n][e]));
+                            s[i][n][2 * j + e] = kv8_exp2(fmaf(s[i][n][2 * j + e], f[n][e], less));
                             w += s[i][n][2 * j + e];
                         }
                     sum[n][e] = fmaf(sum[n][e], shrink[n][e], w);
                 }
-            if (__any_sync(0xffffffffu, grown)) {
+            // every tile: a branch for those whose maximum grew costs as many moves
 #pragma unroll
-                for (int i = 0; i < TILES; i++)
+            for (int i = 0; i < TILES; i++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        o[i][n][0] *= shrink[n][0];
-                        o[i][n][1] *= shrink[n][1];
-                        o[i][n][2] *= shrink[n][0];
-                        o[i][n][3] *= shrink[n][1];
-                    }
-            }
+                for (int n = 0; n < NT; n++) {
+                    o[i][n][0] *= shrink[n][0];
+                    o[i][n][1] *= shrink[n][1];
+                    o[i][n][2] *= shrink[n][0];
+                    o[i][n][3] *= shrink[n][1];
+                }
             // weights as B operands: tokens 16 i + 2 t, + 1 and + 8, + 9 of pair 8 n + g
             uint32_t wh[2][NT][2], wl[2][NT][2];
 #pragma unroll
@@ -359,47 +436,65 @@ __global__ void __launch_bounds__(Kv8Warps<NT>::N * 32, 1)
                         wh[i][n][j] = kv8_turn(hi);
                         wl[i][n][j] = kv8_turn(kv8_half2(s[i][n][2 * j] - f.x, s[i][n][2 * j + 1] - f.y));
                     }
+            const int slot_v = slot + 1 == SLOTS ? 0 : slot + 1;
+            if (!arrived(slot_v)) ok = false;
+            if (!ok) page[1] = page[2] = -1; // nothing after this tile
+            const uint32_t values = dz_smem_addr(ring + slot_v * B::SLOT) + v_at;
+            {                                // this tile's scales are in use: the next one's
+                const int p = page[1] >= 0 ? page[1] : page[0];
+                k_scale = k_scales[(long long)p * a.c.kv_heads];
+                v_scale = v_scales[(long long)p * a.c.kv_heads];
+            }
 #pragma unroll
-            for (int j4 = 0; j4 < COLS / 4; j4++) {
-                // pairs of tokens side by side: bytes (token 0, token 1) of elements 4 j4 + 0, 1 and + 2, 3
-                uint32_t lowb[2][2], highb[2][2];
+            for (int i = 0; i < TILES; i++) {
+                uint32_t v[4];               // elements 16 i + 2 g, + 1 of tokens 8 j + 2 t, + 1
+                kv8_matrices_turned(v, values ^ 16 * i);
+                float part[NT][4];
 #pragma unroll
-                for (int st = 0; st < 2; st++)
-#pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const uint32_t u = v[st][2 * c][j4] ^ 0x80808080u, w = v[st][2 * c + 1][j4] ^ 0x80808080u;
-                        lowb[st][c] = __byte_perm(u, w, 0x5140);
-                        highb[st][c] = __byte_perm(u, w, 0x7362);
-                    }
-#pragma unroll
-                for (int e = 0; e < 2; e++) {                    // elements 4 j4 + 2 e, + 1
-                    const int i = 2 * j4 + e;
-                    float part[NT][4];
-#pragma unroll
-                    for (int st = 0; st < 2; st++) {
-                        const uint32_t (&from2)[2] = e ? highb[st] : lowb[st];
-                        const uint32_t va[4] = {kv8_widen<0>(from2[0]), kv8_widen<1>(from2[0]), kv8_widen<0>(from2[1]),
-                                                kv8_widen<1>(from2[1])};
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            if (st == 0)
-                                kv8_mma_first(part[n], va, wh[st][n][0], wh[st][n][1]);
-                            else
-                                kv8_mma(part[n], va, wh[st][n][0], wh[st][n][1]);
-                            kv8_mma(part[n], va, wl[st][n][0], wl[st][n][1]);
-                        }
-                    }
+                for (int st = 0; st < 2; st++) {
+                    const uint32_t va[4] = {kv8_widen<false>(v[2 * st]), kv8_widen<true>(v[2 * st]),
+                                            kv8_widen<false>(v[2 * st + 1]), kv8_widen<true>(v[2 * st + 1])};
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        o[i][n][0] = fmaf(part[n][0], vs[n][0], o[i][n][0]);
-                        o[i][n][1] = fmaf(part[n][1], vs[n][1], o[i][n][1]);
-                        o[i][n][2] = fmaf(part[n][2], vs[n][0], o[i][n][2]);
-                        o[i][n][3] = fmaf(part[n][3], vs[n][1], o[i][n][3]);
+                        if (st == 0)
+                            kv8_mma_first(part[n], va, wh[st][n][0], wh[st][n][1]);
+                        else
+                            kv8_mma(part[n], va, wh[st][n][0], wh[st][n][1]);
+                        kv8_mma(part[n], va, wl[st][n][0], wl[st][n][1]);
                     }
                 }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    o[i][n][0] = fmaf(part[n][0], vs[n][0], o[i][n][0]);
+                    o[i][n][1] = fmaf(part[n][1], vs[n][1], o[i][n][1]);
+                    o[i][n][2] = fmaf(part[n][2], vs[n][0], o[i][n][2]);
+                    o[i][n][3] = fmaf(part[n][3], vs[n][1], o[i][n][3]);
+                }
             }
-            load_k(page, tile + warps);
+            __syncwarp();                    // the values' slot is free
+            if (SLOTS == 3)
+                copy(slot_v, true, 2);
+            else
+                copy(slot_v, false, 2);
+            tile[0] = tile[1];
+            page[0] = page[1];
+            tile[1] = tile[2];
+            page[1] = page[2];
+            if (ok) look(tile[2], page[2]);
+            slot = slot_v + 1 == SLOTS ? 0 : slot_v + 1;
         }
+        if (!ok) {                           // a copy did not come: the unit reads NaN, once those under way have ended
+            for (int i = 0; i < SLOTS; i++)
+                if (flying >> i & 1u) arrived(i);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    sum[n][e] = __int_as_float(0x7fc00000);
+                    seen[n][e] = 1;
+                }
+        }
+        __syncwarp();
     }
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -410,11 +505,9 @@ __global__ void __launch_bounds__(Kv8Warps<NT>::N * 32, 1)
             w += __shfl_xor_sync(0xffffffffu, w, 4);
             w += __shfl_xor_sync(0xffffffffu, w, 8);
             w += __shfl_xor_sync(0xffffffffu, w, 16);
-            float* at = kv8_join + (warp * PAIRS + r) * HD + g * COLS;
+            float* at = join + warp * (B::RING / 4) + r * HD + 2 * g;
 #pragma unroll
-            for (int i = 0; i < TILES; i += 2)
-                *reinterpret_cast<float4*>(at + 2 * i) =
-                    make_float4(o[i][n][e], o[i][n][2 + e], o[i + 1][n][e], o[i + 1][n][2 + e]);
+            for (int i = 0; i < TILES; i++) *reinterpret_cast<float2*>(at + 16 * i) = make_float2(o[i][n][e], o[i][n][2 + e]);
             if (g == 0) {
                 stats[warp * PAIRS + r] = make_float2(top[n][e], w);
                 seens[warp * PAIRS + r] = seen[n][e];
@@ -443,13 +536,13 @@ __global__ void __launch_bounds__(Kv8Warps<NT>::N * 32, 1)
         float total = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int c = 0; c < cluster; c++) {
             const float2* st = cluster > 1 ? cg::this_cluster().map_shared_rank(stats, c) : stats;
-            const float* jn = cluster > 1 ? cg::this_cluster().map_shared_rank(kv8_join, c) : kv8_join;
+            const float* jn = cluster > 1 ? cg::this_cluster().map_shared_rank(join, c) : join;
             for (int w = 0; w < team; w++) {
                 const int at = (w0 + w) * PAIRS + r;
                 const float2 s = st[at];
                 const float f = s.x == -INFINITY ? 0.0f : s.x == m ? 1.0f : kv8_exp2(s.x - m);
                 // a part that weighs nothing may still hold a NaN, which counts; one that saw nothing is all 0
-                const float4 v = *reinterpret_cast<const float4*>(jn + at * HD + d);
+                const float4 v = *reinterpret_cast<const float4*>(jn + (w0 + w) * (B::RING / 4) + r * HD + d);
                 total = fmaf(s.y, f, total);
                 y[0] = fmaf(v.x, f, y[0]);
                 y[1] = fmaf(v.y, f, y[1]);
@@ -501,7 +594,7 @@ static void kv8_shape(const Kv8Room& room, int block_warps, long long units, lon
 template <typename T, int HD, int NT>
 static cudaError_t kv8_attn_t(const Kv8AttnArgs& a, long long longest, int device, cudaStream_t st) {
     static Kv8Room rooms[KV8_DEVICES];
-    constexpr int PAIRS = 8 * NT, WARPS = Kv8Warps<NT>::N, smem = WARPS * PAIRS * (HD * 4 + (int)sizeof(float2) + 4 + HD * 2 * Kv8Parts<T>::N);
+    constexpr int PAIRS = 8 * NT, WARPS = Kv8Block<HD, NT>::WARPS, smem = Kv8Block<HD, NT>::SMEM;
     const auto kernel = dz_kv8_attn_kernel<T, HD, NT>;
     Kv8Room& room = rooms[device];
     cudaLaunchConfig_t cfg = {};
@@ -536,7 +629,15 @@ static cudaError_t kv8_attn_t(const Kv8AttnArgs& a, long long longest, int devic
     attr[0].val.clusterDim.x = cluster;
     cfg.attrs = cluster > 1 ? attr : attr + 1;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, team, cluster, blocks, (int)units);
+    // code buffers as [pages][kv_heads page][HD]
+    CUtensorMap maps[2];
+    const uint64_t rows = (uint64_t)a.c.kv_heads * a.c.page;
+    const uint64_t dims[3] = {HD, rows, (uint64_t)a.c.pages}, strides[2] = {HD, rows * HD};
+    const uint32_t box[3] = {HD, KV8_TILE, 1};
+    if (!dz_encode_u8_map(&maps[0], a.c.k_codes, 3, dims, strides, box) ||
+        !dz_encode_u8_map(&maps[1], a.c.v_codes, 3, dims, strides, box))
+        return cudaErrorInvalidValue;
+    return cudaLaunchKernelEx(&cfg, kernel, a, maps[0], maps[1], team, cluster, blocks, (int)units);
 }
 
 template <typename T>

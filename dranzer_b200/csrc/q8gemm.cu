@@ -4,14 +4,12 @@
 // columns, so that an output row is written by the lanes of a warp side by
 // side. Both operands are K-major and come by TMA with the 128-byte swizzle,
 // what lies past the rows or past k as zeros.
-#define DZ_KERNEL_LINKAGE static   // the helper headers' own kernels stay private to dz_cuda.cu
-#include "umma.cuh"
-
 #include <atomic>
 #include <cooperative_groups.h>
 
 #include "q8matmul.cuh"
 #include "qlevels.cuh"
+#include "tcgen05.cuh"
 
 namespace dz {
 

@@ -15,8 +15,8 @@ struct QLevels {
 };
 void dz_qmatrix_levels(const dz_cuda_qmatrix_t* matrix, QLevels* out);
 
-// A tiled uint8 TMA map with the 128-byte swizzle over a tensor of `rank` dims
-// (dims[0] innermost, strides in bytes for dims 1..).
+// A tiled uint8 TMA map with the 64- or 128-byte swizzle (as wide as box[0])
+// over a tensor of `rank` dims (dims[0] innermost, strides in bytes for dims 1..).
 bool dz_encode_u8_map(CUtensorMap* tm, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
                       const uint32_t* box);
 
