@@ -2,10 +2,9 @@
 // the newest queries of every sequence, with fp32 sums and running statistics.
 //
 // A unit is one (sequence, key head) and up to 8 NT pairs (query token, query
-// head). Tokens are the rows of the 8-bit integer MMAs (m16n8k32) of the scores,
-// pairs their columns; elements of the head are the rows of the 16-bit MMAs
-// (m16n8k16) of the sums, pairs again their columns, so that few pairs leave few
-// columns idle. Warps take
+// head). Tokens are the rows of the MMAs of the scores, pairs their columns;
+// elements of the head are the rows of the MMAs of the sums, pairs again their
+// columns, so that few pairs leave few columns idle. Warps take
 // tiles of 32 tokens of a unit in turn, a tile lying in one page, so that one
 // scale for keys and one for values serve a whole tile. Its keys and its values
 // come by TMA, each a box of 32 rows into a slot of the warp's own ring, three
@@ -15,14 +14,17 @@
 // of two elements, so that a register holds two elements of two tokens; the
 // weights turn from the scores' result into the sums' operand by movmatrix.
 //
-// Keys enter as their codes. A query is counted in steps of 2^-30 of a power of
-// two above its largest element and cut into four balanced base-256 digits, so
-// that products and sums are exact and nothing is widened (with keys widened to
-// fp16, as values are, a tile took 831 instructions). Values become fp16
-// exactly, two at a time, by setting the exponent of 1024 above the byte and
-// subtracting 1024 + 128; weights are taken times 2^15 in two fp16 parts. Scores
-// of a tile take the page's key scale, the sums of a tile its value scale, both
-// in fp32.
+// Up to 8 pairs, keys enter the 8-bit integer MMA (m16n8k32) as their codes. A
+// query is counted in steps of 2^-30 of a power of two above its largest element
+// and cut into four balanced base-256 digits, so that products and sums are
+// exact and nothing is widened (with keys widened a tile took 831 instructions
+// where it takes 757). With more pairs the digits' sums cost more than keys
+// widened once for all of them: keys are fp16 (m16n8k16), queries fp16 too, bf16
+// and fp32 ones times a power of two of their row (its largest element in [2^13,
+// 2^14)), fp32 ones in two parts. Codes become fp16 exactly, two at a time, by
+// setting the exponent of 1024 above the byte and subtracting 1024 + 128; values
+// always do, and weights are taken times 2^15 in two fp16 parts. Scores of a tile
+// take the page's key scale, the sums of a tile its value scale, both in fp32.
 //
 // Few units of long contexts go to clusters of blocks, many to a warp each
 // (kv8_shape); the parts (maximum, sum of weights, sums) join at the end in
@@ -89,6 +91,9 @@ __device__ __forceinline__ void kv8_matrices(uint32_t (&d)[4], uint32_t at) {
                  : "r"(at)
                  : "memory");
 }
+__device__ __forceinline__ void kv8_half_matrices(uint32_t (&d)[2], uint32_t at) {       // the first two, lanes 0..15
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "r"(at) : "memory");
+}
 __device__ __forceinline__ void kv8_matrices_turned(uint32_t (&d)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
@@ -127,7 +132,7 @@ __device__ __forceinline__ uint32_t kv8_turn(uint32_t x) {
 // queries as operands, maximum, weights and whether anything was seen of each
 // pair, and the ring's barriers.
 template <int HD, int NT> struct Kv8Block {
-    static constexpr int WARPS = NT > 1 ? 8 : HD == 64 ? 16 : 12;
+    static constexpr int WARPS = HD == 64 ? (NT == 1 ? 16 : 12) : NT == 1 ? 12 : 8;
     static constexpr int SLOTS = HD == 128 && NT == 1 ? 3 : 4, SLOT = KV8_TILE * HD, PAIRS = 8 * NT;
     static constexpr int RING = SLOTS * SLOT > PAIRS * HD * 4 ? SLOTS * SLOT : PAIRS * HD * 4;
     static constexpr int QUERIES = PAIRS * HD * 4, STATS = PAIRS * 12;
@@ -141,13 +146,15 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
                        const __grid_constant__ CUtensorMap tm_v, int team, int cluster, int blocks, int units) {
     using B = Kv8Block<HD, NT>;
     constexpr int PAIRS = B::PAIRS, WARPS = B::WARPS, SLOTS = B::SLOTS;
-    constexpr int STEPS = HD / 32;           // score MMAs over a head's elements
+    constexpr bool DIGITS = NT == 1;
+    constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1;      // fp16 parts of a query's element
     constexpr int TILES = HD / 16;           // sum MMAs over a head's elements
     extern __shared__ __align__(1024) uint8_t kv8_raw[];
     uint8_t* sm = kv8_raw + ((1024u - (dz_smem_addr(kv8_raw) & 1023u)) & 1023u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     float* join = reinterpret_cast<float*>(sm);                       // [warps][RING / 4]: [PAIRS][HD]
-    uint2* queries = reinterpret_cast<uint2*>(sm + WARPS * B::RING);  // [warps][NT][STEPS][4 digits][32 lanes]
+    uint2* queries = reinterpret_cast<uint2*>(sm + WARPS * B::RING);  // [warps][NT][HD / 32][4 digits][32 lanes], or
+                                                                      // [warps][PARTS][NT][HD / 16][32 lanes]
     float2* stats = reinterpret_cast<float2*>(sm + WARPS * (B::RING + B::QUERIES));     // [warps][PAIRS] maximum, weights
     uint64_t* bars = reinterpret_cast<uint64_t*>(stats + WARPS * PAIRS);                // [warps][SLOTS]
     int* seens = reinterpret_cast<int*>(bars + WARPS * SLOTS);                          // [warps][PAIRS]
@@ -250,8 +257,8 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
         const float *k_scales = a.c.k_scales + h, *v_scales = a.c.v_scales + h;
         auto scale_of = [&](const float* scales) { return page[0] >= 0 ? scales[(long long)page[0] * a.c.kv_heads] : 0.0f; };
         float k_scale = scale_of(k_scales), v_scale = scale_of(v_scales);
-        // queries as B operands: step s takes elements 32 s + 4 t + 0..3 and 16 further on of pair 8 n + g
-        uint2* qb = queries + warp * (NT * STEPS * 4 * 32) + lane;
+        // queries as B operands, of pair 8 n + g
+        uint2* qb = queries + warp * (B::QUERIES / 8) + lane;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const int r = min(r0 + 8 * n + g, pairs - 1);
@@ -269,8 +276,8 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
             peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
             bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 1);
             bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 2);
-            // 2^e that takes the largest to [2^29, 2^30), in two factors within fp32
-            const int e = peak > 0.0f ? 29 - (int)((__float_as_uint(peak) >> 23) & 255) + 127 : 0;
+            // 2^e that takes the largest to [2^29, 2^30) or [2^13, 2^14), in two factors within fp32
+            const int e = peak > 0.0f ? (DIGITS ? 29 : 13) - (int)((__float_as_uint(peak) >> 23) & 255) + 127 : 0;
             const int e0 = min(max(e, -126), 126), e1 = e - e0;
             const float up0 = __uint_as_float((unsigned)(e0 + 127) << 23), up1 = __uint_as_float((unsigned)(e1 + 127) << 23);
             float own = a.scale * 1.4426950408889634f * __uint_as_float((unsigned)(127 - e0) << 23) *
@@ -278,21 +285,38 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
             if (bad) own = __int_as_float(0x7fc00000);
             factor[n][0] = __shfl_sync(0xffffffffu, own, 8 * t);      // of pair 2 t, which lanes 8 t.. hold
             factor[n][1] = __shfl_sync(0xffffffffu, own, 8 * t + 4);
+            if (DIGITS) {                    // step s: elements 32 s + 4 t + 0..3 and 16 further on
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                unsigned word[8];            // an element's four digits: the carries of 128 a digit, taken off again
+                for (int s = 0; s < HD / 32; s++) {
+                    unsigned word[8];        // an element's four digits: the carries of 128 a digit, taken off again
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float x = dz_to_float(q[32 * s + 16 * (i / 4) + i % 4]);
-                    word[i] = ((unsigned)(bad ? 0 : __float2int_rn(x * up0 * up1)) + 0x80808080u) ^ 0x80808080u;
+                    for (int i = 0; i < 8; i++) {
+                        const float x = dz_to_float(q[32 * s + 16 * (i / 4) + i % 4]);
+                        word[i] = ((unsigned)(bad ? 0 : __float2int_rn(x * up0 * up1)) + 0x80808080u) ^ 0x80808080u;
+                    }
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {                // digit d of four elements side by side
+                        const unsigned pick = (unsigned)(d | (d + 4) << 4);
+                        uint2 v;
+                        v.x = __byte_perm(__byte_perm(word[0], word[1], pick), __byte_perm(word[2], word[3], pick), 0x5410);
+                        v.y = __byte_perm(__byte_perm(word[4], word[5], pick), __byte_perm(word[6], word[7], pick), 0x5410);
+                        qb[((n * (HD / 32) + s) * 4 + d) * 32] = v;
+                    }
                 }
+            } else {                         // step s: elements 16 s + 4 t + 0, 2 and + 1, 3
 #pragma unroll
-                for (int d = 0; d < 4; d++) {                    // digit d of four elements side by side
-                    const unsigned pick = (unsigned)(d | (d + 4) << 4);
-                    uint2 v;
-                    v.x = __byte_perm(__byte_perm(word[0], word[1], pick), __byte_perm(word[2], word[3], pick), 0x5410);
-                    v.y = __byte_perm(__byte_perm(word[4], word[5], pick), __byte_perm(word[6], word[7], pick), 0x5410);
-                    qb[((n * STEPS + s) * 4 + d) * 32] = v;
+                for (int s = 0; s < HD / 16; s++) {
+                    float x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] = dz_to_float(q[16 * s + i]) * up0 * up1;
+                    const uint2 hi = make_uint2(kv8_half2(x[0], x[2]), kv8_half2(x[1], x[3]));
+                    qb[(n * (HD / 16) + s) * 32] = hi;
+                    if (PARTS == 2) {
+                        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+                        const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+                        qb[((NT + n) * (HD / 16) + s) * 32] =
+                            make_uint2(kv8_half2(x[0] - u.x, x[2] - u.y), kv8_half2(x[1] - w.x, x[3] - w.y));
+                    }
                 }
             }
         }
@@ -308,22 +332,20 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
             if (!arrived(slot)) ok = false;
             const uint32_t keys = dz_smem_addr(ring + slot * B::SLOT) + k_at;
             float s[2][NT][4];               // tokens 16 i + g (0, 1) and + 8 (2, 3), pairs 2 t, 2 t + 1
-            constexpr int TOGETHER = NT == 1 ? 2 : 1;            // MMA rows of tokens at a time, by registers
+            if constexpr (DIGITS) {
+                int sums[2][NT][4][4];
 #pragma unroll
-            for (int i0 = 0; i0 < 2; i0 += TOGETHER) {
-                int sums[TOGETHER][NT][4][4];
+                for (int e = 0; e < HD / 32; e++) {
+                    uint32_t k[2][4];
 #pragma unroll
-                for (int e = 0; e < STEPS; e++) {
-                    uint32_t k[TOGETHER][4];
-#pragma unroll
-                    for (int i = 0; i < TOGETHER; i++) kv8_matrices(k[i], (keys ^ 32 * e) + (i0 + i) * (16 * HD));
+                    for (int i = 0; i < 2; i++) kv8_matrices(k[i], (keys ^ 32 * e) + i * (16 * HD));
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
                         for (int d = 0; d < 4; d++) {
-                            const uint2 q = qb[((n * STEPS + e) * 4 + d) * 32];
+                            const uint2 q = qb[((n * (HD / 32) + e) * 4 + d) * 32];
 #pragma unroll
-                            for (int i = 0; i < TOGETHER; i++) {
+                            for (int i = 0; i < 2; i++) {
                                 if (e == 0)
                                     kv8_imma<true>(sums[i][n][d], k[i], q);
                                 else
@@ -332,13 +354,38 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
                         }
                 }
 #pragma unroll
-                for (int i = 0; i < TOGETHER; i++)
+                for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
                         for (int c = 0; c < 4; c++)              // below 2^29 each
-                            s[i0 + i][n][c] = fmaf((float)(sums[i][n][3][c] * 256 + sums[i][n][2][c]), 65536.0f,
-                                                   (float)(sums[i][n][1][c] * 256 + sums[i][n][0][c]));
+                            s[i][n][c] = fmaf((float)(sums[i][n][3][c] * 256 + sums[i][n][2][c]), 65536.0f,
+                                              (float)(sums[i][n][1][c] * 256 + sums[i][n][0][c]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < HD / 16; e++) {
+                    uint2 q[PARTS][NT];
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                        for (int n = 0; n < NT; n++) q[p][n] = qb[((p * NT + n) * (HD / 16) + e) * 32];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        uint32_t k[2];       // tokens 16 i + g and + 8
+                        kv8_half_matrices(k, (keys ^ 16 * e) + i * (16 * HD));
+                        const uint32_t ka[4] = {kv8_widen<false>(k[0]), kv8_widen<false>(k[1]), kv8_widen<true>(k[0]),
+                                                kv8_widen<true>(k[1])};
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int p = 0; p < PARTS; p++) {
+                                if (e == 0 && p == 0)
+                                    kv8_mma_first(s[i][n], ka, q[p][n].x, q[p][n].y);
+                                else
+                                    kv8_mma(s[i][n], ka, q[p][n].x, q[p][n].y);
+                            }
+                    }
+                }
             }
             __syncwarp();                    // the keys' slot is free: the next copy but two
             if (SLOTS == 3)
@@ -642,11 +689,10 @@ static cudaError_t kv8_attn_t(const Kv8AttnArgs& a, long long longest, int devic
 
 template <typename T>
 static cudaError_t kv8_attn_h(const Kv8AttnArgs& a, long long longest, int head_dim, int device, cudaStream_t st) {
-    const int pairs = a.n_tokens * (a.q_heads / a.c.kv_heads);
-    if (head_dim == 128)
-        return pairs <= 8 ? kv8_attn_t<T, 128, 1>(a, longest, device, st) : kv8_attn_t<T, 128, 2>(a, longest, device, st);
-    if (pairs <= 8) return kv8_attn_t<T, 64, 1>(a, longest, device, st);
-    return pairs <= 16 ? kv8_attn_t<T, 64, 2>(a, longest, device, st) : kv8_attn_t<T, 64, 4>(a, longest, device, st);
+    // few pairs in 8 columns, many in 16 (32 of them took 53 us for 128 pairs of heads of 64 where 16 took 52, 8 took 65)
+    const bool few = a.n_tokens * (a.q_heads / a.c.kv_heads) <= 8;
+    if (head_dim == 128) return few ? kv8_attn_t<T, 128, 1>(a, longest, device, st) : kv8_attn_t<T, 128, 2>(a, longest, device, st);
+    return few ? kv8_attn_t<T, 64, 1>(a, longest, device, st) : kv8_attn_t<T, 64, 2>(a, longest, device, st);
 }
 
 cudaError_t dz_kv8_attn_launch(const Kv8AttnArgs& a, long long longest, int type, int head_dim, int device, cudaStream_t st) {

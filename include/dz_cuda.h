@@ -210,7 +210,7 @@ int dz_cuda_kv8_append(const dz_kv8_t *cache, const dz_kv8_append_t *args, const
  * sequence, whose own keys have been appended (positions as in that append):
  * the query at position i sees position p <= i where the table names a page,
  * and with a window p > i - window. A query that sees nothing reads 0. Scores,
- * softmax statistics and sums are fp32. A query's element is held to 2^-24 of
+ * softmax statistics and sums are fp32. A query's element is held to 2^-22 of
  * itself or to 2^-30 of the largest of its head, a softmax weight to 2^-22 of
  * itself or 2^-39 of the largest. A token that is seen makes a NaN of
  * its output where its page's scale is one, whatever its weight. out must not

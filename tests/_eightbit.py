@@ -134,11 +134,12 @@ def near_border(scaled):
 
 def attend(q, k, v, scale, kind):
     """One query over what it sees, and the bound of an evaluation with fp32 sums.
-    Scores: elements held to 2^-22 of themselves or 2^-38 of the head's largest (fp32
-    and bf16); an MMA adds 16 products to a running sum, each alignment and the sum
-    within 2 u of the largest in play, in hd / 16 steps of up to two parts; four
-    roundings of factors and the difference from the maximum, u each of what they
-    round. A weight: the exponential and its parts 2^-21 in all, or 2^-39 of the
+    Scores: an element is held to 2^-22 of itself (two fp16 parts: 11 bits, then the
+    rest to 11) or to 2^-30 of the head's largest (counted in steps of which that has
+    at least 2^29, rounded to half a step); an MMA of 16-bit parts adds 16 products to
+    a running sum, each alignment and the sum within 2 u of the largest in play, in hd
+    / 16 steps of up to two parts; four roundings of factors and the difference from
+    the maximum, u each of what they round. A weight: the exponential and its parts 2^-21 in all, or 2^-39 of the
     largest. Sums: two steps of two parts per tile of 32 tokens and its scale, the
     same again for statistics and joins of parts."""
     q, k, v = (t.astype(np.float64) for t in (q, k, v))
@@ -146,7 +147,7 @@ def attend(q, k, v, scale, kind):
     e = np.exp(s - s.max())
     p = e / e.sum()
     wide = abs(scale) * (np.abs(k) @ np.abs(q)).max()
-    held = 0.0 if kind == "f16" else 2.0 ** -22 * wide + 2.0 ** -38 * abs(scale) * np.abs(q).max() * np.abs(k).sum(1).max()
+    held = 2.0 ** -22 * wide + 2.0 ** -30 * abs(scale) * np.abs(q).max() * np.abs(k).sum(1).max()
     score = (2 * q.size / 16 * 2 + 8) * 2 * U * wide + held
     weight = p @ np.abs(v)
     n = len(s)
