@@ -8,9 +8,13 @@
 // Bound by HBM for many rows (x, residual, sum: 7 bytes an element in 16 bits),
 // by latency for few. A row is held in registers between the reduction and the
 // codes: by a warp when it is short, by a block of 256 threads up to 32 KB, and
-// longer ones are read again.
+// longer ones are read again. Blocks stay: the next rows are on their way into
+// shared memory while one is worked on (each thread copies what it reads itself,
+// so that no barrier is needed; a row ahead in registers took 45 us for 8192 x
+// 4096 in bf16, none 54), and the gains of rows up to 8 KB stay in registers.
 #include "dz_cuda.h"
 
+#include <atomic>
 #include <cmath>
 
 #include "shim.cuh"
@@ -18,6 +22,7 @@
 namespace dz {
 
 constexpr int Q8N_THREADS = 256;
+constexpr int Q8N_DEVICES = 64;    // devices whose launch state is kept
 
 struct Q8NormArgs {
     const void *x, *residual;
@@ -27,7 +32,6 @@ struct Q8NormArgs {
     float* scales;
     long long ldx, ldr, lds, ldc, rows;
     int width, norm;
-    int wide;                // every typed row starts on a 16-byte boundary, gains too, and codes on an 8-byte one
     double eps64;
 };
 
@@ -37,123 +41,134 @@ template <typename T> union Q8Lane {     // 16 bytes of a row
     __device__ Q8Lane() {}
 };
 
-// Sum of squares and the largest magnitude (as bits; above 0x7f7fffff it is not
-// finite) over the TEAM threads of a row.
-template <int TEAM, typename A> __device__ __forceinline__ void q8_reduce(A& sum, unsigned& top) {
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
-    }
-    if (TEAM == 32) return;
-    __shared__ A sums[TEAM / 32];
-    __shared__ unsigned tops[TEAM / 32];
-    if ((threadIdx.x & 31) == 0) {
-        sums[threadIdx.x >> 5] = sum;
-        tops[threadIdx.x >> 5] = top;
-    }
-    __syncthreads();
-    sum = 0;
-    top = 0;
-#pragma unroll
-    for (int w = 0; w < TEAM / 32; w++) {
-        sum += sums[w];
-        top = max(top, tops[w]);
-    }
-    __syncthreads();
-}
-
-// What turns a row's u into codes, and its scale.
-struct Q8Row {
-    float raise, inverse, scale;
-    bool empty;              // zeros, or not finite: codes are 0
-};
-
-__device__ __forceinline__ Q8Row q8_row(const Q8NormArgs& a, unsigned top, double mean) {
-    Q8Row r;
-    const float peak = __uint_as_float(top);
-    r.raise = top < 0x0D800000u ? 0x1p100f : 1.0f;      // below 2^-100 the inverse would leave fp32
-    r.empty = top == 0 || top > 0x7f7fffffu;
-    r.inverse = __fdiv_rn(127.0f, peak * r.raise);
-    r.scale = __fdiv_rn(peak, 127.0f);
-    if (top > 0x7f7fffffu) {
-        r.scale = __int_as_float(0x7fc00000);
-    } else if (top == 0) {
-        r.scale = 0.0f;
-    } else if (a.norm) {
-        const double m = mean + a.eps64;
-        if (m > 1e-30 && m < 1e30) {
-            float s = rsqrtf((float)m);
-            s = s * fmaf(-0.5f * (float)m * s, s, 1.5f);       // a Newton step
-            r.scale = __fdiv_rn(peak * s, 127.0f);
-        } else {
-            r.scale = (float)((double)peak / sqrt(m) / 127.0);
-        }
-    }
+// The larger magnitude; a NaN stays one.
+__device__ __forceinline__ float q8_larger(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
     return r;
 }
 
-__device__ __forceinline__ unsigned q8_code(const Q8Row& r, float u) {
-    const float v = __fmul_rn(u * r.raise, r.inverse);         // at most 127 and two roundings: no clamp
-    return (unsigned)__float2int_rz(__fadd_rn(v, copysignf(0.5f, v))) & 0xffu;
+// Sum of squares and the largest magnitude over the TEAM threads of a row.
+// `turn` alternates from call to call: a place is written again only after a
+// barrier that followed its reads.
+template <int TEAM, typename A> __device__ __forceinline__ void q8_reduce(A& sum, float& top, int turn) {
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        top = q8_larger(top, __shfl_xor_sync(0xffffffffu, top, off));
+    }
+    if (TEAM == 32) return;
+    __shared__ A sums[2][TEAM / 32];
+    __shared__ float tops[2][TEAM / 32];
+    if ((threadIdx.x & 31) == 0) {
+        sums[turn][threadIdx.x >> 5] = sum;
+        tops[turn][threadIdx.x >> 5] = top;
+    }
+    __syncthreads();
+    sum = 0;
+    top = 0.0f;
+#pragma unroll
+    for (int w = 0; w < TEAM / 32; w++) {
+        sum += sums[turn][w];
+        top = q8_larger(top, tops[turn][w]);
+    }
+}
+
+// What turns a row's u into codes.
+struct Q8Row {
+    float raise, inverse;
+    bool plain;              // raise is 1, and there are codes
+    bool empty;              // zeros, or not finite: codes are 0
+};
+
+__device__ __forceinline__ Q8Row q8_row(float peak) {
+    Q8Row r;
+    r.plain = peak >= 0x1p-100f && peak <= 3.402823466e38f;
+    r.raise = r.plain ? 1.0f : 0x1p100f;      // below 2^-100 the inverse would leave fp32
+    r.empty = !(peak > 0.0f && peak <= 3.402823466e38f);
+    r.inverse = __fdiv_rn(127.0f, peak * r.raise);
+    return r;
+}
+
+__device__ __forceinline__ float q8_scale(const Q8NormArgs& a, float peak, double mean) {
+    if (!(peak <= 3.402823466e38f)) return __int_as_float(0x7fc00000);
+    if (peak == 0.0f) return 0.0f;
+    if (!a.norm) return __fdiv_rn(peak, 127.0f);
+    const double m = mean + a.eps64;
+    if (!(m > 1e-30 && m < 1e30)) return (float)((double)peak / sqrt(m) / 127.0);
+    float s = rsqrtf((float)m);
+    s = s * fmaf(-0.5f * (float)m * s, s, 1.5f);               // a Newton step
+    return __fdiv_rn(peak * s, 127.0f);
+}
+
+// At most 127 and two roundings before it is rounded: no clamp.
+__device__ __forceinline__ int q8_round(float v) { return __float2int_rz(__fadd_rn(v, copysignf(0.5f, v))); }
+__device__ __forceinline__ int q8_code(const Q8Row& r, float u) {
+    return r.plain ? q8_round(__fmul_rn(u, r.inverse)) : r.empty ? 0 : q8_round(__fmul_rn(u * r.raise, r.inverse));
 }
 
 // Sums of squares that leave fp32's range are taken again in 64 bits.
 __device__ __forceinline__ bool q8_doubtful(float sum) { return !(sum > 1e-25f && sum < 1e37f); }
 
-template <typename T, int TEAM, int V>
-__global__ void __launch_bounds__(Q8N_THREADS) dz_norm_q8_kernel(const __grid_constant__ Q8NormArgs a) {
+// WIDE: rows are whole numbers of 16 bytes and start on such a boundary, gains
+// too, and codes on an 8-byte one. A thread then has E elements side by side V
+// times and its rows come through shared memory, else each of them TEAM further
+// on, loaded as they are needed.
+template <int V> struct Q8Ring {
+    static constexpr int ROWS = V <= 2 ? 4 : V == 4 ? 3 : 2;         // of a team, in turn
+    static constexpr int PART = V * Q8N_THREADS * 16;                // x or the residual of the teams' rows
+    static constexpr int BLOCKS = V <= 2 ? 3 : V == 4 ? 2 : 1;       // of an SM
+    static constexpr int SMEM = ROWS * 2 * PART;
+};
+
+template <typename T, int TEAM, int V, bool WIDE>
+__global__ void __launch_bounds__(Q8N_THREADS, Q8Ring<V>::BLOCKS) dz_norm_q8_kernel(const __grid_constant__ Q8NormArgs a) {
     constexpr int E = 16 / (int)sizeof(T);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr bool KEPT = V * E <= 16;       // gains stay in registers
+    extern __shared__ __align__(16) uint8_t q8n_ring[];
     const int t = threadIdx.x % TEAM;
-    const long long row = (long long)blockIdx.x * (Q8N_THREADS / TEAM) + threadIdx.x / TEAM;
+    long long row = (long long)blockIdx.x * (Q8N_THREADS / TEAM) + threadIdx.x / TEAM;
+    const long long step = (long long)gridDim.x * (Q8N_THREADS / TEAM);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= a.rows) return;               // whole teams
-    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-    const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
-    T* out = a.sum ? static_cast<T*>(a.sum) + row * a.lds : nullptr;
-    Q8Lane<T> h[V], r[V];
-    auto load = [&](const T* in, Q8Lane<T> (&to)[V]) {
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            const int at = (j * TEAM + t) * E;
-            if (a.wide && at + E <= a.width) {
-                to[j].q = *reinterpret_cast<const uint4*>(in + at);
-            } else {
-#pragma unroll
-                for (int i = 0; i < E; i++) to[j].e[i] = at + i < a.width ? in[at + i] : dz_from_float<T>(0.0f);
-            }
-        }
-    };
-    load(x, h);
-    if (res) {
-        load(res, r);
+    auto place = [&](int j, int i) { return WIDE ? (j * TEAM + t) * E + i : (j * E + i) * TEAM + t; };
+    auto load = [&](const void* base, long long ld, Q8Lane<T> (&to)[V]) {
+        const T* in = static_cast<const T*>(base) + row * ld;
 #pragma unroll
         for (int j = 0; j < V; j++)
 #pragma unroll
-            for (int i = 0; i < E; i++) h[j].e[i] = dz_from_float<T>(dz_to_float(h[j].e[i]) + dz_to_float(r[j].e[i]));
-    }
-    if (out) {
+            for (int i = 0; i < E; i++) to[j].e[i] = place(j, i) < a.width ? in[place(j, i)] : dz_from_float<T>(0.0f);
+    };
+    // this thread's place in a slot's part, vector j
+    auto slot_of = [&](int slot, int part, int j) {
+        return q8n_ring + (slot * 2 + part) * Q8Ring<V>::PART + (j * Q8N_THREADS + (int)threadIdx.x) * 16;
+    };
+    auto copy = [&](int slot, long long r) {
+        if (r < a.rows) {
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            const int at = (j * TEAM + t) * E;
-            if (a.wide && at + E <= a.width) {
-                *reinterpret_cast<uint4*>(out + at) = h[j].q;
-            } else {
+            for (int part = 0; part < 2; part++) {
+                const T* base = static_cast<const T*>(part ? a.residual : a.x);
+                if (!base) continue;
+                base += r * (part ? a.ldr : a.ldx);
 #pragma unroll
-                for (int i = 0; i < E; i++)
-                    if (at + i < a.width) out[at + i] = h[j].e[i];
+                for (int j = 0; j < V; j++)
+                    if (place(j, 0) < a.width)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(slot_of(slot, part, j))),
+                                     "l"(base + place(j, 0))
+                                     : "memory");
             }
         }
-    }
-    // the gains of E elements at `at`
-    auto gains = [&](int at, float (&g)[E]) {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto gains = [&](int j, float (&g)[E]) {
         if (!a.gain) {
 #pragma unroll
             for (int i = 0; i < E; i++) g[i] = 1.0f;
-        } else if (a.wide && at + E <= a.width) {
+        } else if (WIDE) {
 #pragma unroll
             for (int i = 0; i < E; i += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(a.gain + at + i);
+                const float4 v = place(j, 0) < a.width ? *reinterpret_cast<const float4*>(a.gain + place(j, i))
+                                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 g[i] = v.x;
                 g[i + 1] = v.y;
                 g[i + 2] = v.z;
@@ -161,60 +176,118 @@ __global__ void __launch_bounds__(Q8N_THREADS) dz_norm_q8_kernel(const __grid_co
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < E; i++) g[i] = at + i < a.width ? a.gain[at + i] : 0.0f;
+            for (int i = 0; i < E; i++) g[i] = place(j, i) < a.width ? a.gain[place(j, i)] : 0.0f;
         }
     };
-    float sum = 0.0f;
-    unsigned top = 0;
+    constexpr int AHEAD = Q8Ring<V>::ROWS - 1;
+    if (WIDE) {
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-        float g[E];
-        gains((j * TEAM + t) * E, g);
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            const float v = dz_to_float(h[j].e[i]);
-            sum = fmaf(v, v, sum);
-            top = max(top, __float_as_uint(__fmul_rn(g[i], v)) & 0x7fffffffu);
-        }
+        for (int s = 0; s < AHEAD; s++) copy(s, row + s * step);
     }
-    q8_reduce<TEAM>(sum, top);
-    double mean = (double)sum / a.width;
-    if (a.norm && q8_doubtful(sum)) {        // the whole team alike
-        double s = 0.0;
+    float kept[KEPT ? V : 1][E];
+    if (KEPT) {
 #pragma unroll
-        for (int j = 0; j < V; j++)
-#pragma unroll
-            for (int i = 0; i < E; i++) s += (double)dz_to_float(h[j].e[i]) * (double)dz_to_float(h[j].e[i]);
-        unsigned same = top;
-        q8_reduce<TEAM>(s, same);
-        mean = s / a.width;
+        for (int j = 0; j < V; j++) gains(j, kept[KEPT ? j : 0]);
     }
-    const Q8Row k = q8_row(a, top, mean);
-    int8_t* codes = a.codes + row * a.ldc;
+    int slot = 0;
+    for (int turn = 0;; turn ^= 1) {
+        Q8Lane<T> h[V];
+        if (WIDE) {
+            copy(slot + AHEAD >= Q8Ring<V>::ROWS ? slot + AHEAD - Q8Ring<V>::ROWS : slot + AHEAD, row + AHEAD * step);
+            asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-        const int at = (j * TEAM + t) * E;
-        if (at >= a.width) break;
-        float g[E];
-        gains(at, g);
-        unsigned word[E / 4];
+            for (int j = 0; j < V; j++) {
+                h[j].q = place(j, 0) < a.width ? *reinterpret_cast<const uint4*>(slot_of(slot, 0, j)) : make_uint4(0, 0, 0, 0);
+                if (a.residual) {
+                    Q8Lane<T> r;
+                    r.q = place(j, 0) < a.width ? *reinterpret_cast<const uint4*>(slot_of(slot, 1, j)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-            const unsigned c = k.empty ? 0u : q8_code(k, __fmul_rn(g[i], dz_to_float(h[j].e[i])));
-            word[i / 4] = i % 4 ? word[i / 4] | c << (i % 4 * 8) : c;
-        }
-        if (a.wide && at + E <= a.width) {
-            if (E == 8)
-                *reinterpret_cast<uint2*>(codes + at) = make_uint2(word[0], word[E / 4 - 1]);
-            else
-                *reinterpret_cast<unsigned*>(codes + at) = word[0];
+                    for (int i = 0; i < E; i++) h[j].e[i] = dz_from_float<T>(dz_to_float(h[j].e[i]) + dz_to_float(r.e[i]));
+                }
+            }
+            slot = slot + 1 == Q8Ring<V>::ROWS ? 0 : slot + 1;
         } else {
+            load(a.x, a.ldx, h);
+            if (a.residual) {
+                Q8Lane<T> r[V];
+                load(a.residual, a.ldr, r);
 #pragma unroll
-            for (int i = 0; i < E; i++)
-                if (at + i < a.width) codes[at + i] = (int8_t)(word[i / 4] >> (i % 4 * 8));
+                for (int j = 0; j < V; j++)
+#pragma unroll
+                    for (int i = 0; i < E; i++) h[j].e[i] = dz_from_float<T>(dz_to_float(h[j].e[i]) + dz_to_float(r[j].e[i]));
+            }
         }
+        const long long here = row;
+        row += step;
+        if (a.sum) {
+            T* out = static_cast<T*>(a.sum) + here * a.lds;
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                if (WIDE) {
+                    if (place(j, 0) < a.width) *reinterpret_cast<uint4*>(out + place(j, 0)) = h[j].q;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < E; i++)
+                        if (place(j, i) < a.width) out[place(j, i)] = h[j].e[i];
+                }
+            }
+        }
+        float sum = 0.0f, top = 0.0f, u[V][E];
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            float g[E];
+            if (!KEPT) gains(j, g);
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                const float v = dz_to_float(h[j].e[i]);
+                sum = fmaf(v, v, sum);
+                u[j][i] = __fmul_rn(KEPT ? kept[KEPT ? j : 0][i] : g[i], v);
+                top = q8_larger(top, u[j][i]);
+            }
+        }
+        q8_reduce<TEAM>(sum, top, turn);
+        double mean = (double)sum;
+        if (a.norm && q8_doubtful(sum)) {    // the whole team alike
+            mean = 0.0;
+#pragma unroll
+            for (int j = 0; j < V; j++)
+#pragma unroll
+                for (int i = 0; i < E; i++) mean += (double)dz_to_float(h[j].e[i]) * (double)dz_to_float(h[j].e[i]);
+            float same = top;
+            q8_reduce<TEAM>(mean, same, turn);
+        }
+        const Q8Row k = q8_row(top);
+        int8_t* codes = a.codes + here * a.ldc;
+        auto write = [&](auto code) {
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                if (place(j, 0) >= a.width) break;
+                int c[E];
+#pragma unroll
+                for (int i = 0; i < E; i++) c[i] = code(u[j][i]);
+                if (WIDE) {
+                    unsigned word[E / 4];
+#pragma unroll
+                    for (int i = 0; i < E; i += 4)
+                        word[i / 4] = __byte_perm(__byte_perm(c[i], c[i + 1], 0x0040), __byte_perm(c[i + 2], c[i + 3], 0x0040), 0x5410);
+                    if (E == 8)
+                        *reinterpret_cast<uint2*>(codes + place(j, 0)) = make_uint2(word[0], word[E / 4 - 1]);
+                    else
+                        *reinterpret_cast<unsigned*>(codes + place(j, 0)) = word[0];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < E; i++)
+                        if (place(j, i) < a.width) codes[place(j, i)] = (int8_t)c[i];
+                }
+            }
+        };
+        if (k.plain)
+            write([&](float v) { return q8_round(__fmul_rn(v, k.inverse)); });
+        else
+            write([&](float v) { return q8_code(k, v); });
+        if (t == 0) a.scales[here] = q8_scale(a, top, mean / a.width);
+        if (row >= a.rows) return;
     }
-    if (t == 0) a.scales[row] = k.scale;
 }
 
 // Rows of any width, read again for their codes.
@@ -226,27 +299,44 @@ template <typename T> __global__ void __launch_bounds__(Q8N_THREADS) dz_norm_q8_
     T* out = a.sum ? static_cast<T*>(a.sum) + row * a.lds : nullptr;
     auto value = [&](int i) { return res ? dz_from_float<T>(dz_to_float(x[i]) + dz_to_float(res[i])) : x[i]; };
     double sum = 0.0;
-    unsigned top = 0;
+    float top = 0.0f;
 #pragma unroll 4
     for (int i = threadIdx.x; i < a.width; i += Q8N_THREADS) {
         const T h = value(i);
         const float v = dz_to_float(h);
         if (out) out[i] = h;                 // the same thread reads it below
         sum += (double)v * (double)v;
-        top = max(top, __float_as_uint(a.gain ? __fmul_rn(a.gain[i], v) : v) & 0x7fffffffu);
+        top = q8_larger(top, a.gain ? __fmul_rn(a.gain[i], v) : v);
     }
-    q8_reduce<Q8N_THREADS>(sum, top);
-    const Q8Row k = q8_row(a, top, sum / a.width);
+    q8_reduce<Q8N_THREADS>(sum, top, 0);
+    const Q8Row k = q8_row(top);
     int8_t* codes = a.codes + row * a.ldc;
 #pragma unroll 4
     for (int i = threadIdx.x; i < a.width; i += Q8N_THREADS) {
         const float v = dz_to_float(out ? out[i] : value(i));
-        codes[i] = k.empty ? (int8_t)0 : (int8_t)q8_code(k, a.gain ? __fmul_rn(a.gain[i], v) : v);
+        codes[i] = (int8_t)q8_code(k, a.gain ? __fmul_rn(a.gain[i], v) : v);
     }
-    if (threadIdx.x == 0) a.scales[row] = k.scale;
+    if (threadIdx.x == 0) a.scales[row] = q8_scale(a, top, sum / a.width);
 }
 
-template <typename T> static cudaError_t q8_norm_t(const Q8NormArgs& a, cudaStream_t st) {
+template <typename T, int TEAM, int V>
+static cudaError_t q8_norm_v(const Q8NormArgs& a, bool wide, int device, int sms, cudaLaunchConfig_t& cfg) {
+    static std::atomic<bool> ready[Q8N_DEVICES];
+    if (wide && !ready[device].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(dz_norm_q8_kernel<T, TEAM, V, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   Q8Ring<V>::SMEM);
+        if (e != cudaSuccess) return e;
+        ready[device].store(true, std::memory_order_release);
+    }
+    // blocks that stay: as many as the SMs hold at once
+    const long long each = Q8N_THREADS / TEAM, need = (a.rows + each - 1) / each, most = (long long)sms * Q8Ring<V>::BLOCKS;
+    cfg.gridDim = dim3((unsigned)(need < most ? need : most));
+    cfg.dynamicSmemBytes = wide ? Q8Ring<V>::SMEM : 0;
+    return wide ? cudaLaunchKernelEx(&cfg, dz_norm_q8_kernel<T, TEAM, V, true>, a)
+                : cudaLaunchKernelEx(&cfg, dz_norm_q8_kernel<T, TEAM, V, false>, a);
+}
+
+template <typename T> static cudaError_t q8_norm_t(const Q8NormArgs& a, bool wide, int device, int sms, cudaStream_t st) {
     constexpr int E = 16 / (int)sizeof(T);
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(Q8N_THREADS);
@@ -257,13 +347,13 @@ template <typename T> static cudaError_t q8_norm_t(const Q8NormArgs& a, cudaStre
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     const int vectors = (a.width + E - 1) / E;
-    cfg.gridDim = dim3((unsigned)(vectors <= 64 ? (a.rows + Q8N_THREADS / 32 - 1) / (Q8N_THREADS / 32) : a.rows));
-    if (vectors <= 32) return cudaLaunchKernelEx(&cfg, dz_norm_q8_kernel<T, 32, 1>, a);
-    if (vectors <= 64) return cudaLaunchKernelEx(&cfg, dz_norm_q8_kernel<T, 32, 2>, a);
-    if (vectors <= 256) return cudaLaunchKernelEx(&cfg, dz_norm_q8_kernel<T, 256, 1>, a);
-    if (vectors <= 512) return cudaLaunchKernelEx(&cfg, dz_norm_q8_kernel<T, 256, 2>, a);
-    if (vectors <= 1024) return cudaLaunchKernelEx(&cfg, dz_norm_q8_kernel<T, 256, 4>, a);
-    if (vectors <= 2048) return cudaLaunchKernelEx(&cfg, dz_norm_q8_kernel<T, 256, 8>, a);
+    if (vectors <= 32) return q8_norm_v<T, 32, 1>(a, wide, device, sms, cfg);
+    if (vectors <= 64) return q8_norm_v<T, 32, 2>(a, wide, device, sms, cfg);
+    if (vectors <= 256) return q8_norm_v<T, 256, 1>(a, wide, device, sms, cfg);
+    if (vectors <= 512) return q8_norm_v<T, 256, 2>(a, wide, device, sms, cfg);
+    if (vectors <= 1024) return q8_norm_v<T, 256, 4>(a, wide, device, sms, cfg);
+    if (vectors <= 2048) return q8_norm_v<T, 256, 8>(a, wide, device, sms, cfg);
+    cfg.gridDim = dim3((unsigned)a.rows);
     return cudaLaunchKernelEx(&cfg, dz_norm_q8_long_kernel<T>, a);
 }
 
@@ -311,11 +401,18 @@ extern "C" int dz_cuda_norm_q8(const dz_norm_q8_t* p, size_t rows, size_t width,
     a.norm = p->norm;
     a.eps64 = p->norm ? p->eps : 0.0;
     const uintptr_t bases = (uintptr_t)p->x | (uintptr_t)p->residual | (uintptr_t)p->sum_out | (uintptr_t)p->gain;
-    a.wide = bases % 16 == 0 && (a.ldx | a.ldr | a.lds) * (long long)type_bytes(p->type) % 16 == 0 &&
-             ((uintptr_t)p->codes | (uintptr_t)a.ldc) % 8 == 0;
+    const bool wide = bases % 16 == 0 && (a.ldx | a.ldr | a.lds | (long long)width) * (long long)type_bytes(p->type) % 16 == 0 &&
+                      ((uintptr_t)p->codes | (uintptr_t)a.ldc) % 8 == 0;
+    if (p->device >= Q8N_DEVICES) return fail(DZ_E_UNSUPPORTED, "norm_q8: device ordinals below %d", Q8N_DEVICES);
+    static std::atomic<int> known[Q8N_DEVICES];       // SM count per device, looked up once
+    int sms = known[p->device].load(std::memory_order_relaxed);
+    if (!sms) {
+        DZ_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, p->device));
+        known[p->device].store(sms, std::memory_order_relaxed);
+    }
     cudaStream_t st = (cudaStream_t)stream;
-    DZ_CUDA(p->type == DZ_TYPE_F32   ? q8_norm_t<float>(a, st)
-            : p->type == DZ_TYPE_F16 ? q8_norm_t<__half>(a, st)
-                                     : q8_norm_t<__nv_bfloat16>(a, st));
+    DZ_CUDA(p->type == DZ_TYPE_F32   ? q8_norm_t<float>(a, wide, p->device, sms, st)
+            : p->type == DZ_TYPE_F16 ? q8_norm_t<__half>(a, wide, p->device, sms, st)
+                                     : q8_norm_t<__nv_bfloat16>(a, wide, p->device, sms, st));
     return DZ_OK;
 }
