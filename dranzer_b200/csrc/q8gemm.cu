@@ -17,6 +17,7 @@ namespace cg = cooperative_groups;
 
 constexpr int Q8G_THREADS = 256;
 constexpr uint32_t Q8G_A_BYTES = 128 * 128;      // levels of a stage
+constexpr int Q8G_PARTS = 8;                     // blocks that split k at most
 
 template <int TN> struct Q8gShape {
     static constexpr uint32_t B_BYTES = TN * 128;
@@ -46,6 +47,7 @@ __global__ void __launch_bounds__(Q8G_THREADS, TN <= 64 ? 2 : 1)
     dz_q8gemm_kernel(const __grid_constant__ CUtensorMap tm_levels, const __grid_constant__ CUtensorMap tm_rows,
                      const __grid_constant__ Q8MatArgs a, int parts) {
     using S = Q8gShape<TN>;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(1024) uint8_t q8g_raw[];
     uint8_t* sm = q8g_raw + ((1024u - (dz_smem_addr(q8g_raw) & 1023u)) & 1023u);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + (size_t)S::STAGES * S::STAGE);
@@ -162,14 +164,36 @@ __global__ void __launch_bounds__(Q8G_THREADS, TN <= 64 ? 2 : 1)
         const int first = rows * part / parts, last = rows * (part + 1) / parts;
         bool lost = false;
         for (int p = 0; p < parts; p++) lost |= *cluster.map_shared_rank(any, p) != 0;
-        const int n = n0 + (threadIdx.x & 127);
-        if (n < a.N) {
-            const float scale = a.col_scale[n], bias = a.bias ? a.bias[n] : 0.0f;
-            for (int r = first + (threadIdx.x >> 7); r < last; r += 2) {
-                int sum = 0;
-                for (int p = 0; p < parts; p++) sum += cluster.map_shared_rank(sums, p)[r * 128 + (threadIdx.x & 127)];
-                c[(m0 + r) * a.ldc + n] = lost ? nothing : q8_finish<T>(sum, a.a_scales[m0 + r], scale, bias);
+        // a warp has a row, a lane four of its columns, all parts' sums in flight together
+        const int n = n0 + 4 * lane;
+        float scale[4], bias[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            scale[e] = n + e < a.N ? a.col_scale[n + e] : 0.0f;
+            bias[e] = n + e < a.N && a.bias ? a.bias[n + e] : 0.0f;
+        }
+        const int* from[Q8G_PARTS];
+#pragma unroll
+        for (int p = 0; p < Q8G_PARTS; p++) from[p] = cluster.map_shared_rank(sums, p < parts ? p : part) + 4 * lane;
+#pragma unroll 2
+        for (int r = first + warp; r < last; r += Q8G_THREADS / 32) {
+            int4 v[Q8G_PARTS];
+#pragma unroll
+            for (int p = 0; p < Q8G_PARTS; p++)
+                v[p] = p < parts ? *reinterpret_cast<const int4*>(from[p] + r * 128) : make_int4(0, 0, 0, 0);
+            const float row = a.a_scales[m0 + r];
+            int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int p = 0; p < Q8G_PARTS; p++) {
+                sum[0] += v[p].x;
+                sum[1] += v[p].y;
+                sum[2] += v[p].z;
+                sum[3] += v[p].w;
             }
+            T* to = c + (long long)(m0 + r) * a.ldc + n;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < a.N) to[e] = lost ? nothing : q8_finish<T>(sum[e], row, scale[e], bias[e]);
         }
         cluster.sync();                      // no block ends while another reads its shared memory
     }
@@ -204,7 +228,7 @@ static cudaError_t q8gemm_t(const Q8MatArgs& a, const CUtensorMap& levels, int d
     const int tiles = (a.N + 127) / 128, mtiles = (a.M + TN - 1) / TN;
     int parts = 1;
     const int slots = sms * (TN <= 64 ? 2 : 1);
-    while (parts < 8 && 2 * parts * tiles * mtiles <= slots && a.nkb >= 4 * parts) parts *= 2;
+    while (parts < Q8G_PARTS && 2 * parts * tiles * mtiles <= slots && a.nkb >= 4 * parts) parts *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * parts), (unsigned)mtiles);
     cfg.blockDim = dim3(Q8G_THREADS);
@@ -308,6 +332,7 @@ template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q8P_THREADS, 1)
     dz_q8pair_kernel(const __grid_constant__ CUtensorMap tm_levels, const __grid_constant__ CUtensorMap tm_rows,
                      const __grid_constant__ Q8MatArgs a, int ntiles, int mtiles) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(1024) uint8_t q8g_raw[];
     uint8_t* sm = q8g_raw + ((1024u - (dz_smem_addr(q8g_raw) & 1023u)) & 1023u);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + (size_t)Q8P_STAGES * Q8P_STAGE);   // used in the first block

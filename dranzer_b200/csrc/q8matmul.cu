@@ -21,7 +21,9 @@ namespace dz {
 // (m16n8k32, columns as the MMA's rows), the k order within a block being free
 // as long as the activations, staged in shared memory, follow it. Four such
 // pieces are in flight per warp, across tile borders. The warps' sums meet in
-// shared memory once per tile.
+// shared memory once per tile. The next kernel may be launched at once (it waits
+// for this one before it touches memory, but for a matrix's levels): a stream of
+// 1 x 4096 x 32000 products takes 23.9 us each instead of 25.7.
 
 constexpr int Q8V_WARPS = 8;
 constexpr int Q8V_RING = 4;
@@ -76,6 +78,7 @@ __global__ void __launch_bounds__(Q8V_WARPS * 32, 2) dz_q8mv_kernel(const __grid
     };
 #pragma unroll
     for (int i = 0; i < Q8V_RING; i++) load(ring[i]);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");   // the matrix is no kernel's output, the rows are
     const int8_t* x = a.a + (long long)m0 * a.lda;
     const int kept = (a.K + 15) & ~15;       // <= lda: what lies past K meets levels of 0

@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(Q8N_THREADS, Q8Ring<V>::BLOCKS) dz_norm_q8_ker
     const int t = threadIdx.x % TEAM;
     long long row = (long long)blockIdx.x * (Q8N_THREADS / TEAM) + threadIdx.x / TEAM;
     const long long step = (long long)gridDim.x * (Q8N_THREADS / TEAM);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= a.rows) return;               // whole teams
     auto place = [&](int j, int i) { return WIDE ? (j * TEAM + t) * E + i : (j * E + i) * TEAM + t; };
@@ -292,6 +293,7 @@ __global__ void __launch_bounds__(Q8N_THREADS, Q8Ring<V>::BLOCKS) dz_norm_q8_ker
 
 // Rows of any width, read again for their codes.
 template <typename T> __global__ void __launch_bounds__(Q8N_THREADS) dz_norm_q8_long_kernel(const __grid_constant__ Q8NormArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
