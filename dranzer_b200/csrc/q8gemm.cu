@@ -17,14 +17,15 @@ namespace cg = cooperative_groups;
 
 constexpr int Q8G_THREADS = 256;
 constexpr uint32_t Q8G_A_BYTES = 128 * 128;      // levels of a stage
-constexpr int Q8G_PARTS = 8;                     // blocks that split k at most
 
+constexpr int Q8G_STAGES = 10;                   // of a block at most
 template <int TN> struct Q8gShape {
     static constexpr uint32_t B_BYTES = TN * 128;
     static constexpr uint32_t STAGE = Q8G_A_BYTES + B_BYTES;
-    // two blocks to an SM for narrow tiles, one for wide ones
-    static constexpr int STAGES = TN <= 64 ? (int)(100 * 1024 / STAGE) : (int)(200 * 1024 / STAGE);
-    static constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 256;
+    // a block alone on its SM, or one of two
+    static constexpr int ALONE = (int)(200 * 1024 / STAGE), SHARED = (int)(100 * 1024 / STAGE);
+    static_assert(ALONE <= Q8G_STAGES && 2 * STAGE >= TN * 128 * 4, "barriers of a stage; parts' sums in two stages");
+    static constexpr size_t smem(int stages) { return (size_t)stages * STAGE + 1024 + 256; }
 };
 
 // kind::i8, int32 sums, both operands s8 and K-major, 128 lanes, TN columns.
@@ -43,24 +44,25 @@ __device__ __forceinline__ void q8g_tma_2d(void* dst, const CUtensorMap* tm, int
 // A block takes 128 columns, TN rows and a share of k; the blocks of a cluster
 // split k and add their sums through distributed shared memory.
 template <typename T, int TN>
-__global__ void __launch_bounds__(Q8G_THREADS, TN <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(Q8G_THREADS, 2)
     dz_q8gemm_kernel(const __grid_constant__ CUtensorMap tm_levels, const __grid_constant__ CUtensorMap tm_rows,
-                     const __grid_constant__ Q8MatArgs a, int parts) {
+                     const __grid_constant__ Q8MatArgs a, int stages, int mtiles, int parts) {
     using S = Q8gShape<TN>;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(1024) uint8_t q8g_raw[];
     uint8_t* sm = q8g_raw + ((1024u - (dz_smem_addr(q8g_raw) & 1023u)) & 1023u);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm + (size_t)S::STAGES * S::STAGE);
-    uint64_t* empty = full + S::STAGES;
-    uint64_t* accum = empty + S::STAGES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + (size_t)stages * S::STAGE);
+    uint64_t* empty = full + Q8G_STAGES;
+    uint64_t* accum = empty + Q8G_STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum + 1);
     int* progress = reinterpret_cast<int*>(tmem_slot + 1);       // stages issued, consumed; failed
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int part = (int)(blockIdx.x % (unsigned)parts), tile = (int)(blockIdx.x / (unsigned)parts);
-    const int n0 = tile * 128, m0 = blockIdx.y * TN;
+    // parts of a tile side by side, then the tiles of the same levels
+    const int part = (int)(blockIdx.x % (unsigned)parts), where = (int)(blockIdx.x / (unsigned)parts);
+    const int tile = where / mtiles, n0 = tile * 128, m0 = where % mtiles * TN;
     const int kb0 = (int)((long long)a.nkb * part / parts), nkb = (int)((long long)a.nkb * (part + 1) / parts) - kb0;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::STAGES; s++) {
+        for (int s = 0; s < stages; s++) {
             dz_mbar_init(&full[s]);
             dz_mbar_init(&empty[s]);
         }
@@ -79,48 +81,62 @@ __global__ void __launch_bounds__(Q8G_THREADS, TN <= 64 ? 2 : 1)
     ug_fence_after();
     const uint32_t tmem = *tmem_slot;
     if (warp == 0) {
-        if (lane == 0) {
-            // the levels of the first stages are no kernel's output and go out before the one before has ended
-            const int pre = nkb < S::STAGES ? nkb : S::STAGES;
-            for (int kb = 0; kb < pre; kb++) {
+        const bool elected = ug_elect();
+        // the levels of the first stages are no kernel's output and go out before the one before has ended
+        const int pre = nkb < stages ? nkb : stages;
+        for (int kb = 0; kb < pre; kb++)
+            if (elected) {
                 dz_mbar_expect_tx(&full[kb], S::STAGE);
                 ug_tma_4d(sm + (size_t)kb * S::STAGE, &tm_levels, 0, 0, kb0 + kb, tile, &full[kb]);
             }
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            int kb = 0;
-            for (; kb < nkb; kb++) {
-                const int s = kb % S::STAGES;
-                if (kb >= S::STAGES && !dz_mbar_wait(&empty[s], (uint32_t)(((kb / S::STAGES) - 1) & 1))) {
-                    progress[2] = 1;
-                    break;
-                }
-                uint8_t* to = sm + (size_t)s * S::STAGE;
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        int kb = 0, s = 0;
+        uint32_t phase = 1;                  // of the stage's consumption before
+        for (; kb < nkb; kb++) {
+            if (kb >= stages && !dz_mbar_wait(&empty[s], phase)) {
+                if (elected) progress[2] = 1;
+                break;
+            }
+            uint8_t* to = sm + (size_t)s * S::STAGE;
+            if (elected) {
                 if (kb >= pre) {
                     dz_mbar_expect_tx(&full[s], S::STAGE);
                     ug_tma_4d(to, &tm_levels, 0, 0, kb0 + kb, tile, &full[s]);
                 }
                 q8g_tma_2d(to + Q8G_A_BYTES, &tm_rows, (kb0 + kb) * 128, m0, &full[s]);
             }
-            progress[0] = kb;
+            if (++s == stages) {
+                s = 0;
+                phase ^= 1;
+            }
         }
+        if (elected) progress[0] = kb;
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            int kb = 0;
-            for (; kb < nkb; kb++) {
-                const int s = kb % S::STAGES;
-                if (!dz_mbar_wait(&full[s], (uint32_t)((kb / S::STAGES) & 1))) {
-                    progress[2] = 1;
-                    break;
-                }
-                ug_fence_after();
-                const uint32_t at = dz_smem_addr(sm + (size_t)s * S::STAGE);
+        const bool elected = ug_elect();
+        const uint64_t first = ug_desc_kmajor(dz_smem_addr(sm));
+        int kb = 0, s = 0;
+        uint32_t phase = 0;
+        for (; kb < nkb; kb++) {
+            if (!dz_mbar_wait(&full[s], phase)) {
+                if (elected) progress[2] = 1;
+                break;
+            }
+            ug_fence_after();
+            const uint64_t levels = first + (uint64_t)(s * (S::STAGE >> 4)), rows = levels + (Q8G_A_BYTES >> 4);
+            if (elected) {
 #pragma unroll
                 for (int kk = 0; kk < 4; kk++)
-                    ug_mma(tmem, ug_desc_kmajor(at + kk * 32), ug_desc_kmajor(at + Q8G_A_BYTES + kk * 32), q8g_idesc<TN>(),
-                           (kb > 0 || kk > 0) ? 1u : 0u);
+                    ug_mma(tmem, levels + kk * 2, rows + kk * 2, q8g_idesc<TN>(), (kb > 0 || kk > 0) ? 1u : 0u);
                 ug_commit(&empty[s]);
             }
+            __syncwarp();
+            if (++s == stages) {
+                s = 0;
+                phase ^= 1;
+            }
+        }
+        if (elected) {
             progress[1] = kb;
             ug_commit(accum);
         }
@@ -172,19 +188,19 @@ __global__ void __launch_bounds__(Q8G_THREADS, TN <= 64 ? 2 : 1)
             scale[e] = n + e < a.N ? a.col_scale[n + e] : 0.0f;
             bias[e] = n + e < a.N && a.bias ? a.bias[n + e] : 0.0f;
         }
-        const int* from[Q8G_PARTS];
+        const int* from[Q8_PARTS];
 #pragma unroll
-        for (int p = 0; p < Q8G_PARTS; p++) from[p] = cluster.map_shared_rank(sums, p < parts ? p : part) + 4 * lane;
+        for (int p = 0; p < Q8_PARTS; p++) from[p] = cluster.map_shared_rank(sums, p < parts ? p : part) + 4 * lane;
 #pragma unroll 2
         for (int r = first + warp; r < last; r += Q8G_THREADS / 32) {
-            int4 v[Q8G_PARTS];
+            int4 v[Q8_PARTS];
 #pragma unroll
-            for (int p = 0; p < Q8G_PARTS; p++)
+            for (int p = 0; p < Q8_PARTS; p++)
                 v[p] = p < parts ? *reinterpret_cast<const int4*>(from[p] + r * 128) : make_int4(0, 0, 0, 0);
             const float row = a.a_scales[m0 + r];
             int sum[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int p = 0; p < Q8G_PARTS; p++) {
+            for (int p = 0; p < Q8_PARTS; p++) {
                 sum[0] += v[p].x;
                 sum[1] += v[p].y;
                 sum[2] += v[p].z;
@@ -201,7 +217,7 @@ __global__ void __launch_bounds__(Q8G_THREADS, TN <= 64 ? 2 : 1)
     ug_fence_before();
     if (threadIdx.x == 0 && progress[2]) {
         for (int kb = progress[1]; kb < progress[0]; kb++)
-            if (!dz_mbar_wait(&full[kb % S::STAGES], (uint32_t)((kb / S::STAGES) & 1))) break;
+            if (!dz_mbar_wait(&full[kb % stages], (uint32_t)((kb / stages) & 1))) break;
         dz_mbar_wait(accum, 0);
     }
     __syncthreads();
@@ -212,12 +228,12 @@ __global__ void __launch_bounds__(Q8G_THREADS, TN <= 64 ? 2 : 1)
 }
 
 template <typename T, int TN>
-static cudaError_t q8gemm_t(const Q8MatArgs& a, const CUtensorMap& levels, int device, int sms, cudaStream_t st) {
+static cudaError_t q8gemm_t(const Q8MatArgs& a, const CUtensorMap& levels, int parts, int device, int sms, cudaStream_t st) {
     static std::atomic<bool> ready[Q8_DEVICES];
     using S = Q8gShape<TN>;
     const auto kernel = dz_q8gemm_kernel<T, TN>;
     if (!ready[device].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem(S::ALONE));
         if (e != cudaSuccess) return e;
         ready[device].store(true, std::memory_order_release);
     }
@@ -226,13 +242,14 @@ static cudaError_t q8gemm_t(const Q8MatArgs& a, const CUtensorMap& levels, int d
     const uint32_t box[2] = {128, (uint32_t)TN};
     if (!dz_encode_u8_map(&rows, a.a, 2, dims, strides, box)) return cudaErrorInvalidValue;
     const int tiles = (a.N + 127) / 128, mtiles = (a.M + TN - 1) / TN;
-    int parts = 1;
-    const int slots = sms * (TN <= 64 ? 2 : 1);
-    while (parts < Q8G_PARTS && 2 * parts * tiles * mtiles <= slots && a.nkb >= 4 * parts) parts *= 2;
+    const long long blocks = (long long)tiles * mtiles * parts;
+    // no more stages than a block has steps: clusters of blocks that fill an SM each find few places
+    const int most = blocks <= sms ? S::ALONE : S::SHARED, steps = (a.nkb + parts - 1) / parts;
+    const int stages = steps >= most ? most : steps < 2 ? 2 : steps;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * parts), (unsigned)mtiles);
+    cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(Q8G_THREADS);
-    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.dynamicSmemBytes = S::smem(stages);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -242,7 +259,7 @@ static cudaError_t q8gemm_t(const Q8MatArgs& a, const CUtensorMap& levels, int d
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, levels, rows, a, parts);
+    return cudaLaunchKernelEx(&cfg, kernel, levels, rows, a, stages, mtiles, parts);
 }
 
 // ------------------------------------------------- many rows: pairs of SMs
@@ -252,7 +269,7 @@ static cudaError_t q8gemm_t(const Q8MatArgs& a, const CUtensorMap& levels, int d
 // for 256 x 128 x 128 products of its own, where a block alone would load 48.
 // The pairs stay and take tiles in turn. Two accumulators fill the tensor
 // memory, so that eight warps of each block write a tile while the next one's
-// MMAs run (four took 250 us for 4096 x 4096 x 16384, the MMAs waiting). The first block of a pair issues the MMAs for both; its `full`
+// MMAs run. The first block of a pair issues the MMAs for both; its `full`
 // barriers count both blocks' bytes, commits arrive at both blocks' barriers.
 
 constexpr int Q8P_WRITERS = 8;
@@ -372,36 +389,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q8P_THREADS, 1)
     ug_fence_after();
     const uint32_t tmem = *tmem_slot;
     if (warp == 0) {
-        if (lane == 0) {
-            int step = 0;                        // stages since the start
-            bool ok = true, waited = false;
-            for (int i = pair; i < tiles && ok; i += pairs) {
-                int tn, tm;
-                q8p_place(i, ntiles, mtiles, &tn, &tm);
-                for (int kb = 0; kb < a.nkb; kb++, step++) {
-                    const int s = step % Q8P_STAGES;
-                    if (step >= Q8P_STAGES && !q8p_wait(&empty[s], (uint32_t)((step / Q8P_STAGES - 1) & 1))) {
-                        ok = false;
-                        break;
-                    }
-                    uint8_t* to = sm + (size_t)s * Q8P_STAGE;
-                    const uint32_t bar = q8p_at_leader(&full[s]);
+        const bool elected = ug_elect();
+        int step = 0, s = 0;                     // stages since the start; the next one's place
+        uint32_t phase = 1;
+        bool ok = true;
+        for (int i = pair; i < tiles && ok; i += pairs) {
+            int tn, tm;
+            q8p_place(i, ntiles, mtiles, &tn, &tm);
+            for (int kb = 0; kb < a.nkb; kb++, step++) {
+                if (step >= Q8P_STAGES && !q8p_wait(&empty[s], phase)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t* to = sm + (size_t)s * Q8P_STAGE;
+                const uint32_t bar = q8p_at_leader(&full[s]);
+                if (elected) {
                     if (rank == 0) dz_mbar_expect_tx(&full[s], 2 * Q8P_STAGE);
                     q8p_tma_4d(to, &tm_levels, kb, tn * 2 + rank, bar);
-                    if (!waited) {               // the levels are no kernel's output, the rows are
-                        asm volatile("griddepcontrol.wait;" ::: "memory");
-                        waited = true;
-                    }
-                    q8p_tma_2d(to + Q8G_A_BYTES, &tm_rows, kb * 128, tm * Q8P_TILE + rank * 128, bar);
+                }
+                // the levels are no kernel's output, the rows are
+                if (step == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+                if (elected) q8p_tma_2d(to + Q8G_A_BYTES, &tm_rows, kb * 128, tm * Q8P_TILE + rank * 128, bar);
+                if (++s == Q8P_STAGES) {
+                    s = 0;
+                    phase ^= 1;
                 }
             }
+        }
+        if (elected) {
             if (!ok) *failed = 1;
             issued[0] = step;
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            int step = 0, turn = 0;
+        if (rank == 0) {
+            const bool elected = ug_elect();
+            const uint64_t first = ug_desc_kmajor(dz_smem_addr(sm));
+            int step = 0, turn = 0, s = 0;
+            uint32_t phase = 0;
             bool ok = true;
             for (int i = pair; i < tiles && ok; i += pairs, turn++) {
                 const int b = turn & 1;
@@ -411,23 +436,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q8P_THREADS, 1)
                 }
                 ug_fence_after();
                 for (int kb = 0; kb < a.nkb; kb++, step++) {
-                    const int s = step % Q8P_STAGES;
-                    if (!q8p_wait(&full[s], (uint32_t)((step / Q8P_STAGES) & 1))) {
+                    if (!q8p_wait(&full[s], phase)) {
                         ok = false;
                         break;
                     }
                     ug_fence_after();
-                    const uint32_t at = dz_smem_addr(sm + (size_t)s * Q8P_STAGE);
+                    const uint64_t levels = first + (uint64_t)(s * (Q8P_STAGE >> 4)), rows = levels + (Q8G_A_BYTES >> 4);
+                    if (elected) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
-                        q8p_mma(tmem + (uint32_t)(b * 256), ug_desc_kmajor(at + kk * 32),
-                                ug_desc_kmajor(at + Q8G_A_BYTES + kk * 32), (kb > 0 || kk > 0) ? 1u : 0u);
-                    q8p_commit(&empty[s]);
+                        for (int kk = 0; kk < 4; kk++)
+                            q8p_mma(tmem + (uint32_t)(b * 256), levels + kk * 2, rows + kk * 2, (kb > 0 || kk > 0) ? 1u : 0u);
+                        q8p_commit(&empty[s]);
+                    }
+                    __syncwarp();
+                    if (++s == Q8P_STAGES) {
+                        s = 0;
+                        phase ^= 1;
+                    }
                 }
-                if (ok) q8p_commit(&done[b]);
+                if (ok && elected) q8p_commit(&done[b]);
             }
-            if (!ok) *failed = 1;
-            issued[1] = step;
+            if (elected) {
+                if (!ok) *failed = 1;
+                issued[1] = step;
+            }
         }
         __syncwarp();
     } else {
@@ -520,18 +552,19 @@ template <typename T> static cudaError_t q8pair_t(const Q8MatArgs& a, const CUte
     return cudaLaunchKernelEx(&cfg, kernel, levels, rows, a, ntiles, mtiles);
 }
 
-template <typename T> static cudaError_t q8gemm_n(const Q8MatArgs& a, const CUtensorMap& levels, int device, int sms, cudaStream_t st) {
-    if (a.M <= 32) return q8gemm_t<T, 32>(a, levels, device, sms, st);
-    if (a.M <= 64) return q8gemm_t<T, 64>(a, levels, device, sms, st);
-    if (a.M <= 128) return q8gemm_t<T, 128>(a, levels, device, sms, st);
-    if (a.M <= 256) return q8gemm_t<T, 256>(a, levels, device, sms, st);
+template <typename T>
+static cudaError_t q8gemm_n(const Q8MatArgs& a, const CUtensorMap& levels, const Q8Plan& plan, int device, int sms, cudaStream_t st) {
+    if (plan.rows == 32) return q8gemm_t<T, 32>(a, levels, plan.parts, device, sms, st);
+    if (plan.rows == 64) return q8gemm_t<T, 64>(a, levels, plan.parts, device, sms, st);
+    if (plan.rows == 128) return q8gemm_t<T, 128>(a, levels, plan.parts, device, sms, st);
     return q8pair_t<T>(a, levels, device, sms, st);
 }
 
-cudaError_t dz_q8gemm_launch(const Q8MatArgs& a, const CUtensorMap& levels, int type, int device, int sms, cudaStream_t st) {
-    if (type == DZ_TYPE_F32) return q8gemm_n<float>(a, levels, device, sms, st);
-    if (type == DZ_TYPE_F16) return q8gemm_n<__half>(a, levels, device, sms, st);
-    return q8gemm_n<__nv_bfloat16>(a, levels, device, sms, st);
+cudaError_t dz_q8gemm_launch(const Q8MatArgs& a, const CUtensorMap& levels, const Q8Plan& plan, int type, int device, int sms,
+                             cudaStream_t st) {
+    if (type == DZ_TYPE_F32) return q8gemm_n<float>(a, levels, plan, device, sms, st);
+    if (type == DZ_TYPE_F16) return q8gemm_n<__half>(a, levels, plan, device, sms, st);
+    return q8gemm_n<__nv_bfloat16>(a, levels, plan, device, sms, st);
 }
 
 }  // namespace dz

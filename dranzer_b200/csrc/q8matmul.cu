@@ -178,19 +178,17 @@ template <typename T, int G, bool STAGED> static cudaError_t q8mv_g(const Q8MatA
     return cudaLaunchKernelEx(&cfg, dz_q8mv_kernel<T, G, STAGED>, a);
 }
 
-template <typename T> static cudaError_t q8mv_t(const Q8MatArgs& a, int device, int sms, cudaStream_t st) {
-    const size_t pitch = q8v_pitch(a.nkb);
-    auto staged = [&](int g) { return (size_t)(a.M < g * 8 ? a.M : g * 8) * pitch <= (size_t)Q8V_SMEM; };
-    if (a.M > 16 && staged(4)) return q8mv_g<T, 4, true>(a, device, sms, st);
-    if (a.M > 8 && staged(2)) return q8mv_g<T, 2, true>(a, device, sms, st);
-    if (staged(1)) return q8mv_g<T, 1, true>(a, device, sms, st);
+template <typename T> static cudaError_t q8mv_t(const Q8MatArgs& a, int rows, int device, int sms, cudaStream_t st) {
+    if (rows == 16) return q8mv_g<T, 2, true>(a, device, sms, st);
+    // rows that fit are staged, others read from L2 with every piece of levels
+    if ((size_t)(a.M < 8 ? a.M : 8) * q8v_pitch(a.nkb) <= (size_t)Q8V_SMEM) return q8mv_g<T, 1, true>(a, device, sms, st);
     return q8mv_g<T, 1, false>(a, device, sms, st);
 }
 
-static cudaError_t q8mv_launch(const Q8MatArgs& a, int type, int device, int sms, cudaStream_t st) {
-    if (type == DZ_TYPE_F32) return q8mv_t<float>(a, device, sms, st);
-    if (type == DZ_TYPE_F16) return q8mv_t<__half>(a, device, sms, st);
-    return q8mv_t<__nv_bfloat16>(a, device, sms, st);
+static cudaError_t q8mv_launch(const Q8MatArgs& a, int rows, int type, int device, int sms, cudaStream_t st) {
+    if (type == DZ_TYPE_F32) return q8mv_t<float>(a, rows, device, sms, st);
+    if (type == DZ_TYPE_F16) return q8mv_t<__half>(a, rows, device, sms, st);
+    return q8mv_t<__nv_bfloat16>(a, rows, device, sms, st);
 }
 
 }  // namespace dz
@@ -234,8 +232,9 @@ extern "C" int dz_cuda_matmul_q8_async(const int8_t* A, size_t lda, const float*
     a.N = w.N;
     a.K = w.K;
     a.nkb = (w.K + 127) / 128;
-    // few rows go through the matrix at the rate of its bytes either way; the MMAs of registers take 8 rows each time
+    const Q8Plan plan = q8_plan(a.M, a.K, a.N, sms, Q8V_SMEM);
     cudaStream_t st = (cudaStream_t)stream;
-    DZ_CUDA(m <= 16 ? q8mv_launch(a, type, w.device, sms, st) : dz_q8gemm_launch(a, w.map, type, w.device, sms, st));
+    DZ_CUDA(plan.rows <= 16 ? q8mv_launch(a, plan.rows, type, w.device, sms, st)
+                            : dz_q8gemm_launch(a, w.map, plan, type, w.device, sms, st));
     return DZ_OK;
 }

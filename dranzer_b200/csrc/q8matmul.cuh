@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "q8plan.h"
 #include "shim.cuh"
 
 namespace dz {
@@ -27,8 +28,9 @@ template <typename T> __device__ __forceinline__ T q8_finish(int sum, float a_sc
     return dz_from_float<T>(fmaf((float)sum * a_scale, col_scale, bias));
 }
 
-// The product on the tensor cores; `levels` maps the matrix's level blocks.
-[[nodiscard]] cudaError_t dz_q8gemm_launch(const Q8MatArgs& a, const CUtensorMap& levels, int type, int device, int sms,
-                                           cudaStream_t st);
+// The product on the tensor cores, in tiles of 32 rows and more; `levels` maps
+// the matrix's level blocks.
+[[nodiscard]] cudaError_t dz_q8gemm_launch(const Q8MatArgs& a, const CUtensorMap& levels, const Q8Plan& plan, int type,
+                                           int device, int sms, cudaStream_t st);
 
 }  // namespace dz

@@ -33,6 +33,16 @@ __device__ __forceinline__ void ug_mma(uint32_t tmem_d, uint64_t adesc, uint64_t
         : "memory");
 }
 
+// Whether this lane is the one that a converged warp elects. Loops that issue
+// copies or MMAs run in the whole warp and leave only the issue itself to this
+// lane: their addresses and descriptors then are uniform, and an MMA of 128 x 256
+// x 32 bytes takes its 128 cycles where a loop of one thread takes 171.
+__device__ __forceinline__ bool ug_elect() {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    return elected != 0;
+}
+
 // Arrive on `bar` once every MMA this thread issued so far has completed.
 __device__ __forceinline__ void ug_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(dz_smem_addr(bar))
