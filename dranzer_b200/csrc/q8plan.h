@@ -17,7 +17,7 @@ struct Q8Plan {
 // - registers: 1.5 us, then the levels once for every 8 rows at 7.5 MB a
 //   microsecond, or for every 16 at 5.6 where their activations fit shared memory
 //   (2 x 2048 x 2048: 2.3 us, 1 x 4096 x 16384: 9.8, 16 x 4096 x 5120: 7.7);
-// - blocks: 2.9, 3.6 or 5.5 us for 32, 64 or 128 rows each time the SMs are full
+// - blocks: 2.9, 3.6 or 6.8 us for 32, 64 or 128 rows each time the SMs are full
 //   of them, two to an SM, 0.21 us for each step of 128 of k, alone on its SM or
 //   0.33 (0.44) where two share one, 1 us and 0.1 for each part to join parts (32 x
 //   2048 x 2048: 7.5 us whole, 5.0 in four parts; 32 x 4096 x 5120: 6.9 in four, 11.4
@@ -43,11 +43,12 @@ inline Q8Plan q8_plan(long long m, long long k, long long n, long long sms, long
     }
     const long long tiles = (n + 127) / 128;
     for (int rows = 32; rows <= 128; rows *= 2) {
-        const double start = rows == 32 ? 2.9 : rows == 64 ? 3.6 : 5.5, shared = rows == 128 ? 0.44 : 0.33;
+        const double start = rows == 32 ? 2.9 : rows == 64 ? 3.6 : 6.8, shared = rows == 128 ? 0.44 : 0.33;
         for (int parts = 1; parts <= Q8_PARTS && (parts == 1 || 2 * parts <= steps); parts *= 2) {
             const long long blocks = tiles * ((m + rows - 1) / rows) * parts, full = blocks / (2 * sms), rest = blocks % (2 * sms);
             const double each = (double)((steps + parts - 1) / parts);
-            const double step = full * shared + (rest == 0 ? 0.0 : rest <= sms ? 0.21 : shared);
+            const double few = 0.6 + 0.4 * (double)(rest - sms) / (double)sms;       // not all of the SMs have two
+            const double step = full * shared + (rest == 0 ? 0.0 : rest <= sms ? 0.21 : 0.21 + (shared - 0.21) * few);
             const double starts = start * (double)(full + (rest ? 1 : 0));
             consider(rows, parts, least(starts + each * step + (parts > 1 ? 1.0 + 0.1 * parts : 0.0), 6.3e6));
         }
