@@ -23,7 +23,8 @@
 // and fp32 ones times a power of two of their row (its largest element in [2^13,
 // 2^14)), fp32 ones in two parts. Codes become fp16 exactly, two at a time, by
 // setting the exponent of 1024 above the byte and subtracting 1024 + 128; values
-// always do, and weights are taken times 2^15 in two fp16 parts. Scores of a tile
+// always do, and weights are taken times 2^15 in two fp16 parts, in one for bf16,
+// whose outputs' steps are eight times as coarse (6% of a tile's instructions). Scores of a tile
 // take the page's key scale, the sums of a tile its value scale, both in fp32.
 //
 // Few units of long contexts go to clusters of blocks, many to a warp each
@@ -38,6 +39,7 @@
 #include "kv8.cuh"
 #include "qlevels.cuh"
 #include "shim.cuh"
+#include "tcgen05.cuh"
 
 namespace dz {
 
@@ -148,6 +150,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
     constexpr int PAIRS = B::PAIRS, WARPS = B::WARPS, SLOTS = B::SLOTS;
     constexpr bool DIGITS = NT == 1;
     constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1;      // fp16 parts of a query's element
+    constexpr bool WHOLE = !std::is_same<T, __nv_bfloat16>::value;    // weights in two parts
     constexpr int TILES = HD / 16;           // sum MMAs over a head's elements
     extern __shared__ __align__(1024) uint8_t kv8_raw[];
     uint8_t* sm = kv8_raw + ((1024u - (dz_smem_addr(kv8_raw) & 1023u)) & 1023u);
@@ -219,23 +222,26 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
         const int shift = a.c.page == 64 ? 6 : 5;
         const int from = low_of(0), to = min(high_of(rows - 1), (int)reach - 1);
         const int t_first = from >> 5, t_last = to < from ? -1 : to >> 5;                 // tiles
-        // the warp's tiles that have a page, in turn: this one and the two after it, looked up one ahead
-        int at = t_first + me - warps, raw = t_first + me <= t_last ? table[(t_first + me) >> (shift - 5)] : -1;
-        int tile[3], page[3];
-        auto look = [&](int& tile_out, int& page_out) {
-            page_out = -1;
-            while (at + warps <= t_last) {
+        // the warp's tiles that have a page, in turn: this one and the two after it, their entries read three ahead
+        auto entry = [&](int i) { return i <= t_last ? table[i >> (shift - 5)] : -1; };
+        int at = t_first + me, raw[3] = {entry(at), entry(at + warps), entry(at + 2 * warps)};
+        int tile[3] = {0, 0, 0}, page[3] = {-1, -1, -1};
+        auto look = [&](int which) {
+            page[which] = -1;
+            while (at <= t_last && page[which] < 0) {
+                tile[which] = at;
+                page[which] = (unsigned)raw[0] < (unsigned)a.c.pages ? raw[0] : -1;
+                raw[0] = raw[1];
+                raw[1] = raw[2];
+                raw[2] = entry(at + 3 * warps);
                 at += warps;
-                tile_out = at;
-                page_out = (unsigned)raw < (unsigned)a.c.pages ? raw : -1;
-                raw = at + warps <= t_last ? table[(at + warps) >> (shift - 5)] : -1;
-                if (page_out >= 0) break;
             }
         };
+        const bool elected = ug_elect();
         unsigned flying = 0, parity = 0;     // slots that are being filled; their barriers' phases
         auto copy = [&](int slot, bool keys, int which) {
             if (page[which] < 0) return;
-            if (lane == 0) {
+            if (elected) {
                 dz_mbar_expect_tx(&bar[slot], B::SLOT);
                 kv8_copy(ring + slot * B::SLOT, keys ? &tm_k : &tm_v,
                          h * a.c.page + (shift == 6 ? (tile[which] & 1) * KV8_TILE : 0), page[which], &bar[slot]);
@@ -249,7 +255,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
             return ok;
         };
 #pragma unroll
-        for (int i = 0; i < 3; i++) look(tile[i], page[i]);
+        for (int i = 0; i < 3; i++) look(i);
         copy(0, true, 0);
         copy(1, false, 0);
         copy(2, true, 1);
@@ -259,18 +265,33 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
         float k_scale = scale_of(k_scales), v_scale = scale_of(v_scales);
         // queries as B operands, of pair 8 n + g
         uint2* qb = queries + warp * (B::QUERIES / 8) + lane;
+        const bool wide = ((uintptr_t)a.q | (uintptr_t)(a.ldq * (long long)sizeof(T))) % (4 * sizeof(T)) == 0;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const int r = min(r0 + 8 * n + g, pairs - 1);
             const T* q = static_cast<const T*>(a.q) + ((long long)b * a.n_tokens + r / share) * a.ldq +
                          (h * share + r % share) * HD + 4 * t;
-            float peak = 0.0f;
+            float x[HD / 4], peak = 0.0f;    // elements 16 c + 4 t + 0..3 for every c
             bool bad = false;
 #pragma unroll
-            for (int e = 0; e < HD / 4; e++) {
-                const float x = dz_to_float(q[16 * (e / 4) + e % 4]);
-                peak = fmaxf(peak, fabsf(x));
-                bad |= !(fabsf(x) <= 3.402823466e38f);
+            for (int c = 0; c < HD / 16; c++) {
+                T own[4];
+                if (wide) {
+                    if (sizeof(T) == 4)
+                        *reinterpret_cast<uint4*>(own) = *reinterpret_cast<const uint4*>(q + 16 * c);
+                    else
+                        *reinterpret_cast<uint2*>(own) = *reinterpret_cast<const uint2*>(q + 16 * c);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) own[i] = q[16 * c + i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[4 * c + i] = dz_to_float(own[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < HD / 4; i++) {
+                peak = fmaxf(peak, fabsf(x[i]));
+                bad |= !(fabsf(x[i]) <= 3.402823466e38f);
             }
             peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
             peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
@@ -291,8 +312,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
                     unsigned word[8];        // an element's four digits: the carries of 128 a digit, taken off again
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const float x = dz_to_float(q[32 * s + 16 * (i / 4) + i % 4]);
-                        word[i] = ((unsigned)(bad ? 0 : __float2int_rn(x * up0 * up1)) + 0x80808080u) ^ 0x80808080u;
+                        word[i] = ((unsigned)(bad ? 0 : __float2int_rn(x[8 * s + i] * up0 * up1)) + 0x80808080u) ^ 0x80808080u;
                     }
 #pragma unroll
                     for (int d = 0; d < 4; d++) {                // digit d of four elements side by side
@@ -306,16 +326,16 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
             } else {                         // step s: elements 16 s + 4 t + 0, 2 and + 1, 3
 #pragma unroll
                 for (int s = 0; s < HD / 16; s++) {
-                    float x[4];
+                    float v[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x[i] = dz_to_float(q[16 * s + i]) * up0 * up1;
-                    const uint2 hi = make_uint2(kv8_half2(x[0], x[2]), kv8_half2(x[1], x[3]));
+                    for (int i = 0; i < 4; i++) v[i] = x[4 * s + i] * up0 * up1;
+                    const uint2 hi = make_uint2(kv8_half2(v[0], v[2]), kv8_half2(v[1], v[3]));
                     qb[(n * (HD / 16) + s) * 32] = hi;
                     if (PARTS == 2) {
                         const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
                         const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
                         qb[((NT + n) * (HD / 16) + s) * 32] =
-                            make_uint2(kv8_half2(x[0] - u.x, x[2] - u.y), kv8_half2(x[1] - w.x, x[3] - w.y));
+                            make_uint2(kv8_half2(v[0] - u.x, v[2] - u.y), kv8_half2(v[1] - w.x, v[3] - w.y));
                     }
                 }
             }
@@ -479,9 +499,11 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         const uint32_t hi = kv8_half2(s[i][n][2 * j], s[i][n][2 * j + 1]);
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
                         wh[i][n][j] = kv8_turn(hi);
-                        wl[i][n][j] = kv8_turn(kv8_half2(s[i][n][2 * j] - f.x, s[i][n][2 * j + 1] - f.y));
+                        if (WHOLE) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                            wl[i][n][j] = kv8_turn(kv8_half2(s[i][n][2 * j] - f.x, s[i][n][2 * j + 1] - f.y));
+                        }
                     }
             const int slot_v = slot + 1 == SLOTS ? 0 : slot + 1;
             if (!arrived(slot_v)) ok = false;
@@ -507,7 +529,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
                             kv8_mma_first(part[n], va, wh[st][n][0], wh[st][n][1]);
                         else
                             kv8_mma(part[n], va, wh[st][n][0], wh[st][n][1]);
-                        kv8_mma(part[n], va, wl[st][n][0], wl[st][n][1]);
+                        if (WHOLE) kv8_mma(part[n], va, wl[st][n][0], wl[st][n][1]);
                     }
                 }
 #pragma unroll
@@ -527,7 +549,10 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
             page[0] = page[1];
             tile[1] = tile[2];
             page[1] = page[2];
-            if (ok) look(tile[2], page[2]);
+            if (ok)
+                look(2);
+            else
+                page[2] = -1;
             slot = slot_v + 1 == SLOTS ? 0 : slot_v + 1;
         }
         if (!ok) {                           // a copy did not come: the unit reads NaN, once those under way have ended
@@ -575,6 +600,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
         for (int c = 0; c < cluster; c++) {
             const float2* st = cluster > 1 ? cg::this_cluster().map_shared_rank(stats, c) : stats;
             const int* sn = cluster > 1 ? cg::this_cluster().map_shared_rank(seens, c) : seens;
+#pragma unroll 4
             for (int w = 0; w < team; w++) {
                 m = fmaxf(m, st[(w0 + w) * PAIRS + r].x);
                 any |= sn[(w0 + w) * PAIRS + r];
@@ -584,6 +610,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
         for (int c = 0; c < cluster; c++) {
             const float2* st = cluster > 1 ? cg::this_cluster().map_shared_rank(stats, c) : stats;
             const float* jn = cluster > 1 ? cg::this_cluster().map_shared_rank(join, c) : join;
+#pragma unroll 4
             for (int w = 0; w < team; w++) {
                 const int at = (w0 + w) * PAIRS + r;
                 const float2 s = st[at];

@@ -139,8 +139,8 @@ def attend(q, k, v, scale, kind):
     at least 2^29, rounded to half a step); an MMA of 16-bit parts adds 16 products to
     a running sum, each alignment and the sum within 2 u of the largest in play, in hd
     / 16 steps of up to two parts; four roundings of factors and the difference from
-    the maximum, u each of what they round. A weight: the exponential and its parts 2^-21 in all, or 2^-39 of the
-    largest. Sums: two steps of two parts per tile of 32 tokens and its scale, the
+    the maximum, u each of what they round. A weight: the exponential and its parts
+    2^-21 in all, or 2^-39 of the largest, for bf16 its one fp16 part 2^-12 of itself. Sums: two steps of two parts per tile of 32 tokens and its scale, the
     same again for statistics and joins of parts."""
     q, k, v = (t.astype(np.float64) for t in (q, k, v))
     s = scale * (k @ q)
@@ -151,4 +151,5 @@ def attend(q, k, v, scale, kind):
     score = (2 * q.size / 16 * 2 + 8) * 2 * U * wide + held
     weight = p @ np.abs(v)
     n = len(s)
-    return p @ v, (2 * score + 2.0 ** -20 + (n / 32 * 6 + 128) * 2 * U) * weight + 2.0 ** -39 * n * np.abs(v).max() * p.max()
+    one = 2.0 ** -12 if kind == "bf16" else 0.0
+    return p @ v, (2 * score + 2.0 ** -20 + one + (n / 32 * 6 + 128) * 2 * U) * weight + 2.0 ** -39 * n * np.abs(v).max() * p.max()
