@@ -176,12 +176,23 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
     const int share = a.q_heads / a.c.kv_heads, pairs = a.n_tokens * share;
     int b = 0, h = 0, r0 = 0, rows = 0;
     long long first = -1;
+    // entries of the table, those of the warp's next three tiles ahead: without a window they do not wait for the position
+    const int shift = a.c.page == 64 ? 6 : 5;
+    const int32_t* table = a.c.table;
+    auto entry = [&](int i, int last) { return i <= last ? table[i >> (shift - 5)] : -1; };
+    int raw[3] = {-1, -1, -1};
     if (unit < units) {
         const int blk = unit % blocks, bh = unit / blocks;
         h = bh % a.c.kv_heads;
         b = bh / a.c.kv_heads;
         r0 = blk * PAIRS;
         rows = min(PAIRS, pairs - r0);
+        table += (long long)b * a.c.table_pages;
+        if (!a.window) {
+            const int last = (a.c.table_pages << (shift - 5)) - 1;
+#pragma unroll
+            for (int i = 0; i < 3; i++) raw[i] = entry(me + i * warps, last);
+        }
         first = a.positions[b];
         if (kv8_skips(first)) rows = 0;
     }
@@ -218,13 +229,14 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
                 low[n][e] = low_of(8 * n + 2 * t + e);
             }
         const int high_all = high_of(0), low_all = low_of(rows - 1);  // a tile within them is seen by every pair
-        const int32_t* table = a.c.table + (long long)b * a.c.table_pages;
-        const int shift = a.c.page == 64 ? 6 : 5;
         const int from = low_of(0), to = min(high_of(rows - 1), (int)reach - 1);
         const int t_first = from >> 5, t_last = to < from ? -1 : to >> 5;                 // tiles
         // the warp's tiles that have a page, in turn: this one and the two after it, their entries read three ahead
-        auto entry = [&](int i) { return i <= t_last ? table[i >> (shift - 5)] : -1; };
-        int at = t_first + me, raw[3] = {entry(at), entry(at + warps), entry(at + 2 * warps)};
+        int at = t_first + me;
+        if (a.window) {
+#pragma unroll
+            for (int i = 0; i < 3; i++) raw[i] = entry(at + i * warps, t_last);
+        }
         int tile[3] = {0, 0, 0}, page[3] = {-1, -1, -1};
         auto look = [&](int which) {
             page[which] = -1;
@@ -233,7 +245,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
                 page[which] = (unsigned)raw[0] < (unsigned)a.c.pages ? raw[0] : -1;
                 raw[0] = raw[1];
                 raw[1] = raw[2];
-                raw[2] = entry(at + 3 * warps);
+                raw[2] = entry(at + 3 * warps, t_last);
                 at += warps;
             }
         };
