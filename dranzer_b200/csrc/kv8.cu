@@ -34,13 +34,13 @@ namespace dz {
 constexpr int KV8_WARPS = 16;      // warps of a block, many tokens
 constexpr int KV8_ROWS = 4;        // rows of a warp
 constexpr int KV8_ONE_WARPS = 8;   // warps of a block, one token
+constexpr int KV8_QUERY_WARPS = 8; // warps of a block of queries
 constexpr int KV8_TURN = 16;       // rows between angles that are computed afresh
 
 struct Kv8AppendCut {
     int runs;                      // pages that a sequence's new tokens can touch
     int parts;                     // blocks that share a run's (a row's) heads
     int team;                      // warps of a head
-    int table_rows;                // rows of the angle tables
 };
 
 template <typename T> union Kv8Quad {
@@ -214,8 +214,7 @@ template <typename T, int HD, bool WIDE>     // every row of every operand is al
 __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a,
                                                                          const __grid_constant__ Kv8AppendCut cut) {
     constexpr int LANES = HD / 8, SLOTS = 32 / LANES, R = KV8_ROWS / SLOTS, P = HD / 2;
-    extern __shared__ __align__(16) double2 kv8_angles[];                          // [rows][P], then the same in fp32
-    float2* kv8_angles_f = reinterpret_cast<float2*>(kv8_angles + cut.table_rows * P);
+    extern __shared__ __align__(16) double2 kv8_angles[];                          // [rows][P]
     __shared__ unsigned tops[2][KV8_WARPS];
     asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before ends
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, slot = lane / LANES;
@@ -242,7 +241,6 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
             sincos(a.freq[p], &s1, &c1);
             for (int r = r0; r < r1; r++) {
                 kv8_angles[r * P + kv8_angle_at<HD>(p)] = make_double2(c, s);
-                kv8_angles_f[r * P + kv8_angle_at<HD>(p)] = make_float2((float)c, (float)s);
                 const double next = c * c1 - s * s1;
                 s = s * c1 + c * s1;
                 c = next;
@@ -330,47 +328,78 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
             }
         }
     }
-    // queries: a warp takes SLOTS rows at a time, whose angles and gains stay in registers, and this block's heads in
-    // turn, AHEAD of them in flight (two took 57 us of 8000 rows' 115, 16 KB in flight on an SM)
-    constexpr int AHEAD = 8 / (int)sizeof(T);
-    const int h0 = a.q_heads * part / cut.parts, h1 = a.q_heads * (part + 1) / cut.parts;
-    if (h0 == h1) return;
-    gains(a.q_gain);
-    for (int set = warp; set * SLOTS < rows; set += KV8_WARPS) {
-        const int r = set * SLOTS + slot;
-        const bool valid = r < rows;
-        float2 turn[4];
+}
+
+// Queries of many tokens: a warp takes SLOTS rows, whose angles and gains stay in
+// registers, and a share of their heads in turn. Where rows are aligned, the heads
+// after it are on their way into shared memory, each lane copying what it reads
+// itself.
+template <typename T> struct Kv8Ring {
+    static constexpr int HEADS = 8;                    // of a warp's rows, in turn
+    static constexpr int SMEM = HEADS * KV8_QUERY_WARPS * 32 * (int)(2 * sizeof(Kv8Quad<T>));
+};
+
+template <typename T, int HD, bool WIDE>
+__global__ void __launch_bounds__(KV8_QUERY_WARPS * 32, 3) dz_kv8_query_kernel(const __grid_constant__ Kv8AppendArgs a, int parts) {
+    constexpr int LANES = HD / 8, SLOTS = 32 / LANES, P = HD / 2, HEADS = Kv8Ring<T>::HEADS, B = 4 * (int)sizeof(T);
+    extern __shared__ __align__(16) uint8_t kv8_heads[];           // [HEADS][2 quads][threads]
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 31, l = lane % LANES, slot = lane / LANES;
+    const int work = blockIdx.x * KV8_QUERY_WARPS + (threadIdx.x >> 5), set = work / parts, part = work % parts;
+    const int rows = a.c.batch * a.n_tokens;
+    if (set * SLOTS >= rows) return;
+    const int row = min(set * SLOTS + slot, rows - 1), b = row / a.n_tokens;
+    const long long first = a.positions[b];
+    const bool done = set * SLOTS + slot < rows && !kv8_skips(first);
+    const int at = a.halves ? l * 4 : l * 8, quad = a.halves ? P : 4;
+    const int h0 = a.q_heads * part / parts, n = a.q_heads * (part + 1) / parts - h0;
+    const T* in = static_cast<const T*>(a.q) + row * a.ldq + h0 * HD + at;
+    T* out = static_cast<T*>(a.q_out) + row * a.ldqo + h0 * HD + at;
+    auto place = [&](int k, int q) { return kv8_heads + ((k * 2 + q) * (KV8_QUERY_WARPS * 32) + (int)threadIdx.x) * B; };
+    auto copy = [&](int k, int h) {
+        if (h < n) {
 #pragma unroll
-        for (int p = 0; p < 4; p++)
-            if (a.rope) turn[p] = kv8_angles_f[min(r, rows - 1) * P + p * LANES + l];
-        const T* in = static_cast<const T*>(a.q) + (row0 + r) * a.ldq + h0 * HD + at[0];
-        T* out = static_cast<T*>(a.q_out) + (row0 + r) * a.ldqo + h0 * HD + at[0];
-        const int quad = at[1] - at[0];
-        Kv8Quad<T> ring[AHEAD][2];
-        auto fetch = [&](int h, Kv8Quad<T> (&io)[2]) {
-            if (valid && h < h1) {
-                kv8_load<WIDE>(in, io[0]);
-                kv8_load<WIDE>(in + quad, io[1]);
-            }
-            in += HD;
-        };
+            for (int q = 0; q < 2; q++)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(place(k, q))),
+                             "l"(in + h * HD + q * quad), "n"(B)
+                             : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (WIDE) {
 #pragma unroll
-        for (int k = 0; k < AHEAD; k++) fetch(h0 + k, ring[k]);
-        for (int h = h0; h < h1; h += AHEAD) {
+        for (int k = 0; k < HEADS - 1; k++) copy(k, k);
+    }
+    float2 turn[4];
 #pragma unroll
-            for (int k = 0; k < AHEAD; k++) {
-                if (h + k >= h1) break;      // the warp alike
-                float y[8];
+    for (int p = 0; p < 4; p++)
+        if (a.rope) {
+            double c, s;
+            sincos((double)(first + (row - b * a.n_tokens)) * a.freq[l * 4 + p], &s, &c);
+            turn[p] = make_float2((float)c, (float)s);
+        }
+    float gain[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) y[e] = valid ? dz_to_float(ring[k][e / 4].e[e % 4]) : 0.0f;
-                fetch(h + k + AHEAD, ring[k]);
-                kv8_query<HD>(y, gain, turn, a);
-                if (valid) {
-                    kv8_store<WIDE>(out, y);
-                    kv8_store<WIDE>(out + quad, y + 4);
-                }
-                out += HD;
-            }
+    for (int i = 0; i < 8; i++) gain[i] = a.q_gain ? a.q_gain[at + i / 4 * quad + i % 4] : 1.0f;
+#pragma unroll 1
+    for (int h = 0; h < n; h++) {
+        Kv8Quad<T> io[2];
+        if (WIDE) {
+            copy((h + HEADS - 1) % HEADS, h + HEADS - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(HEADS - 1) : "memory");
+#pragma unroll
+            for (int q = 0; q < 2; q++) kv8_load<true>(reinterpret_cast<const T*>(place(h % HEADS, q)), io[q]);
+        } else {
+            kv8_load<false>(in + h * HD, io[0]);
+            kv8_load<false>(in + h * HD + quad, io[1]);
+        }
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = dz_to_float(io[e / 4].e[e % 4]);
+        kv8_query<HD>(y, gain, turn, a);
+        if (done) {
+            kv8_store<WIDE>(out + h * HD, y);
+            kv8_store<WIDE>(out + h * HD + quad, y + 4);
         }
     }
 }
@@ -476,7 +505,6 @@ template <typename T, int HD, bool WIDE> static cudaError_t kv8_append_t(const K
     static std::atomic<bool> ready[KV8_DEVICES];
     const int rows = a.n_tokens < a.c.page ? a.n_tokens : a.c.page;          // of a block at most
     Kv8AppendCut cut;
-    cut.table_rows = a.rope ? rows : 0;
     long long blocks = a.c.batch, most;                  // most: blocks that have heads for their warps
     if (a.n_tokens == 1) {
         constexpr int SLOTS = 256 / HD;
@@ -488,7 +516,6 @@ template <typename T, int HD, bool WIDE> static cudaError_t kv8_append_t(const K
         for (cut.team = 1; cut.team * KV8_ROWS < rows;) cut.team *= 2;
         const int teams = KV8_WARPS / cut.team;
         most = (2 * a.c.kv_heads + teams - 1) / teams;
-        if (most < a.q_heads) most = a.q_heads;
     }
     // as many blocks as the SMs hold at once (four, two of many tokens), as far as there are heads: a part of a wave
     // more cost 8000 rows a third of their time
@@ -504,14 +531,25 @@ template <typename T, int HD, bool WIDE> static cudaError_t kv8_append_t(const K
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     if (a.n_tokens == 1) return cudaLaunchKernelEx(&cfg, dz_kv8_append_one_kernel<T, HD, WIDE>, a, cut);
-    constexpr int most_smem = 64 * (HD / 2) * (int)(sizeof(double2) + sizeof(float2));
+    constexpr int most_smem = 64 * (HD / 2) * (int)sizeof(double2);
     if (!ready[device].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(dz_kv8_append_kernel<T, HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
-        if (e != cudaSuccess) return e;
+        const cudaError_t set = cudaFuncSetAttribute(dz_kv8_append_kernel<T, HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
+        if (set != cudaSuccess) return set;
+        const cudaError_t ring = cudaFuncSetAttribute(dz_kv8_query_kernel<T, HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8Ring<T>::SMEM);
+        if (ring != cudaSuccess) return ring;
         ready[device].store(true, std::memory_order_release);
     }
-    cfg.dynamicSmemBytes = (size_t)cut.table_rows * (HD / 2) * (sizeof(double2) + sizeof(float2));
-    return cudaLaunchKernelEx(&cfg, dz_kv8_append_kernel<T, HD, WIDE>, a, cut);
+    cfg.dynamicSmemBytes = a.rope ? (size_t)rows * (HD / 2) * sizeof(double2) : 0;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, dz_kv8_append_kernel<T, HD, WIDE>, a, cut);
+    if (e != cudaSuccess || a.q_heads == 0) return e;
+    // sets of rows that a warp takes, and its share of their heads where there are few
+    const long long sets = ((long long)a.c.batch * a.n_tokens + 256 / HD - 1) / (256 / HD), fit = 3LL * sms * KV8_QUERY_WARPS;
+    const long long share = (fit + sets - 1) / sets;
+    const int query_parts = (int)(share < a.q_heads ? share : a.q_heads);
+    cfg.gridDim = dim3((unsigned)((sets * query_parts + KV8_QUERY_WARPS - 1) / KV8_QUERY_WARPS));
+    cfg.blockDim = dim3(KV8_QUERY_WARPS * 32);
+    cfg.dynamicSmemBytes = WIDE ? Kv8Ring<T>::SMEM : 0;
+    return cudaLaunchKernelEx(&cfg, dz_kv8_query_kernel<T, HD, WIDE>, a, query_parts);
 }
 
 template <typename T> static cudaError_t kv8_append_h(const Kv8AppendArgs& a, int head_dim, int device, int sms, cudaStream_t st) {
