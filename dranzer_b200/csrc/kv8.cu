@@ -21,8 +21,8 @@ namespace dz {
 // team of 1 to 16 warps, four rows to a warp at most; a key or value head is
 // held in registers until the team knows its peak, so that the page's scale
 // needs no second pass over memory. The rows' angles are computed once per
-// block: sine and cosine of every 16th row in 64 bits, the rows between by
-// turning on by one token's angle (15 roundings of 2^-53).
+// block: sine and cosine of every 8th row in 64 bits, the rows between by
+// turning on by one token's angle (7 roundings of 2^-53).
 //
 // One token: a block takes a share of a row's heads, a warp two or four heads
 // at a time.
@@ -35,7 +35,7 @@ constexpr int KV8_WARPS = 16;      // warps of a block, many tokens
 constexpr int KV8_ROWS = 4;        // rows of a warp
 constexpr int KV8_ONE_WARPS = 8;   // warps of a block, one token
 constexpr int KV8_QUERY_WARPS = 8; // warps of a block of queries
-constexpr int KV8_TURN = 16;       // rows between angles that are computed afresh
+constexpr int KV8_TURN = 8;        // rows between angles that are computed afresh
 
 struct Kv8AppendCut {
     int runs;                      // pages that a sequence's new tokens can touch
@@ -123,10 +123,10 @@ __device__ __forceinline__ void kv8_query(float (&x)[8], const float (&gain)[8],
     if (a.rope) kv8_rotate(x, a.halves, turn);
 }
 
-// A key's eight elements, in 64 bits up to the last rounding; turn(i) is the
-// angle of its i-th pair.
-template <int HD, typename F>
-__device__ __forceinline__ void kv8_key(float (&x)[8], const float (&gain)[8], F turn, const Kv8AppendArgs& a) {
+// A key's eight elements, in 64 bits up to the last rounding; gain(i) is the gain
+// of element i, turn(i) the angle of the i-th pair.
+template <int HD, typename G, typename F>
+__device__ __forceinline__ void kv8_key(float (&x)[8], G gain, F turn, const Kv8AppendArgs& a) {
     if (!a.k_gain && !a.rope) return;
     double y[8];
 #pragma unroll
@@ -134,7 +134,7 @@ __device__ __forceinline__ void kv8_key(float (&x)[8], const float (&gain)[8], F
     if (a.k_gain) {
         const double n = kv4_rsqrt(kv4_square_sum<HD / 8>(y, 0xffffffffu) / HD + a.eps);
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = (double)gain[i] * y[i] * n;
+        for (int i = 0; i < 8; i++) y[i] = gain(i) * y[i] * n;
     }
     if (a.rope) {
         const double2 by[4] = {turn(0), turn(1), turn(2), turn(3)};
@@ -216,6 +216,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
     constexpr int LANES = HD / 8, SLOTS = 32 / LANES, R = KV8_ROWS / SLOTS, P = HD / 2;
     extern __shared__ __align__(16) double2 kv8_angles[];                          // [rows][P]
     __shared__ unsigned tops[2][KV8_WARPS];
+    __shared__ __align__(16) double gains[HD];
     asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before ends
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, slot = lane / LANES;
     const int at[2] = {a.halves ? l * 4 : l * 8, a.halves ? P + l * 4 : l * 8 + 4};
@@ -246,8 +247,10 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
                 c = next;
             }
         }
-        __syncthreads();
     }
+    if (a.k_gain)
+        for (int i = threadIdx.x; i < HD; i += KV8_WARPS * 32) gains[i] = (double)a.k_gain[i];
+    __syncthreads();
     const int team = cut.team, mine = warp / team, rank = warp % team, teams = KV8_WARPS / team;
     const int step = cut.parts * teams, heads = 2 * a.c.kv_heads;
     const long long row0 = (long long)b * a.n_tokens + lo;
@@ -267,12 +270,6 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
             }
         }
     };
-    float gain[8];
-    auto gains = [&](const float* g) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) gain[i] = g ? g[at[i / 4] + i % 4] : 1.0f;
-    };
-    gains(a.k_gain);
     int item = part * teams + mine, parity = 0;
     Kv8Quad<T> next[R][2];
     load(item, next);
@@ -294,7 +291,8 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) dz_kv8_append_kernel(const 
         for (int i = 0; i < R; i++) {
             const int r = min(row_of(i), rows - 1);
             if (key && (i * team + rank) * SLOTS < rows)                 // the warp alike
-                kv8_key<HD>(x[i], gain, [&](int p) { return kv8_angles[r * P + p * LANES + l]; }, a);
+                kv8_key<HD>(x[i], [&](int e) { return gains[at[e / 4] + e % 4]; },
+                            [&](int p) { return kv8_angles[r * P + p * LANES + l]; }, a);
             if (row_of(i) < rows) top = max(top, kv8_top(x[i]));
         }
 #pragma unroll
@@ -462,7 +460,7 @@ __global__ void __launch_bounds__(KV8_ONE_WARPS * 32, 4) dz_kv8_append_one_kerne
         const long long place = (long long)page * a.c.kv_heads + (valid ? h : 0);
         float* scales = key ? a.c.k_scales : a.c.v_scales;
         const float old = offset ? scales[place] : 0.0f;
-        if (key) kv8_key<HD>(x, gain, [&](int p) { return angles[p * LANES + l]; }, a);
+        if (key) kv8_key<HD>(x, [&](int e) { return (double)gain[e]; }, [&](int p) { return angles[p * LANES + l]; }, a);
         unsigned top = kv8_top(x);
 #pragma unroll
         for (int off = LANES / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
