@@ -464,6 +464,7 @@ __global__ void __launch_bounds__(KV8_ONE_WARPS * 32, 4) dz_kv8_append_one_kerne
         unsigned top = kv8_top(x);
 #pragma unroll
         for (int off = LANES / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+        __syncwarp();                        // every lane has the old scale
         if (!valid) continue;
         const Kv8Scale s = kv8_scale(top, old);
         int8_t* codes = (key ? a.c.k_codes : a.c.v_codes) + place * (a.c.page * HD);

@@ -113,6 +113,8 @@ __global__ void __launch_bounds__(Q8G_THREADS, 2)
         if (elected) progress[0] = kb;
         __syncwarp();
     } else if (warp == 1) {
+        // barrier waits are bounded, the kernel before is not: none begins before it has ended
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         const bool elected = ug_elect();
         const uint64_t first = ug_desc_kmajor(dz_smem_addr(sm));
         int kb = 0, s = 0;
@@ -142,9 +144,9 @@ __global__ void __launch_bounds__(Q8G_THREADS, 2)
         }
         __syncwarp();
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows' scales; and the waits above
     const bool ok = dz_mbar_wait(accum, 0);
     ug_fence_after();
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows' scales
     const bool failed = !ok || progress[2];
     T* c = static_cast<T*>(a.c);
     const T nothing = dz_from_float<T>(__int_as_float(0x7fc00000));
@@ -278,6 +280,12 @@ constexpr int Q8P_TILE = 256;
 constexpr uint32_t Q8P_STAGE = 2 * 128 * 128;
 constexpr int Q8P_STAGES = 6;
 constexpr size_t Q8P_SMEM = (size_t)Q8P_STAGES * Q8P_STAGE + 1024 + 256 + 2 * Q8P_TILE * sizeof(float);
+// A block of the next kernel may arrive before those of this one have their
+// tensor memory, and keeps its own until this kernel has ended. So no two blocks
+// that an SM holds at once may want more than 512 columns: a pair's block and
+// any other of a product exceed the shared memory, dz_q8gemm_kernel's two (by
+// their registers) have 128 columns each at most.
+static_assert(Q8P_SMEM + Q8gShape<32>::smem(2) > 227 * 1024, "blocks beside one of a pair");
 constexpr int Q8P_BAND = 8;                      // tiles of rows that neighbouring pairs share columns over
 
 __device__ __forceinline__ uint32_t q8p_at_leader(const void* p) {       // the same place in the pair's first block
@@ -423,6 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Q8P_THREADS, 1)
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");   // before the bounded waits, as in dz_q8gemm_kernel
             const bool elected = ug_elect();
             const uint64_t first = ug_desc_kmajor(dz_smem_addr(sm));
             int step = 0, turn = 0, s = 0;

@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(Q8N_THREADS, Q8Ring<V>::BLOCKS) dz_norm_q8_ker
     const int t = threadIdx.x % TEAM;
     long long row = (long long)blockIdx.x * (Q8N_THREADS / TEAM) + threadIdx.x / TEAM;
     const long long step = (long long)gridDim.x * (Q8N_THREADS / TEAM);
+    // a product that follows may fetch its levels now (it waits for this kernel's end before it reads rows)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= a.rows) return;               // whole teams

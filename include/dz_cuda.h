@@ -199,7 +199,7 @@ int dz_cuda_matmul_q8_async(const int8_t *A_dev, size_t lda, const float *a_scal
  * earlier tokens, S stays unless that is larger, and when it grows, the earlier
  * tokens' codes become round_half_away(fp32(code * fp32(old S / S))). New codes
  * are clamp(round_half_away(fp32(x * fp32(1 / S))), -127, 127), x rounded to
- * fp32 once. New rows that hold an infinity or a NaN make S a NaN, which it
+ * fp32 once (0 where S is 0, and for x = 0). New rows that hold an infinity or a NaN make S a NaN, which it
  * stays until the page is begun anew. k_out and v_out rows of tokens that no
  * page holds are left as they were. An output row may be its own input row
  * (same pointer and stride); otherwise outputs overlap no input. */

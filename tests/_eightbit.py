@@ -140,8 +140,9 @@ def attend(q, k, v, scale, kind):
     a running sum, each alignment and the sum within 2 u of the largest in play, in hd
     / 16 steps of up to two parts; four roundings of factors and the difference from
     the maximum, u each of what they round. A weight: the exponential and its parts
-    2^-21 in all, or 2^-39 of the largest, for bf16 its one fp16 part 2^-12 of itself. Sums: two steps of two parts per tile of 32 tokens and its scale, the
-    same again for statistics and joins of parts."""
+    2^-21 in all, or 2^-39 of the largest, for bf16 its one fp16 part 2^-12 of itself.
+    Sums: two steps of two parts per tile of 32 tokens and its scale, the same again
+    for statistics and joins of parts."""
     q, k, v = (t.astype(np.float64) for t in (q, k, v))
     s = scale * (k @ q)
     e = np.exp(s - s.max())

@@ -208,6 +208,46 @@ def test_product_extremes(gpu, m):
     w.close()
 
 
+@pytest.mark.parametrize("m,k,n", [(40, 512, 300), (1000, 1024, 9000)])
+def test_products_after_a_long_kernel(gpu, m, k, n):
+    """A product waits, however long, for a kernel that lets it start before it ends: the longest row,
+    of one block, takes 3.7 s."""
+    width = 1 << 30
+    x = torch.ones(width, device="cuda")
+    out, scale = torch.empty(width, dtype=torch.int8, device="cuda"), torch.empty(1, device="cuda")
+    levels = np.random.RandomState(m).randint(-127, 128, (k, n)).astype(np.int8)
+    w = _quantized(gpu, levels, np.ones(n, np.float32))
+    codes, ones = torch.ones(m, k, dtype=torch.int8, device="cuda"), torch.ones(m, device="cuda")
+    y = torch.zeros(m, n, device="cuda")
+    for turn in range(2):                    # the first call of a kernel waits for what is under way
+        torch.cuda.synchronize()
+        y.zero_()
+        gpu.norm_q8(1, width if turn else 1000000, type=gpu.TYPE_F32, x=x.data_ptr(), residual=x.data_ptr(),
+                    gain=x.data_ptr(), codes=out.data_ptr(), scales=scale.data_ptr(), stream_ptr=_stream())
+        w.matmul_q8_async(codes.data_ptr(), ones.data_ptr(), y.data_ptr(), m, _stream())
+    assert torch.equal(y, _dev(levels.sum(0, dtype=np.int64).astype(np.float32)).expand(m, n))
+    assert int(out[0]) == int(out[width - 1]) == 127
+    w.close()
+
+
+def test_fp32_products_after_a_long_row(gpu):
+    """The product of fp32 rows, whose waits are bounded too, behind the longest row."""
+    width, m, k, n = 1 << 30, 40, 512, 300
+    x = torch.ones(width, device="cuda")
+    out, scale = torch.empty(width, dtype=torch.int8, device="cuda"), torch.empty(1, device="cuda")
+    levels = np.random.RandomState(1).randint(-127, 128, (k, n)).astype(np.int8)
+    w = _quantized(gpu, levels, np.ones(n, np.float32))
+    ones, y = torch.ones(m, k, device="cuda"), torch.zeros(m, n, device="cuda")
+    for turn in range(2):
+        torch.cuda.synchronize()
+        y.zero_()
+        gpu.norm_q8(1, width if turn else 1000000, type=gpu.TYPE_F32, x=x.data_ptr(), residual=x.data_ptr(),
+                    gain=x.data_ptr(), codes=out.data_ptr(), scales=scale.data_ptr(), stream_ptr=_stream())
+        w.matmul_async(ones.data_ptr(), y.data_ptr(), m, _stream())
+    assert torch.equal(y, _dev(levels.sum(0, dtype=np.int64).astype(np.float32)).expand(m, n))
+    w.close()
+
+
 def test_product_refusals(gpu):
     rng = np.random.RandomState(0)
     v = rng.randn(64, 48).astype(np.float32)
@@ -574,7 +614,7 @@ def test_offsets_past_32_bits(gpu):
     ks, vs = torch.ones(pages, hk, device="cuda"), torch.ones(pages, hk, device="cuda")
     tt, pos = _dev(table), torch.tensor([10], device="cuda")
     cache = gpu.KV8Cache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, page, hk, hd, tt.data_ptr(), 1, 3)
-    c = eb.Cache(rng, pages if False else 3, page, hk, hd, [[0, 1, 2]])
+    c = eb.Cache(rng, 3, page, hk, hd, [[0, 1, 2]])
     for n in "kv":
         c.codes[n][:] = 0
         c.scales[n][:] = 1
