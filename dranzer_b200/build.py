@@ -21,7 +21,7 @@ CC_FLAGS = ["-O2", "-fPIC", "-std=c11", "-Wall", "-Wextra", "-fno-fast-math", "-
             f"-I{INCLUDE}"]
 
 CUDA_SOURCES = ["dz_cuda.cu", "qmvi.cu", "seqgen.cu", "attn.cu", "pfattn.cu", "gmatvec.cu", "kv4.cu", "kv4attn.cu", "kv4chunk.cu",
-                "q8norm.cu", "q8matmul.cu", "q8gemm.cu", "kv8.cu", "kv8attn.cu"]
+                "q8norm.cu", "q8matmul.cu", "q8gemm.cu", "kv8.cu", "kv8attn.cu", "kv8many.cu"]
 C_SOURCES = ["dz_host.c"]
 
 

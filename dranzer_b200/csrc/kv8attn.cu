@@ -1,5 +1,6 @@
 // Attention over the 8-bit paged caches (kv8.cuh): softmax(scale q . k) . v for
-// the newest queries of every sequence, with fp32 sums and running statistics.
+// the newest queries of every sequence, with fp32 sums and running statistics;
+// of many queries in kv8many.cu.
 //
 // A unit is one (sequence, key head) and up to 8 NT pairs (query token, query
 // head). Tokens are the rows of the MMAs of the scores, pairs their columns;
@@ -34,20 +35,15 @@
 #include <cooperative_groups.h>
 #include <type_traits>
 
-#include "async.cuh"
 #include "dz_types.h"
-#include "kv8.cuh"
-#include "qlevels.cuh"
-#include "shim.cuh"
+#include "kv8attn.cuh"
 #include "tcgen05.cuh"
 
 namespace dz {
 
 namespace cg = cooperative_groups;
 
-constexpr int KV8_TILE = 32;       // tokens that a warp takes at a time
-constexpr int KV8_CLUSTER = 16;    // blocks of a cluster at most
-constexpr int KV8_DEVICES = 64;    // devices whose launch state is kept
+
 __device__ __forceinline__ void kv8_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -76,15 +72,6 @@ __device__ __forceinline__ void kv8_imma(int (&d)[4], const uint32_t (&a)[4], ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 
-// A box of 32 tokens' codes of a page's head.
-__device__ __forceinline__ void kv8_copy(void* dst, const CUtensorMap* tm, int row, int page, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-            dz_smem_addr(dst)),
-        "l"(reinterpret_cast<uint64_t>(tm)), "r"(0), "r"(row), "r"(page), "r"(dz_smem_addr(bar))
-        : "memory");
-}
-
 // Four 8 x 8 matrices of 16-bit units from shared memory, lane l giving the
 // address of row l % 8 of matrix l / 8.
 __device__ __forceinline__ void kv8_matrices(uint32_t (&d)[4], uint32_t at) {
@@ -101,25 +88,6 @@ __device__ __forceinline__ void kv8_matrices_turned(uint32_t (&d)[4], uint32_t a
                  : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
                  : "r"(at)
                  : "memory");
-}
-
-// The codes in bytes 0 and 2 (1 and 3) of x as two fp16.
-template <bool ODD> __device__ __forceinline__ uint32_t kv8_widen(uint32_t x) {
-    uint32_t biased;             // (x & bytes) ^ base, 1024 + 128 + code; one instruction, both constants in registers
-    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(biased) : "r"(ODD ? x >> 8 : x), "r"(0x00ff00ffu), "r"(0x64806480u));
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&y);
-}
-
-__device__ __forceinline__ uint32_t kv8_half2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ float kv8_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 // Rows and columns of an 8 x 8 matrix of 16-bit values exchanged: lane 4 r + c held (r, 2c), (r, 2c + 1).
@@ -645,14 +613,6 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
     if (cluster > 1) cg::this_cluster().sync();      // no block ends while another reads its shared memory
 }
 
-// Clusters of 1..16 blocks of a kernel that a device holds at once (a cluster
-// stays within one GPC, so that larger ones leave SMs idle; 0: it cannot hold
-// one). Asked once per kernel and device.
-struct Kv8Room {
-    std::atomic<bool> known{false};
-    std::atomic<int> clusters[KV8_CLUSTER + 1];
-};
-
 // Warps of a team and blocks of a cluster for `units` units of up to `longest`
 // visible tokens: the least number of tiles that a warp works through one
 // after the other, its start (as long as 4 tiles) and the joins (3 each) among
@@ -715,20 +675,14 @@ static cudaError_t kv8_attn_t(const Kv8AttnArgs& a, long long longest, int devic
     attr[0].val.clusterDim.x = cluster;
     cfg.attrs = cluster > 1 ? attr : attr + 1;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    // code buffers as [pages][kv_heads page][HD]
     CUtensorMap maps[2];
-    const uint64_t rows = (uint64_t)a.c.kv_heads * a.c.page;
-    const uint64_t dims[3] = {HD, rows, (uint64_t)a.c.pages}, strides[2] = {HD, rows * HD};
-    const uint32_t box[3] = {HD, KV8_TILE, 1};
-    if (!dz_encode_u8_map(&maps[0], a.c.k_codes, 3, dims, strides, box) ||
-        !dz_encode_u8_map(&maps[1], a.c.v_codes, 3, dims, strides, box))
-        return cudaErrorInvalidValue;
+    if (!kv8_maps(a.c, HD, maps)) return cudaErrorInvalidValue;
     return cudaLaunchKernelEx(&cfg, kernel, a, maps[0], maps[1], team, cluster, blocks, (int)units);
 }
 
 template <typename T>
 static cudaError_t kv8_attn_h(const Kv8AttnArgs& a, long long longest, int head_dim, int device, cudaStream_t st) {
-    // few pairs in 8 columns, many in 16 (32 of them took 53 us for 128 pairs of heads of 64 where 16 took 52, 8 took 65)
+    // up to 8 pairs in 8 columns, more in 16
     const bool few = a.n_tokens * (a.q_heads / a.c.kv_heads) <= 8;
     if (head_dim == 128) return few ? kv8_attn_t<T, 128, 1>(a, longest, device, st) : kv8_attn_t<T, 128, 2>(a, longest, device, st);
     return few ? kv8_attn_t<T, 64, 1>(a, longest, device, st) : kv8_attn_t<T, 64, 2>(a, longest, device, st);
@@ -736,6 +690,9 @@ static cudaError_t kv8_attn_h(const Kv8AttnArgs& a, long long longest, int head_
 
 cudaError_t dz_kv8_attn_launch(const Kv8AttnArgs& a, long long longest, int type, int head_dim, int device, cudaStream_t st) {
     if (device < 0 || device >= KV8_DEVICES) return cudaErrorInvalidDevice;
+    // pairs of a key head: 128 in a block of kv8many.cu, 16 in a warp here (8 sequences of 4000 tokens, 4 key heads. Heads of 64
+    // in fp16: 64 pairs 31 and 26 us, 80 32 and 45, 320 66 and 123. Heads of 128 in bf16: 48 pairs 34 and 38, 128 37 and 70)
+    if (a.n_tokens * (a.q_heads / a.c.kv_heads) > (head_dim == 128 ? 32 : 64)) return dz_kv8_many_launch(a, longest, type, head_dim, device, st);
     if (type == DZ_TYPE_F32) return kv8_attn_h<float>(a, longest, head_dim, device, st);
     if (type == DZ_TYPE_F16) return kv8_attn_h<__half>(a, longest, head_dim, device, st);
     return kv8_attn_h<__nv_bfloat16>(a, longest, head_dim, device, st);

@@ -532,6 +532,104 @@ def test_attention_pages(gpu, kind):
             assert (out[15:] == 0).all()     # a window past the table
 
 
+MANY = [
+    # kind, page, heads, head dim, positions, tokens, window, pad, scale
+    ("f16", 64, (1, 1), 64, [0], 128, 0, 0, None),
+    ("bf16", 64, (2, 2), 128, [0, 37], 128, 0, 0, None),
+    ("f32", 32, (4, 1), 64, [3, 90], 33, 0, 0, None),
+    ("f16", 32, (4, 2), 128, [200], 65, 0, 3, None),
+    ("f32", 64, (8, 2), 128, [1000, 17, 640], 40, 0, 0, -0.2),
+    ("bf16", 32, (16, 1), 64, [700], 24, 130, 0, None),
+    ("f16", 64, (6, 3), 64, [2500, 1], 150, 31, 1, None),
+    ("f32", 32, (1, 1), 128, [0], 300, 0, 0, 0.0),
+    ("f16", 64, (64, 1), 64, [6000], 1, 0, 0, None),
+    ("bf16", 64, (32, 2), 128, [3000, 0, 9], 4, 5, 0, None),
+    ("f32", 64, (12, 1), 64, [1500], 64, 777, 0, None),
+]
+
+
+@pytest.mark.parametrize("kind,page,heads,hd,positions,tokens,window,pad,scale", MANY)
+def test_attention_of_many_queries(gpu, kind, page, heads, hd, positions, tokens, window, pad, scale):
+    """Blocks of 128 pairs, whole and ragged, of few tiles and of many, with and without a cluster."""
+    test_attention(gpu, kind, page, heads, hd, positions, tokens, window, pad, scale)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_pages_of_many_queries(gpu, kind):
+    """What test_attention_pages has, with 72 queries to a key head: shared pages, entries that name none, tokens past the table."""
+    rng = np.random.RandomState(18)
+    table = np.array([[0, 1, 2, 3, 4, 5], [0, 1, 3, -1, 6, 7], [-1, 4, -7, 2, 99, 5], [9, 10, 2 ** 31 - 1, -1, -1, -1],
+                      [5, 99, 6, 0, 1, 2], [0, 1, 2, 3, 4, 5], [6, 7, 0, 1, 2, 3]], np.int32)
+    positions, tokens, hq, hk, hd = [70, 90, 180, 60, 130, 300, -1], 9, 16, 2, 64
+    c = eb.Cache(rng, 8, 32, hk, hd, table)
+    d = Device(gpu, c)
+    qt, qv = _typed(rng.randn(7 * tokens, hq * hd), kind)
+    pos = _dev(np.array(positions, np.int64))
+    positions[6] = 0
+    for window in (0, 20, 100, 1 << 40):
+        out = _np(_attention(gpu, d, pos, tokens, kind, qt, hq, window)).reshape(-1, hq, hd)
+        y, bound = _attend_all(c, qv.reshape(-1, hq, hd), positions, tokens, 8, window, hd ** -0.5, kind)
+        err = np.abs(out - y) - 1.01 * eb.rounding(y, kind)
+        assert (err <= bound)[:6 * tokens].all()
+        assert (out[3 * tokens:4 * tokens] == 0).all() and (out[6 * tokens:] == 8.0).all()
+        if window in (20, 100):
+            assert (out[5 * tokens:6 * tokens] == 0).all()       # a window past the table
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("hd,page", [(64, 32), (128, 64)])
+def test_nan_of_many_queries(gpu, kind, hd, page):
+    """A NaN scale counts where a token of its page is seen, whatever its weight, and nowhere else; so do queries that are not finite."""
+    rng = np.random.RandomState(20)
+    share, tokens = 3, 2 * page
+    c = eb.Cache(rng, 24, page, 1, hd, np.arange(24).reshape(3, 8))
+    c.scales["v"][2] = np.nan                # sequence 0, tokens of its third page
+    c.scales["k"][8 + 3] = np.nan            # sequence 1, of its fourth
+    d = Device(gpu, c)
+    q = rng.randn(3 * tokens, share, hd)
+    q[2 * tokens + 2, 1, 3], q[2 * tokens + 5, 0, 60], q[2 * tokens + 6, 2, 7] = np.inf, np.nan, -np.inf
+    qt, _ = _typed(q.reshape(-1, share * hd), kind)
+    first = [page + 5, 2 * page + 1, page]
+    pos = _dev(np.array(first, np.int64))
+    for window in (0, page // 2):
+        out = _np(_attention(gpu, d, pos, tokens, kind, qt, share, window)).reshape(3, tokens, share, hd)
+        bad = np.isnan(out).all(-1)
+        assert (np.isnan(out).any(-1) == bad).all()
+        want = np.zeros(bad.shape, bool)
+        for b, at in ((0, 2), (1, 3)):
+            p = first[b] + np.arange(tokens)
+            want[b] = ((p >= at * page) & ((p - window + 1 < (at + 1) * page) if window else True))[:, None]
+        for t, h in ((2, 1), (5, 0), (6, 2)):
+            want[2, t, h] = True
+        np.testing.assert_array_equal(bad, want)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_small_beside_large_of_many_queries(gpu, kind):
+    """Elements, scales of either sign and weights beside much larger ones, in pages of 32 that share a thread's tokens."""
+    rng = np.random.RandomState(21)
+    hd, tokens = 64, 80
+    c = eb.Cache(rng, 16, 32, 1, hd, np.arange(16).reshape(2, 8))
+    c.scales["v"][2] *= 2.0 ** 12
+    c.scales["v"][5] *= -1
+    c.scales["v"][10] = 0
+    c.scales["k"][1] *= -0.5
+    c.scales["k"][12] *= 2.0 ** -20
+    c.scales["k"][13] = 0
+    d = Device(gpu, c)
+    q = rng.randn(2 * tokens, hd)
+    q[:40, :32] *= 2.0 ** -10
+    q[100:, 5] *= 100
+    if kind != "f16":
+        q[50:60] *= 2.0 ** -60
+    qt, qv = _typed(q, kind)
+    positions = [170, 100]
+    for scale in (0.1, -0.05):
+        out = _np(_attention(gpu, d, _dev(np.array(positions, np.int64)), tokens, kind, qt, 1, scale=scale)).reshape(-1, 1, hd)
+        y, bound = _attend_all(c, qv.reshape(-1, 1, hd), positions, tokens, 1, 0, float(np.float32(scale)), kind)
+        assert (np.abs(out - y) <= bound + 1.01 * eb.rounding(y, kind)).all()
+
+
 def test_attention_skips(gpu):
     rng = np.random.RandomState(9)
     c = eb.Cache(rng, 8, 32, 1, 128, [[0, 1], [2, 3], [4, 5]])
