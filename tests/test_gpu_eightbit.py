@@ -851,3 +851,45 @@ def test_captured_steps_on_two_streams(gpu):
         for name in ("h", "codes", "scales", "row", "q", "o", "y"):
             assert torch.equal(s[name], eager[name]), name
         assert torch.equal(d.k, d2.k) and torch.equal(d.v, d2.v) and torch.equal(d.ks, d2.ks) and torch.equal(d.vs, d2.vs)
+
+
+def test_products_and_many_queries_side_by_side(gpu):
+    """Kernels with tensor memory one after another on two streams: every turn gives what the first one gives."""
+    lanes = []
+    for seed in range(2):
+        rng = np.random.RandomState(40 + seed)
+        hd, hq, hk, tokens, page = (64, 8, 1, 16, 32) if seed else (128, 16, 2, 16, 64)
+        c = eb.Cache(rng, 40, page, hk, hd, np.arange(40).reshape(2, 20))
+        d = Device(gpu, c)
+        k, m = 256, 2 * tokens
+        w = [_quantized(gpu, rng.randint(-127, 128, (a, b)).astype(np.int8), np.full(b, 1e-4, np.float32))
+             for a, b in ((k, hq * hd), (hq * hd, k))]
+        lanes.append(dict(d=d, w=w, hq=hq, tokens=tokens, m=m, k=k, x=torch.randn(m, k, device="cuda").bfloat16(),
+                          codes=torch.empty(m, hq * hd, dtype=torch.int8, device="cuda"), scales=torch.empty(m, device="cuda"),
+                          q=torch.empty(m, hq * hd, dtype=torch.bfloat16, device="cuda"),
+                          o=torch.empty(m, hq * hd, dtype=torch.bfloat16, device="cuda"),
+                          pos=_dev(np.array([300, 500], np.int64)), stream=torch.cuda.Stream(), outs=[]))
+    torch.cuda.synchronize()
+
+    def turn(s):
+        st, t = s["stream"].cuda_stream, gpu.TYPE_BF16
+        y = torch.empty(s["m"], s["k"], dtype=torch.bfloat16, device="cuda")
+        width = s["hq"] * s["d"].cache.head_dim
+        gpu.norm_q8(s["m"], s["k"], type=t, x=s["x"].data_ptr(), codes=s["codes"].data_ptr(), scales=s["scales"].data_ptr(), stream_ptr=st)
+        s["w"][0].matmul_q8_async(s["codes"].data_ptr(), s["scales"].data_ptr(), s["q"].data_ptr(), s["m"], st, type=t)
+        s["d"].cache.attention(s["pos"].data_ptr(), s["tokens"], type=t, q_heads=s["hq"], q=s["q"].data_ptr(), out=s["o"].data_ptr(),
+                               stream_ptr=st)
+        gpu.norm_q8(s["m"], width, type=t, x=s["o"].data_ptr(), norm=False, codes=s["codes"].data_ptr(),
+                    scales=s["scales"].data_ptr(), stream_ptr=st)
+        s["w"][1].matmul_q8_async(s["codes"].data_ptr(), s["scales"].data_ptr(), y.data_ptr(), s["m"], st, type=t)
+        s["outs"].append(y)
+    for _ in range(40):
+        for s in lanes:
+            with torch.cuda.stream(s["stream"]):
+                turn(s)
+    torch.cuda.synchronize()
+    for s in lanes:
+        assert bool(s["outs"][0].isfinite().all()) and float(s["outs"][0].abs().max()) > 0
+        assert all(torch.equal(s["outs"][0], y) for y in s["outs"])
+        for w in s["w"]:
+            w.close()
