@@ -24,8 +24,9 @@
 // and fp32 ones times a power of two of their row (its largest element in [2^13,
 // 2^14)), fp32 ones in two parts. Codes become fp16 exactly, two at a time, by
 // setting the exponent of 1024 above the byte and subtracting 1024 + 128; values
-// always do, and weights are taken times 2^15 in two fp16 parts, in one for bf16,
-// whose outputs' steps are eight times as coarse (6% of a tile's instructions). Scores of a tile
+// always do, and weights are taken times 2^15 in two fp16 parts (22 bits of each;
+// one part alone, 11 bits, would save 6% of a tile's instructions and show in
+// bf16 outputs where values of both signs cancel). Scores of a tile
 // take the page's key scale, the sums of a tile its value scale, both in fp32.
 //
 // Few units of long contexts go to clusters of blocks, many to a warp each
@@ -118,7 +119,6 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
     constexpr int PAIRS = B::PAIRS, WARPS = B::WARPS, SLOTS = B::SLOTS;
     constexpr bool DIGITS = NT == 1;
     constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1;      // fp16 parts of a query's element
-    constexpr bool WHOLE = !std::is_same<T, __nv_bfloat16>::value;    // weights in two parts
     constexpr int TILES = HD / 16;           // sum MMAs over a head's elements
     extern __shared__ __align__(1024) uint8_t kv8_raw[];
     uint8_t* sm = kv8_raw + ((1024u - (dz_smem_addr(kv8_raw) & 1023u)) & 1023u);
@@ -480,10 +480,8 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
                     for (int j = 0; j < 2; j++) {
                         const uint32_t hi = kv8_half2(s[i][n][2 * j], s[i][n][2 * j + 1]);
                         wh[i][n][j] = kv8_turn(hi);
-                        if (WHOLE) {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                            wl[i][n][j] = kv8_turn(kv8_half2(s[i][n][2 * j] - f.x, s[i][n][2 * j + 1] - f.y));
-                        }
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                        wl[i][n][j] = kv8_turn(kv8_half2(s[i][n][2 * j] - f.x, s[i][n][2 * j + 1] - f.y));
                     }
             const int slot_v = slot + 1 == SLOTS ? 0 : slot + 1;
             if (!arrived(slot_v)) ok = false;
@@ -509,7 +507,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
                             kv8_mma_first(part[n], va, wh[st][n][0], wh[st][n][1]);
                         else
                             kv8_mma(part[n], va, wh[st][n][0], wh[st][n][1]);
-                        if (WHOLE) kv8_mma(part[n], va, wl[st][n][0], wl[st][n][1]);
+                        kv8_mma(part[n], va, wl[st][n][0], wl[st][n][1]);
                     }
                 }
 #pragma unroll

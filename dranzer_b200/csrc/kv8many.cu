@@ -22,7 +22,7 @@
 //
 // Queries are fp16 times a power of two of their row (its largest element in
 // [2^13, 2^14)), fp32 ones in two parts; codes are fp16 exactly; weights are taken
-// times 2^15 in two fp16 parts, in one for bf16. The pages' key scales meet the
+// times 2^15 in two fp16 parts. The pages' key scales meet the
 // scores in fp32. Where two pages of 32 tokens share a thread's 64, the weights
 // take their value scales over the larger one, which the tile's sums take in fp32.
 #include <cooperative_groups.h>
@@ -43,7 +43,6 @@ constexpr int KV8M_CHUNKS = KV8M_KEYS / KV8_TILE;
 
 template <typename T, int HD> struct Kv8Many {
     static constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1;      // fp16 parts of a query's element
-    static constexpr bool WHOLE = !std::is_same<T, __nv_bfloat16>::value;    // weights in two parts
     static constexpr int PANEL = 128 * 128;                // 128 rows of 64 fp16, 128-byte swizzle
     static constexpr int PANELS = HD / 64;
     static constexpr int BOX = KV8_TILE * HD;              // codes of 32 tokens
@@ -389,13 +388,11 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
                             if (scaled.value) w[k] *= ratio;
                         }
                         hw[j / 2] = kv8_half2(w[0], w[1]);
-                        if (B::WHOLE) {
-                            const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&hw[j / 2]));
-                            lw[j / 2] = kv8_half2(w[0] - u.x, w[1] - u.y);
-                        }
+                        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&hw[j / 2]));
+                        lw[j / 2] = kv8_half2(w[0] - u.x, w[1] - u.y);
                     }
                     kv8m_store8(scores + (uint32_t)(c * KV8_TILE + n), hw);
-                    if (B::WHOLE) kv8m_store8(scores + (uint32_t)(c * KV8_TILE + n + 8), lw);
+                    kv8m_store8(scores + (uint32_t)(c * KV8_TILE + n + 8), lw);
                 }
             };
 #pragma unroll
@@ -421,7 +418,7 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
             const uint64_t v = kv8m_desc_values(dz_smem_addr(sm + B::WIDE + B::PANELS * B::PANEL + half * 64 * 128), B::PANEL);
             if (ug_elect()) {
 #pragma unroll
-                for (int part = 0; part < (B::WHOLE ? 2 : 1); part++)
+                for (int part = 0; part < 2; part++)
 #pragma unroll
                     for (int kk = 0; kk < 4; kk++)
                         kv8m_mma_tmem(tmem + (uint32_t)(128 + HD * half), tmem + (uint32_t)(64 * half + kk * 16 + part * 8),
