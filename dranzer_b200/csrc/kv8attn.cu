@@ -437,7 +437,8 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
                         seen[n][e] |= any;
                     }
             }
-            float shrink[NT][2];
+            float shrink[NT][2], less[NT][2];
+            bool far = false;
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -447,19 +448,32 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                     m = fmaxf(top[n][e], m * f[n][e]);
-                    const float less = 15.0f - (m == -INFINITY ? 0.0f : m);      // weights times 2^15
                     shrink[n][e] = top[n][e] == m ? 1.0f : kv8_exp2(top[n][e] - m);
                     top[n][e] = m;
-                    float w = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            s[i][n][2 * j + e] = kv8_exp2(fmaf(s[i][n][2 * j + e], f[n][e], less));
-                            w += s[i][n][2 * j + e];
-                        }
-                    sum[n][e] = fmaf(sum[n][e], shrink[n][e], w);
+                    if (m == -INFINITY) m = 0.0f;
+                    less[n][e] = 15.0f - m;                      // weights times 2^15
+                    far |= fabsf(m) >= KV8_FAR;
                 }
+            auto weigh = [&](auto power) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float w = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+#pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                s[i][n][2 * j + e] = kv8_exp2(power(s[i][n][2 * j + e], n, e));
+                                w += s[i][n][2 * j + e];
+                            }
+                        sum[n][e] = fmaf(sum[n][e], shrink[n][e], w);
+                    }
+            };
+            if (__any_sync(0xffffffffu, far))
+                weigh([&](float x, int n, int e) { return kv8_far_power(x, f[n][e], top[n][e]); });
+            else
+                weigh([&](float x, int n, int e) { return fmaf(x, f[n][e], less[n][e]); });
             // every tile: a branch for those whose maximum grew costs as many moves
 #pragma unroll
             for (int i = 0; i < TILES; i++)

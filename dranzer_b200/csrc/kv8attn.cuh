@@ -42,6 +42,16 @@ __device__ __forceinline__ float kv8_exp2(float x) {
     return y;
 }
 
+// A weight is 2^15 times 2 to the power of its score x f less the largest one m.
+// fma(x, f, 15 - m) does not round x f as m was, and rounds 15 - m: the largest
+// weight is then off by as much as m's steps, half of one from 2^16 on 2^-8 and
+// from 2^24 on 1, where it leaves fp16. From KV8_FAR on scores are rounded first,
+// so that the largest weight is 2^15 exactly.
+constexpr float KV8_FAR = 65536.0f;
+__device__ __forceinline__ float kv8_far_power(float x, float f, float m) {
+    return __fadd_rn(__fadd_rn(__fmul_rn(x, f), m == -INFINITY ? 0.0f : -m), 15.0f);
+}
+
 // Clusters of 1..16 blocks of a kernel that a device holds at once (a cluster
 // stays within one GPC, so that larger ones leave SMs idle; 0: it cannot hold
 // one). Asked once per kernel and device.

@@ -41,3 +41,56 @@ def test_weights_keep_22_bits(gpu, kind, hd, hq, tokens):
     whole = (position + np.arange(tokens)) % 3 == 2                  # rows that see whole triples
     assert (np.abs(y[whole]) < 2.0 ** -11 * 1.3).all() and (bound[whole] < 2.0 ** -14).all()
     assert (np.abs(out - y) <= bound + 1.01 * eb.rounding(y, kind)).all()
+
+
+def _one_hot(c, q, table, positions, tokens, window, scale):
+    """Rows whose scores lie so far apart that only the tokens of the largest one weigh: the mean of their values
+    [rows, heads, hd], and the bound of its evaluation (eb.attend's without the scores', and a weight that is a power of two)."""
+    batch, hd = len(positions), q.shape[-1]
+    y, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(batch):
+        (k, there), (v, _) = (c.values(n, b, 0, positions[b] + tokens, 0) for n in "kv")
+        for t in range(tokens):
+            i = positions[b] + t
+            see = there & (np.arange(len(there)) <= i)
+            if window:
+                see &= np.arange(len(there)) > i - window
+            for h in range(q.shape[1]):
+                s = scale * (k @ q[b * tokens + t, h])
+                best = s == s[see].max()
+                best &= see
+                rest = s[see & ~best]
+                assert not rest.size or s[best].max() - rest.max() > 2.0 ** -17 * np.abs(s[see]).max() + 100
+                y[b * tokens + t, h] = v[best].mean(0)
+                bound[b * tokens + t, h] = (2.0 ** -20 + (see.sum() / 32 * 6 + 128) * 2 * eb.U) * np.abs(v[best]).mean(0)
+    return y, bound
+
+
+def _far_scores(gpu, kind, hd, hq, tokens, size, page=32):
+    """Scores of about +-size, by one element of the query and codes 20..120 of the keys, some of them twice."""
+    rng = np.random.RandomState(hd + hq)
+    per = (200 + tokens) // page + 1
+    c = eb.Cache(rng, 2 * per, page, 1, hd, np.arange(2 * per).reshape(2, per))
+    c.codes["k"][:] = 0
+    c.codes["k"][:, :, :, 3] = rng.randint(20, 121, (2 * per, 1, page))
+    c.scales["k"][:] = np.float32(0.0123)    # of one size: a page's scale does not part equal codes
+    d = Device(gpu, c)
+    q = np.zeros((2 * tokens, hq, hd))
+    q[:, :, 3] = np.exp(rng.uniform(-0.3, 0.3, (2 * tokens, hq))) * rng.choice([-1, 1], (2 * tokens, hq))
+    qt, qv = _typed(q.reshape(2 * tokens, -1), kind)
+    scale = float(np.float32(size / 1.2))
+    positions = [150, 200 - tokens]
+    qv = qv.reshape(-1, hq, hd)
+    for window in (0, 70):
+        out = _np(_attention(gpu, d, _dev(np.array(positions, np.int64)), tokens, kind, qt, hq, window, scale)).reshape(-1, hq, hd)
+        y, bound = _one_hot(c, qv, c.table, positions, tokens, window, scale)
+        assert (np.abs(out - y) <= bound + 1.01 * eb.rounding(y, kind)).all()
+
+
+@pytest.mark.parametrize("hq,tokens", [(1, 1), (4, 2), (4, 4), (3, 10)])
+@pytest.mark.parametrize("size", [2.0 ** 14, 2.0 ** 17, 2.0 ** 24, 2.0 ** 26, 2.0 ** 33, 2.0 ** 41])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_scores_far_from_0(gpu, kind, hd, size, hq, tokens):
+    """The largest score's tokens weigh alone, whatever the scores' steps in fp32 are."""
+    _far_scores(gpu, kind, hd, hq, tokens, size)
