@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
             vt = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
             float total[2] = {0.0f, 0.0f};
             // weights of a box, 16 tokens at a time, in the place of their scores: parts of 8 columns each
-            auto weigh = [&](auto looks, auto scaled, int c, float ratio) {
+            auto weigh = [&](auto looks, auto scaled, auto far, int c, float ratio) {
 #pragma unroll
                 for (int n = 0; n < KV8_TILE; n += 16) {
                     float s[16];
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
                             const int at = n + j + k;
                             float x = s[j + k];
                             if (looks.value) x = at >= lo[c] && at <= hi[c] ? __uint_as_float(__float_as_uint(x) ^ sign[c]) : -INFINITY;
-                            w[k] = kv8_exp2(fmaf(x, f[c], less));
+                            w[k] = kv8_exp2(far.value ? kv8_far_power(x, f[c], m) : fmaf(x, f[c], less));
                             total[k] += w[k];
                             if (scaled.value) w[k] *= ratio;
                         }
@@ -398,12 +398,14 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 const float ratio = vs[c] == vt ? 1.0f : __fdiv_rn(vs[c], vt);
-                if (!__all_sync(0xffffffffu, plain[c]))
-                    weigh(std::true_type(), std::true_type(), c, ratio);
+                if (__any_sync(0xffffffffu, fabsf(less) >= KV8_FAR))
+                    weigh(std::true_type(), std::true_type(), std::true_type(), c, ratio);
+                else if (!__all_sync(0xffffffffu, plain[c]))
+                    weigh(std::true_type(), std::true_type(), std::false_type(), c, ratio);
                 else if (!__all_sync(0xffffffffu, ratio == 1.0f))
-                    weigh(std::false_type(), std::true_type(), c, ratio);
+                    weigh(std::false_type(), std::true_type(), std::false_type(), c, ratio);
                 else
-                    weigh(std::false_type(), std::false_type(), c, ratio);
+                    weigh(std::false_type(), std::false_type(), std::false_type(), c, ratio);
             }
             sum = fmaf(sum, shrink, total[0] + total[1]);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");

@@ -94,3 +94,11 @@ def _far_scores(gpu, kind, hd, hq, tokens, size, page=32):
 def test_scores_far_from_0(gpu, kind, hd, size, hq, tokens):
     """The largest score's tokens weigh alone, whatever the scores' steps in fp32 are."""
     _far_scores(gpu, kind, hd, hq, tokens, size)
+
+
+@pytest.mark.parametrize("hq,tokens,page", [(2, 70, 32), (8, 20, 64), (3, 45, 64)])
+@pytest.mark.parametrize("size", [2.0 ** 14, 2.0 ** 17, 2.0 ** 24, 2.0 ** 26, 2.0 ** 33, 2.0 ** 41])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_scores_far_from_0_of_many_queries(gpu, kind, hd, size, hq, tokens, page):
+    _far_scores(gpu, kind, hd, hq, tokens, size, page)
