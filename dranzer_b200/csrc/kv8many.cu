@@ -279,6 +279,7 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
 #pragma unroll
     for (int i = 0; i < HD; i++) o[i] = 0.0f;
     float top = -INFINITY, sum = 0.0f;
+    bool seen = false;                       // any token, whatever its score
     ug_fence_after();
     const uint32_t tmem = *tmem_slot;
     const float factor = factors[r];
@@ -350,6 +351,7 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
                 ug_tmem_ld32(scores + (uint32_t)(c * 32), raw);
                 float most[2] = {-INFINITY, -INFINITY};
                 if (plain[c]) {
+                    seen = true;
 #pragma unroll
                     for (int j = 0; j < 32; j++) most[j & 1] = fmaxf(most[j & 1], __int_as_float(raw[j]));
                 } else {
@@ -359,6 +361,8 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
                     if (max(lo[c], 0) > min(hi[c], KV8_TILE - 1)) {          // nothing, whatever the scales are
                         f[c] = 1.17549435e-38f;
                         vs[c] = 0.0f;
+                    } else {
+                        seen = true;
                     }
                 }
                 m = fmaxf(m, fmaxf(most[0], most[1]) * f[c]);
@@ -467,7 +471,8 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
 #pragma unroll
     for (int c = 0; c < HD / 4; c++)
         join[(half * KV8M_PAIRS + r) * (HD / 4) + (c ^ (r & 7))] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-    stats[half * KV8M_PAIRS + r] = make_float2(top, sum);
+    // scores that all left fp32 at -inf: no weight, but not a pair that saw nothing
+    stats[half * KV8M_PAIRS + r] = make_float2(top, seen && sum == 0.0f ? 1.0f : sum);
     if (cluster > 1)
         cg::this_cluster().sync();
     else
@@ -479,6 +484,7 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
         for (int x = rank * KV8M_THREADS + (int)threadIdx.x; x < rows * (HD / 4); x += cluster * KV8M_THREADS) {
             const int row = x / (HD / 4), d = x % (HD / 4);
             float m = -INFINITY, total = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            bool any = false;
             for (int p0 = 0; p0 < 2 * cluster; p0 += AT_ONCE) {
                 float2 st[AT_ONCE];
                 float4 v[AT_ONCE];
@@ -505,6 +511,7 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
                     const float f = st[p].x == -INFINITY ? 0.0f : st[p].x == m ? 1.0f : kv8_exp2(st[p].x - m);
                     // a part that weighs nothing may still hold a NaN, which counts; one that saw nothing is all 0
                     total = fmaf(st[p].y, f, total);
+                    any |= st[p].y != 0.0f;
                     y[0] = fmaf(v[p].x, f, y[0]);
                     y[1] = fmaf(v[p].y, f, y[1]);
                     y[2] = fmaf(v[p].z, f, y[2]);
@@ -513,9 +520,8 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
             }
             const int pair = r0 + row;
             T* out = static_cast<T*>(a.out) + ((long long)b * a.n_tokens + pair / share) * a.ldo + (h * share + pair % share) * HD + 4 * d;
-            // the largest weight is 2^15: nothing was seen where they add up to 0
 #pragma unroll
-            for (int e = 0; e < 4; e++) out[e] = dz_from_float<T>(total == 0.0f ? 0.0f : y[e] / total);
+            for (int e = 0; e < 4; e++) out[e] = dz_from_float<T>(any ? y[e] / total : 0.0f);
         }
     };
     if (cluster > 1)

@@ -102,3 +102,27 @@ def test_scores_far_from_0(gpu, kind, hd, size, hq, tokens):
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_scores_far_from_0_of_many_queries(gpu, kind, hd, size, hq, tokens, page):
     _far_scores(gpu, kind, hd, hq, tokens, size, page)
+
+
+@pytest.mark.parametrize("hq,tokens", PAIRS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_scores_past_fp32(gpu, kind, hd, hq, tokens):
+    """A query whose every score is -inf in fp32 reads NaN, as the formula gives it; beside finite ones they weigh nothing;
+    a query that sees nothing reads 0."""
+    page, per = 32, 12
+    c = eb.Cache(np.random.RandomState(hd), 2 * per, page, 1, hd, np.arange(2 * per).reshape(2, per))
+    c.codes["k"][:] = 7
+    c.scales["k"][:] = np.float32(1e30)
+    c.scales["k"][per + 5] = np.float32(1e-30)                   # sequence 1, tokens 160..191: finite
+    table = np.concatenate([c.table, np.full((1, per), -1, np.int32)])
+    c.table = table                          # sequence 2: no page
+    d = Device(gpu, c)
+    q = np.full((3 * tokens, hq, hd), -1e30)
+    qt, _ = _typed(q.reshape(3 * tokens, -1), kind)
+    first = per * page - tokens
+    out = _np(_attention(gpu, d, _dev(np.array([first] * 3, np.int64)), tokens, kind, qt, hq)).reshape(3, tokens, hq, hd)
+    assert np.isnan(out[0]).all() and (out[2] == 0).all()
+    y = c.values("v", 1, 160, 192, 0)[0].mean(0)                 # all 32 scores are alike
+    bound = (2.0 ** -20 + (per + 128) * 2 * eb.U) * np.abs(c.values("v", 1, 160, 192, 0)[0]).mean(0)
+    assert (np.abs(out[1] - y) <= bound + 1.01 * eb.rounding(y, kind)).all()
