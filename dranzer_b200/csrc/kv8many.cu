@@ -23,8 +23,10 @@
 // Queries are fp16 times a power of two of their row (its largest element in
 // [2^13, 2^14)), fp32 ones in two parts; codes are fp16 exactly; weights are taken
 // times 2^15 in two fp16 parts. The pages' key scales meet the
-// scores in fp32. Where two pages of 32 tokens share a thread's 64, the weights
-// take their value scales over the larger one, which the tile's sums take in fp32.
+// scores in fp32. Where two pages of different value scales share a thread's 64
+// tokens, the weights take these over one scale, which the tile's sums take in
+// fp32: that of the page whose largest weight x scale is larger, times that
+// weight, so that what counts keeps its bits whatever the scales are.
 #include <cooperative_groups.h>
 #include <type_traits>
 
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
             if (!dz_mbar_wait(scores_bar, (uint32_t)(i & 1))) ok = false;
             ug_fence_after();
             const int p0 = (start + (rank + i * cluster) * KV8M_CHUNKS) * KV8_TILE + 64 * half;
-            float f[2], m = top;
+            float f[2], box[2], m = top;         // box: each one's largest score
             // a box that every pair sees whole, of scales that leave the scores' order, needs no look at its tokens
             bool plain[2];
             int lo[2], hi[2];                // what this pair sees of it; a page that is not there: nothing
@@ -365,12 +367,21 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
                         seen = true;
                     }
                 }
-                m = fmaxf(m, fmaxf(most[0], most[1]) * f[c]);
+                box[c] = fmaxf(most[0], most[1]) * f[c];
+                m = fmaxf(m, box[c]);
             }
             const float less = 15.0f - (m == -INFINITY ? 0.0f : m);          // weights times 2^15
             shrink = top == m ? 1.0f : kv8_exp2(top - m);
             top = m;
+            // the scale that the tile's sums take: where the boxes' differ, the one that the largest weight x scale sets (no
+            // smaller than 2^-100 of the larger scale, so that quotients stay in range)
             vt = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
+            if (fabsf(vs[0]) != fabsf(vs[1]) && fminf(fabsf(vs[0]), fabsf(vs[1])) > 0.0f) {
+                float most = vt * 0x1p-100f;
+#pragma unroll
+                for (int c = 0; c < 2; c++) most = fmaxf(most, box[c] == -INFINITY ? 0.0f : fabsf(vs[c]) * kv8_exp2(box[c] - m));
+                if (most > 0.0f) vt = most;
+            }
             float total[2] = {0.0f, 0.0f};
             // weights of a box, 16 tokens at a time, in the place of their scores: parts of 8 columns each
             auto weigh = [&](auto looks, auto scaled, auto far, int c, float ratio) {

@@ -211,10 +211,12 @@ int dz_cuda_kv8_append(const dz_kv8_t *cache, const dz_kv8_append_t *args, const
  * the query at position i sees position p <= i where the table names a page,
  * and with a window p > i - window. A query that sees nothing reads 0. Scores,
  * softmax statistics and sums are fp32. A query's element is held to 2^-22 of
- * itself or to 2^-30 of the largest of its head, a softmax weight (with more than
- * 32 queries of a key head: times its value's scale) to 2^-22 of itself or 2^-39
- * of the largest. A token that is seen makes a NaN of its output where its
- * page's scale is one, whatever its weight. out must not overlap q or the cache. */
+ * itself or to 2^-30 of the largest of its head, a softmax weight to 2^-22 of
+ * itself or 2^-39 of the largest (with more than 32 queries of a key head and
+ * pages of different value scales, or its product with its value's scale to
+ * 2^-39 of the largest one). A token that is seen makes a NaN of its output where
+ * its page's scale is one, whatever its weight. out must not overlap q or the
+ * cache. */
 int dz_cuda_kv8_attention(const dz_kv8_t *cache, const dz_kv8_attention_t *args, const int64_t *positions,
                           size_t n_tokens, void *stream);
 

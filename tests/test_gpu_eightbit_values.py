@@ -126,3 +126,47 @@ def test_scores_past_fp32(gpu, kind, hd, hq, tokens):
     y = c.values("v", 1, 160, 192, 0)[0].mean(0)                 # all 32 scores are alike
     bound = (2.0 ** -20 + (per + 128) * 2 * eb.U) * np.abs(c.values("v", 1, 160, 192, 0)[0]).mean(0)
     assert (np.abs(out[1] - y) <= bound + 1.01 * eb.rounding(y, kind)).all()
+
+
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 30, 2.0 ** 60, 2.0 ** 120])
+@pytest.mark.parametrize("hq,tokens,hd", [(4, 4, 64), (8, 17, 64), (2, 90, 128)])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_weights_on_pages_of_small_scales(gpu, kind, hq, tokens, hd, size):
+    """The softmax sits on pages whose neighbours' values are `size` times as large and weigh nothing: every weight keeps its
+    bits. The bound is eb.attend's with the largest weight x value in place of the largest value."""
+    rng = np.random.RandomState(hd)
+    page, per = 32, 7
+    c = eb.Cache(rng, 2 * per, page, 1, hd, np.arange(2 * per).reshape(2, per))
+    c.codes["k"][:, :, :, 0] = 100
+    c.scales["k"][:] = np.float32(0.01)
+    for b in range(2):                       # every second page, from the first or the second on
+        for j in range(b, per, 2):
+            c.codes["k"][b * per + j, :, :, 0] = -100
+            c.scales["v"][b * per + j] *= size * 2.0 ** -40
+    for at in range(2 * per):
+        if (at % per - at // per) % 2:
+            c.scales["v"][at] *= 2.0 ** -40
+    d = Device(gpu, c)
+    q = 0.05 * rng.randn(2 * tokens, hq, hd)
+    q[:, :, 0] = 30
+    qt, qv = _typed(q.reshape(2 * tokens, -1), kind)
+    positions = [190 - tokens, 200 - tokens]
+    scale = float(np.float32(4.0))           # the others' scores lie 240 below: weights of 2^-346
+    out = _np(_attention(gpu, d, _dev(np.array(positions, np.int64)), tokens, kind, qt, hq, scale=scale)).reshape(-1, hq, hd)
+    qv = qv.reshape(-1, hq, hd)
+    seen = 0
+    for b in range(2):
+        k, v = (c.values(n, b, 0, positions[b] + tokens, 0)[0] for n in "kv")
+        for t in range(tokens):
+            n = positions[b] + t + 1
+            for h in range(hq):
+                s = scale * (k[:n] @ qv[b * tokens + t, h])
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                assert p[k[:n, 0] < 0].sum() < 1e-80
+                small = k[:n, 0] > 0
+                y, bound = eb.attend(qv[b * tokens + t, h], k[:n][small], v[:n][small], scale, "f32")
+                o = out[b * tokens + t, h]
+                assert (np.abs(o - y) <= bound + 1.01 * eb.rounding(y, kind)).all()
+                seen += 1
+    assert seen == 2 * tokens * hq
