@@ -673,7 +673,11 @@ DZ_KERNEL_LINKAGE __global__ void __launch_bounds__(UG_THREADS, 1)
       __syncwarp();   // the warp reconverges before the block barriers below
     } else if (warp == 1) {
       if (lane == 0) {
-        // MMA issuer: 3 limbs x 4 k-steps of 32 per stage
+        // MMA issuer: 3 limbs x 4 k-steps of 32 per stage. Barrier waits are
+        // bounded, the kernels before this one are not (one that lets the
+        // split launch early may run for seconds): none begins before they
+        // have ended
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         int kb = 0;
         const uint32_t idesc = ug_idesc();
         for (; kb < nkb; kb++) {
@@ -715,9 +719,10 @@ DZ_KERNEL_LINKAGE __global__ void __launch_bounds__(UG_THREADS, 1)
         // barrier completes): fp32 [128][UG_TILE_LD], or with split-K the
         // int64 totals [128][UG_PART_LD] (exact, so the parts add in any order)
         const int ew = warp - 4;
+        // the split's exponents (and epilogue inputs); ahead of the bounded wait, as above
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         bool ok = dz_mbar_wait(accum, 0);
         ug_fence_after();
-        asm volatile("griddepcontrol.wait;" ::: "memory");   // the split's exponents (and epilogue inputs)
         const int rl = ew * 32 + lane;
         const int row = m0 + rl;
         const uint32_t lane_base = (uint32_t)(ew * 32) << 16;
@@ -1077,6 +1082,7 @@ DZ_KERNEL_LINKAGE __global__ void __launch_bounds__(UG_THREADS, 1)
         __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");   // before the bounded waits, as in dz_ugemm_kernel
             const uint32_t idesc = uv_idesc();
             int i = 0, t = 0;   // stage counter, segment counter
             bool stop = false;

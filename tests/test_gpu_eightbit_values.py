@@ -2,9 +2,10 @@
 weights that nearly cancel, scores, scales and values far from 1."""
 import numpy as np
 import pytest
+import torch
 
 import _eightbit as eb
-from test_gpu_eightbit import TYPES, Device, _attend_all, _attention, _dev, _np, _typed
+from test_gpu_eightbit import TYPES, Device, _attend_all, _attention, _dev, _np, _quantized, _stream, _typed
 
 pytestmark = pytest.mark.gpu
 
@@ -170,3 +171,27 @@ def test_weights_on_pages_of_small_scales(gpu, kind, hq, tokens, hd, size):
                 assert (np.abs(o - y) <= bound + 1.01 * eb.rounding(y, kind)).all()
                 seen += 1
     assert seen == 2 * tokens * hq
+
+
+@pytest.mark.parametrize("m,k,n", [(40, 1024, 1100), (8, 1024, 1100), (40, 4096, 300)])
+def test_fp32_products_on_the_tensor_cores_after_a_long_row(gpu, m, k, n):
+    """The kernels of fp32 products whose waits are bounded (matrices of 2^20 codes and more: the GEMM with and without parts
+    of k, the GEMV) wait without limit behind the longest row, which lets them start early: no NaN, and nothing left for the
+    matrix's next call."""
+    assert k * n >= 1 << 20
+    width = 1 << 30
+    x = torch.ones(width, device="cuda")
+    out, scale = torch.empty(width, dtype=torch.int8, device="cuda"), torch.empty(1, device="cuda")
+    levels = np.random.RandomState(m).randint(-127, 128, (k, n)).astype(np.int8)
+    w = _quantized(gpu, levels, np.ones(n, np.float32))
+    ones, y = torch.ones(m, k, device="cuda"), torch.zeros(m, n, device="cuda")
+    for turn in range(2):                    # the first call of a kernel waits for what is under way
+        torch.cuda.synchronize()
+        y.zero_()
+        gpu.norm_q8(1, width if turn else 1000000, type=gpu.TYPE_F32, x=x.data_ptr(), residual=x.data_ptr(),
+                    gain=x.data_ptr(), codes=out.data_ptr(), scales=scale.data_ptr(), stream_ptr=_stream())
+        w.matmul_async(ones.data_ptr(), y.data_ptr(), m, _stream())
+    want = levels.sum(0, dtype=np.int64).astype(np.float32)
+    assert torch.equal(y, _dev(want).expand(m, n))
+    np.testing.assert_array_equal(w.matmul(np.ones((m, k), np.float32)), np.broadcast_to(want, (m, n)))
+    w.close()
