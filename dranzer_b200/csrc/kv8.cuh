@@ -6,8 +6,8 @@
 
 namespace dz {
 
-// Positions that a table reaches at most: attention counts them in 32 bits, up
-// to two tiles past the end.
+// Positions that a table reaches at most: attention counts them in 32 bits, tiles
+// of 32 tokens with a sign, those of 128, which may pass the end, without.
 constexpr long long KV8_REACH = INT32_MAX - 63;
 
 struct Kv8Cache {

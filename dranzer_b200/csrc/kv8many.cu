@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
         if (busy) {
             if (!dz_mbar_wait(scores_bar, (uint32_t)(i & 1))) ok = false;
             ug_fence_after();
-            const int p0 = (start + (rank + i * cluster) * KV8M_CHUNKS) * KV8_TILE + 64 * half;
+            // without a sign: a tile may pass the end of the longest table
+            const unsigned p0 = (unsigned)(start + (rank + i * cluster) * KV8M_CHUNKS) * KV8_TILE + 64u * half;
             float f[2], box[2], m = top;         // box: each one's largest score
             // a box that every pair sees whole, of scales that leave the scores' order, needs no look at its tokens
             bool plain[2];
@@ -342,11 +343,11 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
             unsigned sign[2];                // scores are f times the dot products, f > 0: signs turned where the scales' differ
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                const int p = p0 + c * KV8_TILE;
+                const unsigned p = p0 + c * KV8_TILE;
                 sign[c] = (ks[c] < 0.0f) != (a.scale < 0.0f) ? 0x80000000u : 0u;
-                plain[c] = page[c] >= 0 && p + KV8_TILE - 1 <= high_all && p >= low_all && !sign[c];
-                lo[c] = page[c] >= 0 ? low - p : KV8_TILE;
-                hi[c] = page[c] >= 0 ? high - p : -1;
+                plain[c] = page[c] >= 0 && p + KV8_TILE - 1 <= (unsigned)high_all && p >= (unsigned)low_all && !sign[c];
+                lo[c] = page[c] >= 0 ? (int)((unsigned)low - p) : KV8_TILE;
+                hi[c] = page[c] >= 0 ? (int)((unsigned)high - p) : -1;
                 f[c] = fabsf(ks[c] * factor);
                 f[c] = f[c] == 0.0f ? 1.17549435e-38f : f[c];                // hidden tokens stay at -inf
                 int32_t raw[32];

@@ -195,3 +195,29 @@ def test_fp32_products_on_the_tensor_cores_after_a_long_row(gpu, m, k, n):
     assert torch.equal(y, _dev(want).expand(m, n))
     np.testing.assert_array_equal(w.matmul(np.ones((m, k), np.float32)), np.broadcast_to(want, (m, n)))
     w.close()
+
+
+@pytest.mark.parametrize("hq,tokens,windows", [(1, 1, (0, 333)), (4, 4, (0, 65)), (8, 40, (1, 100, 300))])
+@pytest.mark.parametrize("page", [32, 64])
+def test_the_end_of_the_longest_table(gpu, page, hq, tokens, windows):
+    """Append and attention at the last positions that a table can reach, and past them."""
+    rng = np.random.RandomState(page)
+    hd, per = 64, ((1 << 31) - 64) // page
+    table = np.full((1, per), -1, np.int32)
+    table[0, -12:] = rng.permutation(13)[:12]
+    c = eb.Cache(rng, 13, page, 1, hd, table)
+    d = Device(gpu, c)
+    for first in (per * page - tokens, per * page - 30):         # up to the end; some tokens past it, where they are many
+        x = rng.randn(tokens, 1, hd).astype(np.float32)
+        xt, pos = _dev(x), _dev(np.array([first], np.int64))
+        d.cache.append(pos.data_ptr(), tokens, k=xt.data_ptr(), v=xt.data_ptr(), stream_ptr=_stream())
+        for n, codes, scales in (("k", d.k, d.ks), ("v", d.v, d.vs)):
+            c.append(n, 0, first, x)
+            np.testing.assert_array_equal(codes.cpu().numpy(), c.codes[n])
+            np.testing.assert_array_equal(scales.cpu().numpy(), c.scales[n])
+        qt, qv = _typed(rng.randn(tokens, hq * hd), "f32")
+        for window in windows:
+            out = _np(_attention(gpu, d, pos, tokens, "f32", qt, hq, window, longest=1000)).reshape(tokens, hq, hd)
+            held = window if window else 12 * page + tokens      # nothing lies before the last twelve pages
+            y, bound = _attend_all(c, qv.reshape(tokens, hq, hd), [first], tokens, hq, held, hd ** -0.5, "f32")
+            assert (np.abs(out - y) <= bound + 1.01 * eb.rounding(y, "f32")).all()
