@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
         if (SLOTS == 4) copy(3, false, 1);
         const float *k_scales = a.c.k_scales + h, *v_scales = a.c.v_scales + h;
         auto scale_of = [&](const float* scales) { return page[0] >= 0 ? scales[(long long)page[0] * a.c.kv_heads] : 0.0f; };
-        float k_scale = scale_of(k_scales), v_scale = scale_of(v_scales);
+        float k_scale = scale_of(k_scales), v_scale = scale_of(v_scales) * KV8_LOWER;
         // queries as B operands, of pair 8 n + g
         uint2* qb = queries + warp * (B::QUERIES / 8) + lane;
         const bool wide = ((uintptr_t)a.q | (uintptr_t)(a.ldq * (long long)sizeof(T))) % (4 * sizeof(T)) == 0;
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
             {                                // this tile's scales are in use: the next one's
                 const int p = page[1] >= 0 ? page[1] : page[0];
                 k_scale = k_scales[(long long)p * a.c.kv_heads];
-                v_scale = v_scales[(long long)p * a.c.kv_heads];
+                v_scale = v_scales[(long long)p * a.c.kv_heads] * KV8_LOWER;
             }
 #pragma unroll
             for (int i = 0; i < TILES; i++) {
@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(Kv8Block<HD, NT>::WARPS * 32, 1)
         T* out = static_cast<T*>(a.out) + ((long long)b * a.n_tokens + pair / share) * a.ldo +
                  (h * share + pair % share) * HD + d;
 #pragma unroll
-        for (int i = 0; i < 4; i++) out[i] = dz_from_float<T>(any ? y[i] / total : 0.0f);
+        for (int i = 0; i < 4; i++) out[i] = dz_from_float<T>(any ? y[i] / (total * KV8_LOWER) : 0.0f);
     }
     if (cluster > 1) cg::this_cluster().sync();      // no block ends while another reads its shared memory
 }

@@ -52,6 +52,10 @@ __device__ __forceinline__ float kv8_far_power(float x, float f, float m) {
     return __fadd_rn(__fadd_rn(__fmul_rn(x, f), m == -INFINITY ? 0.0f : -m), 15.0f);
 }
 
+// What takes the weights' 2^15 off the sums, in the values' scales, so that sums
+// stay in fp32's range as far as those of weights up to 1 do.
+constexpr float KV8_LOWER = 0x1p-15f;
+
 // Clusters of 1..16 blocks of a kernel that a device holds at once (a cluster
 // stays within one GPC, so that larger ones leave SMs idle; 0: it cannot hold
 // one). Asked once per kernel and device.

@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
                 int32_t raw[32];
                 ug_tmem_ld32(sums + (uint32_t)c, raw);
 #pragma unroll
-                for (int j = 0; j < 32; j++) o[c + j] = fmaf(__int_as_float(raw[j]), vt, o[c + j] * shrink);
+                for (int j = 0; j < 32; j++) o[c + j] = fmaf(__int_as_float(raw[j]), vt * KV8_LOWER, o[c + j] * shrink);
             }
         }
         if (!ok) *failed = 1;
@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(KV8M_THREADS, HD == 64 ? 2 : 1)
             const int pair = r0 + row;
             T* out = static_cast<T*>(a.out) + ((long long)b * a.n_tokens + pair / share) * a.ldo + (h * share + pair % share) * HD + 4 * d;
 #pragma unroll
-            for (int e = 0; e < 4; e++) out[e] = dz_from_float<T>(any ? y[e] / total : 0.0f);
+            for (int e = 0; e < 4; e++) out[e] = dz_from_float<T>(any ? y[e] / (total * KV8_LOWER) : 0.0f);
         }
     };
     if (cluster > 1)

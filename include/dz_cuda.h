@@ -215,7 +215,9 @@ int dz_cuda_kv8_append(const dz_kv8_t *cache, const dz_kv8_append_t *args, const
  * itself or 2^-39 of the largest (with more than 32 queries of a key head and
  * pages of different value scales, or its product with its value's scale to
  * 2^-39 of the largest one). A token that is seen makes a NaN of its output where
- * its page's scale is one, whatever its weight. out must not overlap q or the
+ * its page's scale is one, whatever its weight. Sums are of weights up to 1: they
+ * hold while tokens x |value| stay in fp32's range, and scores while |scale| x a
+ * query's largest element is 2^-96 or more (or 0). out must not overlap q or the
  * cache. */
 int dz_cuda_kv8_attention(const dz_kv8_t *cache, const dz_kv8_attention_t *args, const int64_t *positions,
                           size_t n_tokens, void *stream);

@@ -221,3 +221,20 @@ def test_the_end_of_the_longest_table(gpu, page, hq, tokens, windows):
             held = window if window else 12 * page + tokens      # nothing lies before the last twelve pages
             y, bound = _attend_all(c, qv.reshape(tokens, hq, hd), [first], tokens, hq, held, hd ** -0.5, "f32")
             assert (np.abs(out - y) <= bound + 1.01 * eb.rounding(y, "f32")).all()
+
+
+@pytest.mark.parametrize("hq,tokens", PAIRS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_values_near_the_end_of_fp32(gpu, kind, hd, hq, tokens):
+    """Values of up to 2^119, 190 of them: their sum lies in fp32's range."""
+    rng = np.random.RandomState(hd + tokens)
+    c = eb.Cache(rng, 6, 32, 1, hd, [np.arange(6)])
+    c.scales["v"][:] = np.float32(2.0 ** 112)
+    c.scales["v"][2] = np.float32(2.0 ** 90)
+    d = Device(gpu, c)
+    qt, qv = _typed(0.01 * rng.randn(tokens, hq * hd), kind)
+    first = 190 - tokens
+    out = _np(_attention(gpu, d, _dev(np.array([first], np.int64)), tokens, kind, qt, hq)).reshape(tokens, hq, hd)
+    y, bound = _attend_all(c, qv.reshape(tokens, hq, hd), [first], tokens, hq, 0, hd ** -0.5, "f32")
+    assert (np.abs(out - y) <= bound + 1.01 * eb.rounding(y, kind)).all()
