@@ -95,7 +95,8 @@ __device__ __forceinline__ float q8_scale(const Q8NormArgs& a, float peak, doubl
     if (peak == 0.0f) return 0.0f;
     if (!a.norm) return __fdiv_rn(peak, 127.0f);
     const double m = mean + a.eps64;
-    if (!(m > 1e-30 && m < 1e30)) return (float)((double)peak / sqrt(m) / 127.0);
+    // the reciprocal root is below 1e15 there, and its product with the peak within fp32
+    if (!(m > 1e-30 && m < 1e30 && peak < 1e22f)) return (float)((double)peak / sqrt(m) / 127.0);
     float s = rsqrtf((float)m);
     s = s * fmaf(-0.5f * (float)m * s, s, 1.5f);               // a Newton step
     return __fdiv_rn(peak * s, 127.0f);

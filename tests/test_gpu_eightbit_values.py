@@ -238,3 +238,24 @@ def test_values_near_the_end_of_fp32(gpu, kind, hd, hq, tokens):
     out = _np(_attention(gpu, d, _dev(np.array([first], np.int64)), tokens, kind, qt, hq)).reshape(tokens, hq, hd)
     y, bound = _attend_all(c, qv.reshape(tokens, hq, hd), [first], tokens, hq, 0, hd ** -0.5, "f32")
     assert (np.abs(out - y) <= bound + 1.01 * eb.rounding(y, kind)).all()
+
+
+@pytest.mark.parametrize("width", [40, 4096, 5003, 20000])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_row_scales_near_the_end_of_fp32(gpu, kind, width):
+    """Gains so large that peak / root-mean-square leaves fp32 where the scale, a 127th of it, does not."""
+    x = np.zeros((3, width))
+    x[0, width // 2] = 2.0 ** -10            # root-mean-square: 2^-10 / sqrt(width)
+    x[1, :] = 1.0
+    x[2, 3:7] = -2.0 ** -12
+    gain = np.full(width, min(2.0 ** 127, 2.0 ** 134 / np.sqrt(width)), np.float32)
+    xt, xv = _typed(x, kind)
+    gt = _dev(gain)
+    codes = torch.empty(3, -(-width // 16) * 16, dtype=torch.int8, device="cuda")
+    scales = torch.empty(3, device="cuda")
+    gpu.norm_q8(3, width, type={"f32": gpu.TYPE_F32, "f16": gpu.TYPE_F16, "bf16": gpu.TYPE_BF16}[kind], x=xt.data_ptr(),
+                gain=gt.data_ptr(), eps=0.0, codes=codes.data_ptr(), scales=scales.data_ptr(), stream_ptr=_stream())
+    want, scale = eb.norm_rows(xv, gain, True, 0.0)
+    assert 2.0 ** 128 < 127 * scale[0] < 2.0 ** 134.99          # peak / rms of the first row
+    np.testing.assert_array_equal(codes[:, :width].cpu().numpy(), want)
+    assert (np.abs(_np(scales) - scale) <= eb.NORM_SCALE * scale).all()
