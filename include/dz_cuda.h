@@ -180,7 +180,8 @@ int dz_cuda_norm_q8(const dz_norm_q8_t *args, size_t rows, size_t width, void *s
  * A int8 with row stride lda >= k, a multiple of 16, on a 16-byte boundary;
  * what a row holds past k does not matter. bias fp32 or NULL. C has element type `type` and row
  * stride ldc >= n in elements, and overlaps nothing else. Sums are exact, the
- * rest fp32 with one rounding to `type`. The handle holds no scratch for it:
+ * rest fp32 (a sum times its row's scale, then the column's, with the bias added
+ * in the same step) with one rounding to `type`. The handle holds no scratch for it:
  * calls on one matrix may overlap, and a call may be captured. */
 int dz_cuda_matmul_q8_async(const int8_t *A_dev, size_t lda, const float *a_scales_dev,
                             const dz_cuda_qmatrix_t *weights, const float *bias_dev, void *C_dev, size_t ldc, size_t m,

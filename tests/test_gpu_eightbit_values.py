@@ -259,3 +259,54 @@ def test_row_scales_near_the_end_of_fp32(gpu, kind, width):
     assert 2.0 ** 128 < 127 * scale[0] < 2.0 ** 134.99          # peak / rms of the first row
     np.testing.assert_array_equal(codes[:, :width].cpu().numpy(), want)
     assert (np.abs(_np(scales) - scale) <= eb.NORM_SCALE * scale).all()
+
+
+@pytest.mark.parametrize("kind,hd,tokens,halves,pad", [("f32", 64, 1, 0, 0), ("bf16", 128, 1, 1, 0), ("f16", 128, 1, 0, 1), ("bf16", 128, 77, 1, 0),
+                                                       ("f32", 128, 150, 0, 0), ("f16", 64, 40, 1, 0), ("bf16", 64, 33, 0, 3)])
+def test_append_in_place(gpu, kind, hd, tokens, halves, pad):
+    """Outputs that are their own input rows: what other rows of output get, for more heads than are read ahead."""
+    rng = np.random.RandomState(hd + tokens)
+    hq, hk, batch, page = 21, 3, 3, 32
+    per = (60 + tokens) // page + 1
+    caches = [eb.Cache(np.random.RandomState(1), batch * per, page, hk, hd, np.arange(batch * per).reshape(batch, per))
+              for _ in range(2)]
+    devices = [Device(gpu, c) for c in caches]
+    width, rows = (hq + 2 * hk) * hd + pad, batch * tokens
+    xt, _ = _typed(rng.randn(rows, width) * 3, kind)
+    own = xt.clone()
+    gains = [_dev((1 + 0.2 * rng.randn(hd)).astype(np.float32)) for _ in range(2)]
+    pos, size = _dev(np.array([0, 31, 60], np.int64)), xt.element_size()
+    outs = [torch.full_like(xt, 5.0) for _ in range(3)]
+    for x, d, to in ((xt, devices[0], outs), (own, devices[1], None)):
+        at = [x.data_ptr() + n * hd * size for n in (0, hq, hq + hk)]
+        o = at if to is None else [t.data_ptr() + n * hd * size for t, n in zip(to, (0, hq, hq + hk))]
+        d.cache.append(pos.data_ptr(), tokens, type={"f32": gpu.TYPE_F32, "f16": gpu.TYPE_F16, "bf16": gpu.TYPE_BF16}[kind],
+                       q_heads=hq, q=at[0], k=at[1], v=at[2], q_stride=width, k_stride=width, v_stride=width, q_out=o[0],
+                       q_out_stride=width, k_out=o[1], k_out_stride=width, v_out=o[2], v_out_stride=width,
+                       q_gain=gains[0].data_ptr(), k_gain=gains[1].data_ptr(), rope_base=10000.0, halves=bool(halves),
+                       stream_ptr=_stream())
+    parts = [outs[0][:, :hq * hd], outs[1][:, hq * hd:(hq + hk) * hd], outs[2][:, (hq + hk) * hd:(hq + 2 * hk) * hd]]
+    assert torch.equal(own[:, :(hq + 2 * hk) * hd], torch.cat(parts, 1))
+    assert torch.equal(own[:, (hq + 2 * hk) * hd:], xt[:, (hq + 2 * hk) * hd:]) and not torch.equal(own, xt)
+    for name in ("k", "v", "ks", "vs"):
+        assert torch.equal(getattr(devices[0], name), getattr(devices[1], name))
+
+
+def test_many_queries_past_32_bits(gpu):
+    """Pages beyond 2^31 codes of a pool, read by blocks of 128 pairs."""
+    rng = np.random.RandomState(5)
+    page, hk, hd, pages, tokens = 64, 8, 128, 40000, 33          # 2.6e9 codes
+    c = eb.Cache(rng, 4, page, hk, hd, [[0, 1, 2, 3]])
+    at = torch.tensor([39999, 0, 33000, 39001], device="cuda")
+    k = torch.zeros(pages, hk, page, hd, dtype=torch.int8, device="cuda")
+    v = torch.zeros_like(k)
+    ks, vs = torch.ones(pages, hk, device="cuda"), torch.ones(pages, hk, device="cuda")
+    for big, small in ((k, c.codes["k"]), (v, c.codes["v"]), (ks, c.scales["k"]), (vs, c.scales["v"])):
+        big[at] = _dev(small)
+    table, pos = at.to(torch.int32)[None].contiguous(), _dev(np.array([200], np.int64))
+    cache = gpu.KV8Cache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, page, hk, hd, table.data_ptr(), 1, 4)
+    qt, qv = _typed(rng.randn(tokens, 2 * hk * hd), "bf16")
+    out = torch.empty_like(qt)
+    cache.attention(pos.data_ptr(), tokens, type=gpu.TYPE_BF16, q_heads=2 * hk, q=qt.data_ptr(), out=out.data_ptr(), stream_ptr=_stream())
+    y, bound = _attend_all(c, qv.reshape(tokens, 2 * hk, hd), [200], tokens, 2, 0, hd ** -0.5, "f32")
+    assert (np.abs(_np(out).reshape(y.shape) - y) <= bound + 1.01 * eb.rounding(y, "bf16")).all()
