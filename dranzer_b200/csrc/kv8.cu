@@ -27,9 +27,10 @@ namespace dz {
 // One token: a block takes a share of a row's heads, a warp two or four heads
 // at a time.
 //
-// Queries are normed and rotated in fp32. Keys are in 64 bits up to one
-// rounding to fp32, because the codes that follow round values next to a border
-// and two summation orders would otherwise give different codes.
+// Queries are normed and rotated in fp32, as the scores that they enter are. Keys
+// are in 64 bits up to one rounding to fp32, because the codes that follow round
+// values next to a border and two summation orders would otherwise give different
+// codes.
 
 constexpr int KV8_WARPS = 16;      // warps of a block, many tokens
 constexpr int KV8_ROWS = 4;        // rows of a warp

@@ -10,7 +10,7 @@
 // scale for keys and one for values serve a whole tile. Its keys and its values
 // come by TMA, each a box of 32 rows into a slot of the warp's own ring, three
 // or four of them ahead (loads into registers left no room for enough of them:
-// 231 us where this takes less). They
+// 231 us for 24 ragged sequences where the ring took 208). They
 // are read as MMA operands by ldmatrix: keys as they are, values turned in units
 // of two elements, so that a register holds two elements of two tokens; the
 // weights turn from the scores' result into the sums' operand by movmatrix.
@@ -19,15 +19,17 @@
 // query is counted in steps of 2^-30 of a power of two above its largest element
 // and cut into four balanced base-256 digits, so that products and sums are
 // exact and nothing is widened (with keys widened a tile took 831 instructions
-// where it takes 757). With more pairs the digits' sums cost more than keys
+// where the digits took 757). With more pairs the digits' sums cost more than keys
 // widened once for all of them: keys are fp16 (m16n8k16), queries fp16 too, bf16
 // and fp32 ones times a power of two of their row (its largest element in [2^13,
-// 2^14)), fp32 ones in two parts. Codes become fp16 exactly, two at a time, by
-// setting the exponent of 1024 above the byte and subtracting 1024 + 128; values
-// always do, and weights are taken times 2^15 in two fp16 parts (22 bits of each;
-// one part alone, 11 bits, would save 6% of a tile's instructions and show in
-// bf16 outputs where values of both signs cancel). Scores of a tile
-// take the page's key scale, the sums of a tile its value scale, both in fp32.
+// 2^14)), fp32 ones in two parts (22 of their 24 bits: a third part would be half
+// again as many MMAs for less than the fp32 sums of the scores round). Codes
+// become fp16 exactly, two at a time, by setting the exponent of 1024 above the
+// byte and subtracting 1024 + 128; values always do, and weights are taken times
+// 2^15 in two fp16 parts (22 bits of each; one part alone, 11 bits, would save 6%
+// of a tile's instructions and show in bf16 outputs where values of both signs
+// cancel). Scores of a tile take the page's key scale, the sums of a tile its
+// value scale, both in fp32.
 //
 // Few units of long contexts go to clusters of blocks, many to a warp each
 // (kv8_shape); the parts (maximum, sum of weights, sums) join at the end in
@@ -702,8 +704,9 @@ static cudaError_t kv8_attn_h(const Kv8AttnArgs& a, long long longest, int head_
 
 cudaError_t dz_kv8_attn_launch(const Kv8AttnArgs& a, long long longest, int type, int head_dim, int device, cudaStream_t st) {
     if (device < 0 || device >= KV8_DEVICES) return cudaErrorInvalidDevice;
-    // pairs of a key head: 128 in a block of kv8many.cu, 16 in a warp here (8 sequences of 4000 tokens, 4 key heads. Heads of 64
-    // in fp16: 64 pairs 31 and 26 us, 80 32 and 45, 320 66 and 123. Heads of 128 in bf16: 48 pairs 34 and 38, 128 37 and 70)
+    // pairs of a key head: 16 in a warp here, 128 in a block of kv8many.cu (8 sequences of 4000 tokens, 4 key heads, here and
+    // there. Heads of 64 in fp16: 64 pairs 27 and 25 us, 80 46 and 26, 320 125 and 68; in fp32 29 and 26, 50 and 27, 137 and
+    // 70. Heads of 128 in bf16: 32 pairs 28 and 38, 48 44 and 39, 128 79 and 41; in fp32 30 and 40, 49 and 41, 90 and 44)
     if (a.n_tokens * (a.q_heads / a.c.kv_heads) > (head_dim == 128 ? 32 : 64)) return dz_kv8_many_launch(a, longest, type, head_dim, device, st);
     if (type == DZ_TYPE_F32) return kv8_attn_h<float>(a, longest, head_dim, device, st);
     if (type == DZ_TYPE_F16) return kv8_attn_h<__half>(a, longest, head_dim, device, st);

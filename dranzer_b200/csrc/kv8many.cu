@@ -13,20 +13,21 @@
 // threads keeps a maximum, a sum and the sums of values of its tokens; they and
 // the cluster's blocks' join at the end.
 //
-// 32 x 128 pairs over 4112 tokens of heads of 64 in fp16 take 37 us (47 in warps
-// of 16 pairs), 512 tokens of 32 heads of 128 in bf16 over 8512 positions 205 (510),
-// 340 TFLOP/s. Bound by the chain of a tile (2.95 us of a block alone: a fifth
+// 32 x 128 pairs over 4112 tokens of heads of 64 in fp16 take 38 us (49 in warps
+// of 16 pairs), 512 tokens of 32 heads of 128 in bf16 over 8512 positions 244 (560),
+// 284 TFLOP/s. Bound by the chain of a tile (about 3 us of a block alone: a fifth
 // widening, a sixth the scores' maximum, two fifths weights, a fifth sums), not by
 // a unit; only the second block of an SM, with heads of 64, fills its gaps. Packed
 // fp32 operations gained nothing.
 //
 // Queries are fp16 times a power of two of their row (its largest element in
 // [2^13, 2^14)), fp32 ones in two parts; codes are fp16 exactly; weights are taken
-// times 2^15 in two fp16 parts. The pages' key scales meet the
-// scores in fp32. Where two pages of different value scales share a thread's 64
-// tokens, the weights take these over one scale, which the tile's sums take in
-// fp32: that of the page whose largest weight x scale is larger, times that
-// weight, so that what counts keeps its bits whatever the scales are.
+// times 2^15 in two fp16 parts (kv8attn.cu has what these hold, and why). The
+// pages' key scales meet the scores in fp32. Where two pages of different value
+// scales share a thread's 64 tokens, the weights take these over one scale, which
+// the tile's sums take in fp32: that of the page whose largest weight x scale is
+// larger, times that weight, so that what counts keeps its bits whatever the
+// scales are.
 #include <cooperative_groups.h>
 #include <type_traits>
 
@@ -576,7 +577,7 @@ template <typename T, int HD> static cudaError_t kv8_many_t(const Kv8AttnArgs& a
     }
     const int pairs = a.n_tokens * (a.q_heads / a.c.kv_heads), blocks = (pairs + KV8M_PAIRS - 1) / KV8M_PAIRS;
     const long long units = (long long)a.c.batch * a.c.kv_heads * blocks;
-    // the blocks of a cluster: the least estimated time, in tiles of a block alone on its SM (2.95 us with heads of 64). Two on
+    // the blocks of a cluster: the least estimated time, in tiles of a block alone on its SM (about 3 us with heads of 64). Two on
     // an SM, which the occupancy does not count for kernels with tensor memory, take 1.66 times as long, and a cluster then
     // half of the SMs; a start and an end are worth 4 tiles, a join 1 and 0.1 for each block.
     const long long visible = a.window && a.window < longest ? a.window + a.n_tokens : longest;
